@@ -77,6 +77,20 @@ extern "C" {
         block_bytes: i64, src_block_stride_bytes: i64, dst_block_stride_bytes: i64, num_layers: i32,
         src_layer_stride_bytes: i64, dst_layer_stride_bytes: i64, stream: *mut c_void,
     ) -> c_int;
+    /// New: workspace bytes of rg_evict_cache.
+    pub fn rg_evict_cache_workspace_bytes(
+        num_layers: i32, batch_size: i32, num_kv_heads: i32, budget: i32,
+    ) -> usize;
+    /// New: trims sequences to a budget of cached tokens by accumulated attention weight.
+    pub fn rg_evict_cache(
+        key_cache: *mut c_void, value_cache: *mut c_void, scores: *mut f32, block_table: *const i32,
+        dst_block_table: *const i32, context_lens: *const i32, new_context_lens: *mut i32,
+        kept_positions: *mut i32, budget: i32, recent: i32, protected_len: i32, num_layers: i32,
+        num_kv_heads: i32, head_dim: i32, block_size: i32, max_blocks_per_seq: i32,
+        max_dst_blocks_per_seq: i32, batch_size: i32, dtype: i32, layer_stride: i64, kv_block_stride: i64,
+        score_layer_stride: i64, score_block_stride: i64, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
     /// Residual add + RMSNorm around each sublayer (architecture.rs:38-59).
     pub fn rg_rms_norm(
         x: *const c_void, residual: *mut c_void, weight: *const c_void, out: *mut c_void, eps: f32,

@@ -517,6 +517,52 @@ impl PagedAttentionKernels {
                                    src_layer_stride_bytes, dst_layer_stride_bytes, self.stream))
     }
 
+    /// Workspace bytes of `launch_evict`.
+    pub fn evict_workspace_bytes(&self, num_layers: i32, batch_size: i32, num_kv_heads: i32, budget: i32) -> usize {
+        // SAFETY: pure size query.
+        unsafe { ffi::rg_evict_cache_workspace_bytes(num_layers, batch_size, num_kv_heads, budget) }
+    }
+
+    /// Trims every sequence to `budget` cached tokens by `scores`, per layer and kv-head: the first
+    /// `protected_len` and the last `recent` tokens stay, of the others those with the highest
+    /// scores; what stays goes, in order, to the blocks of `dst_block_table` (None: in place).
+    /// `key_cache`, `value_cache` and `scores` point at layer 0; strides in elements.
+    pub unsafe fn launch_evict<T: KvElement>(
+        &self,
+        key_cache: &mut HipSlice<T>,
+        value_cache: &mut HipSlice<T>,
+        scores: &mut HipSlice<f32>,
+        block_table: &HipSlice<i32>,
+        dst_block_table: Option<&HipSlice<i32>>,
+        context_lens: &HipSlice<i32>,
+        new_context_lens: Option<&mut HipSlice<i32>>,
+        kept_positions: Option<&mut HipSlice<i32>>,
+        budget: i32,
+        recent: i32,
+        protected_len: i32,
+        num_layers: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        max_dst_blocks_per_seq: i32,
+        batch_size: i32,
+        layer_stride: i64,
+        score_layer_stride: i64,
+        score_block_stride: i64,
+        workspace: &mut HipSlice<u8>,
+    ) -> CoreResult<()> {
+        let dst = dst_block_table.map_or(std::ptr::null(), |t| t.as_ptr() as *const i32);
+        let lens = new_context_lens.map_or(std::ptr::null_mut(), |t| t.as_mut_ptr() as *mut i32);
+        let kept = kept_positions.map_or(std::ptr::null_mut(), |t| t.as_mut_ptr() as *mut i32);
+        status(ffi::rg_evict_cache(
+            key_cache.as_mut_ptr(), value_cache.as_mut_ptr(), scores.as_mut_ptr() as *mut f32,
+            block_table.as_ptr() as *const i32, dst, context_lens.as_ptr() as *const i32, lens, kept, budget, recent,
+            protected_len, num_layers, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+            max_dst_blocks_per_seq, batch_size, T::DTYPE, layer_stride, self.kv_block_stride, score_layer_stride,
+            score_block_stride, workspace.as_mut_ptr(), workspace.len(), self.stream))
+    }
+
     /// Residual add + RMSNorm over `num_rows` rows (`residual` may be None).
     pub unsafe fn launch_rms_norm<T: KvElement>(
         &self,

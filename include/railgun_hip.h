@@ -173,6 +173,41 @@ int rg_copy_blocks(const void* src_pool, void* dst_pool, const int32_t* block_ma
                    int64_t src_layer_stride_bytes, int64_t dst_layer_stride_bytes,
                    void* stream);
 
+/* Trims sequences to `budget` cached tokens by accumulated attention weight, for every layer and
+ * kv-head on its own.  Sequence s with n = context_lens[s] <= budget tokens keeps them all.  Past
+ * the budget it keeps the positions t < protected_len, those t >= n - recent, and of the others the
+ * budget - protected_len - recent with the highest score; of equal scores (-0 equals +0) the lower
+ * position stays, a NaN ranks as -inf.  scores is fp32, paged like the caches:
+ * [num_blocks, num_kv_heads, block_size] per layer, score_block_stride elements between blocks (0:
+ * dense), filled by rg_paged_attention_v1_scores or by the caller.
+ *
+ * The kept tokens' K and V rows and scores are written, in the order of their positions, to
+ * positions 0, 1, .. of row s of dst_block_table [batch, max_dst_blocks_per_seq], or with
+ * dst_block_table == NULL to the row of block_table itself (in place).  All other cells keep what
+ * they hold.  An entry of the destination row may be the block at the same place of the same row of
+ * block_table (a prefix that stays, or the whole row); every other destination block must appear in
+ * no other entry of either table that the call uses.  Blocks that hold positions below
+ * protected_len only, at the same place in both rows, are not written, so sequences may share them.
+ *
+ * new_context_lens (NULL: not wanted) [batch] gets min(n, budget); kept_positions (NULL: not wanted)
+ * [num_layers, batch, num_kv_heads, budget] the kept positions in order, -1 behind them.
+ * key_cache / value_cache / scores point at layer 0, layer l lies layer_stride (score_layer_stride)
+ * elements further on.  The workspace (rg_evict_cache_workspace_bytes, 4-byte aligned) needs no
+ * clearing; of it the first 4 bytes per (layer, sequence, kv-head), rounded up to 256, suffice with
+ * kept_positions.  New entry: the reference never drops a cached token. */
+size_t rg_evict_cache_workspace_bytes(int32_t num_layers, int32_t batch_size,
+                                      int32_t num_kv_heads, int32_t budget);
+int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
+                   const int32_t* block_table, const int32_t* dst_block_table,
+                   const int32_t* context_lens, int32_t* new_context_lens,
+                   int32_t* kept_positions, int32_t budget, int32_t recent,
+                   int32_t protected_len, int32_t num_layers, int32_t num_kv_heads,
+                   int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq,
+                   int32_t max_dst_blocks_per_seq, int32_t batch_size, int32_t dtype,
+                   int64_t layer_stride, int64_t kv_block_stride,
+                   int64_t score_layer_stride, int64_t score_block_stride,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------- model element-wise ops -- */
 
 /* Fused residual add + RMSNorm over rows of hidden_size elements:

@@ -282,6 +282,24 @@ class PagedAttentionKernels {
                             num_tokens, max_query_len, (int32_t)dtype, kv_block_stride, stream_),
           "launch_prefill_packed");
   }
+  size_t evict_workspace_bytes(int32_t num_layers, int32_t batch_size, int32_t num_kv_heads, int32_t budget) const {
+    return rg_evict_cache_workspace_bytes(num_layers, batch_size, num_kv_heads, budget);
+  }
+  // Trims every sequence to `budget` cached tokens by score, per layer and kv-head; what stays goes,
+  // in order, to the blocks of dst_block_table (nullptr: in place).
+  void launch_evict(void* key_cache, void* value_cache, float* scores, const int32_t* block_table,
+                    const int32_t* dst_block_table, const int32_t* context_lens, int32_t* new_context_lens,
+                    int32_t* kept_positions, int32_t budget, int32_t recent, int32_t protected_len, int32_t num_layers,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq,
+                    int32_t max_dst_blocks_per_seq, int32_t batch_size, void* workspace, size_t workspace_bytes,
+                    DType dtype = DType::BF16, int64_t layer_stride = 0, int64_t kv_block_stride = 0,
+                    int64_t score_layer_stride = 0, int64_t score_block_stride = 0) const {
+    check(rg_evict_cache(key_cache, value_cache, scores, block_table, dst_block_table, context_lens, new_context_lens,
+                         kept_positions, budget, recent, protected_len, num_layers, num_kv_heads, head_dim, block_size,
+                         max_blocks_per_seq, max_dst_blocks_per_seq, batch_size, (int32_t)dtype, layer_stride,
+                         kv_block_stride, score_layer_stride, score_block_stride, workspace, workspace_bytes, stream_),
+          "launch_evict");
+  }
 
  private:
   int ordinal_;

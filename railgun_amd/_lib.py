@@ -74,6 +74,8 @@ SIGNATURES = {
         c_int,
         [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int64, c_int64, c_void_p],
     ),
+    "rg_evict_cache_workspace_bytes": (c_size_t, [c_int32] * 4),
+    "rg_evict_cache": (c_int, [c_void_p] * 8 + [c_int32] * 11 + [c_int64] * 4 + [c_void_p, c_size_t, c_void_p]),
     "rg_rms_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int32, c_int32, c_int32, c_void_p]),
     "rg_silu_and_mul": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p]),
     "rg_silu_and_mul_interleaved": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p]),

@@ -11,6 +11,8 @@ no data (crates/vllm-paged-attention/src/allocator.rs:102-153).  Here:
   kernels take (block stride ``2 H_kv bs D`` elements);
 * :class:`CpuBlockPool` is the host pool in pinned memory, which the GPU reads and writes
   directly;
+* :attr:`GpuBlockPool.scores` and :meth:`GpuBlockPool.evict` trim sequences to a budget of tokens by
+  the attention weight they have gathered (the reference never drops a cached token);
 * :meth:`GpuBlockPool.swap_out`, :meth:`GpuBlockPool.swap_in` and
   :meth:`GpuBlockPool.copy_blocks` are the physical copies behind the allocator's swap and
   copy-on-write, each one ``rg_copy_blocks`` launch over all layers.
@@ -56,6 +58,7 @@ class GpuBlockPool:
         self.block_size = block_size
         self.device = self.storage.device
         self._kernels = kernels
+        self._scores: Optional[torch.Tensor] = None
 
     @staticmethod
     def for_model(cfg, num_blocks: int, block_size: int, device, dtype=torch.bfloat16,
@@ -76,6 +79,27 @@ class GpuBlockPool:
     def v_cache(self, layer: int) -> torch.Tensor:
         """block.rs:93-95: the V view [NB, H_kv, bs, D] of one layer."""
         return self.storage[layer, :, 1]
+
+    @property
+    def scores(self) -> torch.Tensor:
+        """fp32 [layers, NB, H_kv, bs]: the attention weight each cached token has gathered
+        (launch_v1_scores adds to it, evict goes by it); made, with zeros, when first asked for."""
+        if self._scores is None:
+            layers, blocks, _, hkv, bs, _ = self.storage.shape
+            self._scores = torch.zeros((layers, blocks, hkv, bs), device=self.device, dtype=torch.float32)
+        return self._scores
+
+    def evict(self, block_table: torch.Tensor, context_lens: torch.Tensor, budget: int, recent: int,
+              protected_len: int = 0, dst_block_table: Optional[torch.Tensor] = None,
+              kept_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Trims the sequences of ``block_table`` to ``budget`` tokens by ``scores``, every layer in one
+        call (launch_evict); returns the new context lengths, int32 on the device.  In place, the
+        blocks past a sequence's new length hold nothing it needs: the caller frees or refills them."""
+        new_lens = torch.empty_like(context_lens)
+        self.kernels.launch_evict(self.storage[:, :, 0], self.storage[:, :, 1], self.scores, block_table,
+                                  dst_block_table, context_lens, new_lens, kept_positions, budget, recent,
+                                  protected_len)
+        return new_lens
 
     def copy_blocks(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Copy-on-write: block dst[i] becomes a copy of block src[i], K and V, every layer."""

@@ -364,6 +364,60 @@ class PagedAttentionKernels:
             src_pool.stride(bdim) * es, dst_pool.stride(bdim) * es, int(src_pool.shape[0]) if layered else 1,
             src_pool.stride(0) * es if layered else 0, dst_pool.stride(0) * es if layered else 0, stream))
 
+    def evict_workspace_bytes(self, num_layers: int, batch_size: int, num_kv_heads: int, budget: int) -> int:
+        return int(self.lib.rg_evict_cache_workspace_bytes(num_layers, batch_size, num_kv_heads, budget))
+
+    def launch_evict(self, key_cache, value_cache, scores, block_table, dst_block_table, context_lens,
+                     new_context_lens, kept_positions, budget: int, recent: int, protected_len: int = 0,
+                     workspace: Optional[torch.Tensor] = None) -> None:
+        """Trims every sequence to ``budget`` tokens by score, per layer and kv-head (rg_evict_cache):
+        the first ``protected_len`` and the last ``recent`` tokens stay, of the others those with the
+        highest scores; what stays goes, in order, to the blocks of ``dst_block_table`` (None: in
+        place).
+
+        Caches ``[NB, H_kv, bs, D]`` or ``[layers, NB, H_kv, bs, D]`` with contiguous blocks, scores
+        fp32 of the caches' shape without D.  ``new_context_lens`` [B] and ``kept_positions``
+        ``[layers, B, H_kv, budget]`` (int32, either may be None) receive the new lengths and the kept
+        positions.  ``workspace``: evict_workspace_bytes, allocated here when omitted.
+        """
+        def bad(msg: str):
+            return RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "evict: " + msg)
+
+        _require_cuda(key_cache, value_cache, scores, block_table, dst_block_table, context_lens, new_context_lens,
+                      kept_positions, workspace)
+        _require_i32(block_table, context_lens)
+        _require_i32(*(t for t in (dst_block_table, new_context_lens, kept_positions) if t is not None))
+        if key_cache.dim() not in (4, 5) or value_cache.shape != key_cache.shape or \
+                value_cache.dtype != key_cache.dtype or value_cache.stride() != key_cache.stride():
+            raise bad("caches must be [NB, H_kv, bs, D] or [layers, NB, H_kv, bs, D], alike in shape, strides and dtype")
+        layered = key_cache.dim() == 5
+        layers = int(key_cache.shape[0]) if layered else 1
+        nb, hkv, bs, d = (int(x) for x in key_cache.shape[-4:])
+        if key_cache.stride()[-3:] != (bs * d, d, 1):
+            raise bad("cache blocks must be contiguous [H_kv, bs, D]")
+        if scores.dtype != torch.float32 or scores.shape != key_cache.shape[:-1] or scores.stride()[-2:] != (bs, 1):
+            raise bad("scores must be float32 of the caches' shape without head_dim, its blocks contiguous")
+        batch = int(context_lens.numel())
+        if block_table.dim() != 2 or int(block_table.shape[0]) != batch:
+            raise bad("block_table must be [batch, max_blocks]")
+        if dst_block_table is not None and (dst_block_table.dim() != 2 or int(dst_block_table.shape[0]) != batch):
+            raise bad("dst_block_table must be [batch, max_dst_blocks]")
+        if new_context_lens is not None and int(new_context_lens.numel()) != batch:
+            raise bad("new_context_lens needs one entry per sequence")
+        if kept_positions is not None and int(kept_positions.numel()) != layers * batch * hkv * budget:
+            raise bad(f"kept_positions must be [{layers}, {batch}, {hkv}, {budget}]")
+        if workspace is None:
+            nbytes = self.evict_workspace_bytes(layers, batch, hkv, budget if kept_positions is None else 1)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=key_cache.device)
+        check(self.lib.rg_evict_cache(
+            key_cache.data_ptr(), value_cache.data_ptr(), scores.data_ptr(), block_table.data_ptr(),
+            _ptr(dst_block_table), context_lens.data_ptr(), _ptr(new_context_lens), _ptr(kept_positions), budget,
+            recent, protected_len, layers, hkv, d, bs, int(block_table.shape[1]),
+            0 if dst_block_table is None else int(dst_block_table.shape[1]), batch, dtype_code(key_cache),
+            key_cache.stride(0) if layered else 0, key_cache.stride(-4), scores.stride(0) if layered else 0,
+            scores.stride(-3), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            _stream(key_cache)))
+
     def launch_prefill_packed(self, query, key_cache, value_cache, block_table, context_lens, cu_seqlens,
                               output, scale: float, num_heads: int, num_kv_heads: int, head_dim: int,
                               block_size: int, max_blocks_per_seq: int, num_seqs: int, num_tokens: int,
