@@ -517,6 +517,56 @@ impl PagedAttentionKernels {
                                    src_layer_stride_bytes, dst_layer_stride_bytes, self.stream))
     }
 
+    /// Workspace bytes of `launch_v1_scores`.
+    pub fn v1_scores_workspace_bytes(
+        &self,
+        batch_size: i32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+    ) -> usize {
+        // SAFETY: pure size query.
+        unsafe {
+            ffi::rg_paged_attention_v1_scores_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim,
+                                                              block_size, max_blocks_per_seq)
+        }
+    }
+
+    /// `launch_v1_split` that also adds to `scores` (paged like the caches) the softmax weight every
+    /// cached token from position `first_scored` on gets from the kv-head's queries; cells from
+    /// `scored_lens[s]` on are overwritten (None: none are).
+    pub unsafe fn launch_v1_scores<T: KvElement>(
+        &self,
+        query: &HipSlice<T>,
+        key_cache: &HipSlice<T>,
+        value_cache: &HipSlice<T>,
+        block_table: &HipSlice<i32>,
+        context_lens: &HipSlice<i32>,
+        output: &mut HipSlice<T>,
+        scores: &mut HipSlice<f32>,
+        scored_lens: Option<&HipSlice<i32>>,
+        first_scored: i32,
+        scale: f32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        batch_size: i32,
+        score_block_stride: i64,
+        workspace: &mut HipSlice<u8>,
+    ) -> CoreResult<()> {
+        let scored = scored_lens.map_or(std::ptr::null(), |t| t.as_ptr() as *const i32);
+        status(ffi::rg_paged_attention_v1_scores(
+            query.as_ptr(), key_cache.as_ptr(), value_cache.as_ptr(), block_table.as_ptr() as *const i32,
+            context_lens.as_ptr() as *const i32, output.as_mut_ptr(), scores.as_mut_ptr() as *mut f32, scored,
+            first_scored, scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size,
+            T::DTYPE, self.kv_block_stride, score_block_stride, workspace.as_mut_ptr(), workspace.len(),
+            self.stream))
+    }
+
     /// Workspace bytes of `launch_evict`.
     pub fn evict_workspace_bytes(&self, num_layers: i32, batch_size: i32, num_kv_heads: i32, budget: i32) -> usize {
         // SAFETY: pure size query.

@@ -397,6 +397,33 @@ int rg_paged_attention_v1_plus(const void* query, const void* key_cache,
                                int32_t dtype, int64_t kv_block_stride,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* Decode attention that also gathers the attention weight of each cached token: the output of
+ * rg_paged_attention_v1 (up to fp32 rounding), and for every position t of sequence s with
+ * first_scored <= t < context_lens[s], in fp32,
+ *   scores[cell of t, kv-head] <- (t < scored_lens[s] ? scores[same] : 0) + w_t,
+ *   w_t = sum over the kv-head's query heads h of softmax_t(scale * q[s,h].K_t).
+ * scores is paged like the caches: [num_blocks, num_kv_heads, block_size], score_block_stride
+ * elements between blocks (0: dense).  scored_lens [batch] says how many of a sequence's leading
+ * cells hold a score already, so that the cells of new tokens need no clearing; NULL: all of them
+ * do; zeros: this step's weights alone are written.  Cells before first_scored (blocks that several
+ * sequences share) and from context_lens[s] on keep what they hold.  A block with scored positions
+ * belongs to one sequence of the call: two that share one would write the same cells in no set order.
+ * The workspace (rg_paged_attention_v1_scores_workspace_bytes, 16-byte aligned, needed, no clearing)
+ * holds one fp32 per (sequence, query head, token of the table) beside the split-K partials.
+ * num_heads / num_kv_heads at most 512.  New entry: what rg_evict_cache goes by. */
+size_t rg_paged_attention_v1_scores_workspace_bytes(int32_t batch_size, int32_t num_heads,
+                                                    int32_t num_kv_heads, int32_t head_dim,
+                                                    int32_t block_size, int32_t max_blocks_per_seq);
+int rg_paged_attention_v1_scores(const void* query, const void* key_cache,
+                                 const void* value_cache, const int32_t* block_table,
+                                 const int32_t* context_lens, void* output, float* scores,
+                                 const int32_t* scored_lens, int32_t first_scored, float scale,
+                                 int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t block_size, int32_t max_blocks_per_seq,
+                                 int32_t batch_size, int32_t dtype, int64_t kv_block_stride,
+                                 int64_t score_block_stride, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 /* Largest split-K scratch rg_paged_attention_v1_no_alloc can use: 16 MiB, a static
  * device array of the library that every device holds from the library's load until the
  * process ends.  The stream-K form needs (W + batch*num_kv_heads) * (G*head_dim + 2G) * 4

@@ -282,6 +282,25 @@ class PagedAttentionKernels {
                             num_tokens, max_query_len, (int32_t)dtype, kv_block_stride, stream_),
           "launch_prefill_packed");
   }
+  size_t v1_scores_workspace_bytes(int32_t batch_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                   int32_t block_size, int32_t max_blocks_per_seq) const {
+    return rg_paged_attention_v1_scores_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                                                        max_blocks_per_seq);
+  }
+  // launch_v1 that also adds to `scores` (paged like the caches) the softmax weight every cached token
+  // from position first_scored on gets; cells from scored_lens[s] on are overwritten (nullptr: none).
+  void launch_v1_scores(const void* query, const void* key_cache, const void* value_cache, const int32_t* block_table,
+                        const int32_t* context_lens, void* output, float* scores, const int32_t* scored_lens,
+                        int32_t first_scored, float scale, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t block_size, int32_t max_blocks_per_seq, int32_t batch_size, void* workspace,
+                        size_t workspace_bytes, DType dtype = DType::BF16, int64_t kv_block_stride = 0,
+                        int64_t score_block_stride = 0) const {
+    check(rg_paged_attention_v1_scores(query, key_cache, value_cache, block_table, context_lens, output, scores,
+                                       scored_lens, first_scored, scale, num_heads, num_kv_heads, head_dim, block_size,
+                                       max_blocks_per_seq, batch_size, (int32_t)dtype, kv_block_stride,
+                                       score_block_stride, workspace, workspace_bytes, stream_),
+          "launch_v1_scores");
+  }
   size_t evict_workspace_bytes(int32_t num_layers, int32_t batch_size, int32_t num_kv_heads, int32_t budget) const {
     return rg_evict_cache_workspace_bytes(num_layers, batch_size, num_kv_heads, budget);
   }

@@ -98,6 +98,11 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int32, c_int32, c_int32,
          c_int32, c_int32, c_int32, c_int32, c_int64, c_void_p, c_size_t, c_void_p],
     ),
+    "rg_paged_attention_v1_scores_workspace_bytes": (c_size_t, [c_int32] * 6),
+    "rg_paged_attention_v1_scores": (
+        c_int,
+        [c_void_p] * 8 + [c_int32, c_float] + [c_int32] * 7 + [c_int64, c_int64, c_void_p, c_size_t, c_void_p],
+    ),
     "rg_rope_reshape_and_cache_paged_attention_v1": (
         c_int,
         [c_void_p] * 11 + [c_float] + [c_int32] * 7 + [c_int64, c_void_p, c_size_t, c_void_p],

@@ -83,6 +83,12 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 constexpr int kBS = 16;  // tokens per KV block on the MFMA path
 
 
+// What a tile's step hands its raw scores to: nothing, or a function of them.
+struct NoSink {
+  template <typename C>
+  __device__ __forceinline__ void operator()(const C&) const {}
+};
+
 // Online-softmax update of one step of NB blocks, shared by the decode tiles.  c[b] holds the
 // raw scores of block b in the MFMA output layout (lane (col, seg): token col, heads 4*seg + r);
 // tokens at context index >= ctx are masked.  Updates the wave-uniform running max m_run and
@@ -340,9 +346,10 @@ struct DecodeTile {
   // [b*NV, (b+1)*NV)) whose first token has context index tok0; tokens >= ctx are masked.  One
   // running-max update, rescale decision and LDS exchange serve all NB * 16 tokens.
   // p_lds holds NB * 16 rows of GP probabilities.
-  template <int NB = 1>
+  // sink(c) sees the raw scores as they leave the MFMAs.
+  template <int NB = 1, typename Sink = NoSink>
   __device__ __forceinline__ void step(const uint4 (&kr)[NB * NK], const uint4 (&vr)[NB * NV], int tok0, int ctx,
-                                       float scale_log2, float* p_lds, float* alpha_lds) {
+                                       float scale_log2, float* p_lds, float* alpha_lds, Sink sink = {}) {
     f32x4_t c[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -350,6 +357,7 @@ struct DecodeTile {
 #pragma unroll
       for (int i = 0; i < NK; ++i) c[b] = MF::run(qa[i], kr[b * NK + i], c[b]);
     }
+    sink(c);
     const bool tail = tok0 + NB * kBS > ctx;
     const bool rescale = softmax_block<NB, GP, HG>(c, col, seg, tok0, ctx, scale_log2, m_run, l_run, p_lds, alpha_lds);
     if (rescale) {
@@ -472,9 +480,10 @@ struct DecodeTileF32 {
   __device__ __forceinline__ void load(const float* kb, const float* vb, uint4 (&kk)[NK], uint4 (&vv)[NV]) const {
     load_part<1, 0>(kb, vb, kk, vv);
   }
-  template <int NB = 1>
+  // sink(c) sees the raw scores as they leave the MFMAs.
+  template <int NB = 1, typename Sink = NoSink>
   __device__ __forceinline__ void step(const uint4 (&kr)[NB * NK], const uint4 (&vr)[NB * NV], int tok0, int ctx,
-                                       float scale_log2, float* p_lds, float* alpha_lds) {
+                                       float scale_log2, float* p_lds, float* alpha_lds, Sink sink = {}) {
     f32x4_t c[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -488,6 +497,7 @@ struct DecodeTileF32 {
           c[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(qa[4 * i + e], __uint_as_float(kw[e]), c[b], 0, 0, 0);
       }
     }
+    sink(c);
     const bool tail = tok0 + NB * kBS > ctx;
     const bool rescale = softmax_block<NB, GP, HG>(c, col, seg, tok0, ctx, scale_log2, m_run, l_run, p_lds, alpha_lds);
     if (rescale) {
@@ -606,6 +616,7 @@ constexpr int sk_prefetch_for() { return std::is_same_v<T, f32_t> ? (D <= 64 ? 2
 // What a stream-K worker does beside or in place of the plain decode.
 enum class StreamVariant {
   kDecode,
+  kScores,  // also leaves every raw score (q . k) in `logits`
 };
 
 struct StreamArgs {
@@ -630,6 +641,8 @@ struct StreamArgs {
   const float* cos_sin;         // [positions, D]: cos at [d], sin at [D/2 + d]
   const int32_t* positions;     // [batch]
   const int32_t* slot_mapping;  // [batch]; negative: a padding token, not cached
+  // kScores: [batch, H_kv, 16 max_blocks tokens, G].
+  float* logits;
 };
 
 // Cost of a segment start, in KB of K/V streaming.  A worker's end time tracks the segments it
@@ -1024,6 +1037,15 @@ __device__ __forceinline__ void stream_worker(
     }
   };
 
+  // kScores: where this lane's raw scores of the segment's first token go (token tile.col, heads 4 seg ..).
+  // Kept in vector registers: the scalar ones are all taken.
+  float* lg = nullptr;
+  float* lg_all = nullptr;
+  if constexpr (VAR == StreamVariant::kScores) {
+    lg_all = a.logits + tile.col * G + 4 * tile.seg;
+    asm volatile("" : "+v"(lg_all));
+    lg = lg_all + ((int64_t)cur.s * hkv + cur.kvh) * a.max_blocks * (kBS * G);
+  }
   const int64_t n = u1 - u0;
   Cursor ld = cur;
   int64_t ldi = 0;
@@ -1086,8 +1108,28 @@ __device__ __forceinline__ void stream_worker(
         if (tile.vrow == 0) *reinterpret_cast<uint4*>(vdst + tile.vd0) = vnew;
       }
     }
-    tile.template step<BPU>(kbuf[q], vbuf[q], cur.b * BPU * kBS, ctx_cur, a.scale_log2, p_lds[j & 1],
-                            alpha_lds[j & 1]);
+    if constexpr (VAR == StreamVariant::kScores) {
+      const int tok0 = cur.b * BPU * kBS;
+      tile.template step<BPU>(kbuf[q], vbuf[q], tok0, ctx_cur, a.scale_log2, p_lds[j & 1], alpha_lds[j & 1],
+                              [&](const f32x4_t (&c)[BPU]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < BPU; ++b) {
+          if (tile.seg < HG && tok0 + b * kBS + tile.col < ctx_cur) {
+            float* const at = lg + (int64_t)(tok0 + b * kBS) * G;
+            if constexpr (G % 4 == 0) {
+              *reinterpret_cast<float4*>(at) = make_float4(c[b][0], c[b][1], c[b][2], c[b][3]);
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (4 * tile.seg + r < G) at[r] = c[b][r];
+            }
+          }
+        }
+      });
+    } else {
+      tile.template step<BPU>(kbuf[q], vbuf[q], cur.b * BPU * kBS, ctx_cur, a.scale_log2, p_lds[j & 1],
+                              alpha_lds[j & 1]);
+    }
     const bool last_of_segment = cur.b + 1 == cur.nblk || j + 1 == n;
     if (last_of_segment) {
       end_segment(cur);
@@ -1095,6 +1137,9 @@ __device__ __forceinline__ void stream_worker(
         ++seg;
         advance(cur);
         begin_segment(cur, u0 + j + 1);
+        if constexpr (VAR == StreamVariant::kScores) {
+          lg = lg_all + ((int64_t)cur.s * hkv + cur.kvh) * a.max_blocks * (kBS * G);
+        }
         ctx_cur = min(context_lens[cur.s], a.max_blocks * kBS);
       }
     } else {
@@ -1155,6 +1200,21 @@ inline bool mfma_group_size(int G, int head_dim) {
 #ifndef RG_SK_WAVES_PER_CU
 #define RG_SK_WAVES_PER_CU 4
 #endif
+
+// log2(block_size / 16) for the block sizes that the tiles take (-1: another size).
+inline int32_t block_shift(int32_t block_size) {
+  for (int32_t j = 0; j <= 4; ++j)
+    if (block_size == (kBS << j)) return j;
+  return -1;
+}
+
+// Whether the tiles take the call: the MFMA shapes, rows on 16 bytes.  kv_stride: elements, not 0.
+inline bool tiles_take(const Shape& sh, int32_t dtype, int64_t kv_stride, const void* q, const void* kc,
+                       const void* vc, const void* out) {
+  return block_shift(sh.bs) >= 0 && (sh.D == 64 || sh.D == 128 || sh.D == 256) &&
+         mfma_group_size(sh.H / sh.Hkv, sh.D) && aligned16(q) && aligned16(kc) && aligned16(vc) &&
+         kv_stride * dtype_bytes(dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+}
 
 inline int32_t stream_workers(const Shape& sh) {
   const int64_t want = (int64_t)device_cu_count() * RG_SK_WAVES_PER_CU;

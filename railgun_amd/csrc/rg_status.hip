@@ -55,6 +55,7 @@ int probe_cache_kernels();
 int probe_decode_kernels();
 int probe_prefill_kernels();
 int probe_evict_kernels();
+int probe_scores_kernels();
 int setup_no_alloc_scratch();
 }  // namespace rg
 
@@ -87,6 +88,7 @@ extern "C" int rg_init(int device_ordinal) {
   if (st == RG_OK) st = rg::probe_decode_kernels();
   if (st == RG_OK) st = rg::probe_prefill_kernels();
   if (st == RG_OK) st = rg::probe_evict_kernels();
+  if (st == RG_OK) st = rg::probe_scores_kernels();
   if (st == RG_OK) st = rg::setup_no_alloc_scratch();
   (void)hipSetDevice(cur);
   if (st != RG_OK) return st;

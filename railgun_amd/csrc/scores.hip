@@ -1,0 +1,408 @@
+// Decode attention that also gathers, per cached token and kv-head, the softmax weight that the step's
+// queries gave it:
+//   out[s, h]  = sum_t p[h, t] V_t,  p[h, t] = e^(x[h, t] - M_h) / L_h,  x[h, t] = scale q[s, h] . K_t
+//   scores[t] <- (t < scored_lens[s] ? scores[t] : 0) + sum over the kv-head's G query heads of p[h, t].
+//
+// The weights need the row's maximum and sum, which stand only once every key has been seen, and a second
+// pass over K would cost half of the call's bytes again.  So the pass over K and V, the stream-K decode,
+// leaves each raw score q . k in the workspace (4 G bytes a token and kv-head beside the 4 D of K and V in
+// 16 bits: 6 % at G 4, head_dim 128, written and read once), and scores_finish_kernel merges the workers'
+// partials into the output and turns the raw scores into weights with the merged M and L.
+//
+// Shapes outside the tiles (another head_dim, block size or ratio of heads) take scores_generic_kernel, one
+// wave per (partition of kGenTokens tokens, query head, sequence), before the same finish.
+#include "decode_stream.hpp"
+
+namespace rg {
+namespace {
+
+constexpr int kGenTokens = 256;
+constexpr int kFinThreads = 256;
+constexpr int kFinWaves = kFinThreads / 64;
+constexpr int kFinTokens = 1024;   // tokens a workgroup turns into weights at a time
+constexpr int kMaxGroup = 512;     // query heads to a kv-head
+
+struct ScoreArgs {
+  void* out;
+  float* scores;
+  const float* logits;        // [batch, H_kv, tokens, G] raw scores
+  const float* part_acc;      // partials as the stream-K workers leave them
+  const float* part_ml;
+  const int2* seg_desc;       // null: partial p of segment g is g * num_partitions + p
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  const int32_t* scored_lens;  // may be null: every cell holds a score
+  float scale_log2;
+  int32_t first;
+  int32_t num_heads, num_kv_heads, head_dim, block_size, max_blocks, num_partitions;
+  int64_t score_stride;
+};
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(64) void scores_stream_kernel(StreamArgs a, const typename DecodeTileFor<T, D, G>::S* __restrict__ q,
+                                                           const typename DecodeTileFor<T, D, G>::S* __restrict__ kc,
+                                                           const typename DecodeTileFor<T, D, G>::S* __restrict__ vc,
+                                                           const int32_t* __restrict__ block_table,
+                                                           const int32_t* __restrict__ context_lens) {
+  stream_worker<T, D, G, false, StreamVariant::kScores>(a, q, kc, vc, block_table, context_lens, nullptr, nullptr);
+}
+
+struct GenericArgs {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  float* logits;
+  float* part_acc;
+  float* part_ml;
+  float scale_log2;
+  int32_t first;
+  int32_t num_heads, num_kv_heads, head_dim, block_size, max_blocks, num_partitions;
+  int64_t kv_stride;
+};
+
+template <typename T>
+__global__ __launch_bounds__(64) void scores_generic_kernel(GenericArgs a) {
+  using E = elem<T>;
+  using S = typename E::storage;
+  const int p = blockIdx.x, h = blockIdx.y, s = blockIdx.z, lane = threadIdx.x;
+  const int64_t tokens = (int64_t)a.max_blocks * a.block_size;
+  const int ctx = (int)max<int64_t>(0, min<int64_t>(a.context_lens[s], tokens));
+  const int t0 = p * kGenTokens, t1 = min(ctx, t0 + kGenTokens);
+  if (t0 >= t1) return;
+  const int D = a.head_dim, G = a.num_heads / a.num_kv_heads;
+  const int kvh = h / G, g = h - kvh * G;
+  const int d0 = lane * 4;
+  const bool act = d0 < D;
+  const S* qp = static_cast<const S*>(a.q) + ((int64_t)s * a.num_heads + h) * D;
+  const S* kc = static_cast<const S*>(a.k_cache);
+  const S* vc = static_cast<const S*>(a.v_cache);
+  const int32_t* bt = a.block_table + (int64_t)s * a.max_blocks;
+  const int64_t seg = (int64_t)s * a.num_kv_heads + kvh;
+  float qv[4] = {0.f, 0.f, 0.f, 0.f};
+  if (act) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) qv[u] = E::load(qp, d0 + u);
+  }
+  float m = -INFINITY, l = 0.f;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int t = t0; t < t1; ++t) {
+    const int64_t row = bt[t / a.block_size] * a.kv_stride + ((int64_t)kvh * a.block_size + t % a.block_size) * D;
+    float kv[4] = {0.f, 0.f, 0.f, 0.f}, vv[4] = {0.f, 0.f, 0.f, 0.f};
+    if (act) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        kv[u] = E::load(kc, row + d0 + u);
+        vv[u] = E::load(vc, row + d0 + u);
+      }
+    }
+    const float raw = wave_sum(qv[0] * kv[0] + qv[1] * kv[1] + qv[2] * kv[2] + qv[3] * kv[3]);
+    if (lane == 0 && t >= a.first) a.logits[(seg * tokens + t) * G + g] = raw;
+    const float x = raw * a.scale_log2;
+    const float m_new = fmaxf(m, x);
+    const float alpha = exp2f(m - m_new), pe = exp2f(x - m_new);
+    l = l * alpha + pe;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) o[u] = o[u] * alpha + pe * vv[u];
+    m = m_new;
+  }
+  const int64_t part = seg * a.num_partitions + p;
+  if (act) {
+    float* dst = a.part_acc + (part * G + g) * D + d0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) dst[u] = o[u];
+  }
+  if (lane == 0) {
+    a.part_ml[(part * G + g) * 2] = m;
+    a.part_ml[(part * G + g) * 2 + 1] = l;
+  }
+}
+
+// Workgroup (x, kv-head, sequence): x == 0 merges the segment's partials into its G output rows, the others
+// turn raw scores into weights, kFinTokens tokens at a time.  Each works out M and L of its G rows from the
+// partials' pairs itself (a few loads), so one launch does both.  GT: G, or 0 for one known at run time.
+template <typename T, int GT>
+__global__ __launch_bounds__(kFinThreads) void scores_finish_kernel(ScoreArgs a) {
+  using E = elem<T>;
+  using S = typename E::storage;
+  constexpr int GL = GT > 0 ? GT : kMaxGroup;
+  __shared__ float top[GL], inv[GL];
+  const int kvh = blockIdx.y, s = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int G = GT > 0 ? GT : a.num_heads / a.num_kv_heads;
+  const int D = a.head_dim;
+  const int64_t tokens = (int64_t)a.max_blocks * a.block_size;
+  const int64_t seg = (int64_t)s * a.num_kv_heads + kvh;
+  const int ctx = (int)max<int64_t>(0, min<int64_t>(a.context_lens[s], tokens));
+  S* out = static_cast<S*>(a.out) + ((int64_t)s * a.num_heads + (int64_t)kvh * G) * D;
+  if (ctx == 0) {
+    if (blockIdx.x == 0)
+      for (int i = tid; i < G * D; i += kFinThreads) E::store(out, i, 0.f);
+    return;
+  }
+  const int first = max(a.first, 0) + ((int)blockIdx.x - 1) * kFinTokens;
+  if (blockIdx.x > 0 && first >= ctx) return;
+  int64_t pbase;
+  int np;
+  if (a.seg_desc != nullptr) {
+    const int2 d = a.seg_desc[seg];
+    pbase = d.x + seg;
+    np = d.y;
+  } else {
+    pbase = seg * a.num_partitions;
+    np = (ctx + kGenTokens - 1) / kGenTokens;
+  }
+  const float* ml = a.part_ml + pbase * 2 * G;
+  for (int h = w; h < G; h += kFinWaves) {
+    float m = -INFINITY, l = 0.f;
+    for (int q = lane; q < np; q += 64) m = fmaxf(m, ml[((int64_t)q * G + h) * 2]);
+    m = wave_max(m);
+    for (int q = lane; q < np; q += 64) l += ml[((int64_t)q * G + h) * 2 + 1] * exp2f(ml[((int64_t)q * G + h) * 2] - m);
+    l = wave_sum(l);
+    if (lane == 0) {
+      top[h] = m;
+      inv[h] = l != 0.f ? 1.f / l : 1.f;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    const float* acc = a.part_acc + pbase * G * D;
+    for (int i = tid; i < G * D; i += kFinThreads) {
+      const int h = i / D;
+      const float m = top[h];
+      float o = 0.f;
+#pragma unroll 4
+      for (int q = 0; q < np; ++q) o += acc[(int64_t)q * G * D + i] * exp2f(ml[((int64_t)q * G + h) * 2] - m);
+      E::store(out, i, o * inv[h]);
+    }
+    return;
+  }
+  const int scored = a.scored_lens != nullptr ? a.scored_lens[s] : INT32_MAX;
+  const int32_t* bt = a.block_table + (int64_t)s * a.max_blocks;
+  const float* lg = a.logits + seg * tokens * G;
+  const int64_t step = (int64_t)(gridDim.x - 1) * kFinTokens;
+  for (int64_t c0 = first; c0 < ctx; c0 += step) {
+#pragma unroll 4
+    for (int u = 0; u < kFinTokens / kFinThreads; ++u) {
+      const int64_t t = c0 + u * kFinThreads + tid;
+      if (t >= ctx) break;
+      float sum = 0.f;
+      if constexpr (GT > 0 && GT % 4 == 0) {
+#pragma unroll
+        for (int h = 0; h < GT; h += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(lg + t * GT + h);
+          sum += exp2f(x.x * a.scale_log2 - top[h]) * inv[h];
+          sum += exp2f(x.y * a.scale_log2 - top[h + 1]) * inv[h + 1];
+          sum += exp2f(x.z * a.scale_log2 - top[h + 2]) * inv[h + 2];
+          sum += exp2f(x.w * a.scale_log2 - top[h + 3]) * inv[h + 3];
+        }
+      } else {
+        for (int h = 0; h < G; ++h) sum += exp2f(lg[t * G + h] * a.scale_log2 - top[h]) * inv[h];
+      }
+      const int b = (int)t / a.block_size;
+      float* cell = a.scores + bt[b] * a.score_stride + (int64_t)kvh * a.block_size + ((int)t - b * a.block_size);
+      *cell = t < scored ? *cell + sum : sum;
+    }
+  }
+}
+
+template <typename T, int D>
+void launch_scores_stream(const StreamArgs& sa, int G, const void* q, const void* kc, const void* vc, const int32_t* bt,
+                          const int32_t* cl, hipStream_t s) {
+  auto go = [&](auto g) {
+    constexpr int GC = decltype(g)::value;
+    using S = typename DecodeTileFor<T, D, GC>::S;
+    hipLaunchKernelGGL((scores_stream_kernel<T, D, GC>), dim3(sa.num_workers), dim3(64), 0, s, sa,
+                       static_cast<const S*>(q), static_cast<const S*>(kc), static_cast<const S*>(vc), bt, cl);
+  };
+  switch (G) {
+    case 1: go(std::integral_constant<int, 1>{}); break;
+    case 2: go(std::integral_constant<int, 2>{}); break;
+    case 4: go(std::integral_constant<int, 4>{}); break;
+    case 8: go(std::integral_constant<int, 8>{}); break;
+    case 16: go(std::integral_constant<int, 16>{}); break;
+    default:
+      // G 3, 5, 6, 7 (mfma_group_size admits them at head_dim 64 and 128 only)
+      if constexpr (D <= 128) {
+        if (G == 3) go(std::integral_constant<int, 3>{});
+        else if (G == 5) go(std::integral_constant<int, 5>{});
+        else if (G == 6) go(std::integral_constant<int, 6>{});
+        else if (G == 7) go(std::integral_constant<int, 7>{});
+      }
+      break;
+  }
+}
+
+template <typename T>
+void launch_finish(const ScoreArgs& a, int G, dim3 grid, hipStream_t s) {
+  auto go = [&](auto g) {
+    hipLaunchKernelGGL((scores_finish_kernel<T, decltype(g)::value>), grid, dim3(kFinThreads), 0, s, a);
+  };
+  switch (G) {
+    case 1: go(std::integral_constant<int, 1>{}); break;
+    case 2: go(std::integral_constant<int, 2>{}); break;
+    case 4: go(std::integral_constant<int, 4>{}); break;
+    case 7: go(std::integral_constant<int, 7>{}); break;
+    case 8: go(std::integral_constant<int, 8>{}); break;
+    default: go(std::integral_constant<int, 0>{}); break;
+  }
+}
+
+int32_t generic_partitions(const Shape& sh) {
+  return (int32_t)std::max<int64_t>(1, ceil_div((int64_t)sh.MB * sh.bs, kGenTokens));
+}
+
+struct ScoreScratch {
+  float* logits;
+  void* rest;  // stream-K scratch, or the generic kernel's partials
+};
+
+size_t logit_bytes(const Shape& sh) { return align_up((size_t)sh.B * sh.H * sh.MB * sh.bs * 4, 256); }
+size_t generic_acc_bytes(const Shape& sh) {
+  return align_up((size_t)sh.B * sh.H * generic_partitions(sh) * sh.D * 4, 256);
+}
+size_t generic_bytes(const Shape& sh) {
+  return generic_acc_bytes(sh) + align_up((size_t)sh.B * sh.H * generic_partitions(sh) * 8, 256);
+}
+
+}  // namespace
+
+int probe_scores_kernels() {
+  hipFuncAttributes at;
+  if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(scores_stream_kernel<bf16_t, 128, 4>)) != hipSuccess ||
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(scores_finish_kernel<bf16_t, 4>)) != hipSuccess) {
+    return fail(RG_ERR_HIP, "failed to load the scoring decode kernels: %s", hipGetErrorString(hipGetLastError()));
+  }
+  return RG_OK;
+}
+
+}  // namespace rg
+
+using namespace rg;
+
+extern "C" size_t rg_paged_attention_v1_scores_workspace_bytes(int32_t batch_size, int32_t num_heads,
+                                                               int32_t num_kv_heads, int32_t head_dim,
+                                                               int32_t block_size, int32_t max_blocks_per_seq) {
+  if (batch_size <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
+      block_size <= 0 || max_blocks_per_seq <= 0) {
+    return 0;
+  }
+  const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  return logit_bytes(sh) + std::max(generic_bytes(sh), stream_bytes(sh, stream_workers(sh), nullptr, nullptr));
+}
+
+extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_cache, const void* value_cache,
+                                            const int32_t* block_table, const int32_t* context_lens, void* output,
+                                            float* scores, const int32_t* scored_lens, int32_t first_scored,
+                                            float scale, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                            int32_t block_size, int32_t max_blocks_per_seq, int32_t batch_size,
+                                            int32_t dtype, int64_t kv_block_stride, int64_t score_block_stride,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "paged_attention_v1_scores";
+  const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  int st = check_decode_shape(op, sh, dtype, kv_block_stride);
+  if (st != RG_OK) return st;
+  const int64_t block = (int64_t)num_kv_heads * block_size;
+  const int G = num_heads / num_kv_heads;
+  if (G > kMaxGroup) {
+    return fail(RG_ERR_NOT_SUPPORTED, "%s: at most %d query heads to a kv-head, got %d", op, kMaxGroup, G);
+  }
+  if (first_scored < 0) return fail(RG_ERR_INVALID_ARGUMENT, "%s: first_scored %d < 0", op, first_scored);
+  if (score_block_stride != 0 && score_block_stride < block) {
+    return fail(RG_ERR_INVALID_ARGUMENT, "%s: score_block_stride %lld smaller than a block", op,
+                (long long)score_block_stride);
+  }
+  const int64_t tokens = (int64_t)max_blocks_per_seq * block_size;
+  if (tokens > INT32_MAX || batch_size > 65535 || num_heads > 65535) {
+    return fail(RG_ERR_NOT_SUPPORTED, "%s: a block table of %lld tokens, %d sequences, %d heads", op,
+                (long long)tokens, batch_size, num_heads);
+  }
+  if (batch_size == 0) return ok();
+  if (!query || !key_cache || !value_cache || !block_table || !context_lens || !output || !scores) {
+    return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
+  }
+  const int64_t kv_stride = kv_block_stride ? kv_block_stride : block * head_dim;
+  const bool tiles = max_blocks_per_seq > 0 && tiles_take(sh, dtype, kv_stride, query, key_cache, value_cache, output);
+  const int32_t workers = stream_workers(sh);
+  const size_t logits = logit_bytes(sh);
+  const size_t need = logits + (tiles ? stream_bytes(sh, workers, nullptr, nullptr) : generic_bytes(sh));
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) {
+    return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned), %zu required", op,
+                workspace ? workspace_bytes : (size_t)0, need);
+  }
+  char* const ws = static_cast<char*>(workspace);
+  hipStream_t s = as_stream(stream);
+  ScoreArgs f{};
+  f.out = output;
+  f.scores = scores;
+  f.logits = reinterpret_cast<float*>(ws);
+  f.block_table = block_table;
+  f.context_lens = context_lens;
+  f.scored_lens = scored_lens;
+  f.scale_log2 = scale * kLog2e;
+  f.first = first_scored;
+  f.num_heads = num_heads;
+  f.num_kv_heads = num_kv_heads;
+  f.head_dim = head_dim;
+  f.block_size = block_size;
+  f.max_blocks = max_blocks_per_seq;
+  f.num_partitions = generic_partitions(sh);
+  f.score_stride = score_block_stride ? score_block_stride : block;
+  if (tiles) {
+    StreamScratch sc;
+    stream_bytes(sh, workers, &sc, ws + logits);
+    StreamArgs sa{};
+    sa.part_acc = sc.acc;
+    sa.part_ml = sc.ml;
+    sa.seg_desc = sc.desc;
+    sa.scale_log2 = f.scale_log2;
+    sa.num_heads = num_heads;
+    sa.num_kv_heads = num_kv_heads;
+    sa.bs_shift = block_shift(block_size);
+    sa.max_blocks = max_blocks_per_seq << sa.bs_shift;
+    sa.batch = batch_size;
+    sa.num_workers = workers;
+    sa.kv_stride = kv_stride;
+    sa.table_stride = max_blocks_per_seq;
+    sa.logits = reinterpret_cast<float*>(ws);
+    f.part_acc = sc.acc;
+    f.part_ml = sc.ml;
+    f.seg_desc = sc.desc;
+    auto go = [&](auto tag) {
+      using T = decltype(tag);
+      if (head_dim == 256) launch_scores_stream<T, 256>(sa, G, query, key_cache, value_cache, block_table, context_lens, s);
+      else if (head_dim == 128) launch_scores_stream<T, 128>(sa, G, query, key_cache, value_cache, block_table, context_lens, s);
+      else launch_scores_stream<T, 64>(sa, G, query, key_cache, value_cache, block_table, context_lens, s);
+      return check_launch(op);
+    };
+    st = dispatch_dtype(dtype, go);
+    if (st != RG_OK) return st;
+  } else {
+    float* const acc = reinterpret_cast<float*>(ws + logits);
+    float* const ml = reinterpret_cast<float*>(ws + logits + generic_acc_bytes(sh));
+    f.part_acc = acc;
+    f.part_ml = ml;
+    if (max_blocks_per_seq > 0) {
+      GenericArgs ga{query, key_cache, value_cache, block_table, context_lens, reinterpret_cast<float*>(ws), acc, ml,
+                     f.scale_log2, first_scored, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                     f.num_partitions, kv_stride};
+      st = dispatch_dtype(dtype, [&](auto tag) {
+        hipLaunchKernelGGL(scores_generic_kernel<decltype(tag)>, dim3(f.num_partitions, num_heads, batch_size),
+                           dim3(64), 0, s, ga);
+        return check_launch(op);
+      });
+      if (st != RG_OK) return st;
+    }
+  }
+  // One workgroup per segment for the output, and for the weights up to one per kFinTokens of the table but
+  // no more than some 8192 in all (they step on where the table is longer).
+  const int64_t segments = (int64_t)batch_size * num_kv_heads;
+  const int64_t scored = std::max<int64_t>(0, tokens - first_scored);
+  const int64_t chunks = std::min(ceil_div(scored, kFinTokens), std::max<int64_t>(1, 8192 / segments));
+  const dim3 grid((unsigned)(1 + chunks), (unsigned)num_kv_heads, (unsigned)batch_size);
+  return dispatch_dtype(dtype, [&](auto tag) {
+    launch_finish<decltype(tag)>(f, G, grid, s);
+    return check_launch(op);
+  });
+}

@@ -83,6 +83,15 @@ def cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, i
     return hkv, bs, d, k_stride[0]
 
 
+def check_scores(scores: torch.Tensor, cache: torch.Tensor) -> None:
+    """scores: fp32, of the shape of ``cache`` ([..., NB, H_kv, bs, D]) without D, its blocks contiguous."""
+    if scores.dtype != torch.float32 or scores.shape != cache.shape[:-1] or \
+            scores.stride()[-2:] != (int(cache.shape[-2]), 1):
+        raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                           f"scores must be float32 {tuple(cache.shape[:-1])} with contiguous blocks, got "
+                           f"{scores.dtype} {tuple(scores.shape)}")
+
+
 def rope_cos_sin_table(max_position: int, head_dim: int, theta: float,
                        device: Optional[torch.device] = None) -> torch.Tensor:
     """fp32 [max_position, head_dim] table: cos in [:, :D/2], sin in [:, D/2:] (HF Llama)."""
@@ -201,6 +210,34 @@ class PagedAttentionKernels:
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
             context_lens.data_ptr(), output.data_ptr(), float(scale), num_heads, num_kv_heads, head_dim,
             block_size, max_blocks_per_seq, batch_size, dtype_code(query), key_cache.stride(0), _stream(query)))
+
+    def v1_scores_workspace_bytes(self, batch_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                  block_size: int, max_blocks_per_seq: int) -> int:
+        return int(self.lib.rg_paged_attention_v1_scores_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim,
+                                                                         block_size, max_blocks_per_seq))
+
+    def launch_v1_scores(self, query, key_cache, value_cache, block_table, context_lens, output, scores,
+                         scored_lens, first_scored: int, scale: float, num_heads: int, num_kv_heads: int,
+                         head_dim: int, block_size: int, max_blocks_per_seq: int, batch_size: int,
+                         workspace: torch.Tensor) -> None:
+        """launch_v1 that also adds to ``scores`` (fp32 [NB, H_kv, bs], paged like the caches) the softmax
+        weight every cached token from position ``first_scored`` on gets from the kv-head's queries
+        (rg_paged_attention_v1_scores).  ``scored_lens`` [batch]: how many of a sequence's leading cells
+        hold a score to add to, the others are overwritten; None: all.  A block with scored positions
+        belongs to one sequence of the call."""
+        _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens, workspace)
+        _require_i32(block_table, context_lens)
+        if scored_lens is not None:
+            _require_i32(scored_lens)
+            if int(scored_lens.numel()) < batch_size:
+                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "scored_lens needs one entry per sequence")
+        check_scores(scores, key_cache)
+        check(self.lib.rg_paged_attention_v1_scores(
+            query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+            context_lens.data_ptr(), output.data_ptr(), scores.data_ptr(), _ptr(scored_lens), first_scored,
+            float(scale), num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size,
+            dtype_code(query), key_cache.stride(0), scores.stride(0), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream(query)))
 
     # mod.rs:350-399
     def launch_v1_plus(self, query, key_cache, value_cache, block_table, context_lens, output,
@@ -395,8 +432,7 @@ class PagedAttentionKernels:
         nb, hkv, bs, d = (int(x) for x in key_cache.shape[-4:])
         if key_cache.stride()[-3:] != (bs * d, d, 1):
             raise bad("cache blocks must be contiguous [H_kv, bs, D]")
-        if scores.dtype != torch.float32 or scores.shape != key_cache.shape[:-1] or scores.stride()[-2:] != (bs, 1):
-            raise bad("scores must be float32 of the caches' shape without head_dim, its blocks contiguous")
+        check_scores(scores, key_cache)
         batch = int(context_lens.numel())
         if block_table.dim() != 2 or int(block_table.shape[0]) != batch:
             raise bad("block_table must be [batch, max_blocks]")
@@ -477,6 +513,41 @@ class PagedAttentionOp:
             k.launch_v2(q, k_cache, v_cache, block_table, context_lens, out, self.scale, num_heads,
                         self.num_kv_heads, head_dim, block_size, max_blocks, batch, max_context_len,
                         V2_PARTITION_SIZE, ws)
+        return out
+
+    def _check_decode(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      block_table: torch.Tensor, context_lens: torch.Tensor) -> tuple:
+        """(batch, heads, head_dim, block_size, max_blocks) of one decode call, checked against the op."""
+        if q.dim() != 3 or not q.is_contiguous():
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               f"q must be contiguous [batch, heads, head_dim], got {tuple(q.shape)}")
+        _require_cuda(q, k_cache, v_cache, block_table, context_lens)
+        batch, heads, d = (int(x) for x in q.shape)
+        hkv, bs, cache_d, _ = cache_geometry(k_cache, v_cache)
+        if (hkv, heads, d, cache_d, bs) != (self.num_kv_heads, self.num_heads, self.head_dim, self.head_dim,
+                                            self.block_size) or q.dtype != k_cache.dtype:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               f"q {tuple(q.shape)} {q.dtype} and caches {tuple(k_cache.shape)} {k_cache.dtype} do not "
+                               f"fit the op's {self.num_heads} / {self.num_kv_heads} heads of {self.head_dim}, blocks of "
+                               f"{self.block_size}")
+        if block_table.dim() != 2 or int(block_table.shape[0]) != batch or int(context_lens.numel()) != batch:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "block_table and context_lens need one row per sequence")
+        return batch, heads, d, bs, int(block_table.shape[1])
+
+    def execute_with_scores(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            block_table: torch.Tensor, context_lens: torch.Tensor, scores: torch.Tensor,
+                            scored_lens: Optional[torch.Tensor] = None, first_scored: int = 0,
+                            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """execute() that also gathers every cached token's attention weight in ``scores``
+        (launch_v1_scores); the workspace is allocated here when omitted."""
+        batch, heads, d, bs, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
+        out = torch.empty_like(q)
+        k = self.kernels
+        if workspace is None:
+            workspace = torch.empty(k.v1_scores_workspace_bytes(batch, heads, self.num_kv_heads, d, bs, mb),
+                                    dtype=torch.uint8, device=q.device)
+        k.launch_v1_scores(q, k_cache, v_cache, block_table, context_lens, out, scores, scored_lens, first_scored,
+                           self.scale, heads, self.num_kv_heads, d, bs, mb, batch, workspace)
         return out
 
     def reshape_and_cache(self, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -674,6 +745,6 @@ def linear_residual(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tenso
 
 
 __all__ = ["LINEAR_MAX_ROWS", "PagedAttentionKernels", "PagedAttentionOp", "RailgunError", "cache_geometry",
-           "deinterleave_gate_up", "dtype_code", "interleave_gate_up", "linear", "linear_residual",
+           "check_scores", "deinterleave_gate_up", "dtype_code", "interleave_gate_up", "linear", "linear_residual",
            "linear_silu_mul", "linear_workspace_bytes", "rms_norm", "rope_cos_sin_table", "silu_and_mul",
            "silu_and_mul_interleaved", "V1_MAX_CONTEXT", "V2_PARTITION_SIZE"]

@@ -66,3 +66,44 @@ def test_evict_workspace_bytes():
     f = railgun_amd.load_library().rg_evict_cache_workspace_bytes
     assert f(2, 3, 8, 64) == 256 + 48 * 64 * 4
     assert f(0, 3, 8, 64) == f(2, 0, 8, 64) == f(2, 3, 8, 0) == f(2**20, 2**20, 1, 1) == 0
+
+
+def scores(**change):
+    a = dict(q=P, k=P, v=P, table=P, lens=P, out=P, scores=P, scored=P, first=0, scale=0.125, heads=8, kv_heads=2, d=64,
+             bs=16, mb=4, batch=3, dtype=_lib.RG_DTYPE_BF16, kv_stride=0, score_stride=0, ws=P, ws_bytes=1 << 30,
+             stream=None)
+    assert set(change) <= set(a)
+    return call("rg_paged_attention_v1_scores", *{**a, **change}.values())
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=9), UNSUPPORTED, "unknown dtype"),
+    (dict(d=66), UNSUPPORTED, "multiple of 4"),
+    (dict(d=260), UNSUPPORTED, "multiple of 4"),
+    (dict(heads=7), INVALID, "not a multiple"),
+    (dict(kv_heads=0), INVALID, "positive heads"),
+    (dict(batch=-1), INVALID, "batch"),
+    (dict(mb=-1), INVALID, "max_blocks"),
+    (dict(heads=1026), UNSUPPORTED, "query heads to a kv-head"),
+    (dict(first=-1), INVALID, "first_scored"),
+    (dict(kv_stride=2 * 16 * 64 - 1), INVALID, "kv_block_stride"),
+    (dict(score_stride=31), INVALID, "score_block_stride"),
+    (dict(mb=2**31 - 1), UNSUPPORTED, "block table of"),
+    (dict(batch=65536), UNSUPPORTED, "sequences"),
+    (dict(q=None), INVALID, "null pointer"),
+    (dict(scores=None), INVALID, "null pointer"),
+    (dict(lens=None), INVALID, "null pointer"),
+    (dict(ws=None), WORKSPACE, "required"),
+    (dict(ws_bytes=1000), WORKSPACE, "required"),
+    (dict(ws=P // 16 * 16 + 4), WORKSPACE, "aligned"),
+    (dict(batch=0), _lib.RG_OK, ""),
+])
+def test_scores_arguments(change, code, text):
+    st, msg = scores(**change)
+    assert st == code and text in msg, msg
+
+
+def test_scores_workspace_bytes():
+    f = railgun_amd.load_library().rg_paged_attention_v1_scores_workspace_bytes
+    assert f(3, 8, 2, 64, 16, 4) > 3 * 8 * 64 * 4 and f(3, 8, 2, 64, 16, 4) % 256 == 0
+    assert f(0, 8, 2, 64, 16, 4) == f(3, 7, 2, 64, 16, 4) == f(3, 8, 2, 64, 16, 0) == 0
