@@ -77,6 +77,18 @@ extern "C" {
         block_bytes: i64, src_block_stride_bytes: i64, dst_block_stride_bytes: i64, num_layers: i32,
         src_layer_stride_bytes: i64, dst_layer_stride_bytes: i64, stream: *mut c_void,
     ) -> c_int;
+    /// New: workspace bytes of rg_paged_attention_shared_prefix.
+    pub fn rg_paged_attention_shared_prefix_workspace_bytes(
+        batch_size: i32, num_heads: i32, num_kv_heads: i32, head_dim: i32, block_size: i32,
+        max_blocks_per_seq: i32, shared_blocks: i32,
+    ) -> usize;
+    /// New: rg_paged_attention_v1 for sequences that begin with the same cached blocks.
+    pub fn rg_paged_attention_shared_prefix(
+        query: *const c_void, key_cache: *const c_void, value_cache: *const c_void, block_table: *const i32,
+        context_lens: *const i32, output: *mut c_void, scale: f32, num_heads: i32, num_kv_heads: i32,
+        head_dim: i32, block_size: i32, max_blocks_per_seq: i32, batch_size: i32, shared_blocks: i32, dtype: i32,
+        kv_block_stride: i64, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> c_int;
     /// New: workspace bytes of rg_paged_attention_v1_scores.
     pub fn rg_paged_attention_v1_scores_workspace_bytes(
         batch_size: i32, num_heads: i32, num_kv_heads: i32, head_dim: i32, block_size: i32,

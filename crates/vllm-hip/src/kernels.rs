@@ -517,6 +517,51 @@ impl PagedAttentionKernels {
                                    src_layer_stride_bytes, dst_layer_stride_bytes, self.stream))
     }
 
+    /// Workspace bytes of `launch_shared_prefix`.
+    pub fn shared_prefix_workspace_bytes(
+        &self,
+        batch_size: i32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        shared_blocks: i32,
+    ) -> usize {
+        // SAFETY: pure size query.
+        unsafe {
+            ffi::rg_paged_attention_shared_prefix_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim,
+                                                                  block_size, max_blocks_per_seq, shared_blocks)
+        }
+    }
+
+    /// `launch_v1_split` for sequences whose block tables begin with the same `shared_blocks`
+    /// entries: those blocks are read once for many rows.
+    pub unsafe fn launch_shared_prefix<T: KvElement>(
+        &self,
+        query: &HipSlice<T>,
+        key_cache: &HipSlice<T>,
+        value_cache: &HipSlice<T>,
+        block_table: &HipSlice<i32>,
+        context_lens: &HipSlice<i32>,
+        output: &mut HipSlice<T>,
+        scale: f32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        batch_size: i32,
+        shared_blocks: i32,
+        workspace: &mut HipSlice<u8>,
+    ) -> CoreResult<()> {
+        status(ffi::rg_paged_attention_shared_prefix(
+            query.as_ptr(), key_cache.as_ptr(), value_cache.as_ptr(), block_table.as_ptr() as *const i32,
+            context_lens.as_ptr() as *const i32, output.as_mut_ptr(), scale, num_heads, num_kv_heads, head_dim,
+            block_size, max_blocks_per_seq, batch_size, shared_blocks, T::DTYPE, self.kv_block_stride,
+            workspace.as_mut_ptr(), workspace.len(), self.stream))
+    }
+
     /// Workspace bytes of `launch_v1_scores`.
     pub fn v1_scores_workspace_bytes(
         &self,

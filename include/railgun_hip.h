@@ -397,6 +397,33 @@ int rg_paged_attention_v1_plus(const void* query, const void* key_cache,
                                int32_t dtype, int64_t kv_block_stride,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* rg_paged_attention_v1 for a batch whose sequences begin with the same cached blocks (a system
+ * prompt, a document that many rows ask about): the first shared_blocks entries of every row of
+ * block_table name the same blocks (those of any one row are read).  The same output up to
+ * rounding, with the shared blocks read once for many rows instead of once per sequence, as
+ * one product on the matrix cores (in bf16 / f16 with the probabilities of the shared tokens
+ * rounded to that type, as in rg_prefill_packed).  Sequences may be shorter than the prefix or
+ * empty (context_lens[s] == 0 gives zeros); shared_blocks == 0 is rg_paged_attention_v1.  Any shape
+ * of rg_paged_attention_v1; the shared product runs for more than one sequence with a block_size
+ * of 16 * 2^j up to 256 and head_dim 64 or 128, num_heads / num_kv_heads 1 to 8 or 16, the other
+ * shapes read the prefix per sequence.  Needs a workspace of
+ * rg_paged_attention_shared_prefix_workspace_bytes (16-byte aligned, no clearing).  New entry: the
+ * reference shares blocks between sequences (crates/vllm-paged-attention/src/allocator.rs) but
+ * attends to them per sequence. */
+size_t rg_paged_attention_shared_prefix_workspace_bytes(int32_t batch_size, int32_t num_heads,
+                                                        int32_t num_kv_heads, int32_t head_dim,
+                                                        int32_t block_size,
+                                                        int32_t max_blocks_per_seq,
+                                                        int32_t shared_blocks);
+int rg_paged_attention_shared_prefix(const void* query, const void* key_cache,
+                                     const void* value_cache, const int32_t* block_table,
+                                     const int32_t* context_lens, void* output, float scale,
+                                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t block_size, int32_t max_blocks_per_seq,
+                                     int32_t batch_size, int32_t shared_blocks, int32_t dtype,
+                                     int64_t kv_block_stride, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 /* Decode attention that also gathers the attention weight of each cached token: the output of
  * rg_paged_attention_v1 (up to fp32 rounding), and for every position t of sequence s with
  * first_scored <= t < context_lens[s], in fp32,

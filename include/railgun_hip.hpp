@@ -282,6 +282,24 @@ class PagedAttentionKernels {
                             num_tokens, max_query_len, (int32_t)dtype, kv_block_stride, stream_),
           "launch_prefill_packed");
   }
+  size_t shared_prefix_workspace_bytes(int32_t batch_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                       int32_t block_size, int32_t max_blocks_per_seq, int32_t shared_blocks) const {
+    return rg_paged_attention_shared_prefix_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                                                            max_blocks_per_seq, shared_blocks);
+  }
+  // launch_v1 for sequences whose block tables begin with the same shared_blocks entries: those blocks
+  // are read once for many rows.
+  void launch_shared_prefix(const void* query, const void* key_cache, const void* value_cache,
+                            const int32_t* block_table, const int32_t* context_lens, void* output, float scale,
+                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                            int32_t max_blocks_per_seq, int32_t batch_size, int32_t shared_blocks, void* workspace,
+                            size_t workspace_bytes, DType dtype = DType::BF16, int64_t kv_block_stride = 0) const {
+    check(rg_paged_attention_shared_prefix(query, key_cache, value_cache, block_table, context_lens, output, scale,
+                                           num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                                           batch_size, shared_blocks, (int32_t)dtype, kv_block_stride, workspace,
+                                           workspace_bytes, stream_),
+          "launch_shared_prefix");
+  }
   size_t v1_scores_workspace_bytes(int32_t batch_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                    int32_t block_size, int32_t max_blocks_per_seq) const {
     return rg_paged_attention_v1_scores_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,

@@ -24,16 +24,17 @@ LIB_OUT = os.path.join(PKG, "librailgun_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_SOURCES = ["rg_status.hip", "cache_ops.hip", "decode.hip", "prefill.hip", "model_ops.hip", "gemm.hip", "validate.hip",
-               "evict.hip", "scores.hip"]
+               "evict.hip", "scores.hip", "shared_prefix.hip"]
 # -packed-fp32-ops: hipcc must not form v_pk_{add,mul,fma}_f32 on its own.
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++20", f"-I{ROOT}/include",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall",
 ]
-# Per-source additions.  prefill.hip keeps its MFMA accumulators in ordinary VGPRs: with the
-# default heuristic they land in AGPRs and are copied to VGPRs around the softmax rescale
-# on every key tile.
-SOURCE_FLAGS = {"prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# Per-source additions.  prefill.hip and shared_prefix.hip keep their MFMA accumulators in ordinary
+# VGPRs: with the default heuristic they land in AGPRs and are copied to VGPRs around the softmax
+# rescale on every key tile (and in shared_prefix.hip the 80 AGPRs on top of the other half's
+# VGPRs leave room for one workgroup per CU instead of two).
+SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("prefill.hip", "shared_prefix.hip")}
 CPP_TESTS = ["test_paged_attention_op"]
 
 

@@ -303,7 +303,8 @@ __global__ __launch_bounds__(64) RG_SK_OCCUPANCY void decode_stream_kernel(
     const typename DecodeTileFor<T, D, G>::S* __restrict__ kc, const typename DecodeTileFor<T, D, G>::S* __restrict__ vc,
     const int32_t* __restrict__ block_table, const int32_t* __restrict__ context_lens,
     const int32_t* __restrict__ positions, const int32_t* __restrict__ slot_mapping) {
-  stream_worker<T, D, G, ROPE>(a, q_ptr, kc, vc, block_table, context_lens, positions, slot_mapping);
+  stream_worker<T, D, G, ROPE>(a, q_ptr, kc, vc, block_table, context_lens, positions, slot_mapping, blockIdx.x, 0,
+                               threadIdx.x);
 }
 
 // One workgroup per segment (sequence, kv-head), one wave per head of the group: merges the

@@ -617,6 +617,7 @@ constexpr int sk_prefetch_for() { return std::is_same_v<T, f32_t> ? (D <= 64 ? 2
 enum class StreamVariant {
   kDecode,
   kScores,  // also leaves every raw score (q . k) in `logits`
+  kSuffix,  // takes a sequence's tokens from `prefix` on (all of a sequence that has fewer)
 };
 
 struct StreamArgs {
@@ -643,6 +644,8 @@ struct StreamArgs {
   const int32_t* slot_mapping;  // [batch]; negative: a padding token, not cached
   // kScores: [batch, H_kv, 16 max_blocks tokens, G].
   float* logits;
+  // kSuffix: tokens of whole blocks, more than 0.
+  int32_t prefix;
 };
 
 // Cost of a segment start, in KB of K/V streaming.  A worker's end time tracks the segments it
@@ -664,16 +667,21 @@ struct StreamArgs {
 #define RG_SK_SEG_COST_KB_ROPE RG_SK_SEG_COST_KB
 #endif
 
+// Tokens behind the prefix of a context of c tokens that has all of it, else the whole context.
+__device__ __forceinline__ int past_prefix(int c, int prefix) { return c >= prefix ? c - prefix : c; }
+
 // 16-token sub-blocks of sequence s: ceil(ctx/16) per kv-head (context clamped to the table
-// row, max_blocks of them).
-__device__ __forceinline__ int seq_blocks(const int32_t* ctxl, int s, int max_blocks) {
-  const int c = max(0, min(ctxl[s], max_blocks * kBS));
+// row, max_blocks of them); with SUF, of its tokens past the prefix.
+template <bool SUF = false>
+__device__ __forceinline__ int seq_blocks(const int32_t* ctxl, int s, int max_blocks, int prefix = 0) {
+  int c = max(0, min(ctxl[s], max_blocks * kBS));
+  if constexpr (SUF) c = past_prefix(c, prefix);
   return (c + kBS - 1) / kBS;
 }
 // Stream-K units of sequence s per kv-head: its blocks in runs of BPU (the last run may be short).
-template <int BPU>
-__device__ __forceinline__ int seq_units(const int32_t* ctxl, int s, int max_blocks) {
-  return (seq_blocks(ctxl, s, max_blocks) + BPU - 1) / BPU;
+template <int BPU, bool SUF = false>
+__device__ __forceinline__ int seq_units(const int32_t* ctxl, int s, int max_blocks, int prefix = 0) {
+  return (seq_blocks<SUF>(ctxl, s, max_blocks, prefix) + BPU - 1) / BPU;
 }
 
 // A wave-uniform 64-bit value made visibly uniform to the compiler.
@@ -683,8 +691,11 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-// Wave-wide inclusive prefix sum.
+// Wave-wide inclusive prefix sum.  FORGET: the lane masks of its steps are formed anew at each call
+// instead of being held in scalar registers across the caller's loops.
+template <bool FORGET = false>
 __device__ __forceinline__ int64_t wave_incl_scan(int64_t v, int lane) {
+  if constexpr (FORGET) asm volatile("" : "+v"(lane));
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int64_t t = __shfl_up(v, o, 64);
@@ -699,12 +710,14 @@ __device__ __forceinline__ int64_t wave_incl_scan(int64_t v, int lane) {
 // them into its own loaded copy of that block in place of what the cache held.  No worker reads
 // another's store, and the outputs and cache equal those of the RoPE + cache pass followed by
 // the decode bit for bit.  positions / slot_mapping: [batch], token s being sequence s's.
-template <typename T, int D, int G, bool ROPE, StreamVariant VAR = StreamVariant::kDecode>
+// Worker k, one wave: wave `wave` of a workgroup of WAVES that are workers each.
+template <typename T, int D, int G, bool ROPE, StreamVariant VAR = StreamVariant::kDecode, int WAVES = 1>
 __device__ __forceinline__ void stream_worker(
     const StreamArgs& a, const typename DecodeTileFor<T, D, G>::S* __restrict__ q_ptr,
     const typename DecodeTileFor<T, D, G>::S* __restrict__ kc, const typename DecodeTileFor<T, D, G>::S* __restrict__ vc,
     const int32_t* __restrict__ block_table, const int32_t* __restrict__ context_lens,
-    const int32_t* __restrict__ positions, const int32_t* __restrict__ slot_mapping) {
+    const int32_t* __restrict__ positions, const int32_t* __restrict__ slot_mapping, const int64_t k, const int wave,
+    const int lane) {
   using Tile = DecodeTileFor<T, D, G>;
   static_assert(!ROPE || !std::is_same_v<T, f32_t>, "the fused RoPE runs on the 16-bit tiles");
   constexpr int GP = Tile::GP;
@@ -714,11 +727,17 @@ __device__ __forceinline__ void stream_worker(
   constexpr int kSkPrefetch = sk_prefetch_for<T, D, G>();
   constexpr int NBUF = kSkPrefetch + 1;
   constexpr int BPU = sk_bpu_for<T, D, G>();
-  __shared__ float p_lds[2][BPU * kBS * GP];
-  __shared__ float alpha_lds[2][GP];
+  __shared__ float p_all[WAVES][2][BPU * kBS * GP];
+  __shared__ float alpha_all[WAVES][2][GP];
+  auto& p_lds = p_all[wave];
+  auto& alpha_lds = alpha_all[wave];
 
-  const int lane = threadIdx.x;
-  const int64_t k = blockIdx.x;
+  constexpr bool SUF = VAR == StreamVariant::kSuffix;
+  const int prefix = SUF ? a.prefix : 0;
+  auto tokens_of = [&](int sq) __attribute__((always_inline)) -> int {
+    const int c = min(context_lens[sq], a.max_blocks * kBS);
+    return SUF ? past_prefix(c, prefix) : c;
+  };
   const int hkv = a.num_kv_heads;
   // Total units U, this worker's range [u0, u1) and the sequence holding u0: one pass over
   // the context lengths for up to 64 sequences (one per lane), two for larger batches.
@@ -761,8 +780,8 @@ __device__ __forceinline__ void stream_worker(
     int64_t U = 0, ne = 0, n1 = 0, incl1 = 0, nb1 = 0;
     for (int c0 = 0; c0 < a.batch; c0 += 64) {
       const int q = c0 + lane;
-      const int64_t n = q < a.batch ? (int64_t)seq_units<BPU>(context_lens, q, a.max_blocks) * hkv : 0;
-      const int64_t incl = wave_incl_scan(n, lane) + U;
+      const int64_t n = q < a.batch ? (int64_t)seq_units<BPU, SUF>(context_lens, q, a.max_blocks, prefix) * hkv : 0;
+      const int64_t incl = wave_incl_scan<(WAVES > 1)>(n, lane) + U;
       if (c0 == 0) {
         n1 = n;
         incl1 = incl;
@@ -815,8 +834,8 @@ __device__ __forceinline__ void stream_worker(
       int64_t ub = 0, nb = 0;
       for (int c0 = 0; c0 < a.batch && (s < 0 || need1); c0 += 64) {
         const int q = c0 + lane;
-        const int64_t n = q < a.batch ? (int64_t)seq_units<BPU>(context_lens, q, a.max_blocks) * hkv : 0;
-        const int64_t incl = wave_incl_scan(n, lane) + ub;
+        const int64_t n = q < a.batch ? (int64_t)seq_units<BPU, SUF>(context_lens, q, a.max_blocks, prefix) * hkv : 0;
+        const int64_t incl = wave_incl_scan<(WAVES > 1)>(n, lane) + ub;
         resolve(c0, n, incl, nb + below(n > 0));
         ub = uniform64(__shfl(incl, 63, 64));
         nb += __builtin_popcountll(__ballot(n > 0));
@@ -829,8 +848,8 @@ __device__ __forceinline__ void stream_worker(
       s = -1;
       for (int c0 = 0; c0 < a.batch && s < 0; c0 += 64) {
         const int q = c0 + lane;
-        const int64_t n = q < a.batch ? (int64_t)seq_units<BPU>(context_lens, q, a.max_blocks) * hkv : 0;
-        const int64_t incl = wave_incl_scan(n, lane) + ub, excl = incl - n;
+        const int64_t n = q < a.batch ? (int64_t)seq_units<BPU, SUF>(context_lens, q, a.max_blocks, prefix) * hkv : 0;
+        const int64_t incl = wave_incl_scan<(WAVES > 1)>(n, lane) + ub, excl = incl - n;
         const int64_t nb_ = nb + below(n > 0);
         const uint64_t h = __ballot(n > 0 && excl <= u0 && u0 < incl);
         if (h) {
@@ -847,6 +866,14 @@ __device__ __forceinline__ void stream_worker(
     seq_seg = __builtin_amdgcn_readfirstlane(seq_seg);
   }
 
+  // What only a segment's ends use.  With several workers to a workgroup it is kept in vector registers:
+  // the scalar ones are all taken.
+  auto keep = [](int64_t x) __attribute__((always_inline)) -> int64_t {
+    if constexpr (WAVES > 1) asm volatile("" : "+v"(x));
+    return x;
+  };
+  const int64_t k_end = keep(k), C_end = keep(C), W_end = keep(W);
+
   // Cursor of the unit being computed and of the unit being loaded: sequence, kv-head, unit b
   // of the segment's nblk units (blocks b * BPU .. b * BPU + BPU - 1).
   struct Cursor {
@@ -857,7 +884,7 @@ __device__ __forceinline__ void stream_worker(
   // load instead of a vector load whose wait would also drain the K/V prefetches.
   Cursor cur;
   cur.s = s;
-  cur.nblk = __builtin_amdgcn_readfirstlane(seq_units<BPU>(context_lens, s, a.max_blocks));
+  cur.nblk = __builtin_amdgcn_readfirstlane(seq_units<BPU, SUF>(context_lens, s, a.max_blocks, prefix));
   {
     const int r = __builtin_amdgcn_readfirstlane((int)(u0 - seq_start));
     cur.kvh = __builtin_amdgcn_readfirstlane(r / cur.nblk);
@@ -875,7 +902,7 @@ __device__ __forceinline__ void stream_worker(
         c.kvh = 0;
         do {
           ++c.s;
-          c.nblk = c.s < a.batch ? seq_units<BPU>(context_lens, c.s, a.max_blocks) : 1;
+          c.nblk = c.s < a.batch ? seq_units<BPU, SUF>(context_lens, c.s, a.max_blocks, prefix) : 1;
         } while (c.nblk == 0);
       }
     }
@@ -902,13 +929,14 @@ __device__ __forceinline__ void stream_worker(
         kh = 0;
         do {
           ++ss;
-          nb = ss < a.batch ? seq_units<BPU>(context_lens, ss, a.max_blocks) : 1;
+          nb = ss < a.batch ? seq_units<BPU, SUF>(context_lens, ss, a.max_blocks, prefix) : 1;
         } while (nb == 0);
       }
     }
     const bool live = base + lane < u1 - u0 && ss < a.batch;
     const int32_t* row = block_table + (int64_t)(live ? ss : 0) * a.table_stride;
-    const int nbk = live ? seq_blocks(context_lens, ss, a.max_blocks) : 0;
+    if constexpr (SUF) row += live && context_lens[ss] >= prefix ? prefix >> (4 + a.bs_shift) : 0;
+    const int nbk = live ? seq_blocks<SUF>(context_lens, ss, a.max_blocks, prefix) : 0;
 #pragma unroll
     for (int r = 0; r < BPU; ++r) {
       const int bk = b * BPU + r < nbk ? b * BPU + r : b * BPU;
@@ -1004,15 +1032,15 @@ __device__ __forceinline__ void stream_worker(
     if (c.b == 0 && lane == 0) {
       // The worker of the segment's last unit (the last k with k C / W <= its cost).
       const int64_t z = KQ * (ubeg + c.nblk - 1) + KS * (seg + 1);
-      const int64_t last = ((z + 1) * W - 1) / C;
-      a.seg_desc[(int64_t)c.s * hkv + c.kvh] = make_int2((int)k, (int)(last - k + 1));
+      const int64_t last = ((z + 1) * W_end - 1) / C_end;
+      a.seg_desc[(int64_t)c.s * hkv + c.kvh] = make_int2((int)k_end, (int)(last - k_end + 1));
     }
   };
   auto end_segment = [&](const Cursor& c) __attribute__((always_inline)) {
     float lsum[4];
     tile.reduce(lsum);
     const int64_t g = (int64_t)c.s * hkv + c.kvh;
-    const int64_t idx = k + g;
+    const int64_t idx = k_end + g;
     float* pa = a.part_acc + idx * (G * D);
     if (tile.vrow == 0) {
 #pragma unroll
@@ -1049,7 +1077,7 @@ __device__ __forceinline__ void stream_worker(
   const int64_t n = u1 - u0;
   Cursor ld = cur;
   int64_t ldi = 0;
-  int ctx_cur = min(context_lens[cur.s], a.max_blocks * kBS);
+  int ctx_cur = tokens_of(cur.s);
   fill_window(cur, 0);
   uint4 kbuf[NBUF][BPU * NK], vbuf[NBUF][BPU * NV];
   // Prologue: the first kSkPrefetch units (the last one repeated past the end of the range).
@@ -1140,7 +1168,7 @@ __device__ __forceinline__ void stream_worker(
         if constexpr (VAR == StreamVariant::kScores) {
           lg = lg_all + ((int64_t)cur.s * hkv + cur.kvh) * a.max_blocks * (kBS * G);
         }
-        ctx_cur = min(context_lens[cur.s], a.max_blocks * kBS);
+        ctx_cur = tokens_of(cur.s);
       }
     } else {
       advance(cur);

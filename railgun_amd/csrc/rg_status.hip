@@ -56,6 +56,7 @@ int probe_decode_kernels();
 int probe_prefill_kernels();
 int probe_evict_kernels();
 int probe_scores_kernels();
+int probe_shared_prefix_kernels();
 int setup_no_alloc_scratch();
 }  // namespace rg
 
@@ -89,6 +90,7 @@ extern "C" int rg_init(int device_ordinal) {
   if (st == RG_OK) st = rg::probe_prefill_kernels();
   if (st == RG_OK) st = rg::probe_evict_kernels();
   if (st == RG_OK) st = rg::probe_scores_kernels();
+  if (st == RG_OK) st = rg::probe_shared_prefix_kernels();
   if (st == RG_OK) st = rg::setup_no_alloc_scratch();
   (void)hipSetDevice(cur);
   if (st != RG_OK) return st;

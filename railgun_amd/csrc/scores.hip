@@ -44,7 +44,8 @@ __global__ __launch_bounds__(64) void scores_stream_kernel(StreamArgs a, const t
                                                            const typename DecodeTileFor<T, D, G>::S* __restrict__ vc,
                                                            const int32_t* __restrict__ block_table,
                                                            const int32_t* __restrict__ context_lens) {
-  stream_worker<T, D, G, false, StreamVariant::kScores>(a, q, kc, vc, block_table, context_lens, nullptr, nullptr);
+  stream_worker<T, D, G, false, StreamVariant::kScores>(a, q, kc, vc, block_table, context_lens, nullptr, nullptr,
+                                                        blockIdx.x, 0, threadIdx.x);
 }
 
 struct GenericArgs {

@@ -1,0 +1,496 @@
+// Decode attention of a batch whose sequences begin with the same cached blocks.
+//
+// With P prefix tokens in shared blocks, the B rows of the batch ask G query heads each of a kv-head's prefix:
+// B G rows against the same K and V.  Read per sequence, as the plain decode does, the prefix costs B times
+// its bytes; here it is read once per kPreRows rows, as an attention product on the matrix cores:
+//   S^T = K Q^T,  running maximum and sum per row,  O^T += V^T P^T.
+// The tokens behind the prefix differ per sequence and stay with the stream-K decode worker.  Softmax
+// partials (m, l, unnormalised O) of both join in shared_merge_kernel:
+//   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+//
+// One launch computes both: the product is bound by the matrix cores and LDS, the suffixes by HBM, and
+// workgroups of either kind sit on every CU, so the shorter of the two hides under the longer.  A sequence
+// whose context ends inside the prefix is not a row of the product (which then needs no mask per row); the
+// stream-K worker takes all of its tokens.
+#include "decode_stream.hpp"
+
+namespace rg {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+
+template <typename T> struct mfma32;
+template <> struct mfma32<bf16_t> {
+  __device__ static __forceinline__ f32x16_t run(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+};
+template <> struct mfma32<f16_t> {
+  __device__ static __forceinline__ f32x16_t run(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  }
+};
+// acc + lo + hi of a packed pair.
+template <typename T> __device__ __forceinline__ float pair_sum(uint32_t pair, float acc);
+template <> __device__ __forceinline__ float pair_sum<bf16_t>(uint32_t pair, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), __builtin_bit_cast(bf16x2_t, 0x3F803F80u),
+                                         acc, false);
+}
+template <> __device__ __forceinline__ float pair_sum<f16_t>(uint32_t pair, float acc) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), __builtin_bit_cast(f16x2_t, 0x3C003C00u), acc,
+                                false);
+}
+
+constexpr int kPreWaves = 4;
+constexpr int kPreThreads = 64 * kPreWaves;
+constexpr int kPreRows = 32 * kPreWaves;  // rows of a workgroup, 32 a wave
+constexpr int kTileKeys = 32;
+constexpr int kStages = 3;                // key tiles in the LDS ring
+constexpr float kSlack = 8.f;             // log2 headroom of the lazy maximum: 2^8 a probability at most
+
+struct PrefixArgs {
+  float* acc;  // [H_kv, splits, rows, D] unnormalised
+  float* ml;   // [H_kv, splits, rows, 2]: m in log2 units, l
+  float scale_log2;
+  int32_t group, num_heads, num_kv_heads, rows;  // rows = batch * group
+  int32_t prefix, subs;                          // prefix tokens, and its 16-token sub-blocks
+  int32_t tiles, split_tiles, splits;
+  int32_t bs_shift, table_stride_tokens;         // table_stride_tokens: tokens of a block-table row
+  int32_t stream_groups;                         // workgroups of stream-K workers, the first of the grid
+  int64_t kv_stride;
+};
+
+// One key tile in LDS, two sub-blocks of 16 keys.  K: the 16-byte chunk c of key k of sub-block b at
+// b * KB / 2 + 256 c + 16 k, so that a 1 KB copy reads one sub-block only and the A operand of one MFMA is
+// 256 contiguous bytes per 16 lanes.  V: rows [key][D] with the 16-byte chunks of a row XORed by
+// 2 (key & 3), so that the transposing reads of four rows hit different banks.
+template <int D>
+struct KeyTile {
+  static constexpr int KB = kTileKeys * D * 2;
+  static constexpr int BYTES = 2 * KB;
+  static constexpr int VCH = D / 8;        // 16-byte chunks of a V row
+  static constexpr int SUB_COPIES = D / 32;  // 1 KB copies of a sub-block's K, and of its V
+  __device__ static __forceinline__ int vchunk(int key, int c) { return c ^ (2 * (key & 3)); }
+};
+
+// The prefix product of workgroup u: kPreRows rows of one kv-head against the key tiles of one split.
+// Lane l of a wave owns query row l % 32 of it; the other half of that row's keys sits in lane l ^ 32.
+template <typename T, int D>
+__device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16_t* __restrict__ q,
+                                               const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
+                                               const int32_t* __restrict__ table,
+                                               const int32_t* __restrict__ context_lens, char* lds, int u, int w,
+                                               int lane) {
+  using MF = mfma32<T>;
+  using TL = KeyTile<D>;
+  constexpr int NKC = D / 16, NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF;
+  static_assert(HALF >= 1, "two waves copy a sub-block");
+  const int pairs = a.num_kv_heads * a.splits;
+  const int rt = u / pairs, pair = u % pairs;
+  const int kvh = pair % a.num_kv_heads, split = pair / a.num_kv_heads;
+  const int kt0 = split * a.split_tiles, kt1 = min(a.tiles, kt0 + a.split_tiles);
+  const int j = lane & 31, hh = lane >> 5;
+  const int wrow = rt * kPreRows + w * 32;  // the wave's first row
+  const bool busy = wrow < a.rows;          // (a wave without rows copies and waits with the others)
+  const int row = wrow + j;
+  const int b = min(row, a.rows - 1) / a.group, g = min(row, a.rows - 1) - b * a.group;
+
+  // This wave copies half of sub-block cb of every tile.  Lane l of the window holds the entry of tile
+  // wb + l: (physical block << bs_shift) | sub-block within it; past the end the last sub-block's.
+  const int cb = w >> 1, cp = w & 1;
+  int wb = kt0, win;
+  auto fill = [&]() {
+    const int sb = min(2 * (wb + lane) + cb, a.subs - 1);
+    win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
+  };
+  fill();
+  uint4 qb[NKC];
+  {
+    const uint4* qr = reinterpret_cast<const uint4*>(q + ((int64_t)b * a.num_heads + (int64_t)kvh * a.group + g) * D);
+#pragma unroll
+    for (int i = 0; i < NKC; ++i) qb[i] = qr[2 * i + hh];
+  }
+  // Rows whose context lacks part of the prefix are left to the stream-K workers: they compute along
+  // (finite or not, no other lane's row sees it) and write nothing that the merge reads.
+  int32_t lane_off[COPIES];
+  uint32_t ins_lds[COPIES];
+#pragma unroll
+  for (int ld = 0; ld < COPIES; ++ld) {
+    if (ld < HALF) {
+      const int n = cp * HALF + ld;
+      lane_off[ld] = (lane & 15) * D + 8 * (4 * n + (lane >> 4));
+      ins_lds[ld] = cb * (TL::KB / 2) + n * 1024;
+    } else {
+      const int vi = cb * TL::SUB_COPIES + cp * HALF + ld - HALF;  // of the tile's V
+      const int key = vi * (1024 / (D * 2)) + lane / TL::VCH;
+      lane_off[ld] = (key & 15) * D + 8 * TL::vchunk(key, lane % TL::VCH);
+      ins_lds[ld] = TL::KB + vi * 1024;
+    }
+  }
+  const uint32_t lds_base = (uint32_t)(uintptr_t)((RG_LDS char*)lds);
+  const int64_t head = (int64_t)kvh * (kBS << a.bs_shift) * D;
+  auto issue = [&](int kt, int st) {
+    const int e = __builtin_amdgcn_readlane(win, kt - wb);
+    const int64_t off = (int64_t)(e >> a.bs_shift) * a.kv_stride + head + (int64_t)(e & ((1 << a.bs_shift) - 1)) * (kBS * D);
+    const char* kb = reinterpret_cast<const char*>(kc + off);
+    const char* vb = reinterpret_cast<const char*>(vc + off);
+    const uint32_t sbase = lds_base + st * TL::BYTES;
+#pragma unroll
+    for (int ld = 0; ld < COPIES; ++ld) {
+      lds_dma16_s(ld < HALF ? kb : vb, (uint32_t)lane_off[ld] * 2u, sbase + ins_lds[ld]);
+    }
+  };
+
+  f32x16_t o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  const int xor32 = (lane ^ 32) << 2;
+  const int k_lane = (j >> 4) * (TL::KB / 2) + hh * 256 + (j & 15) * 16;
+  const int grp = lane >> 4, e_row = (lane >> 2) & 3, qq = lane & 3;
+
+  // Tile kt from ring stage st.  S^T: c[v] is key 8 (v >> 2) + 4 hh + (v & 3) of the tile for query j.
+  auto compute = [&](int kt, int st) {
+    const char* kbase = lds + st * TL::BYTES + k_lane;
+    f32x16_t c;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NKC; ++i) c = MF::run(*reinterpret_cast<const uint4*>(kbase + i * 512), qb[i], c);
+    if (2 * kt + 1 >= a.subs) {  // an odd number of sub-blocks: the last tile's second half repeats one
+#pragma unroll
+      for (int v = 8; v < 16; ++v) c[v] = -INFINITY;
+    }
+    // The maximum moves only when a tile exceeds it by more than kSlack, for both halves of a row alike;
+    // it is that of the scaled scores, whatever the scale's sign.
+    float x[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = c[v] * a.scale_log2;
+    if (2 * kt + 1 >= a.subs) {
+#pragma unroll
+      for (int v = 8; v < 16; ++v) x[v] = -INFINITY;
+    }
+    float tmax = x[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, x[v]);
+    if (__ballot(tmax > m_run + kSlack)) {
+      const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)));
+      const float both = fmaxf(tmax, other);
+      const float m_new = both > m_run + kSlack ? both : m_run;
+      const float alpha = fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+    }
+    // Probabilities, rounded to the operand type of the PV product; the sum takes the rounded ones, so
+    // the normaliser weighs what enters the product.
+    uint32_t pk[8];
+#pragma unroll
+    for (int v = 0; v < 16; v += 2) pk[v / 2] = pack2<T>(fast_exp2(x[v] - m_run), fast_exp2(x[v + 1] - m_run));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l_run = pair_sum<T>(pk[i], l_run);
+    const char* vbase = lds + st * TL::BYTES + TL::KB;
+#pragma unroll
+    for (int m = 0; m < 2 * NDB; ++m) {
+      const int n = m / NDB, db = m % NDB;
+      const int d = 32 * db + 16 * (grp & 1) + 4 * qq;
+      uint2 part[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int key = 16 * n + 8 * half + 4 * (grp >> 1) + e_row;
+        const int off = key * (D * 2) + TL::vchunk(key, d >> 3) * 16 + (d & 7) * 2;
+        part[half] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((RG_LDS v4i16_t*)(vbase + off)));
+      }
+      o[db] = MF::run(make_uint4(part[0].x, part[0].y, part[1].x, part[1].y),
+                      make_uint4(pk[4 * n], pk[4 * n + 1], pk[4 * n + 2], pk[4 * n + 3]), o[db]);
+    }
+  };
+
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the window and Q have landed: only copies count from here
+#pragma unroll
+  for (int p = 0; p < kStages - 1; ++p)
+    if (kt0 + p < kt1) issue(kt0 + p, p);
+  int st = 0;
+  for (int kt = kt0; kt < kt1; ++kt) {
+    // Tile kt has landed (a newer one may not have), for every wave; all are done with tile kt - 1, whose
+    // stage takes tile kt + kStages - 1.
+    if (kt + 1 < kt1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    static_assert(kStages == 3, "one tile newer than the awaited one");
+    tile_barrier();
+    const int next = kt + kStages - 1;
+    if (next < kt1) {
+      if (next - wb >= 64) {
+        wb = next;
+        fill();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      issue(next, st == 0 ? kStages - 1 : st - 1);
+    }
+    if (busy) compute(kt, st);
+    st = st == kStages - 1 ? 0 : st + 1;
+  }
+  if (row < a.rows) {
+    const float l = l_run + __shfl_xor(l_run, 32, 64);
+    const int64_t at = ((int64_t)kvh * a.splits + split) * a.rows + row;
+    float* acc = a.acc + at * D;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        *reinterpret_cast<float4*>(acc + 32 * db + 8 * p + 4 * hh) =
+            make_float4(o[db][4 * p], o[db][4 * p + 1], o[db][4 * p + 2], o[db][4 * p + 3]);
+    if (hh == 0) {
+      a.ml[2 * at] = m_run;
+      a.ml[2 * at + 1] = l;
+    }
+  }
+}
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(kPreThreads) void shared_prefix_kernel(StreamArgs sa, PrefixArgs pa,
+                                                                    const uint16_t* __restrict__ q,
+                                                                    const uint16_t* __restrict__ kc,
+                                                                    const uint16_t* __restrict__ vc,
+                                                                    const int32_t* __restrict__ block_table,
+                                                                    const int32_t* __restrict__ context_lens) {
+  __shared__ __attribute__((aligned(16))) char ring[kStages * KeyTile<D>::BYTES];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if ((int)blockIdx.x < pa.stream_groups) {
+    const int k = (int)blockIdx.x * kPreWaves + w;
+    if (k < sa.num_workers) {
+      stream_worker<T, D, G, false, StreamVariant::kSuffix, kPreWaves>(sa, q, kc, vc, block_table, context_lens, nullptr,
+                                                                       nullptr, k, w, lane);
+    }
+    return;
+  }
+  prefix_product<T, D>(pa, q, kc, vc, block_table, context_lens, ring, (int)blockIdx.x - pa.stream_groups, w, lane);
+}
+
+// One workgroup per (kv-head, sequence), a wave per query head: lane l folds dims [l PER, (l + 1) PER) of the
+// prefix's splits (if the sequence has the whole prefix) and of the stream-K workers' partials, in that order.
+template <typename T, int D, int G>
+__global__ __launch_bounds__(64 * G) void shared_merge_kernel(StreamArgs sa, PrefixArgs pa,
+                                                              const int32_t* __restrict__ context_lens) {
+  using S = typename elem<T>::storage;
+  constexpr int PER = D / 64;
+  const int kvh = blockIdx.x, s = blockIdx.y, h = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int hkv = sa.num_kv_heads;
+  S* out = static_cast<S*>(sa.out) + ((int64_t)s * sa.num_heads + (int64_t)kvh * G + h) * D + lane * PER;
+  const int ctx = max(0, min(context_lens[s], sa.max_blocks * kBS));
+  float m = -INFINITY, l = 0.f;
+  float acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  auto fold = [&](float2 ml, const float* pa_row) __attribute__((always_inline)) {
+    float v[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) v[e] = pa_row[e];
+    const float mn = fmaxf(m, ml.x);
+    const float fo = exp2f(m - mn), fq = exp2f(ml.x - mn);
+    l = l * fo + ml.y * fq;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = acc[e] * fo + v[e] * fq;
+    m = mn;
+  };
+  if (ctx >= sa.prefix) {
+    const int64_t r0 = (int64_t)kvh * pa.splits * pa.rows + s * G + h;
+#pragma unroll 4
+    for (int p = 0; p < pa.splits; ++p) {
+      const int64_t r = r0 + (int64_t)p * pa.rows;
+      fold(*reinterpret_cast<const float2*>(pa.ml + 2 * r), pa.acc + r * D + lane * PER);
+    }
+  }
+  if (past_prefix(ctx, sa.prefix) > 0) {
+    const int64_t seg = (int64_t)s * hkv + kvh;
+    const int2 dsc = sa.seg_desc[seg];
+    const int64_t p0 = dsc.x + seg;
+#pragma unroll 4
+    for (int p = 0; p < dsc.y; ++p) {
+      fold(*reinterpret_cast<const float2*>(sa.part_ml + (p0 + p) * (2 * G) + 2 * h),
+           sa.part_acc + (p0 + p) * (G * D) + h * D + lane * PER);
+    }
+  }
+  const float inv = l != 0.f ? 1.f / l : 1.f;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) out[e] = elem<T>::from_f32(acc[e] * inv);
+}
+
+template <typename T, int D>
+void launch_shared(const StreamArgs& sa, const PrefixArgs& pa, int G, int groups, const void* q, const void* kc,
+                   const void* vc, const int32_t* bt, const int32_t* cl, hipStream_t s) {
+  auto go = [&](auto g) {
+    constexpr int GC = decltype(g)::value;
+    hipLaunchKernelGGL((shared_prefix_kernel<T, D, GC>), dim3(groups), dim3(kPreThreads), 0, s, sa, pa,
+                       static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(kc),
+                       static_cast<const uint16_t*>(vc), bt, cl);
+    hipLaunchKernelGGL((shared_merge_kernel<T, D, GC>), dim3(sa.num_kv_heads, sa.batch), dim3(64 * GC), 0, s, sa, pa,
+                       cl);
+  };
+  switch (G) {
+    case 1: go(std::integral_constant<int, 1>{}); break;
+    case 2: go(std::integral_constant<int, 2>{}); break;
+    case 3: go(std::integral_constant<int, 3>{}); break;
+    case 4: go(std::integral_constant<int, 4>{}); break;
+    case 5: go(std::integral_constant<int, 5>{}); break;
+    case 6: go(std::integral_constant<int, 6>{}); break;
+    case 7: go(std::integral_constant<int, 7>{}); break;
+    case 8: go(std::integral_constant<int, 8>{}); break;
+    default: go(std::integral_constant<int, 16>{}); break;  // shared_applies
+  }
+}
+
+// Whether the shared product takes the call (else every sequence reads the prefix for itself).
+bool shared_applies(const Shape& sh, int32_t dtype, int64_t kv_stride, const void* q, const void* kc, const void* vc,
+                    const void* out) {
+  return dtype != RG_DTYPE_F32 && sh.D <= 128 && sh.B > 1 && tiles_take(sh, dtype, kv_stride, q, kc, vc, out);
+}
+
+struct SharedPlan {
+  int32_t rows, row_tiles, tiles, split_tiles, splits, workers, stream_groups;
+};
+SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks) {
+  SharedPlan p;
+  const int64_t prefix = (int64_t)shared_blocks * sh.bs;
+  p.rows = sh.B * (sh.H / sh.Hkv);
+  p.row_tiles = (int32_t)ceil_div(p.rows, kPreRows);
+  p.tiles = (int32_t)ceil_div(prefix, kTileKeys);
+  const int64_t want = std::max<int64_t>(1, device_cu_count() / ((int64_t)sh.Hkv * p.row_tiles));
+  p.split_tiles = (int32_t)ceil_div(p.tiles, std::min<int64_t>(want, p.tiles));
+  p.splits = (int32_t)ceil_div(p.tiles, p.split_tiles);
+  p.workers = stream_workers(sh);
+  p.stream_groups = (int32_t)ceil_div(p.workers, kPreWaves);
+  return p;
+}
+size_t prefix_bytes(const Shape& sh, const SharedPlan& p, size_t* ml_at) {
+  const size_t n = (size_t)sh.Hkv * p.splits * p.rows;
+  const size_t acc = align_up(n * sh.D * 4, 256);
+  if (ml_at) *ml_at = acc;
+  return acc + align_up(n * 8, 256);
+}
+
+}  // namespace
+
+int probe_shared_prefix_kernels() {
+  hipFuncAttributes at;
+  if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(shared_prefix_kernel<bf16_t, 128, 4>)) != hipSuccess ||
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(shared_merge_kernel<bf16_t, 128, 4>)) != hipSuccess) {
+    return fail(RG_ERR_HIP, "failed to load the shared-prefix kernels: %s", hipGetErrorString(hipGetLastError()));
+  }
+  return RG_OK;
+}
+
+}  // namespace rg
+
+using namespace rg;
+
+extern "C" size_t rg_paged_attention_shared_prefix_workspace_bytes(int32_t batch_size, int32_t num_heads,
+                                                                   int32_t num_kv_heads, int32_t head_dim,
+                                                                   int32_t block_size, int32_t max_blocks_per_seq,
+                                                                   int32_t shared_blocks) {
+  if (batch_size <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
+      block_size <= 0 || max_blocks_per_seq <= 0 || shared_blocks < 0 || shared_blocks > max_blocks_per_seq) {
+    return 0;
+  }
+  const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  size_t n = rg_paged_attention_v1_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                                                   max_blocks_per_seq);
+  if (shared_blocks > 0) {
+    const SharedPlan p = plan_shared(sh, shared_blocks);
+    n = std::max(n, prefix_bytes(sh, p, nullptr) + stream_bytes(sh, p.workers, nullptr, nullptr));
+  }
+  return n;
+}
+
+extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* key_cache, const void* value_cache,
+                                                const int32_t* block_table, const int32_t* context_lens, void* output,
+                                                float scale, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                int32_t block_size, int32_t max_blocks_per_seq, int32_t batch_size,
+                                                int32_t shared_blocks, int32_t dtype, int64_t kv_block_stride,
+                                                void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "paged_attention_shared_prefix";
+  const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  int st = check_decode_shape(op, sh, dtype, kv_block_stride);
+  if (st != RG_OK) return st;
+  if (shared_blocks < 0 || shared_blocks > max_blocks_per_seq) {
+    return fail(RG_ERR_INVALID_ARGUMENT, "%s: shared_blocks %d outside 0 .. max_blocks_per_seq %d", op, shared_blocks,
+                max_blocks_per_seq);
+  }
+  if ((int64_t)max_blocks_per_seq * block_size > INT32_MAX || batch_size > 65535 ||
+      (int64_t)batch_size * (num_heads / num_kv_heads) > INT32_MAX) {
+    return fail(RG_ERR_NOT_SUPPORTED, "%s: a block table of %lld tokens, %d sequences", op,
+                (long long)max_blocks_per_seq * block_size, batch_size);
+  }
+  if (batch_size == 0) return ok();
+  if (!query || !key_cache || !value_cache || !block_table || !context_lens || !output) {
+    return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
+  }
+  const size_t need = rg_paged_attention_shared_prefix_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim,
+                                                                       block_size, max_blocks_per_seq, shared_blocks);
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) {
+    return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned), %zu required", op,
+                workspace ? workspace_bytes : (size_t)0, need);
+  }
+  const int64_t kv_stride = kv_block_stride ? kv_block_stride : (int64_t)num_kv_heads * block_size * head_dim;
+  if (shared_blocks == 0 || !shared_applies(sh, dtype, kv_stride, query, key_cache, value_cache, output)) {
+    return rg_paged_attention_v1(query, key_cache, value_cache, block_table, context_lens, output, scale, num_heads,
+                                 num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size, dtype,
+                                 kv_block_stride, workspace, workspace_bytes, stream);
+  }
+  const SharedPlan p = plan_shared(sh, shared_blocks);
+  char* const ws = static_cast<char*>(workspace);
+  size_t ml_at;
+  const size_t pre = prefix_bytes(sh, p, &ml_at);
+  StreamScratch sc;
+  stream_bytes(sh, p.workers, &sc, ws + pre);
+  StreamArgs sa{};
+  sa.out = output;
+  sa.part_acc = sc.acc;
+  sa.part_ml = sc.ml;
+  sa.seg_desc = sc.desc;
+  sa.scale_log2 = scale * kLog2e;
+  sa.num_heads = num_heads;
+  sa.num_kv_heads = num_kv_heads;
+  sa.bs_shift = block_shift(block_size);
+  sa.max_blocks = max_blocks_per_seq << sa.bs_shift;
+  sa.batch = batch_size;
+  sa.num_workers = p.workers;
+  sa.kv_stride = kv_stride;
+  sa.table_stride = max_blocks_per_seq;
+  sa.prefix = shared_blocks * block_size;
+  PrefixArgs pa{};
+  pa.acc = reinterpret_cast<float*>(ws);
+  pa.ml = reinterpret_cast<float*>(ws + ml_at);
+  pa.scale_log2 = sa.scale_log2;
+  pa.group = num_heads / num_kv_heads;
+  pa.num_heads = num_heads;
+  pa.num_kv_heads = num_kv_heads;
+  pa.rows = p.rows;
+  pa.prefix = sa.prefix;
+  pa.subs = sa.prefix / kBS;
+  pa.tiles = p.tiles;
+  pa.split_tiles = p.split_tiles;
+  pa.splits = p.splits;
+  pa.bs_shift = sa.bs_shift;
+  pa.stream_groups = p.stream_groups;
+  pa.kv_stride = kv_stride;
+  const int64_t groups = p.stream_groups + (int64_t)num_kv_heads * p.splits * p.row_tiles;
+  if (groups > INT32_MAX) return fail(RG_ERR_NOT_SUPPORTED, "%s: %lld workgroups", op, (long long)groups);
+  hipStream_t s = as_stream(stream);
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    if (head_dim == 128) launch_shared<T, 128>(sa, pa, pa.group, (int)groups, query, key_cache, value_cache, block_table, context_lens, s);
+    else launch_shared<T, 64>(sa, pa, pa.group, (int)groups, query, key_cache, value_cache, block_table, context_lens, s);
+    return check_launch(op);
+  };
+  return dtype == RG_DTYPE_BF16 ? go(bf16_t{}) : go(f16_t{});
+}

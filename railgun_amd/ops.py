@@ -211,6 +211,25 @@ class PagedAttentionKernels:
             context_lens.data_ptr(), output.data_ptr(), float(scale), num_heads, num_kv_heads, head_dim,
             block_size, max_blocks_per_seq, batch_size, dtype_code(query), key_cache.stride(0), _stream(query)))
 
+    def shared_prefix_workspace_bytes(self, batch_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                      block_size: int, max_blocks_per_seq: int, shared_blocks: int) -> int:
+        return int(self.lib.rg_paged_attention_shared_prefix_workspace_bytes(
+            batch_size, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, shared_blocks))
+
+    def launch_shared_prefix(self, query, key_cache, value_cache, block_table, context_lens, output, scale: float,
+                             num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                             max_blocks_per_seq: int, batch_size: int, shared_blocks: int,
+                             workspace: torch.Tensor) -> None:
+        """launch_v1 for a batch whose rows of ``block_table`` begin with the same ``shared_blocks``
+        entries: those blocks are read once for many rows (rg_paged_attention_shared_prefix)."""
+        _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, workspace)
+        _require_i32(block_table, context_lens)
+        check(self.lib.rg_paged_attention_shared_prefix(
+            query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+            context_lens.data_ptr(), output.data_ptr(), float(scale), num_heads, num_kv_heads, head_dim, block_size,
+            max_blocks_per_seq, batch_size, shared_blocks, dtype_code(query), key_cache.stride(0),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(query)))
+
     def v1_scores_workspace_bytes(self, batch_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
                                   block_size: int, max_blocks_per_seq: int) -> int:
         return int(self.lib.rg_paged_attention_v1_scores_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim,
@@ -533,6 +552,21 @@ class PagedAttentionOp:
         if block_table.dim() != 2 or int(block_table.shape[0]) != batch or int(context_lens.numel()) != batch:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "block_table and context_lens need one row per sequence")
         return batch, heads, d, bs, int(block_table.shape[1])
+
+    def execute_shared_prefix(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                              block_table: torch.Tensor, context_lens: torch.Tensor, shared_blocks: int,
+                              workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """execute() for sequences whose block tables begin with the same ``shared_blocks`` entries
+        (launch_shared_prefix); the workspace is allocated here when omitted."""
+        batch, heads, d, bs, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
+        out = torch.empty_like(q)
+        k = self.kernels
+        if workspace is None:
+            workspace = torch.empty(k.shared_prefix_workspace_bytes(batch, heads, self.num_kv_heads, d, bs, mb,
+                                                                    shared_blocks), dtype=torch.uint8, device=q.device)
+        k.launch_shared_prefix(q, k_cache, v_cache, block_table, context_lens, out, self.scale, heads,
+                               self.num_kv_heads, d, bs, mb, batch, shared_blocks, workspace)
+        return out
 
     def execute_with_scores(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                             block_table: torch.Tensor, context_lens: torch.Tensor, scores: torch.Tensor,

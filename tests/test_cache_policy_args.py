@@ -107,3 +107,41 @@ def test_scores_workspace_bytes():
     f = railgun_amd.load_library().rg_paged_attention_v1_scores_workspace_bytes
     assert f(3, 8, 2, 64, 16, 4) > 3 * 8 * 64 * 4 and f(3, 8, 2, 64, 16, 4) % 256 == 0
     assert f(0, 8, 2, 64, 16, 4) == f(3, 7, 2, 64, 16, 4) == f(3, 8, 2, 64, 16, 0) == 0
+
+
+def shared(**change):
+    a = dict(q=P, k=P, v=P, table=P, lens=P, out=P, scale=0.125, heads=8, kv_heads=2, d=64, bs=16, mb=4, batch=3,
+             shared_blocks=2, dtype=_lib.RG_DTYPE_BF16, kv_stride=0, ws=P, ws_bytes=1 << 30, stream=None)
+    assert set(change) <= set(a)
+    return call("rg_paged_attention_shared_prefix", *{**a, **change}.values())
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=9), UNSUPPORTED, "unknown dtype"),
+    (dict(d=66), UNSUPPORTED, "multiple of 4"),
+    (dict(d=260), UNSUPPORTED, "multiple of 4"),
+    (dict(heads=7), INVALID, "not a multiple"),
+    (dict(bs=0), INVALID, "block_size"),
+    (dict(batch=-1), INVALID, "batch"),
+    (dict(shared_blocks=-1), INVALID, "shared_blocks"),
+    (dict(shared_blocks=5), INVALID, "shared_blocks"),
+    (dict(kv_stride=2 * 16 * 64 - 1), INVALID, "kv_block_stride"),
+    (dict(mb=2**31 - 1), UNSUPPORTED, "block table of"),
+    (dict(batch=65536), UNSUPPORTED, "sequences"),
+    (dict(q=None), INVALID, "null pointer"),
+    (dict(table=None), INVALID, "null pointer"),
+    (dict(out=None), INVALID, "null pointer"),
+    (dict(ws=None), WORKSPACE, "required"),
+    (dict(ws_bytes=1000), WORKSPACE, "required"),
+    (dict(ws=P // 16 * 16 + 4), WORKSPACE, "aligned"),
+    (dict(batch=0), _lib.RG_OK, ""),
+])
+def test_shared_prefix_arguments(change, code, text):
+    st, msg = shared(**change)
+    assert st == code and text in msg, msg
+
+
+def test_shared_prefix_workspace_bytes():
+    f = railgun_amd.load_library().rg_paged_attention_shared_prefix_workspace_bytes
+    assert f(3, 8, 2, 64, 16, 40, 20) >= railgun_amd.load_library().rg_paged_attention_v1_workspace_bytes(3, 8, 2, 64, 16, 40)
+    assert f(0, 8, 2, 64, 16, 4, 2) == f(3, 7, 2, 64, 16, 4, 2) == f(3, 8, 2, 64, 16, 4, 5) == 0
