@@ -64,176 +64,223 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kSelBins = 2048;
-constexpr int kSelHeldMost = 32768;  // keys held in LDS: 128 KB beside the 16.5 KB of the tables
-constexpr int kSelGroup = 64;  // strips of kSelThreads candidates whose counts are scanned together
 
-// Inclusive prefix sum over the wave, and the exclusive one over the workgroup's threads
-// (part: kSelWaves words of LDS; ends behind a barrier).
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o, 64);
-    if (lane >= o) v += t;
-  }
+// Inclusive prefix sum over the 64 lanes with DPP: within each row of 16 lanes by shifts of 1, 2, 4 and 8, then
+// lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
-__device__ __forceinline__ int block_scan_excl(int v, int lane, int w, int* part) {
-  const int incl = wave_scan(v, lane);
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+// Sum over the threads before this one; `all`: over the workgroup.  part: NW words of LDS that no thread
+// still reads; holds a barrier.
+template <int NW>
+__device__ __forceinline__ int block_before(int v, int lane, int w, int* part, int& all) {
+  const int incl = wave_scan(v);
   if (lane == 63) part[w] = incl;
   __syncthreads();
-  int before = 0;
-  for (int i = 0; i < w; ++i) before += part[i];
+  const int waves = wave_scan(lane < NW ? part[lane] : 0);
+  all = __builtin_amdgcn_readlane(waves, 63);
+  const int before = w > 0 ? __builtin_amdgcn_readlane(waves, w - 1) : 0;
   return before + incl - v;
 }
 
-// HELD: the candidates' keys are held in LDS (dynamic, one word each), so the scores are read once;
-// longer tables read them again in each pass.
-template <bool HELD>
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  extern __shared__ uint32_t held[];
-  __shared__ int hist[kSelBins];
-  __shared__ int part[kSelWaves];
-  __shared__ int found[2];               // digit, candidates above it
-  __shared__ int strip[2][kSelThreads];  // per (strip, wave): candidates above T, candidates at T
+// NT threads.  VPT > 0: every candidate's key sits in a register (thread t holds candidates t, t + NT, ...: VPT
+// of them), and the scores are read once.  VPT 0: longer tables read them again in each pass.
+//   Measured (16 layers x 16 sequences x 8 kv-heads, 1,500 to 4,096 tokens each; two segments of 48 KB of
+// scores): see the launch.
+template <int NT, int VPT>
+__global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
+  constexpr int NW = NT / 64;
+  constexpr int NR = VPT > 0 ? VPT : 1;
+  constexpr int GROUP = VPT > 0 ? VPT : 64;  // strips of NT candidates whose counts are scanned together
+  constexpr int BPT = kSelBins / NT;         // bins a thread scans
+  constexpr int EPT = (GROUP * NW + NT - 1) / NT;  // (strip, wave) counts a thread scans
+  __shared__ __attribute__((aligned(16))) int hist[kSelBins];
+  __shared__ int part[2][NW];
+  __shared__ int found[3];                          // digit, candidates above it, candidates at it
+  __shared__ int strip[2][GROUP * NW];              // per (strip, wave): candidates above T, candidates at T
   __shared__ int first_hole, alias;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Segment sg = segment_of(a, blockIdx.x);
   const int n = context_of(a, sg.seq);
   const int m = min(n, a.budget);
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.kept_stride;
   const int32_t* row = a.table + (int64_t)sg.seq * a.max_blocks;
   if (a.new_lens != nullptr && sg.layer == 0 && sg.kvh == 0 && tid == 0) a.new_lens[sg.seq] = m;
-  for (int i = m + tid; i < a.kept_stride; i += kSelThreads) kept[i] = -1;
+  for (int i = m + tid; i < a.kept_stride; i += NT) kept[i] = -1;
   if (n <= a.budget) {
-    for (int i = tid; i < n; i += kSelThreads) kept[i] = i;
+    for (int i = tid; i < n; i += NT) kept[i] = i;
     if (tid == 0) a.in_order[blockIdx.x] = 0;
     return;
   }
   const int p0 = a.guarded;
   const int count = n - a.recent - p0;           // candidates, positions p0 ..
   const int take = a.budget - a.recent - p0;     // of which this many stay: 0 <= take < count
-  for (int i = tid; i < p0; i += kSelThreads) kept[i] = i;
-  for (int i = tid; i < a.recent; i += kSelThreads) kept[m - a.recent + i] = n - a.recent + i;
+  const int strips = (count + NT - 1) / NT;
+
+  const float* cells = a.scores + sg.layer * a.score_layer_stride + (int64_t)sg.kvh * a.block_size;
+  auto read_key = [&](int c) -> uint32_t {
+    const uint32_t p = p0 + c, b = p / (uint32_t)a.block_size;
+    return order_key(cells[row[b] * a.score_stride + (p - b * (uint32_t)a.block_size)]);
+  };
+  uint32_t key[NR] = {};
+  if constexpr (VPT > 0) {
+    // (A table entry, then the score it leads to: two round trips, shared by U candidates.)
+    constexpr int U = VPT < 8 || VPT > 16 ? 4 : 8;  // (four with the registers all taken)
+#pragma unroll
+    for (int i0 = 0; i0 < VPT; i0 += U) {
+      if (i0 < strips) {
+#pragma unroll
+        for (int i = i0; i < i0 + U; ++i) key[i] = read_key(min(i * NT + tid, count - 1));
+      }
+#pragma unroll
+      for (int i = i0; i < i0 + U; ++i) {
+        key[i] = i * NT + tid < count ? key[i] : 0u;
+        asm volatile("" : "+v"(key[i]));  // (finished here, not kept as a score and a condition)
+      }
+    }
+  }
+  for (int i = tid; i < a.recent; i += NT) kept[m - a.recent + i] = n - a.recent + i;
+  for (int i = tid; i < p0; i += NT) kept[i] = i;
   if (tid == 0) {
     first_hole = n;
     alias = 0;
   }
-
-  auto read_key = [&](int c) -> uint32_t {
-    const int p = p0 + c;
-    return order_key(a.scores[score_cell(a, sg, row[p / a.block_size], p % a.block_size)]);
-  };
-  // (A thread reads back only keys that it wrote itself.)
-  if constexpr (HELD) {
-    // (A table entry, then the score it leads to: two round trips, shared by eight candidates.)
-    for (int c0 = tid; c0 < count; c0 += 8 * kSelThreads) {
-      uint32_t k[8];
+  // f(strip within the group, candidate, key) over strips g0 .. g0 + gs - 1, the whole wave at once.  The key
+  // of what is no candidate is 0, below every score's.
+  auto each = [&](int g0, int gs, auto f) __attribute__((always_inline)) {
+    if constexpr (VPT > 0) {
+      // (Opaque copies: comparisons are made where they are needed, not kept as masks from call to call.)
+      asm volatile("" : "+s"(gs));
+      int t = tid;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = read_key(min(c0 + i * kSelThreads, count - 1));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (c0 + i * kSelThreads < count) held[c0 + i * kSelThreads] = k[i];
+      for (int i = 0; i < VPT; ++i) {
+        uint32_t k = key[i];
+        asm volatile("" : "+v"(k), "+v"(t));
+        if (i < gs) f(i, i * NT + t, k);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < gs; ++i) {
+        const int c = (g0 + i) * NT + tid;
+        const uint32_t k = read_key(min(c, count - 1));
+        f(i, c, c < count ? k : 0u);
       }
     }
-  }
-  auto key_at = [&](int c) -> uint32_t {
-    if constexpr (HELD) return held[c];
-    else return read_key(c);
   };
 
-  // T: the key of the take-th largest candidate; `left` of those at T are kept.
+  // T: the key of the take-th largest candidate, or below it and above every key that is not kept; `left` of
+  // those at T are kept, the lowest positions first.
   uint32_t T = 0xffffffffu;  // (above every key: nothing kept)
   int left = 0;
+  bool whole = false;  // every candidate at or above T is kept
   if (take > 0) {
     T = 0;
     left = take;
-    const int shifts[3] = {21, 10, 0};
+    constexpr int shifts[4] = {32, 21, 10, 0};
 #pragma unroll
     for (int ps = 0; ps < 3; ++ps) {
-      const int sh = shifts[ps];
-      const uint32_t bins = ps == 2 ? 1024u : 2048u;
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+      if (whole) break;
+      const int sh = shifts[ps + 1], hi = shifts[ps];  // bits from hi on are settled
+      for (int i = 4 * tid; i < kSelBins; i += 4 * NT) *reinterpret_cast<int4*>(&hist[i]) = make_int4(0, 0, 0, 0);
       __syncthreads();
-      const int hi = ps == 0 ? 32 : shifts[ps - 1];  // bits from here on are settled
-      for (int c = tid; c < count; c += kSelThreads) {
-        const uint32_t k = key_at(c);
-        if (ps == 0 || (k >> hi) == (T >> hi)) atomicAdd(&hist[(k >> sh) & (bins - 1)], 1);
+      each(0, strips, [&](int, int, uint32_t k) __attribute__((always_inline)) {
+        if (k != 0 && (ps == 0 || (k >> (hi & 31)) == (T >> (hi & 31))))
+          atomicAdd(&hist[(k >> sh) & (ps == 2 ? 1023u : 2047u)], 1);
+      });
+      __syncthreads();
+      // Candidates in higher bins; BPT bins a thread, from the top.
+      int h[BPT], sum = 0;
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        h[i] = hist[kSelBins - 1 - tid * BPT - i];
+        sum += h[i];
       }
-      __syncthreads();
-      // Candidates in bins above, two bins a thread from the top.
-      const int b1 = kSelBins - 1 - 2 * tid, b0 = b1 - 1;
-      const int h1 = hist[b1], h0 = hist[b0];
-      const int above = block_scan_excl(h1 + h0, lane, w, part);
-      if (above < left && left <= above + h1) {
-        found[0] = b1;
-        found[1] = above;
-      } else if (above + h1 < left && left <= above + h1 + h0) {
-        found[0] = b0;
-        found[1] = above + h1;
+      int all;
+      int above = block_before<NW>(sum, lane, w, part[ps & 1], all);
+      if (above < left && left <= above + sum) {
+#pragma unroll
+        for (int i = 0; i < BPT; ++i) {
+          if (above < left && left <= above + h[i]) {
+            found[0] = kSelBins - 1 - tid * BPT - i;
+            found[1] = above;
+            found[2] = h[i];
+          }
+          above += h[i];
+        }
       }
       __syncthreads();
       T |= (uint32_t)found[0] << sh;
       left -= found[1];
-      __syncthreads();
+      whole = found[2] == left;  // the digit's candidates are all kept: no need to part them further
     }
   }
 
-  // The kept candidates in order.  Strip i holds candidates i * kSelThreads ..; the counts of
-  // every (strip, wave) of a group go to LDS and are scanned at once.
+  // The kept candidates in order: the counts of every (strip, wave) of a group go to LDS and are scanned.
+  const uint32_t above_T = whole ? T - 1 : T, at_T = whole ? 0xffffffffu : T;  // (no key is 0xffffffff)
+  const int ties = whole ? 0 : left;
   int gt_before = 0, eq_before = 0;  // in the groups before
-  const int strips = (count + kSelThreads - 1) / kSelThreads;
   int hole = n;
-  for (int g0 = 0; g0 < strips; g0 += kSelGroup) {
-    const int gs = min(kSelGroup, strips - g0);
-    __syncthreads();
-    for (int i = 0; i < gs; ++i) {
-      const int c = (g0 + i) * kSelThreads + tid;
-      const bool in = c < count;
-      const uint32_t k = in ? key_at(c) : 0u;
-      const int gt = __popcll(__ballot(in && k > T)), eq = __popcll(__ballot(in && k == T));
+  for (int g0 = 0; g0 < strips; g0 += GROUP) {
+    const int gs = min(GROUP, strips - g0);
+    if (g0 > 0) __syncthreads();
+    each(g0, gs, [&](int i, int, uint32_t k) __attribute__((always_inline)) {
+      const int gt = __popcll(__ballot(k > above_T)), eq = __popcll(__ballot(k == at_T));
       if (lane == 0) {
-        strip[0][i * kSelWaves + w] = gt;
-        strip[1][i * kSelWaves + w] = eq;
+        strip[0][i * NW + w] = gt;
+        strip[1][i * NW + w] = eq;
       }
+    });
+    __syncthreads();
+    int gt[EPT], eq[EPT], gsum = 0, esum = 0;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int e = tid * EPT + i;
+      gt[i] = e < gs * NW ? strip[0][e] : 0;
+      eq[i] = e < gs * NW ? strip[1][e] : 0;
+      gsum += gt[i];
+      esum += eq[i];
+    }
+    int gall, eall = 0, ge, ee = 0;
+    ge = gt_before + block_before<NW>(gsum, lane, w, part[1], gall);
+    if (!whole) ee = eq_before + block_before<NW>(esum, lane, w, part[0], eall);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int e = tid * EPT + i;
+      if (e < gs * NW) {
+        strip[0][e] = ge;
+        strip[1][e] = ee;
+      }
+      ge += gt[i];
+      ee += eq[i];
     }
     __syncthreads();
-    const bool have = tid < gs * kSelWaves;
-    const int gt = have ? strip[0][tid] : 0, eq = have ? strip[1][tid] : 0;
-    const int gt_ex = block_scan_excl(gt, lane, w, part);
-    int gt_all = 0;
-    for (int i = 0; i < kSelWaves; ++i) gt_all += part[i];
-    __syncthreads();
-    const int eq_ex = block_scan_excl(eq, lane, w, part);
-    int eq_all = 0;
-    for (int i = 0; i < kSelWaves; ++i) eq_all += part[i];
-    strip[0][tid] = gt_before + gt_ex;
-    strip[1][tid] = eq_before + eq_ex;
-    __syncthreads();
-    auto below = [&](uint64_t x) {
-      return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(x >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)x, 0));
-    };
-    for (int i = 0; i < gs; ++i) {
-      const int c = (g0 + i) * kSelThreads + tid;
-      const bool in = c < count;
-      const uint32_t k = in ? key_at(c) : 0u;
-      const bool is_gt = in && k > T, is_eq = in && k == T;
-      const int g = strip[0][i * kSelWaves + w] + below(__ballot(is_gt));
-      const int e = strip[1][i * kSelWaves + w] + below(__ballot(is_eq));
-      if (is_gt || (is_eq && e < left)) kept[p0 + g + min(e, left)] = p0 + c;
-      else if (in) hole = min(hole, p0 + c);
-    }
-    gt_before += gt_all;
-    eq_before += eq_all;
+    each(g0, gs, [&](int i, int c, uint32_t k) __attribute__((always_inline)) {
+      const bool is_gt = k > above_T, is_eq = k == at_T;
+      const int g = strip[0][i * NW + w] + lanes_below(__ballot(is_gt));
+      const int e = strip[1][i * NW + w] + lanes_below(__ballot(is_eq));
+      if (is_gt || (is_eq && e < ties)) kept[p0 + g + min(e, ties)] = p0 + c;
+      else if (k != 0) hole = min(hole, p0 + c);
+    });
+    gt_before += gall;
+    eq_before += eall;
   }
   // Rows from the first hole on move.  Where a block that receives them is also the block they may
   // come from (the same entry of both tables: eviction in place), the chunks go in order.
   atomicMin(&first_hole, hole);
   __syncthreads();
   const int32_t* drow = a.dst_table + (int64_t)sg.seq * a.max_dst_blocks;
-  for (int i = first_hole / a.block_size + tid; i < (m + a.block_size - 1) / a.block_size; i += kSelThreads) {
+  for (int i = first_hole / a.block_size + tid; i < (m + a.block_size - 1) / a.block_size; i += NT) {
     if (row[i] == drow[i]) alias = 1;
   }
   __syncthreads();
@@ -325,7 +372,7 @@ size_t evict_bytes(int64_t segments, int64_t budget, bool own_list) {
 
 int probe_evict_kernels() {
   hipFuncAttributes at;
-  if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_select_kernel<true>)) != hipSuccess ||
+  if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_select_kernel<256, 16>)) != hipSuccess ||
       hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_move_kernel<rg_u32x4_t>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the eviction kernels: %s", hipGetErrorString(hipGetLastError()));
   }
@@ -426,11 +473,12 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   a.batch = batch_size;
   hipStream_t s = as_stream(stream);
   const dim3 sel((unsigned)segments);
-  if (table_tokens <= kSelHeldMost) {
-    hipLaunchKernelGGL(evict_select_kernel<true>, sel, dim3(kSelThreads), (size_t)table_tokens * 4, s, a);
-  } else {
-    hipLaunchKernelGGL(evict_select_kernel<false>, sel, dim3(kSelThreads), 0, s, a);
-  }
+  auto select = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, sel, dim3(threads), 0, s, a); };
+  if (table_tokens <= 256 * 4) select(evict_select_kernel<256, 4>, 256);
+  else if (table_tokens <= 256 * 16) select(evict_select_kernel<256, 16>, 256);
+  else if (table_tokens <= 1024 * 16) select(evict_select_kernel<1024, 16>, 1024);
+  else if (table_tokens <= 1024 * 64) select(evict_select_kernel<1024, 64>, 1024);
+  else select(evict_select_kernel<1024, 0>, 1024);
   int st = check_launch(op);
   if (st != RG_OK || most == 0) return st;
   // Rows move in 16-byte pieces where every row starts on one, else in 2-byte ones.
