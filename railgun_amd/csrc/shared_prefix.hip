@@ -54,7 +54,8 @@ constexpr float kSlack = 8.f;             // log2 headroom of the lazy maximum: 
 struct PrefixArgs {
   float* acc;  // [H_kv, splits, rows, D] unnormalised
   float* ml;   // [H_kv, splits, rows, 2]: m in log2 units, l
-  float scale_log2;
+  float scale_log2;  // > 0
+  uint32_t q_sign;   // bit 0: q is taken (else zeros, a scale of 0), bits 15 and 31: negated (a negative scale)
   int32_t group, num_heads, num_kv_heads, rows;  // rows = batch * group
   int32_t prefix, subs;                          // prefix tokens, and its 16-token sub-blocks
   int32_t tiles, split_tiles, splits;
@@ -112,6 +113,11 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
     const uint4* qr = reinterpret_cast<const uint4*>(q + ((int64_t)b * a.num_heads + (int64_t)kvh * a.group + g) * D);
 #pragma unroll
     for (int i = 0; i < NKC; ++i) qb[i] = qr[2 * i + hh];
+    // scale_log2 > 0 here: the host passes its magnitude (1 for a scale of 0) and what becomes of q.
+    const uint32_t flip = a.q_sign & 0x80008000u, on = a.q_sign & 1 ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int i = 0; i < NKC; ++i)
+      qb[i] = make_uint4((qb[i].x ^ flip) & on, (qb[i].y ^ flip) & on, (qb[i].z ^ flip) & on, (qb[i].w ^ flip) & on);
   }
   // Rows whose context lacks part of the prefix are left to the stream-K workers: they compute along
   // (finite or not, no other lane's row sees it) and write nothing that the merge reads.
@@ -150,40 +156,67 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
+  float m_thr = -INFINITY;  // m_run + kSlack in raw score units, so a tile's test needs no multiply
   const int xor32 = (lane ^ 32) << 2;
   const int k_lane = (j >> 4) * (TL::KB / 2) + hh * 256 + (j & 15) * 16;
   const int grp = lane >> 4, e_row = (lane >> 2) & 3, qq = lane & 3;
 
-  // Tile kt from ring stage st.  S^T: c[v] is key 8 (v >> 2) + 4 hh + (v & 3) of the tile for query j.
-  auto compute = [&](int kt, int st) {
-    const char* kbase = lds + st * TL::BYTES + k_lane;
+  // A operand m = n NDB + db of the PV product (keys 16 n .., 32-dim block db) by the transposing LDS read: in
+  // each 16-lane group, lane 4 e + p points at V[key0 + e][d0 + 4 p ..] and lane i receives V[key0 ..][d0 + i].
+  auto v_operand = [&](const char* vbase, int m) {
+    const int n = m / NDB, db = m % NDB;
+    const int d = 32 * db + 16 * (grp & 1) + 4 * qq;
+    uint2 part[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = 16 * n + 8 * half + 4 * (grp >> 1) + e_row;
+      const int off = key * (D * 2) + TL::vchunk(key, d >> 3) * 16 + (d & 7) * 2;
+      part[half] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((RG_LDS v4i16_t*)(vbase + off)));
+    }
+    return make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+  };
+  constexpr int KA = NKC < 4 ? NKC : 4;          // K operands read ahead of their MFMA
+  constexpr int VA = 2 * NDB < 3 ? 2 * NDB : 3;  // V operands, the first of them before the softmax
+  // Tile kt from ring stage ST.  S^T: c[v] is key 8 (v >> 2) + 4 hh + (v & 3) of the tile for query j.
+  auto scores = [&](int kt, auto stc) __attribute__((always_inline)) -> f32x16_t {
+    const char* kbase = lds + decltype(stc)::value * TL::BYTES + k_lane;
+    uint4 ka[KA];
+#pragma unroll
+    for (int i = 0; i < KA; ++i) ka[i] = *reinterpret_cast<const uint4*>(kbase + i * 512);
     f32x16_t c;
 #pragma unroll
     for (int v = 0; v < 16; ++v) c[v] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NKC; ++i) c = MF::run(*reinterpret_cast<const uint4*>(kbase + i * 512), qb[i], c);
+    for (int i = 0; i < NKC; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      c = MF::run(ka[i % KA], qb[i], c);
+      if (i + KA < NKC) ka[i % KA] = *reinterpret_cast<const uint4*>(kbase + (i + KA) * 512);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    return c;
+  };
+  auto finish = [&](int kt, f32x16_t c, auto stc) __attribute__((always_inline)) {
+    const char* vbase = lds + decltype(stc)::value * TL::BYTES + TL::KB;
+    uint4 va[VA];
+#pragma unroll
+    for (int m = 0; m < VA; ++m) va[m] = v_operand(vbase, m);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     if (2 * kt + 1 >= a.subs) {  // an odd number of sub-blocks: the last tile's second half repeats one
 #pragma unroll
       for (int v = 8; v < 16; ++v) c[v] = -INFINITY;
     }
-    // The maximum moves only when a tile exceeds it by more than kSlack, for both halves of a row alike;
-    // it is that of the scaled scores, whatever the scale's sign.
-    float x[16];
+    // The maximum moves only when a tile exceeds it by more than kSlack, for both halves of a row alike.
+    float tmax = c[0];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) x[v] = c[v] * a.scale_log2;
-    if (2 * kt + 1 >= a.subs) {
-#pragma unroll
-      for (int v = 8; v < 16; ++v) x[v] = -INFINITY;
-    }
-    float tmax = x[0];
-#pragma unroll
-    for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, x[v]);
-    if (__ballot(tmax > m_run + kSlack)) {
+    for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, c[v]);
+    if (__ballot(tmax > m_thr)) {
       const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)));
-      const float both = fmaxf(tmax, other);
+      const float both = fmaxf(tmax, other) * a.scale_log2;
       const float m_new = both > m_run + kSlack ? both : m_run;
       const float alpha = fast_exp2(m_run - m_new);
       m_run = m_new;
+      m_thr = (m_run + kSlack) / a.scale_log2;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -194,49 +227,62 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
     // the normaliser weighs what enters the product.
     uint32_t pk[8];
 #pragma unroll
-    for (int v = 0; v < 16; v += 2) pk[v / 2] = pack2<T>(fast_exp2(x[v] - m_run), fast_exp2(x[v + 1] - m_run));
+    for (int v = 0; v < 16; v += 2)
+      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, -m_run)), fast_exp2(fmaf(c[v + 1], a.scale_log2, -m_run)));
+    float s0 = pair_sum<T>(pk[0], l_run), s1 = pair_sum<T>(pk[1], 0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) l_run = pair_sum<T>(pk[i], l_run);
-    const char* vbase = lds + st * TL::BYTES + TL::KB;
+    for (int i = 2; i < 8; i += 2) {
+      s0 = pair_sum<T>(pk[i], s0);
+      s1 = pair_sum<T>(pk[i + 1], s1);
+    }
+    l_run = s0 + s1;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int m = 0; m < 2 * NDB; ++m) {
       const int n = m / NDB, db = m % NDB;
-      const int d = 32 * db + 16 * (grp & 1) + 4 * qq;
-      uint2 part[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int key = 16 * n + 8 * half + 4 * (grp >> 1) + e_row;
-        const int off = key * (D * 2) + TL::vchunk(key, d >> 3) * 16 + (d & 7) * 2;
-        part[half] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((RG_LDS v4i16_t*)(vbase + off)));
-      }
-      o[db] = MF::run(make_uint4(part[0].x, part[0].y, part[1].x, part[1].y),
-                      make_uint4(pk[4 * n], pk[4 * n + 1], pk[4 * n + 2], pk[4 * n + 3]), o[db]);
+      __builtin_amdgcn_sched_barrier(0);
+      o[db] = MF::run(va[m % VA], make_uint4(pk[4 * n], pk[4 * n + 1], pk[4 * n + 2], pk[4 * n + 3]), o[db]);
+      if (m + VA < 2 * NDB) va[m % VA] = v_operand(vbase, m + VA);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
   };
 
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the window and Q have landed: only copies count from here
+  // The window and Q have landed (the builtin, which the compiler's own counting follows: behind an asm
+  // wait it would wait for Q again in every tile, and with it for every copy in flight).
+  __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0)
 #pragma unroll
   for (int p = 0; p < kStages - 1; ++p)
     if (kt0 + p < kt1) issue(kt0 + p, p);
-  int st = 0;
-  for (int kt = kt0; kt < kt1; ++kt) {
-    // Tile kt has landed (a newer one may not have), for every wave; all are done with tile kt - 1, whose
-    // stage takes tile kt + kStages - 1.
-    if (kt + 1 < kt1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    static_assert(kStages == 3, "one tile newer than the awaited one");
+  // Tile kt has landed (a newer one may not have), for every wave; all are done with tile kt - 1, whose
+  // stage takes tile kt + kStages - 1.
+  auto step = [&](int kt, auto stc) __attribute__((always_inline)) {
+    constexpr int st = decltype(stc)::value;
+    static_assert(kStages == 3 && COPIES < 16, "one tile newer than the awaited one; low bits of vmcnt");
+    asm volatile("" ::: "memory");
+    if (kt + 1 < kt1) __builtin_amdgcn_s_waitcnt(COPIES | 0x70 | 0xF00);
+    else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
     tile_barrier();
     const int next = kt + kStages - 1;
-    if (next < kt1) {
-      if (next - wb >= 64) {
-        wb = next;
-        fill();
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      issue(next, st == 0 ? kStages - 1 : st - 1);
+    if (next - wb >= 64) {
+      wb = next;
+      fill();
+      __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
     }
-    if (busy) compute(kt, st);
-    st = st == kStages - 1 ? 0 : st + 1;
+    if (!busy) {
+      if (next < kt1) issue(next, st == 0 ? kStages - 1 : st - 1);
+      return;
+    }
+    __builtin_amdgcn_s_setprio(1);
+    const f32x16_t c = scores(kt, stc);
+    if (next < kt1) issue(next, st == 0 ? kStages - 1 : st - 1);  // while the QK MFMAs run
+    finish(kt, c, stc);
+  };
+  for (int kt = kt0; kt < kt1; kt += kStages) {
+    step(kt, std::integral_constant<int, 0>{});
+    if (kt + 1 < kt1) step(kt + 1, std::integral_constant<int, 1>{});
+    if (kt + 2 < kt1) step(kt + 2, std::integral_constant<int, 2>{});
   }
   if (row < a.rows) {
     const float l = l_run + __shfl_xor(l_run, 32, 64);
@@ -278,47 +324,64 @@ __global__ __launch_bounds__(kPreThreads) void shared_prefix_kernel(StreamArgs s
 
 // One workgroup per (kv-head, sequence), a wave per query head: lane l folds dims [l PER, (l + 1) PER) of the
 // prefix's splits (if the sequence has the whole prefix) and of the stream-K workers' partials, in that order.
+// A chain of memory round trips and little else, so the prefix's partials are asked for together with the
+// length and the segment's descriptor: they are there for every row, if only as numbers that do not count.
 template <typename T, int D, int G>
 __global__ __launch_bounds__(64 * G) void shared_merge_kernel(StreamArgs sa, PrefixArgs pa,
                                                               const int32_t* __restrict__ context_lens) {
   using S = typename elem<T>::storage;
   constexpr int PER = D / 64;
+  constexpr int AHEAD = 4;
   const int kvh = blockIdx.x, s = blockIdx.y, h = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int hkv = sa.num_kv_heads;
+  const int64_t seg = (int64_t)s * sa.num_kv_heads + kvh;
   S* out = static_cast<S*>(sa.out) + ((int64_t)s * sa.num_heads + (int64_t)kvh * G + h) * D + lane * PER;
-  const int ctx = max(0, min(context_lens[s], sa.max_blocks * kBS));
+  const int2 dsc = sa.seg_desc[seg];  // (stale, and not used, where the segment has no tokens of its own)
+  const int len = context_lens[s];
+  struct Part {
+    float2 ml;
+    float v[PER];
+  };
+  auto load = [&](const float* ml, const float* acc) __attribute__((always_inline)) {
+    Part p;
+    p.ml = *reinterpret_cast<const float2*>(ml);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) p.v[e] = acc[lane * PER + e];
+    return p;
+  };
+  const int64_t r0 = (int64_t)kvh * pa.splits * pa.rows + s * G + h;
+  auto split = [&](int p) __attribute__((always_inline)) {
+    const int64_t r = r0 + (int64_t)min(p, pa.splits - 1) * pa.rows;
+    return load(pa.ml + 2 * r, pa.acc + r * D);
+  };
   float m = -INFINITY, l = 0.f;
   float acc[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-  auto fold = [&](float2 ml, const float* pa_row) __attribute__((always_inline)) {
-    float v[PER];
+  auto fold = [&](const Part& p, bool counts) __attribute__((always_inline)) {
+    const float x = counts ? p.ml.x : -INFINITY;
+    const float mn = fmaxf(m, x);
+    const float fo = m == -INFINITY ? 0.f : exp2f(m - mn), fq = counts ? exp2f(x - mn) : 0.f;
+    l = l * fo + (counts ? p.ml.y : 0.f) * fq;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = pa_row[e];
-    const float mn = fmaxf(m, ml.x);
-    const float fo = exp2f(m - mn), fq = exp2f(ml.x - mn);
-    l = l * fo + ml.y * fq;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = acc[e] * fo + v[e] * fq;
-    m = mn;
+    for (int e = 0; e < PER; ++e) acc[e] = acc[e] * fo + (counts ? p.v[e] : 0.f) * fq;
+    m = counts ? mn : m;
   };
-  if (ctx >= sa.prefix) {
-    const int64_t r0 = (int64_t)kvh * pa.splits * pa.rows + s * G + h;
+  Part first[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) first[i] = split(i);
+  const int ctx = max(0, min(len, sa.max_blocks * kBS));
+  const bool has = ctx >= sa.prefix;
+  const int np = past_prefix(ctx, sa.prefix) > 0 ? dsc.y : 0;
+  const int64_t p0 = dsc.x + seg;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fold(first[i], has && i < pa.splits);
+  if (has) {
 #pragma unroll 4
-    for (int p = 0; p < pa.splits; ++p) {
-      const int64_t r = r0 + (int64_t)p * pa.rows;
-      fold(*reinterpret_cast<const float2*>(pa.ml + 2 * r), pa.acc + r * D + lane * PER);
-    }
+    for (int p = AHEAD; p < pa.splits; ++p) fold(split(p), true);
   }
-  if (past_prefix(ctx, sa.prefix) > 0) {
-    const int64_t seg = (int64_t)s * hkv + kvh;
-    const int2 dsc = sa.seg_desc[seg];
-    const int64_t p0 = dsc.x + seg;
 #pragma unroll 4
-    for (int p = 0; p < dsc.y; ++p) {
-      fold(*reinterpret_cast<const float2*>(sa.part_ml + (p0 + p) * (2 * G) + 2 * h),
-           sa.part_acc + (p0 + p) * (G * D) + h * D + lane * PER);
-    }
+  for (int p = 0; p < np; ++p) {
+    fold(load(sa.part_ml + (p0 + p) * (2 * G) + 2 * h, sa.part_acc + (p0 + p) * (G * D) + h * D), true);
   }
   const float inv = l != 0.f ? 1.f / l : 1.f;
 #pragma unroll
@@ -364,7 +427,17 @@ SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks) {
   p.rows = sh.B * (sh.H / sh.Hkv);
   p.row_tiles = (int32_t)ceil_div(p.rows, kPreRows);
   p.tiles = (int32_t)ceil_div(prefix, kTileKeys);
-  const int64_t want = std::max<int64_t>(1, device_cu_count() / ((int64_t)sh.Hkv * p.row_tiles));
+  // One workgroup of the product per CU beside the one of stream-K workers that its CU also holds.  Two where
+  // that leaves splits of many row tiles (few of them, then, for the merge to read) and the table leaves the
+  // sequences so little behind the prefix that the product (at 0.7 PFLOP/s) outlasts the workers (at 5 TB/s).
+  // Splits of fewer than 8 key tiles are not made: each writes 4 D bytes a row for the merge to read.
+  //   Measured (bf16, 32 / 8 heads of 128, us): 256 rows' 16,384 tokens with nothing behind them 113 with one,
+  // 93 with two, with 64 to 1,024 tokens behind them 177 and 189; 16 rows of 16,384 22.2 and 26.7; 16 rows of
+  // 2,048 with up to 700 behind them 18.7 with 8 tiles to a split, 21.7 with 2, 22.7 with 16.
+  const double product = 4.0 * sh.B * sh.H * sh.D * (double)prefix / 0.7e15;
+  const double stream = 4.0 * sh.B * sh.Hkv * sh.D * ((double)sh.MB * sh.bs - (double)prefix) / 5e12;
+  const int64_t one = std::max<int64_t>(1, device_cu_count() / ((int64_t)sh.Hkv * p.row_tiles));
+  const int64_t want = std::min(product > stream && one <= 8 ? 2 * one : one, ceil_div(p.tiles, 8));
   p.split_tiles = (int32_t)ceil_div(p.tiles, std::min<int64_t>(want, p.tiles));
   p.splits = (int32_t)ceil_div(p.tiles, p.split_tiles);
   p.workers = stream_workers(sh);
@@ -470,7 +543,9 @@ extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* k
   PrefixArgs pa{};
   pa.acc = reinterpret_cast<float*>(ws);
   pa.ml = reinterpret_cast<float*>(ws + ml_at);
-  pa.scale_log2 = sa.scale_log2;
+  // The product works with a positive scale: a negative one turns q's signs, 0 takes zeros for q.
+  pa.scale_log2 = scale != 0.f ? fabsf(sa.scale_log2) : 1.f;
+  pa.q_sign = scale == 0.f ? 0u : scale < 0.f ? 0x80008001u : 1u;
   pa.group = num_heads / num_kv_heads;
   pa.num_heads = num_heads;
   pa.num_kv_heads = num_kv_heads;
