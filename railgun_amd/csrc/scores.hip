@@ -36,6 +36,7 @@ struct ScoreArgs {
   int32_t first;
   int32_t num_heads, num_kv_heads, head_dim, block_size, max_blocks, num_partitions;
   int64_t score_stride;
+  int32_t merge_groups, merge_heads;  // workgroups of a segment that merge, and query heads to each (1 or 4)
 };
 
 template <typename T, int D, int G>
@@ -120,90 +121,153 @@ __global__ __launch_bounds__(64) void scores_generic_kernel(GenericArgs a) {
   }
 }
 
-// Workgroup (x, kv-head, sequence): x == 0 merges the segment's partials into its G output rows, the others
-// turn raw scores into weights, kFinTokens tokens at a time.  Each works out M and L of its G rows from the
-// partials' pairs itself (a few loads), so one launch does both.  GT: G, or 0 for one known at run time.
+// Workgroup (x, kv-head, sequence): the first merge_groups merge the partials of merge_heads query heads each
+// into their output rows, the others turn raw scores into weights, kFinTokens tokens at a time.  Each works out the maxima and sums it needs
+// from the partials' pairs itself (a few loads), so one launch does both.  The call is short against memory
+// latency: what does not depend on the pairs (the accumulators of the merge, the raw scores, the old ones) is
+// asked for before they are waited for.  GT: G, or 0 for one known at run time.
 template <typename T, int GT>
 __global__ __launch_bounds__(kFinThreads) void scores_finish_kernel(ScoreArgs a) {
   using E = elem<T>;
   using S = typename E::storage;
   constexpr int GL = GT > 0 ? GT : kMaxGroup;
+  constexpr int UNROLL = kFinTokens / kFinThreads;
   __shared__ float top[GL], inv[GL];
+  __shared__ float4 sums[kFinThreads];
   const int kvh = blockIdx.y, s = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int G = GT > 0 ? GT : a.num_heads / a.num_kv_heads;
   const int D = a.head_dim;
   const int64_t tokens = (int64_t)a.max_blocks * a.block_size;
   const int64_t seg = (int64_t)s * a.num_kv_heads + kvh;
+  const int2 desc = a.seg_desc != nullptr ? a.seg_desc[seg] : make_int2(0, 0);  // (with the length: one round trip)
   const int ctx = (int)max<int64_t>(0, min<int64_t>(a.context_lens[s], tokens));
+  const bool merges = (int)blockIdx.x < a.merge_groups;
   S* out = static_cast<S*>(a.out) + ((int64_t)s * a.num_heads + (int64_t)kvh * G) * D;
   if (ctx == 0) {
     if (blockIdx.x == 0)
       for (int i = tid; i < G * D; i += kFinThreads) E::store(out, i, 0.f);
     return;
   }
-  const int first = max(a.first, 0) + ((int)blockIdx.x - 1) * kFinTokens;
-  if (blockIdx.x > 0 && first >= ctx) return;
-  int64_t pbase;
-  int np;
-  if (a.seg_desc != nullptr) {
-    const int2 d = a.seg_desc[seg];
-    pbase = d.x + seg;
-    np = d.y;
-  } else {
-    pbase = seg * a.num_partitions;
-    np = (ctx + kGenTokens - 1) / kGenTokens;
-  }
+  const int64_t first = max(a.first, 0) + (int64_t)((int)blockIdx.x - a.merge_groups) * kFinTokens;
+  if (!merges && first >= ctx) return;
+  const int64_t pbase = a.seg_desc != nullptr ? desc.x + seg : seg * a.num_partitions;
+  const int np = a.seg_desc != nullptr ? desc.y : (ctx + kGenTokens - 1) / kGenTokens;
   const float* ml = a.part_ml + pbase * 2 * G;
-  for (int h = w; h < G; h += kFinWaves) {
-    float m = -INFINITY, l = 0.f;
-    for (int q = lane; q < np; q += 64) m = fmaxf(m, ml[((int64_t)q * G + h) * 2]);
-    m = wave_max(m);
-    for (int q = lane; q < np; q += 64) l += ml[((int64_t)q * G + h) * 2 + 1] * exp2f(ml[((int64_t)q * G + h) * 2] - m);
-    l = wave_sum(l);
-    if (lane == 0) {
-      top[h] = m;
-      inv[h] = l != 0.f ? 1.f / l : 1.f;
+  auto pair = [&](int q, int h) { return *reinterpret_cast<const float2*>(ml + ((int64_t)q * G + h) * 2); };
+  // Maximum and sum of head h over its partials, in every lane of the wave.
+  auto stats = [&](int h, float& m, float& l) {
+    m = -INFINITY;
+    l = 0.f;
+    for (int q0 = 0; q0 < np; q0 += 64) {
+      const float2 p = q0 + lane < np ? pair(q0 + lane, h) : make_float2(-INFINITY, 0.f);
+      const float mn = fmaxf(m, wave_max(p.x));
+      l = l * exp2f(m - mn) + wave_sum(p.y * exp2f(p.x - mn));
+      m = mn;
     }
-  }
-  __syncthreads();
-  if (blockIdx.x == 0) {
-    const float* acc = a.part_acc + pbase * G * D;
-    for (int i = tid; i < G * D; i += kFinThreads) {
-      const int h = i / D;
-      const float m = top[h];
-      float o = 0.f;
+  };
+  if (merges) {
+    // Whole waves to a head; in it four dims a thread, R partials at a time, their sums added in a fixed order.
+    const int per = kFinThreads / a.merge_heads, hw = tid / per, t = tid - hw * per;
+    const int h = min((int)blockIdx.x * a.merge_heads + hw, G - 1);
+    const int C = D / 4, R = per / C, c = t % C, r = t / C;
+    const float* acc = a.part_acc + (pbase * G + h) * D + 4 * c;
+    constexpr int AHEAD = 2;
+    float4 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int q = r + i * R;
+      v[i] = r < R && q < np ? *reinterpret_cast<const float4*>(acc + (int64_t)q * G * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float m, l;
+    stats(h, m, l);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float4 x, int q) {
+      const float f = exp2f(pair(q, h).x - m);
+      o.x += f * x.x;
+      o.y += f * x.y;
+      o.z += f * x.z;
+      o.w += f * x.w;
+    };
+    if (r < R) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (r + i * R < np) add(v[i], r + i * R);
 #pragma unroll 4
-      for (int q = 0; q < np; ++q) o += acc[(int64_t)q * G * D + i] * exp2f(ml[((int64_t)q * G + h) * 2] - m);
-      E::store(out, i, o * inv[h]);
+      for (int q = r + AHEAD * R; q < np; q += R) add(*reinterpret_cast<const float4*>(acc + (int64_t)q * G * D), q);
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (t < C && (int)blockIdx.x * a.merge_heads + hw < G) {
+      for (int i = 1; i < min(R, np); ++i) {
+        const float4 x = sums[tid + i * C];
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+      }
+      const float f = l != 0.f ? 1.f / l : 1.f;
+      S* row = out + (int64_t)h * D + 4 * t;
+      E::store(row, 0, o.x * f);
+      E::store(row, 1, o.y * f);
+      E::store(row, 2, o.z * f);
+      E::store(row, 3, o.w * f);
     }
     return;
   }
   const int scored = a.scored_lens != nullptr ? a.scored_lens[s] : INT32_MAX;
   const int32_t* bt = a.block_table + (int64_t)s * a.max_blocks;
   const float* lg = a.logits + seg * tokens * G;
-  const int64_t step = (int64_t)(gridDim.x - 1) * kFinTokens;
+  float* const cells = a.scores + (int64_t)kvh * a.block_size;
+  const int64_t step = (int64_t)(gridDim.x - a.merge_groups) * kFinTokens;
+  bool known = false;
   for (int64_t c0 = first; c0 < ctx; c0 += step) {
-#pragma unroll 4
-    for (int u = 0; u < kFinTokens / kFinThreads; ++u) {
-      const int64_t t = c0 + u * kFinThreads + tid;
-      if (t >= ctx) break;
-      float sum = 0.f;
+    // The chunk's cells, old scores and raw scores (a token past the end reads the last one's).
+    float* cell[UNROLL];
+    float old[UNROLL], raw[UNROLL][GT > 0 ? GT : 1];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int t = (int)min<int64_t>(c0 + u * kFinThreads + tid, ctx - 1), b = t / a.block_size;
+      cell[u] = cells + bt[b] * a.score_stride + (t - b * a.block_size);
       if constexpr (GT > 0 && GT % 4 == 0) {
 #pragma unroll
         for (int h = 0; h < GT; h += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(lg + t * GT + h);
-          sum += exp2f(x.x * a.scale_log2 - top[h]) * inv[h];
-          sum += exp2f(x.y * a.scale_log2 - top[h + 1]) * inv[h + 1];
-          sum += exp2f(x.z * a.scale_log2 - top[h + 2]) * inv[h + 2];
-          sum += exp2f(x.w * a.scale_log2 - top[h + 3]) * inv[h + 3];
+          const float4 x = *reinterpret_cast<const float4*>(lg + (int64_t)t * GT + h);
+          raw[u][h] = x.x;
+          raw[u][h + 1] = x.y;
+          raw[u][h + 2] = x.z;
+          raw[u][h + 3] = x.w;
         }
-      } else {
+      } else if constexpr (GT > 0) {
+#pragma unroll
+        for (int h = 0; h < GT; ++h) raw[u][h] = lg[(int64_t)t * GT + h];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) old[u] = *cell[u];
+    if (!known) {
+      for (int h = w; h < G; h += kFinWaves) {
+        float m, l;
+        stats(h, m, l);
+        if (lane == 0) {
+          top[h] = m;
+          inv[h] = l != 0.f ? 1.f / l : 1.f;
+        }
+      }
+      __syncthreads();
+      known = true;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t t = c0 + u * kFinThreads + tid;
+      float sum = 0.f;
+      if constexpr (GT > 0) {
+#pragma unroll
+        for (int h = 0; h < GT; ++h) sum += exp2f(raw[u][h] * a.scale_log2 - top[h]) * inv[h];
+      } else if (t < ctx) {
         for (int h = 0; h < G; ++h) sum += exp2f(lg[t * G + h] * a.scale_log2 - top[h]) * inv[h];
       }
-      const int b = (int)t / a.block_size;
-      float* cell = a.scores + bt[b] * a.score_stride + (int64_t)kvh * a.block_size + ((int)t - b * a.block_size);
-      *cell = t < scored ? *cell + sum : sum;
+      if (t < ctx) *cell[u] = t < scored ? old[u] + sum : sum;
     }
   }
 }
@@ -396,12 +460,15 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
       if (st != RG_OK) return st;
     }
   }
-  // One workgroup per segment for the output, and for the weights up to one per kFinTokens of the table but
-  // no more than some 8192 in all (they step on where the table is longer).
+  // The output: a workgroup per head where a segment has many partials (a worker of the grid each, so known
+  // here up to the contexts), one per four heads where it has few.  The weights: up to one per kFinTokens of the
+  // table but no more than some 8192 in all (they step on where the table is longer).
   const int64_t segments = (int64_t)batch_size * num_kv_heads;
+  f.merge_heads = (tiles ? workers / segments : f.num_partitions) >= 8 ? 1 : 4;
+  f.merge_groups = (int32_t)ceil_div(G, f.merge_heads);
   const int64_t scored = std::max<int64_t>(0, tokens - first_scored);
   const int64_t chunks = std::min(ceil_div(scored, kFinTokens), std::max<int64_t>(1, 8192 / segments));
-  const dim3 grid((unsigned)(1 + chunks), (unsigned)num_kv_heads, (unsigned)batch_size);
+  const dim3 grid((unsigned)(f.merge_groups + chunks), (unsigned)num_kv_heads, (unsigned)batch_size);
   return dispatch_dtype(dtype, [&](auto tag) {
     launch_finish<decltype(tag)>(f, G, grid, s);
     return check_launch(op);
