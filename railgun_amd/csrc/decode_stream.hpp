@@ -642,7 +642,7 @@ struct StreamArgs {
   const float* cos_sin;         // [positions, D]: cos at [d], sin at [D/2 + d]
   const int32_t* positions;     // [batch]
   const int32_t* slot_mapping;  // [batch]; negative: a padding token, not cached
-  // kScores: [batch, H_kv, 16 max_blocks tokens, G].
+  // kScores: [batch, H_kv, 16 max_blocks tokens, G], a (sequence, kv-head)'s below 4 GB.
   float* logits;
   // kSuffix: tokens of whole blocks, more than 0.
   int32_t prefix;
@@ -1065,12 +1065,11 @@ __device__ __forceinline__ void stream_worker(
     }
   };
 
-  // kScores: where this lane's raw scores of the segment's first token go (token tile.col, heads 4 seg ..).
-  // Kept in vector registers: the scalar ones are all taken.
+  // kScores: where the segment's raw scores go.  Kept in vector registers: the scalar ones are all taken.
   float* lg = nullptr;
   float* lg_all = nullptr;
   if constexpr (VAR == StreamVariant::kScores) {
-    lg_all = a.logits + tile.col * G + 4 * tile.seg;
+    lg_all = a.logits;
     asm volatile("" : "+v"(lg_all));
     lg = lg_all + ((int64_t)cur.s * hkv + cur.kvh) * a.max_blocks * (kBS * G);
   }
@@ -1137,20 +1136,24 @@ __device__ __forceinline__ void stream_worker(
       }
     }
     if constexpr (VAR == StreamVariant::kScores) {
+      // Stores that the buffer's bounds mask, not a branch: a store that may or may not have been issued would
+      // make the compiler wait for it whenever it waits for the loads issued before it.
       const int tok0 = cur.b * BPU * kBS;
+      auto* base = reinterpret_cast<float*>((uint64_t)uniform64(reinterpret_cast<int64_t>(lg)));
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)((uint32_t)ctx_cur * (G * 4)), 0x00020000);
       tile.template step<BPU>(kbuf[q], vbuf[q], tok0, ctx_cur, a.scale_log2, p_lds[j & 1], alpha_lds[j & 1],
                               [&](const f32x4_t (&c)[BPU]) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < BPU; ++b) {
-          if (tile.seg < HG && tok0 + b * kBS + tile.col < ctx_cur) {
-            float* const at = lg + (int64_t)(tok0 + b * kBS) * G;
-            if constexpr (G % 4 == 0) {
-              *reinterpret_cast<float4*>(at) = make_float4(c[b][0], c[b][1], c[b][2], c[b][3]);
-            } else {
+          const uint32_t at = ((uint32_t)(tok0 + b * kBS + tile.col) * G + 4 * tile.seg) * 4;
+          if constexpr (G % 4 == 0) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(rg_u32x4_t, c[b]), rsrc,
+                                                   tile.seg < HG ? at : ~15u, 0, 0);
+          } else {
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (4 * tile.seg + r < G) at[r] = c[b][r];
-            }
+            for (int r = 0; r < (G < 4 ? G : 4); ++r)
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(c[b][r]), rsrc,
+                                                    4 * tile.seg + r < G ? at + 4 * r : ~15u, 0, 0);
           }
         }
       });

@@ -388,7 +388,9 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
   }
   const int64_t kv_stride = kv_block_stride ? kv_block_stride : block * head_dim;
-  const bool tiles = max_blocks_per_seq > 0 && tiles_take(sh, dtype, kv_stride, query, key_cache, value_cache, output);
+  // (The workers address a segment's raw scores with 32 bits.)
+  const bool tiles = max_blocks_per_seq > 0 && tokens * G * 4 < (int64_t)UINT32_MAX - 64 &&
+                     tiles_take(sh, dtype, kv_stride, query, key_cache, value_cache, output);
   const int32_t workers = stream_workers(sh);
   const size_t logits = logit_bytes(sh);
   const size_t need = logits + (tiles ? stream_bytes(sh, workers, nullptr, nullptr) : generic_bytes(sh));
