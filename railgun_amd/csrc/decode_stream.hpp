@@ -642,7 +642,7 @@ struct StreamArgs {
   const float* cos_sin;         // [positions, D]: cos at [d], sin at [D/2 + d]
   const int32_t* positions;     // [batch]
   const int32_t* slot_mapping;  // [batch]; negative: a padding token, not cached
-  // kScores: [batch, H_kv, 16 max_blocks tokens, G], a (sequence, kv-head)'s below 4 GB.
+  // kScores: [batch, H_kv, 16 max_blocks tokens, G].
   float* logits;
   // kSuffix: tokens of whole blocks, more than 0.
   int32_t prefix;
@@ -733,6 +733,9 @@ __device__ __forceinline__ void stream_worker(
   auto& alpha_lds = alpha_all[wave];
 
   constexpr bool SUF = VAR == StreamVariant::kSuffix;
+  // The variants hold a few scalars more than the plain decode, which takes every scalar register: what
+  // they can form anew or keep in vector registers, they do.
+  constexpr bool LEAN = VAR != StreamVariant::kDecode;
   const int prefix = SUF ? a.prefix : 0;
   auto tokens_of = [&](int sq) __attribute__((always_inline)) -> int {
     const int c = min(context_lens[sq], a.max_blocks * kBS);
@@ -781,7 +784,7 @@ __device__ __forceinline__ void stream_worker(
     for (int c0 = 0; c0 < a.batch; c0 += 64) {
       const int q = c0 + lane;
       const int64_t n = q < a.batch ? (int64_t)seq_units<BPU, SUF>(context_lens, q, a.max_blocks, prefix) * hkv : 0;
-      const int64_t incl = wave_incl_scan<(WAVES > 1)>(n, lane) + U;
+      const int64_t incl = wave_incl_scan<LEAN>(n, lane) + U;
       if (c0 == 0) {
         n1 = n;
         incl1 = incl;
@@ -835,7 +838,7 @@ __device__ __forceinline__ void stream_worker(
       for (int c0 = 0; c0 < a.batch && (s < 0 || need1); c0 += 64) {
         const int q = c0 + lane;
         const int64_t n = q < a.batch ? (int64_t)seq_units<BPU, SUF>(context_lens, q, a.max_blocks, prefix) * hkv : 0;
-        const int64_t incl = wave_incl_scan<(WAVES > 1)>(n, lane) + ub;
+        const int64_t incl = wave_incl_scan<LEAN>(n, lane) + ub;
         resolve(c0, n, incl, nb + below(n > 0));
         ub = uniform64(__shfl(incl, 63, 64));
         nb += __builtin_popcountll(__ballot(n > 0));
@@ -849,7 +852,7 @@ __device__ __forceinline__ void stream_worker(
       for (int c0 = 0; c0 < a.batch && s < 0; c0 += 64) {
         const int q = c0 + lane;
         const int64_t n = q < a.batch ? (int64_t)seq_units<BPU, SUF>(context_lens, q, a.max_blocks, prefix) * hkv : 0;
-        const int64_t incl = wave_incl_scan<(WAVES > 1)>(n, lane) + ub, excl = incl - n;
+        const int64_t incl = wave_incl_scan<LEAN>(n, lane) + ub, excl = incl - n;
         const int64_t nb_ = nb + below(n > 0);
         const uint64_t h = __ballot(n > 0 && excl <= u0 && u0 < incl);
         if (h) {
@@ -866,10 +869,9 @@ __device__ __forceinline__ void stream_worker(
     seq_seg = __builtin_amdgcn_readfirstlane(seq_seg);
   }
 
-  // What only a segment's ends use.  With several workers to a workgroup it is kept in vector registers:
-  // the scalar ones are all taken.
+  // What only a segment's ends use.
   auto keep = [](int64_t x) __attribute__((always_inline)) -> int64_t {
-    if constexpr (WAVES > 1) asm volatile("" : "+v"(x));
+    if constexpr (LEAN) asm volatile("" : "+v"(x));
     return x;
   };
   const int64_t k_end = keep(k), C_end = keep(C), W_end = keep(W);
@@ -1065,13 +1067,28 @@ __device__ __forceinline__ void stream_worker(
     }
   };
 
-  // kScores: where the segment's raw scores go.  Kept in vector registers: the scalar ones are all taken.
+  // kScores: raw scores gather in LDS and leave at the segment's end or when the ring of LGU units (a power of
+  // two; 32 KB, the most that four workers on a CU find) is full.  The vector-memory counter retires in order,
+  // so a wait for the next unit's loads also waits for stores issued before them, and a store takes longer
+  // than a unit: with a store per unit, or one per 16, 64 sequences of 512 to 4,096 tokens (32 / 8 heads of
+  // 128) took 131 us instead of 115.
+  // lg: where the segment's go, lg_from: its first unit here.
+  constexpr int LGU = []() {
+    int n = 1;
+    while (2 * n * BPU * kBS * G <= 8192) n *= 2;
+    return n;
+  }();
+  __shared__ __attribute__((aligned(16))) float lg_lds[VAR == StreamVariant::kScores ? LGU * BPU * kBS * G : 4];
+  float* const lg_ring = lg_lds;
+  int lg_from = 0;
   float* lg = nullptr;
   float* lg_all = nullptr;
   if constexpr (VAR == StreamVariant::kScores) {
     lg_all = a.logits;
     asm volatile("" : "+v"(lg_all));
     lg = lg_all + ((int64_t)cur.s * hkv + cur.kvh) * a.max_blocks * (kBS * G);
+    lg_from = cur.b;
+    asm volatile("" : "+v"(lg_from));
   }
   const int64_t n = u1 - u0;
   Cursor ld = cur;
@@ -1136,27 +1153,37 @@ __device__ __forceinline__ void stream_worker(
       }
     }
     if constexpr (VAR == StreamVariant::kScores) {
-      // Stores that the buffer's bounds mask, not a branch: a store that may or may not have been issued would
-      // make the compiler wait for it whenever it waits for the loads issued before it.
-      const int tok0 = cur.b * BPU * kBS;
-      auto* base = reinterpret_cast<float*>((uint64_t)uniform64(reinterpret_cast<int64_t>(lg)));
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)((uint32_t)ctx_cur * (G * 4)), 0x00020000);
-      tile.template step<BPU>(kbuf[q], vbuf[q], tok0, ctx_cur, a.scale_log2, p_lds[j & 1], alpha_lds[j & 1],
-                              [&](const f32x4_t (&c)[BPU]) __attribute__((always_inline)) {
+      const int slot = (int)(j & (LGU - 1));
+      float* const ring = lg_ring + slot * (BPU * kBS * G);
+      tile.template step<BPU>(kbuf[q], vbuf[q], cur.b * BPU * kBS, ctx_cur, a.scale_log2, p_lds[j & 1],
+                              alpha_lds[j & 1], [&](const f32x4_t (&c)[BPU]) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < BPU; ++b) {
-          const uint32_t at = ((uint32_t)(tok0 + b * kBS + tile.col) * G + 4 * tile.seg) * 4;
+          float* const at = ring + (b * kBS + tile.col) * G + 4 * tile.seg;
           if constexpr (G % 4 == 0) {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(rg_u32x4_t, c[b]), rsrc,
-                                                   tile.seg < HG ? at : ~15u, 0, 0);
+            if (tile.seg < HG) *reinterpret_cast<float4*>(at) = make_float4(c[b][0], c[b][1], c[b][2], c[b][3]);
           } else {
 #pragma unroll
-            for (int r = 0; r < (G < 4 ? G : 4); ++r)
-              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(c[b][r]), rsrc,
-                                                    4 * tile.seg + r < G ? at + 4 * r : ~15u, 0, 0);
+            for (int r = 0; r < 4; ++r)
+              if (4 * tile.seg + r < G) at[r] = c[b][r];
           }
         }
       });
+      if (slot == LGU - 1 || cur.b + 1 == cur.nblk || j + 1 == n) {
+        // The units gathered since the last time, contiguous in the ring and in the segment, up to its last
+        // block (whose rows behind the context go along: nobody reads them).
+        const int held = min(slot + 1, cur.b + 1 - lg_from);
+        const float* const from = ring - (held - 1) * (BPU * kBS * G);
+        const int at = (cur.b + 1 - held) * (BPU * kBS);  // first token
+        const int floats = min(held * (BPU * kBS), ((ctx_cur + kBS - 1) & ~(kBS - 1)) - at) * G;
+        // (Global stores by their address space: as generic ones, out of order with the loads, they would make
+        // every wait for a load a wait for all.)
+        typedef __attribute__((address_space(1))) rg_u32x4_t* global_ptr;
+        const global_ptr to = (global_ptr) reinterpret_cast<uintptr_t>(lg + (int64_t)at * G);
+        wave_lds_sync();
+#pragma unroll 1
+        for (int i = lane; i < floats / 4; i += 64) to[i] = reinterpret_cast<const rg_u32x4_t*>(from)[i];
+      }
     } else {
       tile.template step<BPU>(kbuf[q], vbuf[q], cur.b * BPU * kBS, ctx_cur, a.scale_log2, p_lds[j & 1],
                               alpha_lds[j & 1]);
@@ -1170,6 +1197,8 @@ __device__ __forceinline__ void stream_worker(
         begin_segment(cur, u0 + j + 1);
         if constexpr (VAR == StreamVariant::kScores) {
           lg = lg_all + ((int64_t)cur.s * hkv + cur.kvh) * a.max_blocks * (kBS * G);
+          lg_from = 0;
+          asm volatile("" : "+v"(lg_from));
         }
         ctx_cur = tokens_of(cur.s);
       }

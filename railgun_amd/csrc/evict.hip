@@ -134,13 +134,34 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   };
   uint32_t key[NR] = {};
   if constexpr (VPT > 0) {
-    // (A table entry, then the score it leads to: two round trips, shared by U candidates.)
-    constexpr int U = VPT < 8 || VPT > 16 ? 4 : 8;  // (four with the registers all taken)
+    // A table entry, then the score it leads to: two round trips, shared by U candidates.  Where a thread
+    // has many candidates, the entries come to LDS first, all at once (where they fit), and the batches cost
+    // one round trip each.
+    constexpr int U = VPT < 8 ? VPT : 8;
+    constexpr int kEntries = VPT > 16 ? 4096 : 1;
+    __shared__ int32_t entries[kEntries];
+    const int e0 = p0 / a.block_size, ne = (p0 + count - 1) / a.block_size - e0 + 1;
+    const bool staged = VPT > 16 && ne <= kEntries;
+    if constexpr (VPT > 16) {
+      if (staged) {
+        for (int i = tid; i < ne; i += NT) entries[i] = row[e0 + i];
+        __syncthreads();
+      }
+    }
+    auto staged_key = [&](int c) -> uint32_t {
+      const uint32_t p = p0 + c, b = p / (uint32_t)a.block_size;
+      return order_key(cells[entries[b - e0] * a.score_stride + (p - b * (uint32_t)a.block_size)]);
+    };
 #pragma unroll
     for (int i0 = 0; i0 < VPT; i0 += U) {
       if (i0 < strips) {
+        if (VPT > 16 && staged) {
 #pragma unroll
-        for (int i = i0; i < i0 + U; ++i) key[i] = read_key(min(i * NT + tid, count - 1));
+          for (int i = i0; i < i0 + U; ++i) key[i] = staged_key(min(i * NT + tid, count - 1));
+        } else {
+#pragma unroll
+          for (int i = i0; i < i0 + U; ++i) key[i] = read_key(min(i * NT + tid, count - 1));
+        }
       }
 #pragma unroll
       for (int i = i0; i < i0 + U; ++i) {

@@ -286,7 +286,9 @@ void launch_scores_stream(const StreamArgs& sa, int G, const void* q, const void
     case 2: go(std::integral_constant<int, 2>{}); break;
     case 4: go(std::integral_constant<int, 4>{}); break;
     case 8: go(std::integral_constant<int, 8>{}); break;
-    case 16: go(std::integral_constant<int, 16>{}); break;
+    case 16:
+      if constexpr (D <= 128) go(std::integral_constant<int, 16>{});
+      break;
     default:
       // G 3, 5, 6, 7 (mfma_group_size admits them at head_dim 64 and 128 only)
       if constexpr (D <= 128) {
@@ -388,8 +390,8 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
   }
   const int64_t kv_stride = kv_block_stride ? kv_block_stride : block * head_dim;
-  // (The workers address a segment's raw scores with 32 bits.)
-  const bool tiles = max_blocks_per_seq > 0 && tokens * G * 4 < (int64_t)UINT32_MAX - 64 &&
+  // (head_dim 256 with 16 heads to a kv-head fills the registers without the ring of raw scores.)
+  const bool tiles = max_blocks_per_seq > 0 && !(head_dim == 256 && G == 16) &&
                      tiles_take(sh, dtype, kv_stride, query, key_cache, value_cache, output);
   const int32_t workers = stream_workers(sh);
   const size_t logits = logit_bytes(sh);

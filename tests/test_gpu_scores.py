@@ -199,3 +199,8 @@ def test_refusals(device, kernels):
                    dict(workspace=torch.empty(16, dtype=torch.uint8, device=device))):
         with pytest.raises(RailgunError):
             op.execute_with_scores(**{**good, **change})
+
+
+def test_workers_with_more_tokens_than_they_gather_at_once(device, kernels):
+    """16 heads to a kv-head at head_dim 64: a worker gathers the raw scores of 512 tokens, and has 586."""
+    Batch(device, [150000], heads=64, hkv=4, d=64, seed=15).check(kernels, scored=np.array([149000]))
