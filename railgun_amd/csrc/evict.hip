@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelBins = 2048;
+constexpr uint32_t kZeroKey = 0x80000000u;  // order_key(0)
 
 // Inclusive prefix sum over the 64 lanes with DPP: within each row of 16 lanes by shifts of 1, 2, 4 and 8, then
 // lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
@@ -102,13 +102,17 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   constexpr int NW = NT / 64;
   constexpr int NR = VPT > 0 ? VPT : 1;
   constexpr int GROUP = VPT > 0 ? VPT : 64;  // strips of NT candidates whose counts are scanned together
-  constexpr int BPT = kSelBins / NT;         // bins a thread scans
+  // Bits of the three passes: with many candidates a first pass over more bins meets fewer equal addresses in
+  // the LDS atomics of a wave (65,000 candidates: 9 us over 2,048 bins).
+  constexpr int FIRST = VPT > 16 ? 13 : 11, BINS = 1 << FIRST;
+  constexpr int shifts[4] = {32, 32 - FIRST, 21 - FIRST, 0};
+  constexpr int BPT = BINS / NT;  // bins a thread scans
   constexpr int EPT = (GROUP * NW + NT - 1) / NT;  // (strip, wave) counts a thread scans
-  __shared__ __attribute__((aligned(16))) int hist[kSelBins];
+  __shared__ __attribute__((aligned(16))) int hist[BINS];
   __shared__ int part[2][NW];
   __shared__ int found[3];                          // digit, candidates above it, candidates at it
   __shared__ int strip[2][GROUP * NW];              // per (strip, wave): candidates above T, candidates at T
-  __shared__ int first_hole, alias;
+  __shared__ int first_hole, last_alias;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Segment sg = segment_of(a, blockIdx.x);
   const int n = context_of(a, sg.seq);
@@ -116,9 +120,8 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.kept_stride;
   const int32_t* row = a.table + (int64_t)sg.seq * a.max_blocks;
   if (a.new_lens != nullptr && sg.layer == 0 && sg.kvh == 0 && tid == 0) a.new_lens[sg.seq] = m;
-  for (int i = m + tid; i < a.kept_stride; i += NT) kept[i] = -1;
   if (n <= a.budget) {
-    for (int i = tid; i < n; i += NT) kept[i] = i;
+    for (int i = tid; i < a.kept_stride; i += NT) kept[i] = i < n ? i : -1;
     if (tid == 0) a.in_order[blockIdx.x] = 0;
     return;
   }
@@ -137,7 +140,7 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
     // A table entry, then the score it leads to: two round trips, shared by U candidates.  Where a thread
     // has many candidates, the entries come to LDS first, all at once (where they fit), and the batches cost
     // one round trip each.
-    constexpr int U = VPT < 8 ? VPT : 8;
+    constexpr int U = VPT < 16 ? VPT : 16;
     constexpr int kEntries = VPT > 16 ? 4096 : 1;
     __shared__ int32_t entries[kEntries];
     const int e0 = p0 / a.block_size, ne = (p0 + count - 1) / a.block_size - e0 + 1;
@@ -170,11 +173,18 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
       }
     }
   }
+  // The last entry that both tables have alike (before the first stores: a load behind them waits for them).
+  const int32_t* drow = a.dst_table + (int64_t)sg.seq * a.max_dst_blocks;
+  int alias = -1;
+  for (int i = tid; i < (m + a.block_size - 1) / a.block_size; i += NT) {
+    if (row[i] == drow[i]) alias = i;
+  }
+  for (int i = m + tid; i < a.kept_stride; i += NT) kept[i] = -1;
   for (int i = tid; i < a.recent; i += NT) kept[m - a.recent + i] = n - a.recent + i;
   for (int i = tid; i < p0; i += NT) kept[i] = i;
   if (tid == 0) {
     first_hole = n;
-    alias = 0;
+    last_alias = -1;
   }
   // f(strip within the group, candidate, key) over strips g0 .. g0 + gs - 1, the whole wave at once.  The key
   // of what is no candidate is 0, below every score's.
@@ -208,23 +218,30 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   if (take > 0) {
     T = 0;
     left = take;
-    constexpr int shifts[4] = {32, 21, 10, 0};
 #pragma unroll
     for (int ps = 0; ps < 3; ++ps) {
       if (whole) break;
       const int sh = shifts[ps + 1], hi = shifts[ps];  // bits from hi on are settled
-      for (int i = 4 * tid; i < kSelBins; i += 4 * NT) *reinterpret_cast<int4*>(&hist[i]) = make_int4(0, 0, 0, 0);
+      for (int i = 4 * tid; i < BINS; i += 4 * NT) *reinterpret_cast<int4*>(&hist[i]) = make_int4(0, 0, 0, 0);
       __syncthreads();
+      int zeros = 0;
       each(0, strips, [&](int, int, uint32_t k) __attribute__((always_inline)) {
+        // Lanes on one address go one after the other, and a score of 0 is the one that many tokens have in
+        // common (weights that underflowed): those are counted in a register.
+        if (ps == 0) {
+          zeros += __popcll(__ballot(k == kZeroKey));
+          if (k == kZeroKey) return;
+        }
         if (k != 0 && (ps == 0 || (k >> (hi & 31)) == (T >> (hi & 31))))
-          atomicAdd(&hist[(k >> sh) & (ps == 2 ? 1023u : 2047u)], 1);
+          atomicAdd(&hist[(k >> sh) & ((1u << (shifts[ps] - sh)) - 1u)], 1);
       });
+      if (ps == 0 && lane == 0 && zeros > 0) atomicAdd(&hist[kZeroKey >> sh], zeros);
       __syncthreads();
       // Candidates in higher bins; BPT bins a thread, from the top.
       int h[BPT], sum = 0;
 #pragma unroll
       for (int i = 0; i < BPT; ++i) {
-        h[i] = hist[kSelBins - 1 - tid * BPT - i];
+        h[i] = hist[BINS - 1 - tid * BPT - i];
         sum += h[i];
       }
       int all;
@@ -233,7 +250,7 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
 #pragma unroll
         for (int i = 0; i < BPT; ++i) {
           if (above < left && left <= above + h[i]) {
-            found[0] = kSelBins - 1 - tid * BPT - i;
+            found[0] = BINS - 1 - tid * BPT - i;
             found[1] = above;
             found[2] = h[i];
           }
@@ -296,16 +313,20 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
     gt_before += gall;
     eq_before += eall;
   }
-  // Rows from the first hole on move.  Where a block that receives them is also the block they may
-  // come from (the same entry of both tables: eviction in place), the chunks go in order.
-  atomicMin(&first_hole, hole);
-  __syncthreads();
-  const int32_t* drow = a.dst_table + (int64_t)sg.seq * a.max_dst_blocks;
-  for (int i = first_hole / a.block_size + tid; i < (m + a.block_size - 1) / a.block_size; i += NT) {
-    if (row[i] == drow[i]) alias = 1;
+  // Rows from the first hole on move.  Where a block that receives them is also the block they may come
+  // from (the same entry of both tables: eviction in place), the chunks go in order.
+  // (One LDS atomic a wave: lanes on one address go one after the other.)
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    hole = min(hole, __shfl_xor(hole, o, 64));
+    alias = max(alias, __shfl_xor(alias, o, 64));
+  }
+  if (lane == 0) {
+    atomicMin(&first_hole, hole);
+    atomicMax(&last_alias, alias);
   }
   __syncthreads();
-  if (tid == 0) a.in_order[blockIdx.x] = alias;
+  if (tid == 0) a.in_order[blockIdx.x] = last_alias >= first_hole / a.block_size;
 }
 
 // ----------------------------------------------------------------- move -----
