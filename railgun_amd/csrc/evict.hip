@@ -95,8 +95,9 @@ __device__ __forceinline__ int block_before(int v, int lane, int w, int* part, i
 
 // NT threads.  VPT > 0: every candidate's key sits in a register (thread t holds candidates t, t + NT, ...: VPT
 // of them), and the scores are read once.  VPT 0: longer tables read them again in each pass.
-//   Measured (16 layers x 16 sequences x 8 kv-heads, 1,500 to 4,096 tokens each; two segments of 48 KB of
-// scores): see the launch.
+//   A chain of memory round trips and barriers, and past some 16,000 candidates a workgroup's issue rate.  Per
+// segment (16 layers x 16 sequences x 8 kv-heads of up to 4,096 tokens, all at once / one of 65,000): keys there
+// after 5.6 / 10.7 us, T known at 9.6 / 24, positions written at 12.6 / 33.
 template <int NT, int VPT>
 __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   constexpr int NW = NT / 64;
@@ -331,17 +332,21 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
 
 // ----------------------------------------------------------------- move -----
 
-constexpr int kMoveThreads = 256;
-constexpr int kMoveUnroll = 8;     // V-sized pieces of K and V a thread holds
-constexpr int kMoveMaxTokens = 128;
+constexpr int kMoveMaxTokens = 512;
+constexpr int kInPlacePieces = 8;
 
-// Workgroup (chunk, segment): tokens chunk * TOK .. of the segment's kept list, TOK such that its K
-// and V rows fill kMoveUnroll pieces a thread, all of them read before the first is written.  A
-// segment that is evicted in place is walked by its first workgroup alone: the chunk at hand is
-// written once every thread has read its part of it.  That is enough: kept[j] >= j, so rows
-// j .. of the destination never hold a row that a later chunk has yet to read.
-template <typename V>
-__global__ __launch_bounds__(kMoveThreads, 4) void evict_move_kernel(EvictArgs a, int row_vecs, int tok) {
+// Workgroup (chunk, segment), NT threads: tokens chunk * tok .. of the segment's kept list, tok such that their K
+// and V rows fill U pieces V a thread, all of them read before the first is written.  A segment that is evicted in
+// place is walked by its first workgroup alone: the chunk at hand is written once every thread has read its part
+// of it.  That is enough: kept[j] >= j, so rows j .. of the destination never hold a row that a later chunk has
+// yet to read.
+//   Bound by the copy: every row is read and written once, with non-temporal accesses (no row is met again).
+// 16 layers x 16 sequences x 8 kv-heads of 1,024 kept tokens, head_dim 64 in 16 bits (1.07 GB): 215 us with 256
+// threads of 4 pieces, 238 with 8 and ordinary accesses, a 1 GiB copy's rate being 5.2 TB/s.  In place the
+// round trips of a segment's chunks follow each other, so fewer, larger ones win: two sequences of 65,000
+// tokens down to 8,192 (16 segments) took 447 us with 256 threads of 8 pieces, 197 with 1,024 of 8, 223 of 16.
+template <typename V, int NT, int U>
+__global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a, int row_vecs, int tok) {
   __shared__ int64_t src_off[2][kMoveMaxTokens], dst_off[2][kMoveMaxTokens];  // in pieces V; -1: not moved
   const int tid = threadIdx.x;
   const Segment sg = segment_of(a, blockIdx.x);
@@ -374,13 +379,13 @@ __global__ __launch_bounds__(kMoveThreads, 4) void evict_move_kernel(EvictArgs a
       }
     }
     __syncthreads();
-    V piece[kMoveUnroll] = {};
+    V piece[U] = {};
 #pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = u * kMoveThreads + tid, t = i / per_token, c = i - t * per_token;
+    for (int u = 0; u < U; ++u) {
+      const int i = u * NT + tid, t = i / per_token, c = i - t * per_token;
       if (t < nt && src_off[buf][t] >= 0) {
         const int64_t at = src_off[buf][t];
-        piece[u] = *((c >= row_vecs ? vb - row_vecs : kb) + at + c);
+        piece[u] = __builtin_nontemporal_load((c >= row_vecs ? vb - row_vecs : kb) + at + c);
       }
     }
     if (in_order) {
@@ -389,11 +394,11 @@ __global__ __launch_bounds__(kMoveThreads, 4) void evict_move_kernel(EvictArgs a
       __syncthreads();
     }
 #pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = u * kMoveThreads + tid, t = i / per_token, c = i - t * per_token;
+    for (int u = 0; u < U; ++u) {
+      const int i = u * NT + tid, t = i / per_token, c = i - t * per_token;
       if (t < nt && src_off[buf][t] >= 0) {
         const int64_t at = dst_off[buf][t];
-        *((c >= row_vecs ? vb - row_vecs : kb) + at + c) = piece[u];
+        __builtin_nontemporal_store(piece[u], (c >= row_vecs ? vb - row_vecs : kb) + at + c);
       }
     }
     if (to_cell >= 0) a.scores[to_cell] = score;
@@ -415,7 +420,7 @@ size_t evict_bytes(int64_t segments, int64_t budget, bool own_list) {
 int probe_evict_kernels() {
   hipFuncAttributes at;
   if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_select_kernel<256, 16>)) != hipSuccess ||
-      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_move_kernel<rg_u32x4_t>)) != hipSuccess) {
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_move_kernel<rg_u32x4_t, 256, 4>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the eviction kernels: %s", hipGetErrorString(hipGetLastError()));
   }
   return RG_OK;
@@ -528,14 +533,17 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   const bool wide = whole(head_dim) && whole(kv_stride) && whole(a.layer_stride) &&
                     ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15u) == 0;
   const int row_vecs = head_dim * eb / (wide ? 16 : 2);
-  const int tok = std::max(1, std::min(kMoveMaxTokens, kMoveThreads * kMoveUnroll / (2 * row_vecs)));
-  const int64_t chunks = ceil_div(most, tok);
-  if (chunks > 65535) return fail(RG_ERR_NOT_SUPPORTED, "%s: a budget of %lld tokens", op, (long long)most);
-  const dim3 grid((unsigned)segments, (unsigned)chunks);
-  if (wide) {
-    hipLaunchKernelGGL(evict_move_kernel<rg_u32x4_t>, grid, dim3(kMoveThreads), 0, s, a, row_vecs, tok);
-  } else {
-    hipLaunchKernelGGL(evict_move_kernel<uint16_t>, grid, dim3(kMoveThreads), 0, s, a, row_vecs, tok);
+  auto move = [&](auto kernel, int threads, int pieces) {
+    const int tok = std::max(1, std::min(kMoveMaxTokens, threads * pieces / (2 * row_vecs)));
+    const int64_t chunks = dst_block_table == nullptr ? 1 : ceil_div(most, tok);
+    if (chunks > 65535) return fail(RG_ERR_NOT_SUPPORTED, "%s: a budget of %lld tokens", op, (long long)most);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)segments, (unsigned)chunks), dim3(threads), 0, s, a, row_vecs, tok);
+    return check_launch(op);
+  };
+  // (In place without a second table no segment has use for more than one workgroup.)
+  if (dst_block_table == nullptr) {
+    return wide ? move(evict_move_kernel<rg_u32x4_t, 1024, kInPlacePieces>, 1024, kInPlacePieces)
+                : move(evict_move_kernel<uint16_t, 1024, kInPlacePieces>, 1024, kInPlacePieces);
   }
-  return check_launch(op);
+  return wide ? move(evict_move_kernel<rg_u32x4_t, 256, 4>, 256, 4) : move(evict_move_kernel<uint16_t, 256, 4>, 256, 4);
 }
