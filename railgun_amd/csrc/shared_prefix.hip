@@ -82,9 +82,7 @@ struct KeyTile {
 template <typename T, int D>
 __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16_t* __restrict__ q,
                                                const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-                                               const int32_t* __restrict__ table,
-                                               const int32_t* __restrict__ context_lens, char* lds, int u, int w,
-                                               int lane) {
+                                               const int32_t* __restrict__ table, char* lds, int u, int w, int lane) {
   using MF = mfma32<T>;
   using TL = KeyTile<D>;
   constexpr int NKC = D / 16, NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF;
@@ -301,14 +299,183 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
   }
 }
 
+// The fp32 product, on v_mfma_f32_32x32x2: step m of S^T = K Q^T takes the k-slot of lane half hh from dim
+// hh D/2 + m, so a lane reads its K row in 16-byte pieces; step v of O^T += V^T P^T takes the keys
+// 8 (v >> 2) + 4 hh + (v & 3), which is where S^T leaves them, so the probabilities stay in fp32 and in their
+// registers.  A key tile is twice as long as in 16 bits and its product 16 times (128 MFMAs of 64 cycles at
+// head_dim 128), so one tile in flight ahead of the one at hand is enough: two stages.
+// K in LDS: rows [key][D], the 16-byte chunk c of a row at c ^ (key & 7) (rows of 256 or 512 bytes would put all
+// keys of a read on the same banks); V: rows [key][D] as they are (a read takes 32 neighbours of one row).
+template <int D>
+struct KeyTileF32 {
+  static constexpr int KB = kTileKeys * D * 4;
+  static constexpr int BYTES = 2 * KB;
+  static constexpr int STAGES = 2;
+  static constexpr int CH = D / 4;            // 16-byte chunks of a row
+  static constexpr int SUB_COPIES = D / 16;   // 1 KB copies of a sub-block's K, and of its V
+};
+
+template <int D>
+__device__ __forceinline__ void prefix_product_f32(const PrefixArgs& a, const float* __restrict__ q,
+                                                   const float* __restrict__ kc, const float* __restrict__ vc,
+                                                   const int32_t* __restrict__ table, char* lds, int u, int w,
+                                                   int lane) {
+  using TL = KeyTileF32<D>;
+  constexpr int NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF, HD = D / 2;
+  const int pairs = a.num_kv_heads * a.splits;
+  const int rt = u / pairs, pair = u % pairs;
+  const int kvh = pair % a.num_kv_heads, split = pair / a.num_kv_heads;
+  const int kt0 = split * a.split_tiles, kt1 = min(a.tiles, kt0 + a.split_tiles);
+  const int j = lane & 31, hh = lane >> 5;
+  const int wrow = rt * kPreRows + w * 32;
+  const bool busy = wrow < a.rows;
+  const int row = wrow + j;
+  const int b = min(row, a.rows - 1) / a.group, g = min(row, a.rows - 1) - b * a.group;
+  const int cb = w >> 1, cp = w & 1;
+  int wb = kt0, win;
+  auto fill = [&]() {
+    const int sb = min(2 * (wb + lane) + cb, a.subs - 1);
+    win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
+  };
+  fill();
+  float qf[HD];
+  {
+    const float4* qr = reinterpret_cast<const float4*>(q + ((int64_t)b * a.num_heads + (int64_t)kvh * a.group + g) * D + hh * HD);
+    const float on = a.q_sign == 0 ? 0.f : a.q_sign & 0x8000u ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) {
+      const float4 x = qr[i];
+      qf[4 * i] = on != 0.f ? x.x * on : 0.f;
+      qf[4 * i + 1] = on != 0.f ? x.y * on : 0.f;
+      qf[4 * i + 2] = on != 0.f ? x.z * on : 0.f;
+      qf[4 * i + 3] = on != 0.f ? x.w * on : 0.f;
+    }
+  }
+  // Copy n of a sub-block's K or V (1 KB): chunk positions 64 n + lane of its rows.
+  uint32_t k_off[HALF], v_off[HALF];  // bytes within the sub-block
+#pragma unroll
+  for (int i = 0; i < HALF; ++i) {
+    const int at = (cp * HALF + i) * 64 + lane, key = at / TL::CH, c = at % TL::CH;
+    k_off[i] = (uint32_t)(key * D * 4 + 16 * (c ^ (key & 7)));
+    v_off[i] = (uint32_t)(at * 16);
+  }
+  const uint32_t lds_base = (uint32_t)(uintptr_t)((RG_LDS char*)lds);
+  const int64_t head = (int64_t)kvh * (kBS << a.bs_shift) * D;
+  auto issue = [&](int kt, int st) {
+    const int e = __builtin_amdgcn_readlane(win, kt - wb);
+    const int64_t off = (int64_t)(e >> a.bs_shift) * a.kv_stride + head + (int64_t)(e & ((1 << a.bs_shift) - 1)) * (kBS * D);
+    const uint32_t at = lds_base + st * TL::BYTES + cb * (TL::KB / 2) + cp * HALF * 1024;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) lds_dma16_s(reinterpret_cast<const char*>(kc + off), k_off[i], at + i * 1024);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) lds_dma16_s(reinterpret_cast<const char*>(vc + off), v_off[i], at + TL::KB + i * 1024);
+  };
+  f32x16_t o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  const int xor32 = (lane ^ 32) << 2;
+  auto compute = [&](int kt, int st) __attribute__((always_inline)) {
+    const char* krow = lds + st * TL::BYTES + j * (D * 4);
+    f32x16_t c;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) {
+      const float4 k4 = *reinterpret_cast<const float4*>(krow + 16 * ((hh * (HD / 4) + i) ^ (j & 7)));
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.x, qf[4 * i], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.y, qf[4 * i + 1], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.z, qf[4 * i + 2], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.w, qf[4 * i + 3], c, 0, 0, 0);
+    }
+    if (2 * kt + 1 >= a.subs) {  // the last tile's second half repeats a sub-block
+#pragma unroll
+      for (int v = 8; v < 16; ++v) c[v] = -INFINITY;
+    }
+    float tmax = c[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, c[v]);
+    tmax = fmaxf(tmax, __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)))) * a.scale_log2;
+    if (__ballot(tmax > m_run)) {
+      const float m_new = fmaxf(m_run, tmax);
+      const float alpha = fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      c[v] = fast_exp2(fmaf(c[v], a.scale_log2, -m_run));
+      l_run += c[v];
+    }
+    const float* vrow = reinterpret_cast<const float*>(lds + st * TL::BYTES + TL::KB) + 4 * hh * D + j;
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[(8 * (v >> 2) + (v & 3)) * D + 32 * db], c[v], o[db], 0, 0, 0);
+  };
+  __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0): the window and Q
+  issue(kt0, 0);
+  if (kt0 + 1 < kt1) issue(kt0 + 1, 1);
+  static_assert(COPIES < 16, "low bits of vmcnt");
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const int st = (kt - kt0) & 1;
+    asm volatile("" ::: "memory");
+    if (kt + 1 < kt1) __builtin_amdgcn_s_waitcnt(COPIES | 0x70 | 0xF00);
+    else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+    tile_barrier();  // tile kt has landed for every wave
+    if (busy) compute(kt, st);
+    if (kt + 2 < kt1) {
+      if (kt + 2 - wb >= 64) {
+        wb = kt + 2;
+        fill();
+        __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+      }
+      tile_barrier();  // every wave is done with the stage
+      issue(kt + 2, st);
+    }
+  }
+  if (row < a.rows) {
+    const float l = l_run + __shfl_xor(l_run, 32, 64);
+    const int64_t at = ((int64_t)kvh * a.splits + split) * a.rows + row;
+    float* acc = a.acc + at * D;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        *reinterpret_cast<float4*>(acc + 32 * db + 8 * p + 4 * hh) =
+            make_float4(o[db][4 * p], o[db][4 * p + 1], o[db][4 * p + 2], o[db][4 * p + 3]);
+    if (hh == 0) {
+      a.ml[2 * at] = m_run;
+      a.ml[2 * at + 1] = l;
+    }
+  }
+}
+
+// LDS of the product's ring.
+template <typename T, int D>
+constexpr int ring_bytes() {
+  if constexpr (std::is_same_v<T, f32_t>) return KeyTileF32<D>::STAGES * KeyTileF32<D>::BYTES;
+  else return kStages * KeyTile<D>::BYTES;
+}
+
+// Workgroups to a CU that the compiler is held to: two (256 registers a wave) where that costs the worker's tile
+// few of its own.
 template <typename T, int D, int G>
-__global__ __launch_bounds__(kPreThreads) void shared_prefix_kernel(StreamArgs sa, PrefixArgs pa,
-                                                                    const uint16_t* __restrict__ q,
-                                                                    const uint16_t* __restrict__ kc,
-                                                                    const uint16_t* __restrict__ vc,
-                                                                    const int32_t* __restrict__ block_table,
-                                                                    const int32_t* __restrict__ context_lens) {
-  __shared__ __attribute__((aligned(16))) char ring[kStages * KeyTile<D>::BYTES];
+constexpr int groups_per_cu() { return std::is_same_v<T, f32_t> && D == 128 && G <= 4 ? 2 : 1; }
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(kPreThreads, (groups_per_cu<T, D, G>())) void shared_prefix_kernel(
+    StreamArgs sa, PrefixArgs pa, const typename DecodeTileFor<T, D, G>::S* __restrict__ q,
+    const typename DecodeTileFor<T, D, G>::S* __restrict__ kc, const typename DecodeTileFor<T, D, G>::S* __restrict__ vc,
+    const int32_t* __restrict__ block_table, const int32_t* __restrict__ context_lens) {
+  __shared__ __attribute__((aligned(16))) char ring[ring_bytes<T, D>()];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x < pa.stream_groups) {
@@ -319,7 +486,9 @@ __global__ __launch_bounds__(kPreThreads) void shared_prefix_kernel(StreamArgs s
     }
     return;
   }
-  prefix_product<T, D>(pa, q, kc, vc, block_table, context_lens, ring, (int)blockIdx.x - pa.stream_groups, w, lane);
+  const int u = (int)blockIdx.x - pa.stream_groups;
+  if constexpr (std::is_same_v<T, f32_t>) prefix_product_f32<D>(pa, q, kc, vc, block_table, ring, u, w, lane);
+  else prefix_product<T, D>(pa, q, kc, vc, block_table, ring, u, w, lane);
 }
 
 // One workgroup per (kv-head, sequence), a wave per query head: lane l folds dims [l PER, (l + 1) PER) of the
@@ -393,9 +562,9 @@ void launch_shared(const StreamArgs& sa, const PrefixArgs& pa, int G, int groups
                    const void* vc, const int32_t* bt, const int32_t* cl, hipStream_t s) {
   auto go = [&](auto g) {
     constexpr int GC = decltype(g)::value;
+    using S = typename DecodeTileFor<T, D, GC>::S;
     hipLaunchKernelGGL((shared_prefix_kernel<T, D, GC>), dim3(groups), dim3(kPreThreads), 0, s, sa, pa,
-                       static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(kc),
-                       static_cast<const uint16_t*>(vc), bt, cl);
+                       static_cast<const S*>(q), static_cast<const S*>(kc), static_cast<const S*>(vc), bt, cl);
     hipLaunchKernelGGL((shared_merge_kernel<T, D, GC>), dim3(sa.num_kv_heads, sa.batch), dim3(64 * GC), 0, s, sa, pa,
                        cl);
   };
@@ -415,13 +584,13 @@ void launch_shared(const StreamArgs& sa, const PrefixArgs& pa, int G, int groups
 // Whether the shared product takes the call (else every sequence reads the prefix for itself).
 bool shared_applies(const Shape& sh, int32_t dtype, int64_t kv_stride, const void* q, const void* kc, const void* vc,
                     const void* out) {
-  return dtype != RG_DTYPE_F32 && sh.D <= 128 && sh.B > 1 && tiles_take(sh, dtype, kv_stride, q, kc, vc, out);
+  return sh.D <= 128 && sh.B > 1 && tiles_take(sh, dtype, kv_stride, q, kc, vc, out);
 }
 
 struct SharedPlan {
   int32_t rows, row_tiles, tiles, split_tiles, splits, workers, stream_groups;
 };
-SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks) {
+SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks, bool f32) {
   SharedPlan p;
   const int64_t prefix = (int64_t)shared_blocks * sh.bs;
   p.rows = sh.B * (sh.H / sh.Hkv);
@@ -430,14 +599,15 @@ SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks) {
   // One workgroup of the product per CU beside the one of stream-K workers that its CU also holds.  Two where
   // that leaves splits of many row tiles (few of them, then, for the merge to read) and the table leaves the
   // sequences so little behind the prefix that the product (at 0.7 PFLOP/s) outlasts the workers (at 5 TB/s).
-  // Splits of fewer than 8 key tiles are not made: each writes 4 D bytes a row for the merge to read.
+  // Splits of fewer than 8 key tiles (2 in fp32, whose tiles take 16 times the time) are not made: each writes
+  // 4 D bytes a row for the merge to read.
   //   Measured (bf16, 32 / 8 heads of 128, us): 256 rows' 16,384 tokens with nothing behind them 113 with one,
   // 93 with two, with 64 to 1,024 tokens behind them 177 and 189; 16 rows of 16,384 22.2 and 26.7; 16 rows of
   // 2,048 with up to 700 behind them 18.7 with 8 tiles to a split, 21.7 with 2, 22.7 with 16.
-  const double product = 4.0 * sh.B * sh.H * sh.D * (double)prefix / 0.7e15;
-  const double stream = 4.0 * sh.B * sh.Hkv * sh.D * ((double)sh.MB * sh.bs - (double)prefix) / 5e12;
+  const double product = 4.0 * sh.B * sh.H * sh.D * (double)prefix / (f32 ? 0.1e15 : 0.7e15);
+  const double stream = (f32 ? 8.0 : 4.0) * sh.B * sh.Hkv * sh.D * ((double)sh.MB * sh.bs - (double)prefix) / 5e12;
   const int64_t one = std::max<int64_t>(1, device_cu_count() / ((int64_t)sh.Hkv * p.row_tiles));
-  const int64_t want = std::min(product > stream && one <= 8 ? 2 * one : one, ceil_div(p.tiles, 8));
+  const int64_t want = std::min(product > stream && one <= 8 ? 2 * one : one, ceil_div(p.tiles, f32 ? 2 : 8));
   p.split_tiles = (int32_t)ceil_div(p.tiles, std::min<int64_t>(want, p.tiles));
   p.splits = (int32_t)ceil_div(p.tiles, p.split_tiles);
   p.workers = stream_workers(sh);
@@ -478,8 +648,10 @@ extern "C" size_t rg_paged_attention_shared_prefix_workspace_bytes(int32_t batch
   size_t n = rg_paged_attention_v1_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,
                                                    max_blocks_per_seq);
   if (shared_blocks > 0) {
-    const SharedPlan p = plan_shared(sh, shared_blocks);
-    n = std::max(n, prefix_bytes(sh, p, nullptr) + stream_bytes(sh, p.workers, nullptr, nullptr));
+    for (const bool f32 : {false, true}) {
+      const SharedPlan p = plan_shared(sh, shared_blocks, f32);
+      n = std::max(n, prefix_bytes(sh, p, nullptr) + stream_bytes(sh, p.workers, nullptr, nullptr));
+    }
   }
   return n;
 }
@@ -519,7 +691,7 @@ extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* k
                                  num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size, dtype,
                                  kv_block_stride, workspace, workspace_bytes, stream);
   }
-  const SharedPlan p = plan_shared(sh, shared_blocks);
+  const SharedPlan p = plan_shared(sh, shared_blocks, dtype == RG_DTYPE_F32);
   char* const ws = static_cast<char*>(workspace);
   size_t ml_at;
   const size_t pre = prefix_bytes(sh, p, &ml_at);
@@ -567,5 +739,5 @@ extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* k
     else launch_shared<T, 64>(sa, pa, pa.group, (int)groups, query, key_cache, value_cache, block_table, context_lens, s);
     return check_launch(op);
   };
-  return dtype == RG_DTYPE_BF16 ? go(bf16_t{}) : go(f16_t{});
+  return dispatch_dtype(dtype, go);
 }
