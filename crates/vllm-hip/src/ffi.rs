@@ -82,6 +82,11 @@ extern "C" {
         batch_size: i32, num_heads: i32, num_kv_heads: i32, head_dim: i32, block_size: i32,
         max_blocks_per_seq: i32, shared_blocks: i32,
     ) -> usize;
+    /// New: 1 where rg_paged_attention_shared_prefix is expected to beat rg_paged_attention_v1.
+    pub fn rg_paged_attention_shared_prefix_pays(
+        batch_size: i32, num_heads: i32, num_kv_heads: i32, head_dim: i32, block_size: i32,
+        max_blocks_per_seq: i32, shared_blocks: i32, dtype: i32,
+    ) -> c_int;
     /// New: rg_paged_attention_v1 for sequences that begin with the same cached blocks.
     pub fn rg_paged_attention_shared_prefix(
         query: *const c_void, key_cache: *const c_void, value_cache: *const c_void, block_table: *const i32,

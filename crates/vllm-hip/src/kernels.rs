@@ -535,6 +535,24 @@ impl PagedAttentionKernels {
         }
     }
 
+    /// Whether `launch_shared_prefix` is expected to be faster than `launch_v1_split`.
+    pub fn shared_prefix_pays<T: KvElement>(
+        &self,
+        batch_size: i32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        shared_blocks: i32,
+    ) -> bool {
+        // SAFETY: pure query.
+        unsafe {
+            ffi::rg_paged_attention_shared_prefix_pays(batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                                                       max_blocks_per_seq, shared_blocks, T::DTYPE) != 0
+        }
+    }
+
     /// `launch_v1_split` for sequences whose block tables begin with the same `shared_blocks`
     /// entries: those blocks are read once for many rows.
     pub unsafe fn launch_shared_prefix<T: KvElement>(

@@ -415,6 +415,12 @@ size_t rg_paged_attention_shared_prefix_workspace_bytes(int32_t batch_size, int3
                                                         int32_t block_size,
                                                         int32_t max_blocks_per_seq,
                                                         int32_t shared_blocks);
+/* 1 where rg_paged_attention_shared_prefix is expected to be faster than rg_paged_attention_v1 on the
+ * current device (the bytes it saves against what its product and merge add), else 0. */
+int rg_paged_attention_shared_prefix_pays(int32_t batch_size, int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t head_dim,
+                                          int32_t block_size, int32_t max_blocks_per_seq,
+                                          int32_t shared_blocks, int32_t dtype);
 int rg_paged_attention_shared_prefix(const void* query, const void* key_cache,
                                      const void* value_cache, const int32_t* block_table,
                                      const int32_t* context_lens, void* output, float scale,

@@ -287,6 +287,12 @@ class PagedAttentionKernels {
     return rg_paged_attention_shared_prefix_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,
                                                             max_blocks_per_seq, shared_blocks);
   }
+  // Whether launch_shared_prefix is expected to be faster than launch_v1.
+  bool shared_prefix_pays(int32_t batch_size, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t block_size, int32_t max_blocks_per_seq, int32_t shared_blocks, DType dtype) const {
+    return rg_paged_attention_shared_prefix_pays(batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                                                 max_blocks_per_seq, shared_blocks, (int32_t)dtype) != 0;
+  }
   // launch_v1 for sequences whose block tables begin with the same shared_blocks entries: those blocks
   // are read once for many rows.
   void launch_shared_prefix(const void* query, const void* key_cache, const void* value_cache,

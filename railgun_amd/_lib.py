@@ -99,6 +99,7 @@ SIGNATURES = {
          c_int32, c_int32, c_int32, c_int32, c_int64, c_void_p, c_size_t, c_void_p],
     ),
     "rg_paged_attention_shared_prefix_workspace_bytes": (c_size_t, [c_int32] * 7),
+    "rg_paged_attention_shared_prefix_pays": (c_int, [c_int32] * 8),
     "rg_paged_attention_shared_prefix": (
         c_int,
         [c_void_p] * 6 + [c_float] + [c_int32] * 8 + [c_int64, c_void_p, c_size_t, c_void_p],

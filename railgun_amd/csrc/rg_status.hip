@@ -1,4 +1,5 @@
 // Error reporting, initialisation and host-only helpers of the C ABI.
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -34,12 +35,16 @@ int check_launch(const char* what) {
   return ok();
 }
 
+// (Asked of the runtime once per device: plans and workspace queries ask several times per call.)
 int device_cu_count() {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];
   int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) {
-    n = 256;
-  }
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  const bool keep = dev >= 0 && dev < kDevices;
+  if (keep && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+  if (keep) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

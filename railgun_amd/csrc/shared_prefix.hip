@@ -581,12 +581,6 @@ void launch_shared(const StreamArgs& sa, const PrefixArgs& pa, int G, int groups
   }
 }
 
-// Whether the shared product takes the call (else every sequence reads the prefix for itself).
-bool shared_applies(const Shape& sh, int32_t dtype, int64_t kv_stride, const void* q, const void* kc, const void* vc,
-                    const void* out) {
-  return sh.D <= 128 && sh.B > 1 && tiles_take(sh, dtype, kv_stride, q, kc, vc, out);
-}
-
 struct SharedPlan {
   int32_t rows, row_tiles, tiles, split_tiles, splits, workers, stream_groups;
 };
@@ -614,6 +608,27 @@ SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks, bool f32) {
   p.stream_groups = (int32_t)ceil_div(p.workers, kPreWaves);
   return p;
 }
+// Whether the shared product takes the call (else every sequence reads the prefix for itself).
+bool shared_applies(const Shape& sh, int32_t dtype, int64_t kv_stride, const void* q, const void* kc, const void* vc,
+                    const void* out) {
+  return sh.D <= 128 && sh.B > 1 && tiles_take(sh, dtype, kv_stride, q, kc, vc, out);
+}
+
+// Whether the product saves more than it adds.  It saves all but one reading of the prefix, at the 8 TB/s at which
+// the plain decode reads blocks that its sequences share; it adds the product's time over the CUs (a key tile of
+// kPreRows rows, full or not: 0.45 us in 16 bits, 3.4 in fp32 at head_dim 128) and the merge's splits and its
+// launch where the plain decode of a short table is one kernel (4 us).
+//   Measured (32 / 8 heads, 1 to 200 tokens behind the prefix; shared and plain, us): bf16, head_dim 128, 4
+// sequences: 512 tokens 15.0 / 13.3, 8,192 19.4 / 29.9; 32: 128 tokens 15.9 / 14.5, 512 16.8 / 20.5, 8,192
+// 24.6 / 141; head_dim 64, 32: 512 tokens 18.3 / 11.5, 2,048 19.7 / 29.9.  fp32, head_dim 128, 2: 8,192 tokens
+// 48.1 / 35.1; 8: 49.6 / 75.9, 512 tokens 20.4 / 17.5; 64: 512 tokens 28.6 / 48.4.
+bool shared_pays(const Shape& sh, int32_t dtype, const SharedPlan& p) {
+  const double saved = 2.0 * (sh.B - 1) * p.tiles * kTileKeys * sh.Hkv * sh.D * dtype_bytes(dtype) / 8e12;
+  const double product = (double)p.tiles * sh.Hkv * p.row_tiles * sh.D * (dtype == RG_DTYPE_F32 ? 27e-9 : 3.5e-9) /
+                         device_cu_count();
+  return saved > product + 4e-6;
+}
+
 size_t prefix_bytes(const Shape& sh, const SharedPlan& p, size_t* ml_at) {
   const size_t n = (size_t)sh.Hkv * p.splits * p.rows;
   const size_t acc = align_up(n * sh.D * 4, 256);
@@ -654,6 +669,20 @@ extern "C" size_t rg_paged_attention_shared_prefix_workspace_bytes(int32_t batch
     }
   }
   return n;
+}
+
+extern "C" int rg_paged_attention_shared_prefix_pays(int32_t batch_size, int32_t num_heads, int32_t num_kv_heads,
+                                                     int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq,
+                                                     int32_t shared_blocks, int32_t dtype) {
+  if (batch_size <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
+      block_size <= 0 || shared_blocks <= 0 || shared_blocks > max_blocks_per_seq || dtype_bytes(dtype) == 0) {
+    return 0;
+  }
+  const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  return shared_applies(sh, dtype, 16, nullptr, nullptr, nullptr, nullptr) &&
+                 shared_pays(sh, dtype, plan_shared(sh, shared_blocks, dtype == RG_DTYPE_F32))
+             ? 1
+             : 0;
 }
 
 extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* key_cache, const void* value_cache,

@@ -62,6 +62,21 @@ def _require_i32(*tensors: torch.Tensor) -> None:
             )
 
 
+def _require_table(block_table: torch.Tensor, context_lens: torch.Tensor, batch: int, max_blocks: int) -> None:
+    if block_table.dim() != 2 or block_table.shape[0] < batch or block_table.shape[1] != max_blocks or \
+            context_lens.numel() < batch:
+        raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                           f"block_table must be [batch, {max_blocks}] and context_lens [batch] with {batch} rows, got "
+                           f"{tuple(block_table.shape)} and {tuple(context_lens.shape)}")
+
+
+def _require_scored_lens(scored_lens: Optional[torch.Tensor], batch: int) -> None:
+    if scored_lens is not None:
+        _require_i32(scored_lens)
+        if scored_lens.numel() < batch:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "scored_lens needs one entry per sequence")
+
+
 def cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
     """(num_kv_heads, block_size, head_dim, kv_block_stride) of a [NB, H_kv, bs, D] cache view.
 
@@ -115,6 +130,16 @@ class PagedAttentionKernels:
         ordinal = device.index if isinstance(device, torch.device) else int(device)
         self.ordinal = 0 if ordinal is None else ordinal
         check(self.lib.rg_init(self.ordinal))
+        # What the execute_* forms asked the library, by entry and shape: a query costs as much host time
+        # as a tenth of a small call, and its answer depends on the shape and the device alone.
+        self._answers: dict = {}
+
+    def _ask(self, entry: str, *shape: int) -> int:
+        key = (entry, shape)
+        n = self._answers.get(key)
+        if n is None:
+            n = self._answers[key] = int(getattr(self.lib, entry)(*shape))
+        return n
 
     # mod.rs:196-225
     def launch_rope(self, x, cos_sin, positions, num_heads: int, head_dim: int, num_tokens: int) -> None:
@@ -216,6 +241,13 @@ class PagedAttentionKernels:
         return int(self.lib.rg_paged_attention_shared_prefix_workspace_bytes(
             batch_size, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, shared_blocks))
 
+    def shared_prefix_pays(self, batch_size: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                           max_blocks_per_seq: int, shared_blocks: int, dtype: torch.dtype) -> bool:
+        """Whether launch_shared_prefix is expected to be faster than launch_v1 for this shape."""
+        code = _DTYPES.get(dtype)
+        return code is not None and bool(self.lib.rg_paged_attention_shared_prefix_pays(
+            batch_size, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, shared_blocks, code))
+
     def launch_shared_prefix(self, query, key_cache, value_cache, block_table, context_lens, output, scale: float,
                              num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
                              max_blocks_per_seq: int, batch_size: int, shared_blocks: int,
@@ -224,9 +256,17 @@ class PagedAttentionKernels:
         entries: those blocks are read once for many rows (rg_paged_attention_shared_prefix)."""
         _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, workspace)
         _require_i32(block_table, context_lens)
+        _require_table(block_table, context_lens, batch_size, max_blocks_per_seq)
+        self._shared_prefix(query, key_cache, value_cache, block_table, context_lens, output, scale, num_heads,
+                            num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size, shared_blocks,
+                            workspace)
+
+    def _shared_prefix(self, query, key_cache, value_cache, block_table, context_lens, output, scale, num_heads,
+                       num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size, shared_blocks,
+                       workspace) -> None:
         check(self.lib.rg_paged_attention_shared_prefix(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
-            context_lens.data_ptr(), output.data_ptr(), float(scale), num_heads, num_kv_heads, head_dim, block_size,
+            context_lens.data_ptr(), output.data_ptr(), scale, num_heads, num_kv_heads, head_dim, block_size,
             max_blocks_per_seq, batch_size, shared_blocks, dtype_code(query), key_cache.stride(0),
             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(query)))
 
@@ -246,15 +286,20 @@ class PagedAttentionKernels:
         belongs to one sequence of the call."""
         _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens, workspace)
         _require_i32(block_table, context_lens)
-        if scored_lens is not None:
-            _require_i32(scored_lens)
-            if int(scored_lens.numel()) < batch_size:
-                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "scored_lens needs one entry per sequence")
+        _require_scored_lens(scored_lens, batch_size)
         check_scores(scores, key_cache)
+        _require_table(block_table, context_lens, batch_size, max_blocks_per_seq)
+        self._v1_scores(query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens,
+                        first_scored, scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                        batch_size, workspace)
+
+    def _v1_scores(self, query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens,
+                   first_scored, scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                   batch_size, workspace) -> None:
         check(self.lib.rg_paged_attention_v1_scores(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
             context_lens.data_ptr(), output.data_ptr(), scores.data_ptr(), _ptr(scored_lens), first_scored,
-            float(scale), num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size,
+            scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size,
             dtype_code(query), key_cache.stride(0), scores.stride(0), workspace.data_ptr(),
             workspace.numel() * workspace.element_size(), _stream(query)))
 
@@ -462,7 +507,8 @@ class PagedAttentionKernels:
         if kept_positions is not None and int(kept_positions.numel()) != layers * batch * hkv * budget:
             raise bad(f"kept_positions must be [{layers}, {batch}, {hkv}, {budget}]")
         if workspace is None:
-            nbytes = self.evict_workspace_bytes(layers, batch, hkv, budget if kept_positions is None else 1)
+            nbytes = self._ask("rg_evict_cache_workspace_bytes", layers, batch, hkv,
+                               budget if kept_positions is None else 1)
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=key_cache.device)
         check(self.lib.rg_evict_cache(
             key_cache.data_ptr(), value_cache.data_ptr(), scores.data_ptr(), block_table.data_ptr(),
@@ -536,36 +582,46 @@ class PagedAttentionOp:
 
     def _check_decode(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       block_table: torch.Tensor, context_lens: torch.Tensor) -> tuple:
-        """(batch, heads, head_dim, block_size, max_blocks) of one decode call, checked against the op."""
-        if q.dim() != 3 or not q.is_contiguous():
-            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                               f"q must be contiguous [batch, heads, head_dim], got {tuple(q.shape)}")
+        """(batch, max_blocks) of one decode call, its tensors checked against the op and each other."""
         _require_cuda(q, k_cache, v_cache, block_table, context_lens)
-        batch, heads, d = (int(x) for x in q.shape)
-        hkv, bs, cache_d, _ = cache_geometry(k_cache, v_cache)
-        if (hkv, heads, d, cache_d, bs) != (self.num_kv_heads, self.num_heads, self.head_dim, self.head_dim,
-                                            self.block_size) or q.dtype != k_cache.dtype:
+        _require_i32(block_table, context_lens)
+        hkv, bs, d, _ = cache_geometry(k_cache, v_cache)
+        qs, ts = q.shape, block_table.shape
+        if len(qs) != 3 or not q.is_contiguous():
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                               f"q {tuple(q.shape)} {q.dtype} and caches {tuple(k_cache.shape)} {k_cache.dtype} do not "
+                               f"q must be contiguous [batch, heads, head_dim], got {tuple(qs)}")
+        if qs[1] != self.num_heads or qs[2] != self.head_dim or d != self.head_dim or hkv != self.num_kv_heads or \
+                bs != self.block_size or q.dtype != k_cache.dtype:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               f"q {tuple(qs)} {q.dtype} and caches {tuple(k_cache.shape)} {k_cache.dtype} do not "
                                f"fit the op's {self.num_heads} / {self.num_kv_heads} heads of {self.head_dim}, blocks of "
                                f"{self.block_size}")
-        if block_table.dim() != 2 or int(block_table.shape[0]) != batch or int(context_lens.numel()) != batch:
+        if len(ts) != 2 or ts[0] != qs[0] or context_lens.numel() != qs[0]:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "block_table and context_lens need one row per sequence")
-        return batch, heads, d, bs, int(block_table.shape[1])
+        return qs[0], ts[1]
 
     def execute_shared_prefix(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                               block_table: torch.Tensor, context_lens: torch.Tensor, shared_blocks: int,
                               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """execute() for sequences whose block tables begin with the same ``shared_blocks`` entries
-        (launch_shared_prefix); the workspace is allocated here when omitted."""
-        batch, heads, d, bs, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
+        """execute() for sequences whose block tables begin with the same ``shared_blocks`` entries:
+        launch_shared_prefix where it pays, else launch_v1.  The workspace
+        (shared_prefix_workspace_bytes) is allocated here when omitted."""
+        batch, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
+        if not 0 <= shared_blocks <= mb:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, f"shared_blocks {shared_blocks} outside 0 .. {mb}")
         out = torch.empty_like(q)
-        k = self.kernels
+        k, heads, hkv, d, bs = self.kernels, self.num_heads, self.num_kv_heads, self.head_dim, self.block_size
+        if not k._ask("rg_paged_attention_shared_prefix_pays", batch, heads, hkv, d, bs, mb, shared_blocks,
+                      dtype_code(q)):
+            shared_blocks = 0
         if workspace is None:
-            workspace = torch.empty(k.shared_prefix_workspace_bytes(batch, heads, self.num_kv_heads, d, bs, mb,
-                                                                    shared_blocks), dtype=torch.uint8, device=q.device)
-        k.launch_shared_prefix(q, k_cache, v_cache, block_table, context_lens, out, self.scale, heads,
-                               self.num_kv_heads, d, bs, mb, batch, shared_blocks, workspace)
+            nbytes = k._ask("rg_paged_attention_shared_prefix_workspace_bytes", batch, heads, hkv, d, bs, mb,
+                            shared_blocks)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        else:
+            _require_cuda(workspace)
+        k._shared_prefix(q, k_cache, v_cache, block_table, context_lens, out, self.scale, heads, hkv, d, bs, mb, batch,
+                         shared_blocks, workspace)
         return out
 
     def execute_with_scores(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -574,14 +630,17 @@ class PagedAttentionOp:
                             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """execute() that also gathers every cached token's attention weight in ``scores``
         (launch_v1_scores); the workspace is allocated here when omitted."""
-        batch, heads, d, bs, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
+        batch, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
+        _require_cuda(scores, scored_lens, workspace)
+        _require_scored_lens(scored_lens, batch)
+        check_scores(scores, k_cache)
         out = torch.empty_like(q)
-        k = self.kernels
+        k, heads, hkv, d, bs = self.kernels, self.num_heads, self.num_kv_heads, self.head_dim, self.block_size
         if workspace is None:
-            workspace = torch.empty(k.v1_scores_workspace_bytes(batch, heads, self.num_kv_heads, d, bs, mb),
-                                    dtype=torch.uint8, device=q.device)
-        k.launch_v1_scores(q, k_cache, v_cache, block_table, context_lens, out, scores, scored_lens, first_scored,
-                           self.scale, heads, self.num_kv_heads, d, bs, mb, batch, workspace)
+            nbytes = k._ask("rg_paged_attention_v1_scores_workspace_bytes", batch, heads, hkv, d, bs, mb)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        k._v1_scores(q, k_cache, v_cache, block_table, context_lens, out, scores, scored_lens, first_scored,
+                     self.scale, heads, hkv, d, bs, mb, batch, workspace)
         return out
 
     def reshape_and_cache(self, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

@@ -145,3 +145,13 @@ def test_shared_prefix_workspace_bytes():
     f = railgun_amd.load_library().rg_paged_attention_shared_prefix_workspace_bytes
     assert f(3, 8, 2, 64, 16, 40, 20) >= railgun_amd.load_library().rg_paged_attention_v1_workspace_bytes(3, 8, 2, 64, 16, 40)
     assert f(0, 8, 2, 64, 16, 4, 2) == f(3, 7, 2, 64, 16, 4, 2) == f(3, 8, 2, 64, 16, 4, 5) == 0
+
+
+def test_shared_prefix_pays():
+    f = railgun_amd.load_library().rg_paged_attention_shared_prefix_pays
+    assert f(64, 32, 8, 128, 16, 200, 128, _lib.RG_DTYPE_BF16) == 1
+    assert f(1, 32, 8, 128, 16, 2000, 1280, _lib.RG_DTYPE_BF16) == 0    # one sequence
+    assert f(3, 32, 8, 64, 16, 9, 6, _lib.RG_DTYPE_F32) == 0            # little to save
+    assert f(64, 32, 8, 96, 16, 200, 128, _lib.RG_DTYPE_BF16) == 0      # no such tile
+    assert f(64, 32, 7, 128, 16, 200, 128, _lib.RG_DTYPE_BF16) == f(64, 32, 8, 128, 16, 200, 201, _lib.RG_DTYPE_BF16) == 0
+    assert f(64, 32, 8, 128, 16, 200, 0, _lib.RG_DTYPE_BF16) == f(64, 32, 8, 128, 16, 200, 128, 9) == 0

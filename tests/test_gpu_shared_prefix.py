@@ -48,9 +48,17 @@ class Batch:
         return PagedAttentionOp(self.scale, self.heads, self.hkv, self.d, self.bs, kernels)
 
     def run(self, kernels, workspace=None, lens=None):
-        return self.op(kernels).execute_shared_prefix(self.q, self.kc, self.vc, i32(self.table, self.device),
-                                                      i32(self.ctx if lens is None else lens, self.device), self.shared,
-                                                      workspace)
+        """launch_shared_prefix: the shared product wherever its shapes allow it."""
+        out = torch.full_like(self.q, float("nan"))
+        b, mb = self.table.shape
+        shape = (b, self.heads, self.hkv, self.d, self.bs, mb)
+        if workspace is None:
+            n = kernels.shared_prefix_workspace_bytes(*shape, self.shared)
+            workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
+        kernels.launch_shared_prefix(self.q, self.kc, self.vc, i32(self.table, self.device),
+                                     i32(self.ctx if lens is None else lens, self.device), out, self.scale,
+                                     self.heads, self.hkv, self.d, self.bs, mb, b, self.shared, workspace)
+        return out
 
     def verify(self, out):
         want, tol, _, _ = attention64(self.q, self.kc, self.vc, self.table, self.ctx, self.scale, self.dtype,
@@ -148,18 +156,18 @@ def test_equals_the_plain_decode_of_the_same_tables(device, kernels):
 
 def test_replayed_graph(device, kernels):
     b = Batch(device, [400, 330, 0, 321], 20, heads=16, hkv=4, d=128, seed=11)
-    op, table, lens = b.op(kernels), i32(b.table, device), i32(b.ctx, device)
-    ws = torch.empty(kernels.shared_prefix_workspace_bytes(4, 16, 4, 128, 16, b.table.shape[1], 20), dtype=torch.uint8,
-                     device=device)
+    table, lens, mb = i32(b.table, device), i32(b.ctx, device), b.table.shape[1]
+    ws = torch.empty(kernels.shared_prefix_workspace_bytes(4, 16, 4, 128, 16, mb, 20), dtype=torch.uint8, device=device)
+    out = torch.empty_like(b.q)
 
     def step():
-        return op.execute_shared_prefix(b.q, b.kc, b.vc, table, lens, 20, ws)
+        kernels.launch_shared_prefix(b.q, b.kc, b.vc, table, lens, out, b.scale, 16, 4, 128, 16, mb, 4, 20, ws)
 
     step()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out = step()
+        step()
     for i in range(3):
         b.q.copy_(torch.randn_like(b.q))
         graph.replay()
@@ -185,6 +193,21 @@ def test_pool_far_past_32_bits(device, kernels):
     b.check(kernels)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch,shared,pays", [(3, 4, False), (150, 40, True)])
+def test_op(device, kernels, dtype, batch, shared, pays):
+    """The op takes the shared product where it pays, and is right on either side."""
+    ctx = [shared * 16 + i % 50 for i in range(batch - 1)] + [0]
+    b = Batch(device, ctx, shared, dtype, heads=16, hkv=4, d=128, seed=batch)
+    mb = b.table.shape[1]
+    assert kernels.shared_prefix_pays(batch, 16, 4, 128, 16, mb, shared, b.q.dtype) is pays
+    table, lens = i32(b.table, device), i32(b.ctx, device)
+    b.verify(b.op(kernels).execute_shared_prefix(b.q, b.kc, b.vc, table, lens, shared))
+    ws = torch.empty(kernels.shared_prefix_workspace_bytes(batch, 16, 4, 128, 16, mb, shared), dtype=torch.uint8,
+                     device=device)
+    b.verify(b.op(kernels).execute_shared_prefix(b.q, b.kc, b.vc, table, lens, shared, ws))
+
+
 def test_refusals(device, kernels):
     b = Batch(device, [40, 30], 1, seed=14)
     op, table, lens = b.op(kernels), i32(b.table, device), i32(b.ctx, device)
@@ -195,3 +218,9 @@ def test_refusals(device, kernels):
                    dict(workspace=torch.empty(16, dtype=torch.uint8, device=device))):
         with pytest.raises(RailgunError):
             op.execute_shared_prefix(**{**good, **change})
+    ws = torch.empty(kernels.shared_prefix_workspace_bytes(2, 8, 2, 64, 16, table.shape[1], 1), dtype=torch.uint8,
+                     device=device)
+    for t, n in ((table[:1], 2), (table, 3)):  # a row short, rows of another width than said
+        with pytest.raises(RailgunError):
+            kernels.launch_shared_prefix(b.q, b.kc, b.vc, t, lens, torch.empty_like(b.q), 0.1, 8, 2, 64, 16,
+                                         table.shape[1] + (n == 3), 2, 1, ws)
