@@ -394,10 +394,6 @@ __global__ __launch_bounds__(64 * G) void decode_stream_merge_kernel(StreamArgs 
 // 3.4 of the two kernels and the gap between them; fp32 heads of 64 at 400 tokens 10.4 against 8.8 +
 // 3.4.  Its slope is P.V on the VALU, ~1,100 cycles a sub-block and
 // wave; 16 tokens a wave more cost 1.1 us.
-constexpr int kShortWaves = 8;
-constexpr int kShortThreads = 64 * kShortWaves;
-constexpr int kShortMaxTokens = 16 * 64 * kShortWaves;  // one table entry per lane and wave
-
 template <typename T, int D, int G, bool ROPE>
 __global__ __launch_bounds__(kShortThreads) void decode_short_kernel(
     StreamArgs a, const typename DecodeTileFor<T, D, G>::S* __restrict__ q_ptr,
@@ -828,28 +824,6 @@ int32_t v1_num_partitions(const Shape& sh) {
 }
 
 // ---- stream-K path ----
-
-// Whether the one-launch kernel takes the call: G 1 to 8 at head_dim 64 or 128, and the lines below
-// on the table's width, which stands for the contexts that the host does not know (contexts shorter
-// than it only make the call shorter), and on the segments.  One CU streams a segment, and a second
-// workgroup does not fit beside the first, so the segments past one per CU run after the others.
-//   Up to one segment per CU: the last width at which no ratio of heads (1, 4, 7, 8) at 8 to 256
-// segments was slower than the two kernels back to back (time here over time there, mean and worst):
-// head_dim 128 in 16 bits 0.90 / 0.96 at 320 tokens, 0.96 / 1.05 at 384, 1.08 / 1.19 at 512; in
-// fp32 0.88 / 0.92 at 192, 0.97 / 1.08 at 256; head_dim 64 in 16 bits 0.89 / 1.00 at 896, 0.95 / 1.06
-// at 1,024; in fp32 0.92 / 0.98 at 512.
-//   Up to two per CU: 64 tokens, 0.92 at worst (264 to 512 segments); at 128 already 1.33, at 320
-// 1.48.  More: never (1,024 segments of 64 tokens 1.27 to 1.60).
-bool short_applies(const Shape& sh, int elem_bytes) {
-  const int64_t tokens = (int64_t)sh.MB * sh.bs, segments = (int64_t)sh.B * sh.Hkv;
-  const int64_t widest = (sh.D == 64 ? 224 : 160) + (elem_bytes == 4 ? 32 : 0);  // KB of K and V
-  if ((sh.D != 64 && sh.D != 128) || sh.H / sh.Hkv > 8 || tokens > kShortMaxTokens || sh.B > 65535 ||
-      tokens * sh.D * 2 * elem_bytes > widest << 10) {
-    return false;
-  }
-  const int64_t cus = device_cu_count();  // (two calls of the runtime: asked for small tables only)
-  return segments <= cus || (segments <= 2 * cus && tokens <= 64);
-}
 
 template <typename T, int D, int G, bool ROPE = false>
 void launch_stream(const StreamArgs& sa, const DecodeArgs& a, hipStream_t s) {

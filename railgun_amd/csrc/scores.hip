@@ -21,6 +21,7 @@ constexpr int kFinThreads = 256;
 constexpr int kFinWaves = kFinThreads / 64;
 constexpr int kFinTokens = 1024;   // tokens a workgroup turns into weights at a time
 constexpr int kMaxGroup = 512;     // query heads to a kv-head
+constexpr int kShortMaxScored = 1024;  // tokens of table that the one-launch kernel takes (short_applies admits no more)
 
 struct ScoreArgs {
   void* out;
@@ -272,6 +273,174 @@ __global__ __launch_bounds__(kFinThreads) void scores_finish_kernel(ScoreArgs a)
   }
 }
 
+// Tables of few tokens (short_applies): one workgroup per segment does it all, one launch.  Its waves take the
+// 16-token sub-blocks in turn, as the plain decode's kernel for such tables does; the raw scores stay in LDS
+// (`raw`, [tokens][G]), and once the waves' partials are merged every thread turns some tokens' into weights.
+//   Bound by latency: two sequences of up to 77 tokens in fp32 (32 / 8 heads of 64) 11.5 us a call, with the worker and the finish kernel 14.5.
+template <typename T, int D, int G>
+__global__ __launch_bounds__(kShortThreads) void scores_short_kernel(
+    ScoreArgs a, int64_t kv_stride, int bs_shift, const typename DecodeTileFor<T, D, G>::S* __restrict__ q,
+    const typename DecodeTileFor<T, D, G>::S* __restrict__ kc, const typename DecodeTileFor<T, D, G>::S* __restrict__ vc) {
+  using Tile = DecodeTileFor<T, D, G>;
+  using E = elem<T>;
+  constexpr int GP = Tile::GP, HG = Tile::HG, NK = Tile::NK, NV = Tile::NV;
+  constexpr int AHEAD = std::is_same_v<T, f32_t> && D == 128 ? 1 : 2, NBUF = AHEAD + 1;
+  extern __shared__ float raw[];
+  __shared__ float p_lds[kShortWaves][2][kBS * GP];
+  __shared__ float alpha_lds[kShortWaves][2][GP];
+  __shared__ float acc_lds[kShortWaves][G * D];
+  __shared__ float ml_lds[kShortWaves][2][GP];
+  const int kvh = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int max_subs = a.max_blocks << bs_shift, sub_mask = (1 << bs_shift) - 1;
+  // Sub-block w + kShortWaves lane of the table row, within the row whatever the context is.
+  const int sb = w + kShortWaves * lane;
+  const int32_t* row = a.block_table + (int64_t)s * a.max_blocks;
+  const int entry = sb < max_subs ? row[sb >> bs_shift] : 0;
+  const int len = a.context_lens[s];
+  const int scored = a.scored_lens != nullptr ? a.scored_lens[s] : INT32_MAX;
+  Tile tile;
+  tile.init(lane);
+  tile.reset();
+  tile.load_q(q + ((int64_t)s * a.num_heads + (int64_t)kvh * G) * D);
+  const int ctx = max(0, min(len, max_subs * kBS));
+  // The old scores of this thread's tokens, behind nothing but the table.
+  constexpr int PER = (kShortMaxScored + kShortThreads - 1) / kShortThreads;
+  float old[PER];
+  float* cell[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = a.first + tid + i * kShortThreads;
+    cell[i] = nullptr;
+    old[i] = 0.f;
+    if (t < ctx) {
+      const int b = t >> (4 + bs_shift);
+      cell[i] = a.scores + row[b] * a.score_stride + (int64_t)kvh * a.block_size + (t - (b << (4 + bs_shift)));
+      if (t < scored) old[i] = *cell[i];
+    }
+  }
+  const int nblk = (ctx + kBS - 1) / kBS;
+  const int nb = w < nblk ? (nblk - w + kShortWaves - 1) / kShortWaves : 0;  // this wave's sub-blocks
+  if (nb > 0) {
+    const int64_t head = (int64_t)kvh * (kBS << bs_shift) * D;
+    uint4 kbuf[NBUF][NK], vbuf[NBUF][NV];
+    auto load_block = [&](int j, uint4 (&kk)[NK], uint4 (&vv)[NV]) __attribute__((always_inline)) {
+      const int e = __builtin_amdgcn_readlane(entry, j);
+      const int64_t off = (int64_t)e * kv_stride + head + (int64_t)((w + kShortWaves * j) & sub_mask) * (kBS * D);
+      tile.template load_part<1, 0>(kc + off, vc + off, kk, vv);
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) load_block(min(u, nb - 1), kbuf[u], vbuf[u]);
+    for (int j0 = 0; j0 < nb; j0 += NBUF) {
+#pragma unroll
+      for (int u = 0; u < NBUF; ++u) {
+        const int j = j0 + u;
+        if (j < nb) {
+          load_block(min(j + AHEAD, nb - 1), kbuf[(u + AHEAD) % NBUF], vbuf[(u + AHEAD) % NBUF]);
+          const int tok0 = (w + kShortWaves * j) * kBS;
+          tile.step(kbuf[u], vbuf[u], tok0, ctx, a.scale_log2, p_lds[w][j & 1], alpha_lds[w][j & 1],
+                    [&](const f32x4_t (&c)[1]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (4 * tile.seg + r < G) raw[(tok0 + tile.col) * G + 4 * tile.seg + r] = c[0][r];
+          });
+        }
+      }
+    }
+  }
+  float lsum[4];
+  tile.reduce(lsum);
+  if (tile.vrow == 0) {
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      float4* dst = reinterpret_cast<float4*>(&acc_lds[w][h * D + tile.vd0]);
+#pragma unroll
+      for (int q4 = 0; q4 < Tile::ACC / 4; ++q4)
+        dst[q4] = make_float4(tile.acc[h][4 * q4], tile.acc[h][4 * q4 + 1], tile.acc[h][4 * q4 + 2],
+                              tile.acc[h][4 * q4 + 3]);
+    }
+  }
+  if (tile.seg < HG && tile.col == 0) {
+    *reinterpret_cast<float4*>(&ml_lds[w][0][4 * tile.seg]) =
+        make_float4(tile.m_run[0], tile.m_run[1], tile.m_run[2], tile.m_run[3]);
+    *reinterpret_cast<float4*>(&ml_lds[w][1][4 * tile.seg]) = make_float4(lsum[0], lsum[1], lsum[2], lsum[3]);
+  }
+  __syncthreads();
+  // M and 1 / L of head h over the waves.
+  auto stats = [&](int h, float& M, float& inv) __attribute__((always_inline)) {
+    M = -INFINITY;
+#pragma unroll
+    for (int ww = 0; ww < kShortWaves; ++ww) M = fmaxf(M, ml_lds[ww][0][h]);
+    float L = 0.f;
+#pragma unroll
+    for (int ww = 0; ww < kShortWaves; ++ww) {
+      const float mw = ml_lds[ww][0][h];
+      L += (mw == -INFINITY ? 0.f : exp2f(mw - M)) * ml_lds[ww][1][h];
+    }
+    inv = L != 0.f ? 1.f / L : 1.f;
+  };
+  for (int i = tid; i < G * D; i += kShortThreads) {
+    const int h = i / D;
+    float M, inv, o = 0.f;
+    stats(h, M, inv);
+#pragma unroll
+    for (int ww = 0; ww < kShortWaves; ++ww) {
+      const float mw = ml_lds[ww][0][h];
+      o += (mw == -INFINITY ? 0.f : exp2f(mw - M)) * acc_lds[ww][i];
+    }
+    E::store(static_cast<typename E::storage*>(a.out), ((int64_t)s * a.num_heads + (int64_t)kvh * G) * D + i, o * inv);
+  }
+  if (a.first >= ctx) return;
+  float M[G], inv[G];
+#pragma unroll
+  for (int h = 0; h < G; ++h) stats(h, M[h], inv[h]);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = a.first + tid + i * kShortThreads;
+    if (t < ctx) {
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < G; ++h) sum += exp2f(raw[t * G + h] * a.scale_log2 - M[h]) * inv[h];
+      *cell[i] = old[i] + sum;
+    }
+  }
+}
+
+// The one-launch kernel takes what the plain decode's takes, up to kShortMaxScored tokens of table; fp32 at
+// head_dim 128 with 8 heads to a kv-head fills the registers without the scores.
+bool scores_short_applies(const Shape& sh, int32_t dtype) {
+  return (int64_t)sh.MB * sh.bs <= kShortMaxScored && short_applies(sh, dtype_bytes(dtype)) &&
+         !(dtype == RG_DTYPE_F32 && sh.D == 128 && sh.H / sh.Hkv == 8);
+}
+
+template <typename T>
+void launch_scores_short(const ScoreArgs& f, int64_t kv_stride, int bs_shift, const Shape& sh, const void* q,
+                         const void* kc, const void* vc, hipStream_t s) {
+  auto go = [&](auto d, auto g) {
+    constexpr int D = decltype(d)::value, G = decltype(g)::value;
+    using S = typename DecodeTileFor<T, D, G>::S;
+    hipLaunchKernelGGL((scores_short_kernel<T, D, G>), dim3(sh.Hkv, sh.B), dim3(kShortThreads),
+                       (size_t)sh.MB * sh.bs * G * 4, s, f, kv_stride, bs_shift, static_cast<const S*>(q),
+                       static_cast<const S*>(kc), static_cast<const S*>(vc));
+  };
+  auto by_group = [&](auto d) {
+    switch (sh.H / sh.Hkv) {
+      case 1: go(d, std::integral_constant<int, 1>{}); break;
+      case 2: go(d, std::integral_constant<int, 2>{}); break;
+      case 3: go(d, std::integral_constant<int, 3>{}); break;
+      case 4: go(d, std::integral_constant<int, 4>{}); break;
+      case 5: go(d, std::integral_constant<int, 5>{}); break;
+      case 6: go(d, std::integral_constant<int, 6>{}); break;
+      case 7: go(d, std::integral_constant<int, 7>{}); break;
+      default:  // 8
+        if constexpr (!(std::is_same_v<T, f32_t> && decltype(d)::value == 128)) go(d, std::integral_constant<int, 8>{});
+        break;
+    }
+  };
+  if (sh.D == 128) by_group(std::integral_constant<int, 128>{});
+  else by_group(std::integral_constant<int, 64>{});
+}
+
 template <typename T, int D>
 void launch_scores_stream(const StreamArgs& sa, int G, const void* q, const void* kc, const void* vc, const int32_t* bt,
                           const int32_t* cl, hipStream_t s) {
@@ -418,6 +587,12 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
   f.max_blocks = max_blocks_per_seq;
   f.num_partitions = generic_partitions(sh);
   f.score_stride = score_block_stride ? score_block_stride : block;
+  if (tiles && scores_short_applies(sh, dtype)) {
+    return dispatch_dtype(dtype, [&](auto tag) {
+      launch_scores_short<decltype(tag)>(f, kv_stride, block_shift(block_size), sh, query, key_cache, value_cache, s);
+      return check_launch(op);
+    });
+  }
   if (tiles) {
     StreamScratch sc;
     stream_bytes(sh, workers, &sc, ws + logits);

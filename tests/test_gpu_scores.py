@@ -204,3 +204,17 @@ def test_refusals(device, kernels):
 def test_workers_with_more_tokens_than_they_gather_at_once(device, kernels):
     """16 heads to a kv-head at head_dim 64: a worker gathers the raw scores of 512 tokens, and has 586."""
     Batch(device, [150000], heads=64, hkv=4, d=64, seed=15).check(kernels, scored=np.array([149000]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,hkv,d", [(4, 4, 64), (8, 4, 128), (6, 2, 64), (8, 2, 128), (10, 2, 64), (12, 2, 128),
+                                         (14, 2, 128), (16, 2, 64), (16, 2, 128)])
+@pytest.mark.parametrize("first", [0, 70])
+def test_short_tables(device, kernels, dtype, heads, hkv, d, first):
+    """Tables that one launch takes (and, fp32 with 8 heads of 128, the one it does not)."""
+    b = Batch(device, [150, 0, 1, 16, 17, 129, 128], dtype, heads, hkv, d, bs=32 if d == 64 else 16, seed=heads + d)
+    b.check(kernels, scored=np.array([149, 0, 0, 3, 17, 0, 500]), first=first)
+
+
+def test_widest_short_tables(device, kernels):
+    Batch(device, [890, 3, 512, 513], "bf16", 16, 2, 64, seed=16).check(kernels, scored=np.array([300, 0, 512, 9]))
