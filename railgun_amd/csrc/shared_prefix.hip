@@ -491,19 +491,22 @@ __global__ __launch_bounds__(kPreThreads, (groups_per_cu<T, D, G>())) void share
   else prefix_product<T, D>(pa, q, kc, vc, block_table, ring, u, w, lane);
 }
 
-// One workgroup per (kv-head, sequence), a wave per query head: lane l folds dims [l PER, (l + 1) PER) of the
-// prefix's splits (if the sequence has the whole prefix) and of the stream-K workers' partials, in that order.
-// A chain of memory round trips and little else, so the prefix's partials are asked for together with the
-// length and the segment's descriptor: they are there for every row, if only as numbers that do not count.
-template <typename T, int D, int G>
-__global__ __launch_bounds__(64 * G) void shared_merge_kernel(StreamArgs sa, PrefixArgs pa,
-                                                              const int32_t* __restrict__ context_lens) {
+// One workgroup per (kv-head, sequence), R waves per query head: lane l of wave r folds dims [l PER, (l + 1) PER) of
+// every R-th of the prefix's splits (if the sequence has the whole prefix) and of the stream-K workers' partials,
+// in that order; the R results join through LDS.  A chain of memory round trips and little else, so the first of
+// the prefix's partials are asked for together with the length and the segment's descriptor: they are there for
+// every row, if only as numbers that do not count.
+//   Two waves a head: 16 rows over 16,384 shared tokens (32 splits) 22.2 -> 20.9 us a call, 4 over 8,192 18.9 ->
+// 17.3; with four splits or fewer one is as fast.
+template <typename T, int D, int G, int R>
+__global__ __launch_bounds__(64 * G * R) void shared_merge_kernel(StreamArgs sa, PrefixArgs pa,
+                                                                  const int32_t* __restrict__ context_lens) {
   using S = typename elem<T>::storage;
   constexpr int PER = D / 64;
   constexpr int AHEAD = 4;
-  const int kvh = blockIdx.x, s = blockIdx.y, h = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int kvh = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63;
+  const int h = (threadIdx.x >> 6) % G, r = (threadIdx.x >> 6) / G;
   const int64_t seg = (int64_t)s * sa.num_kv_heads + kvh;
-  S* out = static_cast<S*>(sa.out) + ((int64_t)s * sa.num_heads + (int64_t)kvh * G + h) * D + lane * PER;
   const int2 dsc = sa.seg_desc[seg];  // (stale, and not used, where the segment has no tokens of its own)
   const int len = context_lens[s];
   struct Part {
@@ -519,8 +522,8 @@ __global__ __launch_bounds__(64 * G) void shared_merge_kernel(StreamArgs sa, Pre
   };
   const int64_t r0 = (int64_t)kvh * pa.splits * pa.rows + s * G + h;
   auto split = [&](int p) __attribute__((always_inline)) {
-    const int64_t r = r0 + (int64_t)min(p, pa.splits - 1) * pa.rows;
-    return load(pa.ml + 2 * r, pa.acc + r * D);
+    const int64_t at = r0 + (int64_t)min(p, pa.splits - 1) * pa.rows;
+    return load(pa.ml + 2 * at, pa.acc + at * D);
   };
   float m = -INFINITY, l = 0.f;
   float acc[PER];
@@ -537,21 +540,41 @@ __global__ __launch_bounds__(64 * G) void shared_merge_kernel(StreamArgs sa, Pre
   };
   Part first[AHEAD];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) first[i] = split(i);
+  for (int i = 0; i < AHEAD; ++i) first[i] = split(r + i * R);
   const int ctx = max(0, min(len, sa.max_blocks * kBS));
   const bool has = ctx >= sa.prefix;
   const int np = past_prefix(ctx, sa.prefix) > 0 ? dsc.y : 0;
   const int64_t p0 = dsc.x + seg;
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) fold(first[i], has && i < pa.splits);
+  for (int i = 0; i < AHEAD; ++i) fold(first[i], has && r + i * R < pa.splits);
   if (has) {
 #pragma unroll 4
-    for (int p = AHEAD; p < pa.splits; ++p) fold(split(p), true);
+    for (int p = r + AHEAD * R; p < pa.splits; p += R) fold(split(p), true);
   }
 #pragma unroll 4
-  for (int p = 0; p < np; ++p) {
+  for (int p = r; p < np; p += R) {
     fold(load(sa.part_ml + (p0 + p) * (2 * G) + 2 * h, sa.part_acc + (p0 + p) * (G * D) + h * D), true);
   }
+  if constexpr (R > 1) {
+    __shared__ float2 ml_lds[R][G];
+    __shared__ float acc_lds[R][G][D];
+    if (r > 0) {
+      if (lane == 0) ml_lds[r][h] = make_float2(m, l);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc_lds[r][h][lane * PER + e] = acc[e];
+    }
+    __syncthreads();
+    if (r > 0) return;
+#pragma unroll
+    for (int i = 1; i < R; ++i) {
+      Part p;
+      p.ml = ml_lds[i][h];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) p.v[e] = acc_lds[i][h][lane * PER + e];
+      fold(p, p.ml.x != -INFINITY);
+    }
+  }
+  S* out = static_cast<S*>(sa.out) + ((int64_t)s * sa.num_heads + (int64_t)kvh * G + h) * D + lane * PER;
   const float inv = l != 0.f ? 1.f / l : 1.f;
 #pragma unroll
   for (int e = 0; e < PER; ++e) out[e] = elem<T>::from_f32(acc[e] * inv);
@@ -565,8 +588,15 @@ void launch_shared(const StreamArgs& sa, const PrefixArgs& pa, int G, int groups
     using S = typename DecodeTileFor<T, D, GC>::S;
     hipLaunchKernelGGL((shared_prefix_kernel<T, D, GC>), dim3(groups), dim3(kPreThreads), 0, s, sa, pa,
                        static_cast<const S*>(q), static_cast<const S*>(kc), static_cast<const S*>(vc), bt, cl);
-    hipLaunchKernelGGL((shared_merge_kernel<T, D, GC>), dim3(sa.num_kv_heads, sa.batch), dim3(64 * GC), 0, s, sa, pa,
-                       cl);
+    // (Two waves to a head where there are more than four splits, and room in the workgroup.)
+    constexpr int R = GC <= 8 ? 2 : 1;
+    if (pa.splits > 4) {
+      hipLaunchKernelGGL((shared_merge_kernel<T, D, GC, R>), dim3(sa.num_kv_heads, sa.batch), dim3(64 * GC * R), 0, s,
+                         sa, pa, cl);
+    } else {
+      hipLaunchKernelGGL((shared_merge_kernel<T, D, GC, 1>), dim3(sa.num_kv_heads, sa.batch), dim3(64 * GC), 0, s, sa,
+                         pa, cl);
+    }
   };
   switch (G) {
     case 1: go(std::integral_constant<int, 1>{}); break;
@@ -641,7 +671,7 @@ size_t prefix_bytes(const Shape& sh, const SharedPlan& p, size_t* ml_at) {
 int probe_shared_prefix_kernels() {
   hipFuncAttributes at;
   if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(shared_prefix_kernel<bf16_t, 128, 4>)) != hipSuccess ||
-      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(shared_merge_kernel<bf16_t, 128, 4>)) != hipSuccess) {
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(shared_merge_kernel<bf16_t, 128, 4, 1>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the shared-prefix kernels: %s", hipGetErrorString(hipGetLastError()));
   }
   return RG_OK;
