@@ -38,11 +38,19 @@ class PrefillChunk:
 
 @dataclass
 class DecodeSlot:
-    """batch.rs:8-19: one new token; ``seq_len`` counts it (prompt + generated so far)."""
+    """batch.rs:8-19: one new token; ``seq_len`` counts it (prompt + generated so far, less what eviction
+    dropped: the cached tokens).
+
+    ``position`` is the token's place in the text, which its rotation goes by (default: seq_len - 1;
+    larger once tokens have been evicted).  ``scored_len``, for a step that gathers attention weights:
+    how many of the cached tokens hold a gathered score (0 after a prefill; seq_len - 1 while every
+    step since gathered)."""
 
     last_token_id: int
     seq_len: int
     block_table: Sequence[int]
+    position: Optional[int] = None
+    scored_len: Optional[int] = None
 
 
 def slot_of(block_table: Sequence[int], pos: int, block_size: int) -> int:
@@ -70,6 +78,10 @@ class StepBatch:
     max_context_len: int
     max_query_len: int
     last_rows: np.ndarray = field(default=None)  # int64 [R]: row of each request's last token
+    # Leading block-table entries that all decode rows share (0 unless asked for).
+    shared_decode_blocks: int = 0
+    # int32 [decode rows]: cached tokens that hold a score, for a step that gathers attention weights.
+    scored_lens: Optional[np.ndarray] = None
 
     @property
     def num_tokens(self) -> int:
@@ -90,10 +102,40 @@ def _check_ids(table: Sequence[int]) -> None:
             raise ValueError(f"block id {int(b):#x} is not a GPU block (bit 31 marks CPU blocks, block.rs:15-36)")
 
 
+def shared_prefix_blocks(decode_slots: Sequence[DecodeSlot], block_size: int) -> int:
+    """Leading entries that the block tables of all slots have in common, whole blocks that end before
+    every slot's new token (allocator.rs forks them; a block that is written to is never shared)."""
+    if len(decode_slots) < 2:
+        return 0
+    n = min((d.seq_len - 1) // block_size for d in decode_slots)
+    first = [int(b) for b in decode_slots[0].block_table[:n]]
+    for d in decode_slots[1:]:
+        same = 0
+        while same < len(first) and int(d.block_table[same]) == first[same]:
+            same += 1
+        first = first[:same]
+    return len(first)
+
+
+def _scored_lens(decode_slots: Sequence[DecodeSlot], block_size: int, shared: int) -> np.ndarray:
+    """The slots' scored lengths; every scored block has to belong to one slot alone."""
+    seen: set = set()
+    for d in decode_slots:
+        if d.scored_len is None or not 0 <= d.scored_len < d.seq_len:
+            raise ValueError(f"decode slot of length {d.seq_len} with scored_len {d.scored_len}")
+        for b in d.block_table[shared:(d.seq_len + block_size - 1) // block_size]:
+            if int(b) in seen:
+                raise ValueError(f"block {int(b)} is scored twice in a step")
+            seen.add(int(b))
+    return np.asarray([d.scored_len for d in decode_slots], np.int32)
+
+
 def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[DecodeSlot], block_size: int,
-              max_blocks: Optional[int] = None) -> StepBatch:
+              max_blocks: Optional[int] = None, share_prefix: bool = False, gather_scores: bool = False) -> StepBatch:
     """engine.rs:184-227 plus positions / cu_seqlens; ``max_blocks`` (default: the longest
-    table) fixes the padded row length, e.g. to keep one shape across steps."""
+    table) fixes the padded row length, e.g. to keep one shape across steps.  ``share_prefix`` looks for
+    blocks that all decode rows begin with, ``gather_scores`` makes the step add the attention weights of
+    the decode rows' cached tokens, behind such a prefix, to the pool's scores."""
     tokens, positions, slots, ctx, tables = [], [], [], [], []
     cu = [0]
     for c in prefill_chunks:
@@ -118,7 +160,9 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
         if (d.seq_len + block_size - 1) // block_size > len(d.block_table):
             raise ValueError(f"decode slot of length {d.seq_len} needs more than {len(d.block_table)} blocks")
         tokens.append(int(d.last_token_id))
-        positions.append(d.seq_len - 1)
+        positions.append(d.seq_len - 1 if d.position is None else int(d.position))
+        if positions[-1] < d.seq_len - 1:
+            raise ValueError(f"decode slot at position {positions[-1]} with {d.seq_len} cached tokens")
         slots.append(slot_of(d.block_table, d.seq_len - 1, block_size))
         ctx.append(d.seq_len)
         tables.append(list(d.block_table))
@@ -129,6 +173,7 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     bt = np.zeros((len(tables), mb), np.int32)
     for r, t in enumerate(tables):
         bt[r, :len(t)] = np.asarray(t, dtype=np.int64).astype(np.int32)
+    shared = shared_prefix_blocks(decode_slots, block_size) if share_prefix else 0
     lens = np.diff(np.asarray(cu))
     last = np.concatenate([np.asarray(cu[1:], np.int64) - 1,
                            cu[-1] + np.arange(len(decode_slots), dtype=np.int64)])
@@ -136,7 +181,9 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
         tokens=np.asarray(tokens, np.int64), positions=np.asarray(positions, np.int32),
         slot_mapping=np.asarray(slots, np.int32), context_lens=np.asarray(ctx, np.int32), block_table=bt,
         cu_seqlens=np.asarray(cu, np.int32), num_prefill_seqs=len(prefill_chunks), num_prefill_tokens=cu[-1],
-        max_context_len=max(ctx, default=0), max_query_len=int(lens.max()) if len(lens) else 0, last_rows=last)
+        max_context_len=max(ctx, default=0), max_query_len=int(lens.max()) if len(lens) else 0, last_rows=last,
+        shared_decode_blocks=shared,
+        scored_lens=_scored_lens(decode_slots, block_size, shared) if gather_scores else None)
 
 
-__all__ = ["CPU_BLOCK_FLAG", "DecodeSlot", "PrefillChunk", "StepBatch", "pack_step", "slot_of"]
+__all__ = ["CPU_BLOCK_FLAG", "DecodeSlot", "PrefillChunk", "StepBatch", "pack_step", "shared_prefix_blocks", "slot_of"]

@@ -496,7 +496,7 @@ __global__ __launch_bounds__(kPreThreads, (groups_per_cu<T, D, G>())) void share
 // in that order; the R results join through LDS.  A chain of memory round trips and little else, so the first of
 // the prefix's partials are asked for together with the length and the segment's descriptor: they are there for
 // every row, if only as numbers that do not count.
-//   Two waves a head: 16 rows over 16,384 shared tokens (32 splits) 22.2 -> 20.9 us a call, 4 over 8,192 18.9 ->
+//   Two waves a head: 16 rows over 16,384 shared tokens (32 splits) 22.8 -> 20.9 us a call, 4 over 8,192 18.9 ->
 // 17.3; with four splits or fewer one is as fast.
 template <typename T, int D, int G, int R>
 __global__ __launch_bounds__(64 * G * R) void shared_merge_kernel(StreamArgs sa, PrefixArgs pa,

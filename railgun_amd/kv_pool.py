@@ -83,8 +83,11 @@ class GpuBlockPool:
     @property
     def scores(self) -> torch.Tensor:
         """fp32 [layers, NB, H_kv, bs]: the attention weight each cached token has gathered
-        (launch_v1_scores adds to it, evict goes by it); made, with zeros, when first asked for."""
+        (launch_v1_scores adds to it, evict goes by it); made, with zeros, when first asked for.
+        copy_blocks, swap_out and swap_in leave it as it is."""
         if self._scores is None:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the pool's scores are first asked for in a graph's capture: ask for them before it")
             layers, blocks, _, hkv, bs, _ = self.storage.shape
             self._scores = torch.zeros((layers, blocks, hkv, bs), device=self.device, dtype=torch.float32)
         return self._scores

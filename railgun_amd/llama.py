@@ -11,7 +11,9 @@ then decode slots, :mod:`railgun_amd.batch`) runs as:
   one pass (the reference writes the cache but never applies RoPE, defect D10);
 * attention: ``rg_prefill_packed`` for the prefill rows (causal, MFMA), the stream-K
   ``rg_paged_attention_v1`` for the decode rows (the reference sends prefill rows through
-  the decode op, D7);
+  the decode op, D7); decode rows that begin with the same blocks read those once
+  (``rg_paged_attention_shared_prefix``) where the step was packed so and it pays, and a step packed
+  to gather attention weights adds them to the pool's scores (``rg_paged_attention_v1_scores``);
 * ``rg_rms_norm`` fuses each residual add with the next RMSNorm; ``rg_silu_and_mul`` is the
   SwiGLU gate;
 * the projections of decode-sized steps (at most 128 rows) run on ``rg_linear``, the skinny
@@ -190,6 +192,7 @@ class DeviceStep:
     block_table: torch.Tensor
     cu_seqlens: torch.Tensor
     last_rows: torch.Tensor
+    scored_lens: Optional[torch.Tensor] = None
 
     @staticmethod
     def from_host(b: StepBatch, device) -> "DeviceStep":
@@ -197,7 +200,7 @@ class DeviceStep:
             return torch.from_numpy(np.ascontiguousarray(a)).to(device)
 
         return DeviceStep(b, d(b.tokens), d(b.positions), d(b.slot_mapping), d(b.context_lens), d(b.block_table),
-                          d(b.cu_seqlens), d(b.last_rows))
+                          d(b.cu_seqlens), d(b.last_rows), None if b.scored_lens is None else d(b.scored_lens))
 
 
 class RailgunLlama:
@@ -262,7 +265,18 @@ class RailgunLlama:
             k.launch_prefill_packed(q[:TP], kc, vc, st.block_table[:P], st.context_lens[:P], st.cu_seqlens,
                                     out[:TP], self.scale, H, Hkv, D, bs, mb, P, TP, b.max_query_len)
         nd = b.num_decode
-        if nd:
+        if nd and st.scored_lens is not None:
+            # A step that gathers attention weights, of the tokens behind a prefix that the rows share.
+            ws = self._workspace(k.v1_scores_workspace_bytes(nd, H, Hkv, D, bs, mb))
+            k.launch_v1_scores(q[TP:], kc, vc, st.block_table[P:], st.context_lens[P:], out[TP:],
+                               self.pool.scores[layer], st.scored_lens, b.shared_decode_blocks * bs, self.scale, H, Hkv,
+                               D, bs, mb, nd, ws)
+        elif nd and b.shared_decode_blocks and k.shared_prefix_pays(nd, H, Hkv, D, bs, mb, b.shared_decode_blocks,
+                                                                    self.dtype):
+            ws = self._workspace(k.shared_prefix_workspace_bytes(nd, H, Hkv, D, bs, mb, b.shared_decode_blocks))
+            k.launch_shared_prefix(q[TP:], kc, vc, st.block_table[P:], st.context_lens[P:], out[TP:], self.scale, H,
+                                   Hkv, D, bs, mb, nd, b.shared_decode_blocks, ws)
+        elif nd:
             ws = self._workspace(k.v1_workspace_bytes(nd, H, Hkv, D, bs, mb))
             k.launch_v1(q[TP:], kc, vc, st.block_table[P:], st.context_lens[P:], out[TP:], self.scale, H, Hkv, D,
                         bs, mb, nd, workspace=ws if ws.numel() else None)
