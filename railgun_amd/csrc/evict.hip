@@ -534,7 +534,8 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
                     ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15u) == 0;
   const int row_vecs = head_dim * eb / (wide ? 16 : 2);
   auto move = [&](auto kernel, int threads, int pieces) {
-    const int tok = std::max(1, std::min(kMoveMaxTokens, threads * pieces / (2 * row_vecs)));
+    // (A thread looks one token up: no more tokens than threads, which rows of a single piece would allow.)
+    const int tok = std::max(1, std::min({kMoveMaxTokens, threads, threads * pieces / (2 * row_vecs)}));
     const int64_t chunks = dst_block_table == nullptr ? 1 : ceil_div(most, tok);
     if (chunks > 65535) return fail(RG_ERR_NOT_SUPPORTED, "%s: a budget of %lld tokens", op, (long long)most);
     hipLaunchKernelGGL(kernel, dim3((unsigned)segments, (unsigned)chunks), dim3(threads), 0, s, a, row_vecs, tok);

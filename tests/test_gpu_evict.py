@@ -123,6 +123,13 @@ def test_shapes(device, kernels, dtype, hkv, bs, d, dst):
     c.check(kernels, 10, 3)
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 8), ("f32", 4), ("f16", 1), ("bf16", 2)])
+@pytest.mark.parametrize("dst", ["apart", "in place"])
+def test_many_short_rows(device, kernels, dtype, d, dst):
+    """Rows of one piece of the move: its workgroups take no more tokens than they have threads."""
+    Case(device, [3000, 1200], 1100, dtype=dtype, d=d, dst=dst, seed=d).check(kernels, 40, 20)
+
+
 def test_layers_and_shared_prefix(device, kernels):
     """Sequences that share their first blocks, protected: the shared blocks stay as they are."""
     c = Case(device, [700, 128, 90, 401], 128, layers=5, hkv=4, shared=2, seed=5)
