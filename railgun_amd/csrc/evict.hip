@@ -10,11 +10,12 @@
 // evict_select_kernel (one workgroup per segment) finds the threshold: scores become 32-bit keys in
 // the order of the values, and three passes over 11, 11 and 10 bits narrow the key T of the last one
 // to be kept, each with a histogram in LDS over the candidates that agree with the bits found so
-// far.  A kept candidate's place is then known without a list: before position t lie
+// far (after the first pass mostly few, which are then listed).  A kept candidate's place is then known without a list: before position t lie
 //   #{key > T before t} + min(#{key == T before t}, ties to keep)
-// kept candidates.  It leaves the kept positions in order (the caller's array, or workspace).
+// kept candidates.  The kernel leaves the kept positions in order (the caller's array, or workspace).
 // evict_move_kernel copies: what a segment has to move is cut into chunks, a workgroup each.
 #include <algorithm>
+#include <type_traits>
 
 #include "rg_common.hpp"
 
@@ -34,6 +35,7 @@ struct EvictArgs {
   int64_t layer_stride, kv_stride, score_layer_stride, score_stride;  // elements
   int32_t kept_stride, budget, recent, guarded;
   int32_t num_kv_heads, head_dim, block_size, max_blocks, max_dst_blocks, batch;
+  int32_t block_shift;  // log2(block_size) where four scores from a multiple of four on are one load, else -1
 };
 
 struct Segment {
@@ -77,9 +79,6 @@ __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
-__device__ __forceinline__ int lanes_below(uint64_t m) {
-  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-}
 // Sum over the threads before this one; `all`: over the workgroup.  part: NW words of LDS that no thread
 // still reads; holds a barrier.
 template <int NW>
@@ -93,27 +92,27 @@ __device__ __forceinline__ int block_before(int v, int lane, int w, int* part, i
   return before + incl - v;
 }
 
-// NT threads.  VPT > 0: every candidate's key sits in a register (thread t holds candidates t, t + NT, ...: VPT
-// of them), and the scores are read once.  VPT 0: longer tables read them again in each pass.
+// NT threads.  VPT > 0: every candidate's key sits in a register (VPT a thread, in quads of consecutive ones; a
+// wave's candidates are one run), and the scores are read once.  VPT 0: longer tables read them in each pass.
 //   A chain of memory round trips and barriers, and past some 16,000 candidates a workgroup's issue rate.  Per
 // segment (16 layers x 16 sequences x 8 kv-heads of up to 4,096 tokens, all at once / one of 65,000): keys there
-// after 5.6 / 10.7 us, T known at 9.6 / 24, positions written at 12.6 / 33.
+// after 3.0 / 7.9 us, T known at 8 / 16.5, positions written at 10 / 22; the launch 21-23 / 24-25 us.
 template <int NT, int VPT>
 __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   constexpr int NW = NT / 64;
-  constexpr int NR = VPT > 0 ? VPT : 1;
-  constexpr int GROUP = VPT > 0 ? VPT : 64;  // strips of NT candidates whose counts are scanned together
+  constexpr int NQ = VPT / 4;                    // quads of candidates in a thread's registers
+  constexpr int GROUP = VPT > 0 ? NQ : 16;       // strips of 4 NT candidates whose counts are scanned together
   // Bits of the three passes: with many candidates a first pass over more bins meets fewer equal addresses in
-  // the LDS atomics of a wave (65,000 candidates: 9 us over 2,048 bins).
+  // the LDS atomics of a wave (65,000 candidates: 9 us over 2,048 bins, 3 over 8,192).
   constexpr int FIRST = VPT > 16 ? 13 : 11, BINS = 1 << FIRST;
   constexpr int shifts[4] = {32, 32 - FIRST, 21 - FIRST, 0};
   constexpr int BPT = BINS / NT;  // bins a thread scans
-  constexpr int EPT = (GROUP * NW + NT - 1) / NT;  // (strip, wave) counts a thread scans
+  constexpr int kList = NT == 1024 ? 2048 : 512;
   __shared__ __attribute__((aligned(16))) int hist[BINS];
   __shared__ int part[2][NW];
   __shared__ int found[3];                          // digit, candidates above it, candidates at it
-  __shared__ int strip[2][GROUP * NW];              // per (strip, wave): candidates above T, candidates at T
-  __shared__ int first_hole, last_alias;
+  __shared__ uint32_t list[kList];                  // the candidates of the first pass's digit, where they fit
+  __shared__ int listed, first_hole, last_alias;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Segment sg = segment_of(a, blockIdx.x);
   const int n = context_of(a, sg.seq);
@@ -129,48 +128,56 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   const int p0 = a.guarded;
   const int count = n - a.recent - p0;           // candidates, positions p0 ..
   const int take = a.budget - a.recent - p0;     // of which this many stay: 0 <= take < count
-  const int strips = (count + NT - 1) / NT;
+  // Four consecutive positions, from base + c on with c a multiple of four, are a lane's: quads that lie in one
+  // block where the block size is a power of two, and are then read in one load (`aligned`).  Keys one at a
+  // time cost an address each, which bounded this phase: 65,000 candidates 14.7 us, in quads 7.9.
+  const int lead = p0 & 3, base = p0 - lead, extent = lead + count;
+  const int strips = (extent + 4 * NT - 1) / (4 * NT);
+  const bool aligned = a.block_shift >= 0;
 
   const float* cells = a.scores + sg.layer * a.score_layer_stride + (int64_t)sg.kvh * a.block_size;
-  auto read_key = [&](int c) -> uint32_t {
-    const uint32_t p = p0 + c, b = p / (uint32_t)a.block_size;
-    return order_key(cells[row[b] * a.score_stride + (p - b * (uint32_t)a.block_size)]);
+  auto entry = [&](int c) { return row[(uint32_t)(base + min(c, extent - 1)) >> a.block_shift]; };
+  auto read_aligned = [&](int c, int blk, uint32_t (&k)[4]) {
+    const int off = (base + (min(c, extent - 1) & ~3)) & (a.block_size - 1);
+    const float4 v = *reinterpret_cast<const float4*>(&cells[blk * a.score_stride + off]);
+    k[0] = __float_as_uint(v.x), k[1] = __float_as_uint(v.y);
+    k[2] = __float_as_uint(v.z), k[3] = __float_as_uint(v.w);
   };
-  uint32_t key[NR] = {};
-  if constexpr (VPT > 0) {
-    // A table entry, then the score it leads to: two round trips, shared by U candidates.  Where a thread
-    // has many candidates, the entries come to LDS first, all at once (where they fit), and the batches cost
-    // one round trip each.
-    constexpr int U = VPT < 16 ? VPT : 16;
-    constexpr int kEntries = VPT > 16 ? 4096 : 1;
-    __shared__ int32_t entries[kEntries];
-    const int e0 = p0 / a.block_size, ne = (p0 + count - 1) / a.block_size - e0 + 1;
-    const bool staged = VPT > 16 && ne <= kEntries;
-    if constexpr (VPT > 16) {
-      if (staged) {
-        for (int i = tid; i < ne; i += NT) entries[i] = row[e0 + i];
-        __syncthreads();
-      }
+  auto read_each = [&](int c, uint32_t (&k)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t p = base + min(c + j, extent - 1), b = p / (uint32_t)a.block_size;
+      k[j] = __float_as_uint(cells[row[b] * a.score_stride + (p - b * (uint32_t)a.block_size)]);
     }
-    auto staged_key = [&](int c) -> uint32_t {
-      const uint32_t p = p0 + c, b = p / (uint32_t)a.block_size;
-      return order_key(cells[entries[b - e0] * a.score_stride + (p - b * (uint32_t)a.block_size)]);
-    };
+  };
+  auto to_keys = [&](int c, uint32_t (&k)[4]) {  // of scores; of what is no candidate 0
 #pragma unroll
-    for (int i0 = 0; i0 < VPT; i0 += U) {
+    for (int j = 0; j < 4; ++j) k[j] = c + j >= lead && c + j < extent ? order_key(__uint_as_float(k[j])) : 0u;
+  };
+  uint32_t key[NQ > 0 ? NQ : 1][4] = {};
+  if constexpr (VPT > 0) {
+    // A table entry, then the scores it leads to: two round trips, shared by U quads.
+    constexpr int U = NQ < 8 ? NQ : 8;
+#pragma unroll
+    for (int i0 = 0; i0 < NQ; i0 += U) {
       if (i0 < strips) {
-        if (VPT > 16 && staged) {
+        if (aligned) {
+          int blk[U];
 #pragma unroll
-          for (int i = i0; i < i0 + U; ++i) key[i] = staged_key(min(i * NT + tid, count - 1));
+          for (int i = 0; i < U; ++i) blk[i] = entry(((w * strips + i0 + i) * 64 + lane) * 4);
+#pragma unroll
+          for (int i = 0; i < U; ++i) read_aligned(((w * strips + i0 + i) * 64 + lane) * 4, blk[i], key[i0 + i]);
         } else {
 #pragma unroll
-          for (int i = i0; i < i0 + U; ++i) key[i] = read_key(min(i * NT + tid, count - 1));
+          for (int i = i0; i < i0 + U; ++i) read_each(((w * strips + i) * 64 + lane) * 4, key[i]);
         }
       }
 #pragma unroll
       for (int i = i0; i < i0 + U; ++i) {
-        key[i] = i * NT + tid < count ? key[i] : 0u;
-        asm volatile("" : "+v"(key[i]));  // (finished here, not kept as a score and a condition)
+        to_keys(i < strips ? ((w * strips + i) * 64 + lane) * 4 : extent, key[i]);
+        // (Finished here, not kept as scores and conditions.)
+        asm volatile("" : "+v"(key[i][0]), "+v"(key[i][1]), "+v"(key[i][2]), "+v"(key[i][3]));
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -184,29 +191,33 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   for (int i = tid; i < a.recent; i += NT) kept[m - a.recent + i] = n - a.recent + i;
   for (int i = tid; i < p0; i += NT) kept[i] = i;
   if (tid == 0) {
+    listed = 0;
     first_hole = n;
     last_alias = -1;
   }
-  // f(strip within the group, candidate, key) over strips g0 .. g0 + gs - 1, the whole wave at once.  The key
-  // of what is no candidate is 0, below every score's.
+  // f(c, the four keys of candidates c ..) over the wave's candidates of the gs strips from g0 on, 256 consecutive
+  // ones at a time.  The key of what is no candidate is 0, below every score's.
   auto each = [&](int g0, int gs, auto f) __attribute__((always_inline)) {
     if constexpr (VPT > 0) {
       // (Opaque copies: comparisons are made where they are needed, not kept as masks from call to call.)
       asm volatile("" : "+s"(gs));
-      int t = tid;
+      int c = (w * gs * 64 + lane) * 4;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        uint32_t k = key[i];
-        asm volatile("" : "+v"(k), "+v"(t));
-        if (i < gs) f(i, i * NT + t, k);
-        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < NQ; ++i) {
+        uint32_t k[4] = {key[i][0], key[i][1], key[i][2], key[i][3]};
+        asm volatile("" : "+v"(k[0]), "+v"(k[1]), "+v"(k[2]), "+v"(k[3]), "+v"(c));
+        if (i < gs) f(c + i * 256, k);
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
 #pragma unroll 1
       for (int i = 0; i < gs; ++i) {
-        const int c = (g0 + i) * NT + tid;
-        const uint32_t k = read_key(min(c, count - 1));
-        f(i, c, c < count ? k : 0u);
+        const int c = g0 * NT * 4 + ((w * gs + i) * 64 + lane) * 4;
+        uint32_t k[4];
+        if (aligned) read_aligned(c, entry(c), k);
+        else read_each(c, k);
+        to_keys(c, k);
+        f(c, k);
       }
     }
   };
@@ -216,6 +227,10 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   uint32_t T = 0xffffffffu;  // (above every key: nothing kept)
   int left = 0;
   bool whole = false;  // every candidate at or above T is kept
+  bool few = false;    // `list` holds the candidates that agree with T's first digit
+  auto each_group = [&](auto f) __attribute__((always_inline)) {
+    for (int g0 = 0; g0 < (VPT > 0 ? 1 : strips); g0 += GROUP) each(g0, min(GROUP, strips - g0), f);
+  };
   if (take > 0) {
     T = 0;
     left = take;
@@ -226,7 +241,7 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
       for (int i = 4 * tid; i < BINS; i += 4 * NT) *reinterpret_cast<int4*>(&hist[i]) = make_int4(0, 0, 0, 0);
       __syncthreads();
       int zeros = 0;
-      each(0, strips, [&](int, int, uint32_t k) __attribute__((always_inline)) {
+      auto count_in = [&](uint32_t k) __attribute__((always_inline)) {
         // Lanes on one address go one after the other, and a score of 0 is the one that many tokens have in
         // common (weights that underflowed): those are counted in a register.
         if (ps == 0) {
@@ -235,7 +250,15 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
         }
         if (k != 0 && (ps == 0 || (k >> (hi & 31)) == (T >> (hi & 31))))
           atomicAdd(&hist[(k >> sh) & ((1u << (shifts[ps] - sh)) - 1u)], 1);
-      });
+      };
+      if (ps > 0 && few) {
+        for (int i = tid; i < listed; i += NT) count_in(list[i]);
+      } else {
+        each_group([&](int, const uint32_t (&k)[4]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) count_in(k[j]);
+        });
+      }
       if (ps == 0 && lane == 0 && zeros > 0) atomicAdd(&hist[kZeroKey >> sh], zeros);
       __syncthreads();
       // Candidates in higher bins; BPT bins a thread, from the top.
@@ -262,58 +285,80 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
       T |= (uint32_t)found[0] << sh;
       left -= found[1];
       whole = found[2] == left;  // the digit's candidates are all kept: no need to part them further
+      if (ps == 0) few = !whole && found[2] <= kList;
+      if (ps == 0 && few) {
+        // The other passes part those alone (in no order: they are only counted).
+        auto in_digit = [&](uint32_t k) { return k - T < (1u << sh); };  // (T > 0: every score's key is)
+        int mine = 0;
+        each_group([&](int, const uint32_t (&k)[4]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mine += in_digit(k[j]);
+        });
+        const int incl = wave_scan(mine);
+        int at = 0;
+        if (lane == 63 && incl > 0) at = atomicAdd(&listed, incl);
+        at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+        each_group([&](int, const uint32_t (&k)[4]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (in_digit(k[j])) list[at++] = k[j];
+          }
+        });
+      }
     }
   }
 
-  // The kept candidates in order: the counts of every (strip, wave) of a group go to LDS and are scanned.
-  const uint32_t above_T = whole ? T - 1 : T, at_T = whole ? 0xffffffffu : T;  // (no key is 0xffffffff)
-  const int ties = whole ? 0 : left;
-  int gt_before = 0, eq_before = 0;  // in the groups before
+  // The kept candidates in order: a wave's run of candidates is counted, and the waves' counts are scanned.  Where
+  // all at T stay, which is so unless scores are equal, there are no ties to count.
   int hole = n;
-  for (int g0 = 0; g0 < strips; g0 += GROUP) {
-    const int gs = min(GROUP, strips - g0);
-    if (g0 > 0) __syncthreads();
-    each(g0, gs, [&](int i, int, uint32_t k) __attribute__((always_inline)) {
-      const int gt = __popcll(__ballot(k > above_T)), eq = __popcll(__ballot(k == at_T));
-      if (lane == 0) {
-        strip[0][i * NW + w] = gt;
-        strip[1][i * NW + w] = eq;
-      }
-    });
-    __syncthreads();
-    int gt[EPT], eq[EPT], gsum = 0, esum = 0;
+  auto place = [&](auto with_ties) __attribute__((always_inline)) {
+    constexpr bool TIES = decltype(with_ties)::value;
+    const uint32_t above_T = TIES ? T : T - 1;
+    int gt_before = 0, eq_before = 0;  // in the groups before
+    for (int g0 = 0; g0 < (VPT > 0 ? 1 : strips); g0 += GROUP) {
+      const int gs = min(GROUP, strips - g0);
+      if (g0 > 0) __syncthreads();
+      int gt = 0, eq = 0;
+      each(g0, gs, [&](int, const uint32_t (&k)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int e = tid * EPT + i;
-      gt[i] = e < gs * NW ? strip[0][e] : 0;
-      eq[i] = e < gs * NW ? strip[1][e] : 0;
-      gsum += gt[i];
-      esum += eq[i];
-    }
-    int gall, eall = 0, ge, ee = 0;
-    ge = gt_before + block_before<NW>(gsum, lane, w, part[1], gall);
-    if (!whole) ee = eq_before + block_before<NW>(esum, lane, w, part[0], eall);
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int e = tid * EPT + i;
-      if (e < gs * NW) {
-        strip[0][e] = ge;
-        strip[1][e] = ee;
+        for (int j = 0; j < 4; ++j) {
+          gt += k[j] > above_T;
+          if constexpr (TIES) eq += k[j] == T;
+        }
+      });
+      const int gt_scan = wave_scan(gt), eq_scan = TIES ? wave_scan(eq) : 0;
+      if (lane == 63) {
+        part[0][w] = gt_scan;
+        part[1][w] = eq_scan;
       }
-      ge += gt[i];
-      ee += eq[i];
+      __syncthreads();
+      const int gsum = wave_scan(lane < NW ? part[0][lane] : 0), esum = TIES ? wave_scan(lane < NW ? part[1][lane] : 0) : 0;
+      const int gall = __builtin_amdgcn_readlane(gsum, 63), eall = __builtin_amdgcn_readlane(esum, 63);
+      int g = gt_before + (w > 0 ? __builtin_amdgcn_readlane(gsum, w - 1) : 0);
+      int e = eq_before + (w > 0 ? __builtin_amdgcn_readlane(esum, w - 1) : 0);
+      each(g0, gs, [&](int c, const uint32_t (&k)[4]) __attribute__((always_inline)) {
+        int mine = 0;  // (both counts in one scan, ties from bit 16 on)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine += (k[j] > above_T) + (TIES && k[j] == T ? 65536 : 0);
+        const int incl = wave_scan(mine), all = __builtin_amdgcn_readlane(incl, 63);
+        int gl = g + ((incl - mine) & 0xffff), el = e + ((incl - mine) >> 16);
+        g += all & 0xffff;
+        e += all >> 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool is_gt = k[j] > above_T, is_eq = TIES && k[j] == T;
+          if (is_gt || (is_eq && el < left)) kept[p0 + gl + (TIES ? min(el, left) : 0)] = base + c + j;
+          else if (k[j] != 0) hole = min(hole, base + c + j);
+          gl += is_gt;
+          el += is_eq;
+        }
+      });
+      gt_before += gall;
+      eq_before += eall;
     }
-    __syncthreads();
-    each(g0, gs, [&](int i, int c, uint32_t k) __attribute__((always_inline)) {
-      const bool is_gt = k > above_T, is_eq = k == at_T;
-      const int g = strip[0][i * NW + w] + lanes_below(__ballot(is_gt));
-      const int e = strip[1][i * NW + w] + lanes_below(__ballot(is_eq));
-      if (is_gt || (is_eq && e < ties)) kept[p0 + g + min(e, ties)] = p0 + c;
-      else if (k != 0) hole = min(hole, p0 + c);
-    });
-    gt_before += gall;
-    eq_before += eall;
-  }
+  };
+  if (whole) place(std::false_type{});
+  else place(std::true_type{});
   // Rows from the first hole on move.  Where a block that receives them is also the block they may come
   // from (the same entry of both tables: eviction in place), the chunks go in order.
   // (One LDS atomic a wave: lanes on one address go one after the other.)
@@ -472,7 +517,7 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: layer strides must be positive with num_layers > 1", op);
   }
   const int64_t table_tokens = (int64_t)max_blocks_per_seq * block_size;
-  if (table_tokens > INT32_MAX) {
+  if (table_tokens > INT32_MAX - 65536) {  // (positions are counted in 32 bits, up to a group past the last)
     return fail(RG_ERR_NOT_SUPPORTED, "%s: a block table of %lld tokens", op, (long long)table_tokens);
   }
   const int64_t most = std::min<int64_t>(budget, table_tokens);  // tokens a segment keeps at most
@@ -518,6 +563,9 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   a.max_blocks = max_blocks_per_seq;
   a.max_dst_blocks = dst_block_table ? max_dst_blocks_per_seq : max_blocks_per_seq;
   a.batch = batch_size;
+  const bool quads = block_size >= 4 && (block_size & (block_size - 1)) == 0 && score_stride % 4 == 0 &&
+                     a.score_layer_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(scores) & 15u) == 0;
+  a.block_shift = quads ? __builtin_ctz((unsigned)block_size) : -1;
   hipStream_t s = as_stream(stream);
   const dim3 sel((unsigned)segments);
   auto select = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, sel, dim3(threads), 0, s, a); };

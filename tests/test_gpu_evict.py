@@ -144,6 +144,32 @@ def test_long(device, kernels, lens, budget, dst):
     c.check(kernels, 100, 16)
 
 
+@pytest.mark.parametrize("bs,protected,recent", [(24, 5, 1), (6, 7, 33), (4, 1, 0), (2, 3, 2), (32, 30, 99)])
+@pytest.mark.parametrize("lens", [[700, 90, 91], [3000, 41], [13001], [30000], [70001]])
+def test_candidates_that_begin_anywhere(device, kernels, bs, protected, recent, lens):
+    """First and last candidates inside a group of four, blocks that hold whole groups and blocks that do not, in
+    each of the selection's forms."""
+    c = Case(device, lens, max(40 + recent, lens[0] // 7), hkv=1, bs=bs, d=4, seed=lens[0] + bs)
+    c.check(kernels, recent, protected)
+
+
+@pytest.mark.parametrize("n", [500, 40000])
+def test_scores_off_16_bytes(device, kernels, n):
+    c = Case(device, [n], n // 3, d=8, seed=n)
+    room = torch.zeros(c.scores.numel() + 1, device=device)
+    room[1:] = c.scores.flatten()
+    c.scores = room[1:].view(c.scores.shape)
+    c.check(kernels, 9, 6)
+
+
+@pytest.mark.parametrize("n", [900, 3900, 16000, 60000, 80000])
+@pytest.mark.parametrize("values", [2, 40])
+def test_few_distinct_scores(device, kernels, n, values):
+    """Ties at the threshold, more of them than the later passes list."""
+    c = Case(device, [n], n // 4, hkv=1, d=4, seed=n, scores=lambda s, g: torch.ceil(s * values))
+    c.check(kernels, 20, 3)
+
+
 def test_wide_table_of_short_contexts(device, kernels):
     c = Case(device, [70, 3, 200], 64, seed=11, wide=3000)
     c.check(kernels, 5, 0)
