@@ -399,8 +399,9 @@ int rg_paged_attention_v1_plus(const void* query, const void* key_cache,
 
 /* rg_paged_attention_v1 for a batch whose sequences begin with the same cached blocks (a system
  * prompt, a document that many rows ask about): the first shared_blocks entries of every row of
- * block_table name the same blocks (those of any one row are read).  The same output up to
- * rounding, with the shared blocks read once for many rows instead of once per sequence, as
+ * block_table whose context holds them all name the same blocks.  Shorter rows (empty ones that pad
+ * a batch among them) may have other blocks there, and anything behind their own tokens.  The same
+ * output up to rounding, with the shared blocks read once for many rows instead of once per sequence, as
  * one product on the matrix cores (in bf16 / f16 with the probabilities of the shared tokens
  * rounded to that type, as in rg_prefill_packed).  Sequences may be shorter than the prefix or
  * empty (context_lens[s] == 0 gives zeros); shared_blocks == 0 is rg_paged_attention_v1.  Any shape

@@ -59,7 +59,7 @@ struct PrefixArgs {
   int32_t group, num_heads, num_kv_heads, rows;  // rows = batch * group
   int32_t prefix, subs;                          // prefix tokens, and its 16-token sub-blocks
   int32_t tiles, split_tiles, splits;
-  int32_t bs_shift, table_stride_tokens;         // table_stride_tokens: tokens of a block-table row
+  int32_t bs_shift;
   int32_t stream_groups;                         // workgroups of stream-K workers, the first of the grid
   int64_t kv_stride;
 };
@@ -486,9 +486,18 @@ __global__ __launch_bounds__(kPreThreads, (groups_per_cu<T, D, G>())) void share
     }
     return;
   }
+  // The prefix's blocks come from the first row that holds all of it: what the rows of a padded batch have in
+  // their tables is not looked at.
+  int holder = -1;
+  for (int s0 = 0; s0 < sa.batch && holder < 0; s0 += 64) {
+    const uint64_t mask = __ballot(s0 + lane < sa.batch && context_lens[min(s0 + lane, sa.batch - 1)] >= pa.prefix);
+    if (mask != 0) holder = s0 + __builtin_ctzll(mask);
+  }
+  if (holder < 0) return;
+  const int32_t* table = block_table + (int64_t)holder * sa.table_stride;
   const int u = (int)blockIdx.x - pa.stream_groups;
-  if constexpr (std::is_same_v<T, f32_t>) prefix_product_f32<D>(pa, q, kc, vc, block_table, ring, u, w, lane);
-  else prefix_product<T, D>(pa, q, kc, vc, block_table, ring, u, w, lane);
+  if constexpr (std::is_same_v<T, f32_t>) prefix_product_f32<D>(pa, q, kc, vc, table, ring, u, w, lane);
+  else prefix_product<T, D>(pa, q, kc, vc, table, ring, u, w, lane);
 }
 
 // One workgroup per (kv-head, sequence), R waves per query head: lane l of wave r folds dims [l PER, (l + 1) PER) of

@@ -119,6 +119,27 @@ def test_no_sequence_has_the_whole_prefix(device, kernels):
     Batch(device, [40, 100, 0, 7], 20, seed=4).check(kernels)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("ctx", [[0, 0, 700, 330, 0], [319, 40, 0, 320, 500], [0] * 150 + [400] + [0] * 70 + [321],
+                                 [100, 0, 7]])
+def test_shorter_rows_have_tables_of_their_own(device, kernels, dtype, ctx):
+    """Rows that pad the batch, or end inside the prefix, hold other blocks and no valid entry behind their
+    tokens; the prefix's blocks come from a row that has them all."""
+    c = Batch(device, ctx, 20, dtype=dtype, seed=len(ctx), wide=2)
+    spare = iter(range(len(c.pool), len(c.pool) + 64))
+    own = []
+    for s, n in enumerate(ctx):
+        if n < 320:
+            used = -(-n // 16)
+            c.table[s] = -7
+            for i in range(used):
+                c.table[s, i] = next(spare)
+                own.append(torch.randn(c.pool.shape[1:], device=device).to(c.pool.dtype))
+    c.pool = torch.cat([c.pool, torch.stack(own)]) if own else c.pool
+    c.kc, c.vc = c.pool[:, 0], c.pool[:, 1]
+    c.check(kernels)
+
+
 def test_all_rows_empty_and_nothing_shared(device, kernels):
     Batch(device, [0, 0, 0], 4, seed=5).check(kernels)
     Batch(device, [70, 0, 5], 0, seed=5).check(kernels)
