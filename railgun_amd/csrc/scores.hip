@@ -123,10 +123,10 @@ __global__ __launch_bounds__(64) void scores_generic_kernel(GenericArgs a) {
 }
 
 // Workgroup (x, kv-head, sequence): the first merge_groups merge the partials of merge_heads query heads each
-// into their output rows, the others turn raw scores into weights, kFinTokens tokens at a time.  Each works out the maxima and sums it needs
-// from the partials' pairs itself (a few loads), so one launch does both.  The call is short against memory
-// latency: what does not depend on the pairs (the accumulators of the merge, the raw scores, the old ones) is
-// asked for before they are waited for.  GT: G, or 0 for one known at run time.
+// into their output rows, the others turn raw scores into weights, kFinTokens tokens at a time.  Each works out
+// the maxima and sums it needs from the partials' pairs itself (a few loads), so one launch does both.  The call
+// is short against memory latency: what does not depend on the pairs (the accumulators of the merge, the raw
+// scores, the old ones) is asked for before they are waited for.  GT: G, or 0 for one known at run time.
 template <typename T, int GT>
 __global__ __launch_bounds__(kFinThreads) void scores_finish_kernel(ScoreArgs a) {
   using E = elem<T>;
@@ -276,7 +276,8 @@ __global__ __launch_bounds__(kFinThreads) void scores_finish_kernel(ScoreArgs a)
 // Tables of few tokens (short_applies): one workgroup per segment does it all, one launch.  Its waves take the
 // 16-token sub-blocks in turn, as the plain decode's kernel for such tables does; the raw scores stay in LDS
 // (`raw`, [tokens][G]), and once the waves' partials are merged every thread turns some tokens' into weights.
-//   Bound by latency: two sequences of up to 77 tokens in fp32 (32 / 8 heads of 64) 11.5 us a call, with the worker and the finish kernel 14.5.
+//   Bound by latency: two sequences of up to 77 tokens in fp32 (32 / 8 heads of 64) 11.5 us a call, with the
+// worker and the finish kernel 14.5.
 template <typename T, int D, int G>
 __global__ __launch_bounds__(kShortThreads) void scores_short_kernel(
     ScoreArgs a, int64_t kv_stride, int bs_shift, const typename DecodeTileFor<T, D, G>::S* __restrict__ q,
@@ -579,7 +580,7 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
   f.context_lens = context_lens;
   f.scored_lens = scored_lens;
   f.scale_log2 = scale * kLog2e;
-  f.first = first_scored;
+  f.first = (int32_t)std::min<int64_t>(first_scored, tokens);  // (so that positions counted from it fit 32 bits)
   f.num_heads = num_heads;
   f.num_kv_heads = num_kv_heads;
   f.head_dim = head_dim;
@@ -629,7 +630,7 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
     f.part_ml = ml;
     if (max_blocks_per_seq > 0) {
       GenericArgs ga{query, key_cache, value_cache, block_table, context_lens, reinterpret_cast<float*>(ws), acc, ml,
-                     f.scale_log2, first_scored, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                     f.scale_log2, f.first, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
                      f.num_partitions, kv_stride};
       st = dispatch_dtype(dtype, [&](auto tag) {
         hipLaunchKernelGGL(scores_generic_kernel<decltype(tag)>, dim3(f.num_partitions, num_heads, batch_size),
@@ -645,7 +646,7 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
   const int64_t segments = (int64_t)batch_size * num_kv_heads;
   f.merge_heads = (tiles ? workers / segments : f.num_partitions) >= 8 ? 1 : 4;
   f.merge_groups = (int32_t)ceil_div(G, f.merge_heads);
-  const int64_t scored = std::max<int64_t>(0, tokens - first_scored);
+  const int64_t scored = tokens - f.first;
   const int64_t chunks = std::min(ceil_div(scored, kFinTokens), std::max<int64_t>(1, 8192 / segments));
   const dim3 grid((unsigned)(f.merge_groups + chunks), (unsigned)num_kv_heads, (unsigned)batch_size);
   return dispatch_dtype(dtype, [&](auto tag) {

@@ -98,6 +98,25 @@ def test_block_sizes(device, kernels, bs, fused):
     b.check(kernels)
 
 
+@pytest.mark.parametrize("ctx", [[70, 33], [2000, 900]])
+@pytest.mark.parametrize("d", [64, 96])
+def test_nothing_scored(device, kernels, ctx, d):
+    """first_scored at and past the table's end, up to the largest: the output alone."""
+    c = Batch(device, ctx, d=d, seed=d)
+    before = c.scores.clone()
+    for first in (max(ctx), 2048, 2**31 - 300, 2**31 - 1):
+        c.check(kernels, first=first)
+        assert torch.equal(c.scores, before)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.4, 3.0])
+@pytest.mark.parametrize("ctx", [[70, 33], [2000, 900]])
+def test_scales(device, kernels, scale, ctx):
+    c = Batch(device, ctx, seed=9)
+    c.scale = scale
+    c.check(kernels, scored=[20, 900])
+
+
 @pytest.mark.parametrize("first", [0, 1, 16, 100, 299, 300, 5000])
 def test_first_scored(device, kernels, first):
     Batch(device, [300, 120, 7], seed=first).check(kernels, scored=np.array([0, 120, 3]), first=first)
