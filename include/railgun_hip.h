@@ -189,7 +189,7 @@ int rg_copy_blocks(const void* src_pool, void* dst_pool, const int32_t* block_ma
  * no other entry of either table that the call uses.  Blocks that hold positions below
  * protected_len only, at the same place in both rows, are not written, so sequences may share them.
  *
- * new_context_lens (NULL: not wanted) [batch] gets min(n, budget); kept_positions (NULL: not wanted)
+ * new_context_lens (NULL: not wanted; apart from context_lens) [batch] gets min(n, budget); kept_positions (NULL: not wanted)
  * [num_layers, batch, num_kv_heads, budget] the kept positions in order, -1 behind them.
  * key_cache / value_cache / scores point at layer 0, layer l lies layer_stride (score_layer_stride)
  * elements further on.  The workspace (rg_evict_cache_workspace_bytes, 4-byte aligned) needs no

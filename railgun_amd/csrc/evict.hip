@@ -10,7 +10,8 @@
 // evict_select_kernel (one workgroup per segment) finds the threshold: scores become 32-bit keys in
 // the order of the values, and three passes over 11, 11 and 10 bits narrow the key T of the last one
 // to be kept, each with a histogram in LDS over the candidates that agree with the bits found so
-// far (after the first pass mostly few, which are then listed).  A kept candidate's place is then known without a list: before position t lie
+// far (after the first pass mostly few, which are then listed).  A kept candidate's place is then known: before
+// position t lie
 //   #{key > T before t} + min(#{key == T before t}, ties to keep)
 // kept candidates.  The kernel leaves the kept positions in order (the caller's array, or workspace).
 // evict_move_kernel copies: what a segment has to move is cut into chunks, a workgroup each.
@@ -537,6 +538,12 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0) {
     return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (4-byte aligned), %zu required", op,
                 workspace ? workspace_bytes : (size_t)0, need);
+  }
+  // (The lengths are read by every segment while the new ones are written.)
+  const auto lens_at = reinterpret_cast<uintptr_t>(context_lens), new_at = reinterpret_cast<uintptr_t>(new_context_lens);
+  if (new_context_lens != nullptr && lens_at < new_at + 4 * (uintptr_t)batch_size &&
+      new_at < lens_at + 4 * (uintptr_t)batch_size) {
+    return fail(RG_ERR_INVALID_ARGUMENT, "%s: new_context_lens overlaps context_lens", op);
   }
   EvictArgs a{};
   a.k = key_cache;

@@ -54,6 +54,10 @@ def evict(**change):
     (dict(ws_bytes=255), WORKSPACE, "256 required"),
     (dict(ws=P + 2), WORKSPACE, "aligned"),
     (dict(kept=None), WORKSPACE, "required"),          # the list goes to the workspace then
+    (dict(), INVALID, "overlaps"),                      # lengths read while the new ones are written
+    (dict(new_lens=P + 8), INVALID, "overlaps"),
+    (dict(new_lens=P - 8), INVALID, "overlaps"),
+    (dict(mb=2**27 - 1), UNSUPPORTED, "block table of"),
     (dict(layers=0), _lib.RG_OK, ""),
     (dict(batch=0), _lib.RG_OK, ""),
 ])
