@@ -15,6 +15,7 @@
 //   #{key > T before t} + min(#{key == T before t}, ties to keep)
 // kept candidates.  The kernel leaves the kept positions in order (the caller's array, or workspace).
 // evict_move_kernel copies: what a segment has to move is cut into chunks, a workgroup each.
+// evict_segment_kernel does both, for many or small segments.
 #include <algorithm>
 #include <type_traits>
 
@@ -98,8 +99,9 @@ __device__ __forceinline__ int block_before(int v, int lane, int w, int* part, i
 //   A chain of memory round trips and barriers, and past some 16,000 candidates a workgroup's issue rate.  Per
 // segment (16 layers x 16 sequences x 8 kv-heads of up to 4,096 tokens, all at once / one of 65,000): keys there
 // after 3.0 / 7.9 us, T known at 8 / 16.5, positions written at 10 / 22; the launch 21-23 / 24-25 us.
+// Returns, to all threads alike, whether the segment's chunks have to move in order.
 template <int NT, int VPT>
-__global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
+__device__ __forceinline__ bool select_segment(const EvictArgs a, const Segment sg, int64_t index) {
   constexpr int NW = NT / 64;
   constexpr int NQ = VPT / 4;                    // quads of candidates in a thread's registers
   constexpr int GROUP = VPT > 0 ? NQ : 16;       // strips of 4 NT candidates whose counts are scanned together
@@ -115,16 +117,14 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   __shared__ uint32_t list[kList];                  // the candidates of the first pass's digit, where they fit
   __shared__ int listed, first_hole, last_alias;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Segment sg = segment_of(a, blockIdx.x);
   const int n = context_of(a, sg.seq);
   const int m = min(n, a.budget);
-  int32_t* kept = a.kept + (int64_t)blockIdx.x * a.kept_stride;
+  int32_t* kept = a.kept + index * a.kept_stride;
   const int32_t* row = a.table + (int64_t)sg.seq * a.max_blocks;
   if (a.new_lens != nullptr && sg.layer == 0 && sg.kvh == 0 && tid == 0) a.new_lens[sg.seq] = m;
   if (n <= a.budget) {
     for (int i = tid; i < a.kept_stride; i += NT) kept[i] = i < n ? i : -1;
-    if (tid == 0) a.in_order[blockIdx.x] = 0;
-    return;
+    return false;
   }
   const int p0 = a.guarded;
   const int count = n - a.recent - p0;           // candidates, positions p0 ..
@@ -373,7 +373,13 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
     atomicMax(&last_alias, alias);
   }
   __syncthreads();
-  if (tid == 0) a.in_order[blockIdx.x] = last_alias >= first_hole / a.block_size;
+  return last_alias >= first_hole / a.block_size;
+}
+
+template <int NT, int VPT>
+__global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
+  const bool in_order = select_segment<NT, VPT>(a, segment_of(a, blockIdx.x), blockIdx.x);
+  if (threadIdx.x == 0) a.in_order[blockIdx.x] = in_order;
 }
 
 // ----------------------------------------------------------------- move -----
@@ -387,19 +393,21 @@ constexpr int kInPlacePieces = 8;
 // of it.  That is enough: kept[j] >= j, so rows j .. of the destination never hold a row that a later chunk has
 // yet to read.
 //   Bound by the copy: every row is read and written once, with non-temporal accesses (no row is met again).
-// 16 layers x 16 sequences x 8 kv-heads of 1,024 kept tokens, head_dim 64 in 16 bits (1.07 GB): 215 us with 256
-// threads of 4 pieces, 238 with 8 and ordinary accesses, a 1 GiB copy's rate being 5.2 TB/s.  In place the
-// round trips of a segment's chunks follow each other, so fewer, larger ones win: two sequences of 65,000
-// tokens down to 8,192 (16 segments) took 447 us with 256 threads of 8 pieces, 197 with 1,024 of 8, 223 of 16.
-template <typename V, int NT, int U>
-__global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a, int row_vecs, int tok) {
+// Four layers x 17 sequences x 4 kv-heads of up to 1,500 kept tokens of 512 bytes (0.33 GB): 56 us with 256 threads
+// of 4 pieces, the rate of a 1 GiB copy being 5.2 TB/s (64 us for these bytes); 8 pieces and ordinary accesses were
+// 10 % slower.  In place the round trips of a segment's chunks follow each other, so fewer, larger ones win: two
+// sequences of 65,000 tokens down to 8,192 (16 segments) took 447 us a call with 256 threads of 8 pieces, 184 with
+// 1,024 of 8, 223 of 16.
+//   (The arguments come by value: behind a reference the compiler kept the addresses of all pieces at once, 1,700
+// registers of them spilled.)
+// Chunk j0 of the segment; in order, or with ALL, that and all later ones.
+template <typename V, int NT, int U, bool ALL>
+__device__ __forceinline__ void move_rows(const EvictArgs a, const Segment sg, int64_t index, int row_vecs, int tok,
+                                          int j0, bool in_order) {
   __shared__ int64_t src_off[2][kMoveMaxTokens], dst_off[2][kMoveMaxTokens];  // in pieces V; -1: not moved
   const int tid = threadIdx.x;
-  const Segment sg = segment_of(a, blockIdx.x);
   const int m = min(context_of(a, sg.seq), a.budget);
-  const bool in_order = a.in_order[blockIdx.x] != 0;
-  if (in_order && blockIdx.y != 0) return;
-  const int32_t* kept = a.kept + (int64_t)blockIdx.x * a.kept_stride;
+  const int32_t* kept = a.kept + index * a.kept_stride;
   const int32_t* row = a.table + (int64_t)sg.seq * a.max_blocks;
   const int32_t* drow = a.dst_table + (int64_t)sg.seq * a.max_dst_blocks;
   constexpr int kSize = (int)sizeof(V);
@@ -408,7 +416,8 @@ __global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a, int row_vec
   V* const vb = static_cast<V*>(a.v);
   const int64_t layer = sg.layer * a.layer_stride, head = (int64_t)sg.kvh * a.block_size;
   const int per_token = 2 * row_vecs;
-  for (int j0 = (int)blockIdx.y * tok, buf = 0; j0 < m; j0 += tok, buf ^= 1) {
+#pragma unroll 1
+  for (int buf = 0; j0 < m; j0 += tok, buf ^= 1) {
     const int nt = min(tok, m - j0);
     float score = 0.f;
     int64_t to_cell = -1;
@@ -448,8 +457,29 @@ __global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a, int row_vec
       }
     }
     if (to_cell >= 0) a.scores[to_cell] = score;
-    if (!in_order) break;
+    if (!ALL && !in_order) break;
   }
+}
+
+template <typename V, int NT, int U>
+__global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a, int row_vecs, int tok) {
+  const bool in_order = a.in_order[blockIdx.x] != 0;
+  if (in_order && blockIdx.y != 0) return;
+  move_rows<V, NT, U, false>(a, segment_of(a, blockIdx.x), blockIdx.x, row_vecs, tok, (int)blockIdx.y * tok, in_order);
+}
+
+// Both in one launch, a workgroup per segment: where there are segments enough to fill the chip with one each (the
+// moves of some then hide the selection of others), or where a segment moves no more than two chunks.  Else the
+// chunks that follow each other in a workgroup cost more than the second launch.  Measured (us, two launches / one;
+// rows of 128 bytes): 2,048 segments of 1,024 kept tokens 249 / 231 (in place 225 / 209), 1,024 of 2,000 230 / 225, 48
+// of 128 with 256-byte rows 13.0 / 10.6, 256 of 256 15.7 / 14.4; 272 of up to 1,500 with 256-byte rows 64 / 92,
+// 64 of 512 13.3 / 16.0.
+constexpr int kSegThreads = 512, kSegKeys = 8, kSegPieces = 4;
+__global__ __launch_bounds__(kSegThreads) void evict_segment_kernel(EvictArgs a, int row_vecs, int tok) {
+  const Segment sg = segment_of(a, blockIdx.x);
+  const bool in_order = select_segment<kSegThreads, kSegKeys>(a, sg, blockIdx.x);
+  __syncthreads();  // the kept positions stand for the workgroup
+  move_rows<rg_u32x4_t, kSegThreads, kSegPieces, true>(a, sg, blockIdx.x, row_vecs, tok, 0, in_order);
 }
 
 // Segments of the call, -1 past what one launch numbers.
@@ -466,6 +496,7 @@ size_t evict_bytes(int64_t segments, int64_t budget, bool own_list) {
 int probe_evict_kernels() {
   hipFuncAttributes at;
   if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_select_kernel<256, 16>)) != hipSuccess ||
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_segment_kernel)) != hipSuccess ||
       hipFuncGetAttributes(&at, reinterpret_cast<const void*>(evict_move_kernel<rg_u32x4_t, 256, 4>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the eviction kernels: %s", hipGetErrorString(hipGetLastError()));
   }
@@ -575,6 +606,21 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   a.block_shift = quads ? __builtin_ctz((unsigned)block_size) : -1;
   hipStream_t s = as_stream(stream);
   const dim3 sel((unsigned)segments);
+  // Rows move in 16-byte pieces where every row starts on one, else in 2-byte ones.
+  auto whole = [&](int64_t elements) { return elements * eb % 16 == 0; };
+  const bool wide = whole(head_dim) && whole(kv_stride) && whole(a.layer_stride) &&
+                    ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15u) == 0;
+  const int row_vecs = head_dim * eb / (wide ? 16 : 2);
+  // Tokens of a chunk.  (A thread looks one token up: no more tokens than threads, which rows of a single piece
+  // would allow.)
+  auto chunk = [&](int threads, int pieces) {
+    return std::max(1, std::min({kMoveMaxTokens, threads, threads * pieces / (2 * row_vecs)}));
+  };
+  if (wide && table_tokens <= kSegThreads * kSegKeys &&
+      (segments >= 4 * (int64_t)device_cu_count() || most * 2 * row_vecs <= 2 * kSegThreads * kSegPieces)) {
+    hipLaunchKernelGGL(evict_segment_kernel, sel, dim3(kSegThreads), 0, s, a, row_vecs, chunk(kSegThreads, kSegPieces));
+    return check_launch(op);
+  }
   auto select = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, sel, dim3(threads), 0, s, a); };
   if (table_tokens <= 256 * 4) select(evict_select_kernel<256, 4>, 256);
   else if (table_tokens <= 256 * 16) select(evict_select_kernel<256, 16>, 256);
@@ -583,14 +629,8 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   else select(evict_select_kernel<1024, 0>, 1024);
   int st = check_launch(op);
   if (st != RG_OK || most == 0) return st;
-  // Rows move in 16-byte pieces where every row starts on one, else in 2-byte ones.
-  auto whole = [&](int64_t elements) { return elements * eb % 16 == 0; };
-  const bool wide = whole(head_dim) && whole(kv_stride) && whole(a.layer_stride) &&
-                    ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15u) == 0;
-  const int row_vecs = head_dim * eb / (wide ? 16 : 2);
   auto move = [&](auto kernel, int threads, int pieces) {
-    // (A thread looks one token up: no more tokens than threads, which rows of a single piece would allow.)
-    const int tok = std::max(1, std::min({kMoveMaxTokens, threads, threads * pieces / (2 * row_vecs)}));
+    const int tok = chunk(threads, pieces);
     const int64_t chunks = dst_block_table == nullptr ? 1 : ceil_div(most, tok);
     if (chunks > 65535) return fail(RG_ERR_NOT_SUPPORTED, "%s: a budget of %lld tokens", op, (long long)most);
     hipLaunchKernelGGL(kernel, dim3((unsigned)segments, (unsigned)chunks), dim3(threads), 0, s, a, row_vecs, tok);

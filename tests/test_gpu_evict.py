@@ -130,6 +130,21 @@ def test_many_short_rows(device, kernels, dtype, d, dst):
     Case(device, [3000, 1200], 1100, dtype=dtype, d=d, dst=dst, seed=d).check(kernels, 40, 20)
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f32", 128)])
+@pytest.mark.parametrize("dst", ["apart", "in place", "mixed"])
+@pytest.mark.parametrize("lens,budget", [([1000, 640, 30], 600), ([3900, 1300, 999], 1200)])
+def test_few_large_segments(device, kernels, dtype, d, dst, lens, budget):
+    """Selection and move as two launches."""
+    Case(device, lens, budget, dtype=dtype, d=d, dst=dst, seed=d).check(kernels, 77, 35)
+
+
+@pytest.mark.parametrize("dst", ["apart", "in place", "mixed"])
+def test_many_segments(device, kernels, dst):
+    """More than four segments a CU, of several chunks each: one workgroup a segment."""
+    lens = np.random.default_rng(1).integers(1, 700, 18)
+    Case(device, lens, 300, layers=15, hkv=4, d=128, dst=dst).check(kernels, 50, 17)
+
+
 def test_layers_and_shared_prefix(device, kernels):
     """Sequences that share their first blocks, protected: the shared blocks stay as they are."""
     c = Case(device, [700, 128, 90, 401], 128, layers=5, hkv=4, shared=2, seed=5)
