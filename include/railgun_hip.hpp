@@ -293,8 +293,8 @@ class PagedAttentionKernels {
     return rg_paged_attention_shared_prefix_pays(batch_size, num_heads, num_kv_heads, head_dim, block_size,
                                                  max_blocks_per_seq, shared_blocks, (int32_t)dtype) != 0;
   }
-  // launch_v1 for sequences whose block tables begin with the same shared_blocks entries: those blocks
-  // are read once for many rows.
+  // launch_v1 for sequences whose block tables begin with the same shared_blocks entries (all whose
+  // context holds those): those blocks are read once for many rows.
   void launch_shared_prefix(const void* query, const void* key_cache, const void* value_cache,
                             const int32_t* block_table, const int32_t* context_lens, void* output, float scale,
                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,

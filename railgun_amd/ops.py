@@ -70,6 +70,13 @@ def _require_table(block_table: torch.Tensor, context_lens: torch.Tensor, batch:
                            f"{tuple(block_table.shape)} and {tuple(context_lens.shape)}")
 
 
+def _require_int32(**values: int) -> None:
+    """Counts that ctypes would cut to 32 bits without a word."""
+    for name, v in values.items():
+        if not -2**31 <= v < 2**31:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, f"{name} {v} does not fit 32 bits")
+
+
 def _require_scored_lens(scored_lens: Optional[torch.Tensor], batch: int) -> None:
     if scored_lens is not None:
         _require_i32(scored_lens)
@@ -130,15 +137,17 @@ class PagedAttentionKernels:
         ordinal = device.index if isinstance(device, torch.device) else int(device)
         self.ordinal = 0 if ordinal is None else ordinal
         check(self.lib.rg_init(self.ordinal))
-        # What the execute_* forms asked the library, by entry and shape: a query costs as much host time
-        # as a tenth of a small call, and its answer depends on the shape and the device alone.
-        self._answers: dict = {}
+        # Workspace sizes and choices of form by entry and shape (they depend on nothing else but the device):
+        # asking the library costs as much host time as a tenth of a small call.
+        self._plans: dict = {}
 
     def _ask(self, entry: str, *shape: int) -> int:
         key = (entry, shape)
-        n = self._answers.get(key)
+        n = self._plans.get(key)
         if n is None:
-            n = self._answers[key] = int(getattr(self.lib, entry)(*shape))
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            n = self._plans[key] = int(getattr(self.lib, entry)(*shape))
         return n
 
     # mod.rs:196-225
@@ -252,8 +261,9 @@ class PagedAttentionKernels:
                              num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
                              max_blocks_per_seq: int, batch_size: int, shared_blocks: int,
                              workspace: torch.Tensor) -> None:
-        """launch_v1 for a batch whose rows of ``block_table`` begin with the same ``shared_blocks``
-        entries: those blocks are read once for many rows (rg_paged_attention_shared_prefix)."""
+        """launch_v1 for a batch whose rows of ``block_table``, as far as their context holds them all,
+        begin with the same ``shared_blocks`` entries: those blocks are read once for many rows
+        (rg_paged_attention_shared_prefix)."""
         _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, workspace)
         _require_i32(block_table, context_lens)
         _require_table(block_table, context_lens, batch_size, max_blocks_per_seq)
@@ -296,6 +306,7 @@ class PagedAttentionKernels:
     def _v1_scores(self, query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens,
                    first_scored, scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
                    batch_size, workspace) -> None:
+        _require_int32(first_scored=first_scored)
         check(self.lib.rg_paged_attention_v1_scores(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
             context_lens.data_ptr(), output.data_ptr(), scores.data_ptr(), _ptr(scored_lens), first_scored,
@@ -491,6 +502,7 @@ class PagedAttentionKernels:
         if key_cache.dim() not in (4, 5) or value_cache.shape != key_cache.shape or \
                 value_cache.dtype != key_cache.dtype or value_cache.stride() != key_cache.stride():
             raise bad("caches must be [NB, H_kv, bs, D] or [layers, NB, H_kv, bs, D], alike in shape, strides and dtype")
+        _require_int32(budget=budget, recent=recent, protected_len=protected_len)
         layered = key_cache.dim() == 5
         layers = int(key_cache.shape[0]) if layered else 1
         nb, hkv, bs, d = (int(x) for x in key_cache.shape[-4:])
@@ -603,8 +615,8 @@ class PagedAttentionOp:
     def execute_shared_prefix(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                               block_table: torch.Tensor, context_lens: torch.Tensor, shared_blocks: int,
                               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """execute() for sequences whose block tables begin with the same ``shared_blocks`` entries:
-        launch_shared_prefix where it pays, else launch_v1.  The workspace
+        """execute() for sequences whose block tables begin with the same ``shared_blocks`` entries (all
+        whose context holds those): launch_shared_prefix where it pays, else launch_v1.  The workspace
         (shared_prefix_workspace_bytes) is allocated here when omitted."""
         batch, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
         if not 0 <= shared_blocks <= mb:

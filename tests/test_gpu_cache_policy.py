@@ -128,6 +128,60 @@ def test_decode_score_evict_decode(device, kernels, dtype, heads, hkv, d, in_pla
         step()
 
 
+def test_two_streams_at_once(device, kernels):
+    """A shared-prefix decode and a scored decode of one pool, and an eviction of another, on streams of their
+    own: the results of the calls one after the other, bit for bit."""
+    g = torch.Generator(device=device).manual_seed(4)
+    b, shared, hkv, heads, d = 24, 40, 2, 8, 128
+    table = np.zeros((b, 80), np.int32)
+    order = iter(np.random.default_rng(4).permutation(40 + 40 * b).astype(np.int32))
+    table[:, :shared] = [next(order) for _ in range(shared)]
+    for s in range(b):
+        table[s, shared:] = [next(order) for _ in range(40)]
+    lens = np.random.default_rng(5).integers(640, 1280, b)
+    pool, other = (GpuBlockPool(1, 40 + 40 * b, hkv, BS, d, device) for _ in range(2))
+    for x in (pool, other):
+        x.storage.copy_(torch.randn(x.storage.shape, generator=g, device=device))
+        x.scores.copy_(torch.rand(x.scores.shape, generator=g, device=device))
+    q = torch.randn((b, heads, d), generator=g, device=device).to(torch.bfloat16)
+    op = PagedAttentionOp(1 / math.sqrt(d), heads, hkv, d, BS, kernels)
+    dt, dl = i32(table, device), i32(lens, device)
+    kc, vc = pool.k_cache(0), pool.v_cache(0)
+    shape = (b, heads, hkv, d, BS, 80)
+    start = pool.scores.clone(), other.storage.clone(), other.scores.clone()
+
+    def prefix():
+        out = torch.empty_like(q)
+        ws = torch.empty(kernels.shared_prefix_workspace_bytes(*shape, shared), dtype=torch.uint8, device=device)
+        kernels.launch_shared_prefix(q, kc, vc, dt, dl, out, op.scale, *shape[1:], b, shared, ws)
+        return out
+
+    calls = [prefix, lambda: op.execute_with_scores(q, kc, vc, dt, dl, pool.scores[0], None, shared * BS),
+             lambda: other.evict(dt, dl, 800, 100, shared * BS)]
+
+    def reset():
+        pool.scores.copy_(start[0])
+        other.storage.copy_(start[1])
+        other.scores.copy_(start[2])
+        torch.cuda.synchronize()
+
+    def results(outs):
+        torch.cuda.synchronize()
+        return [x.clone() for x in (*outs, pool.scores, other.storage, other.scores)]
+
+    reset()
+    want = results([f() for f in calls])
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        reset()
+        outs = []
+        for f, st in zip(calls, streams):
+            with torch.cuda.stream(st):
+                outs.append(f())
+        for got, w in zip(results(outs), want):
+            assert torch.equal(got, w)
+
+
 class _EvictedReference(llama_ref.ReferenceLlama):
     """The CPU model where a decode token sees all cached tokens, fewer than its position says."""
 

@@ -326,6 +326,25 @@ def test_refusals_of_the_binding(device, kernels):
         kernels.launch_evict(**{**ok, "scores": c.scores.cpu()})
 
 
+@pytest.mark.parametrize("name", ["budget", "recent", "protected_len"])
+def test_counts_past_32_bits(device, name):
+    pool = GpuBlockPool(1, 4, 2, 16, 64, device)
+    counts = dict(budget=20, recent=4, protected_len=4)
+    counts[name] += 2**32
+    with pytest.raises(RailgunError, match="32 bits"):
+        pool.evict(i32(np.arange(4).reshape(1, 4), device), i32([60], device), **counts)
+
+
+def test_new_lengths_over_the_old_ones(device, kernels):
+    c = Case(device, [90, 40], 32, seed=2)
+    before = c.pool.clone()
+    lens = i32(c.lens, device)
+    with pytest.raises(RailgunError, match="overlaps"):
+        kernels.launch_evict(c.pool[:, :, 0], c.pool[:, :, 1], c.scores, i32(c.table, device), i32(c.dst, device), lens,
+                             lens, c.kept, 32, 4, 0)
+    assert torch.equal(c.pool, before)
+
+
 def test_pool_evicts_every_layer(device):
     """GpuBlockPool.evict: the pool's own storage and scores."""
     pool = GpuBlockPool(3, 40, 2, 16, 64, device, fill=torch.Generator(device=device).manual_seed(1))

@@ -207,6 +207,13 @@ def test_pool_far_past_32_bits(device, kernels):
     assert float(before.abs().max()) == 0 and float(wide[:, hkv * bs:].abs().max()) == 0
 
 
+def test_first_scored_past_32_bits(device, kernels):
+    c = Batch(device, [70, 33], seed=3)
+    with pytest.raises(RailgunError, match="32 bits"):
+        c.op(kernels).execute_with_scores(c.q, c.kc, c.vc, i32(c.table, device), i32(c.ctx, device), c.scores,
+                                          first_scored=2**32)
+
+
 def test_refusals(device, kernels):
     b = Batch(device, [40, 30], seed=12)
     op, table, lens = b.op(kernels), i32(b.table, device), i32(b.ctx, device)
