@@ -634,7 +634,7 @@ SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks, bool f32) {
   // sequences so little behind the prefix that the product (at 0.7 PFLOP/s) outlasts the workers (at 5 TB/s).
   // Splits of fewer than 8 key tiles (2 in fp32, whose tiles take 16 times the time) are not made: each writes
   // 4 D bytes a row for the merge to read.
-  //   Measured (bf16, 32 / 8 heads of 128, us): 256 rows' 16,384 tokens with nothing behind them 113 with one,
+  //   Measured (bf16, 32 / 8 heads of 128, us, with one wave to a head in the merge): 256 rows' 16,384 tokens with nothing behind them 113 with one,
   // 93 with two, with 64 to 1,024 tokens behind them 177 and 189; 16 rows of 16,384 22.2 and 26.7; 16 rows of
   // 2,048 with up to 700 behind them 18.7 with 8 tiles to a split, 21.7 with 2, 22.7 with 16.
   const double product = 4.0 * sh.B * sh.H * sh.D * (double)prefix / (f32 ? 0.1e15 : 0.7e15);
@@ -658,9 +658,9 @@ bool shared_applies(const Shape& sh, int32_t dtype, int64_t kv_stride, const voi
 // kPreRows rows, full or not: 0.45 us in 16 bits, 3.4 in fp32 at head_dim 128) and the merge's splits and its
 // launch where the plain decode of a short table is one kernel (4 us).
 //   Measured (32 / 8 heads, 1 to 200 tokens behind the prefix; shared and plain, us): bf16, head_dim 128, 4
-// sequences: 512 tokens 15.0 / 13.3, 8,192 19.4 / 29.9; 32: 128 tokens 15.9 / 14.5, 512 16.8 / 20.5, 8,192
-// 24.6 / 141; head_dim 64, 32: 512 tokens 18.3 / 11.5, 2,048 19.7 / 29.9.  fp32, head_dim 128, 2: 8,192 tokens
-// 48.1 / 35.1; 8: 49.6 / 75.9, 512 tokens 20.4 / 17.5; 64: 512 tokens 28.6 / 48.4.
+// sequences: 512 tokens 15.0 / 13.3, 8,192 18.6 / 30.0; 32: 128 tokens 15.9 / 14.5, 512 16.9 / 20.3, 8,192
+// 22.3 / 143; head_dim 64, 32: 512 tokens 18.3 / 11.5, 2,048 18.7 / 29.4.  fp32, head_dim 128, 2: 8,192 tokens
+// 48.1 / 35.1; 8: 47.3 / 75.2, 512 tokens 20.4 / 17.5; 64: 512 tokens 29.4 / 48.0.
 bool shared_pays(const Shape& sh, int32_t dtype, const SharedPlan& p) {
   const double saved = 2.0 * (sh.B - 1) * p.tiles * kTileKeys * sh.Hkv * sh.D * dtype_bytes(dtype) / 8e12;
   const double product = (double)p.tiles * sh.Hkv * p.row_tiles * sh.D * (dtype == RG_DTYPE_F32 ? 27e-9 : 3.5e-9) /
