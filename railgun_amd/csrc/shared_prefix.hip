@@ -12,6 +12,9 @@
 // workgroups of either kind sit on every CU, so the shorter of the two hides under the longer.  A sequence
 // whose context ends inside the prefix is not a row of the product (which then needs no mask per row); the
 // stream-K worker takes all of its tokens.
+//   Measured (bf16, 32 / 8 heads of 128): 256 sequences over 16,384 shared tokens alone 87-92 us a call
+// (0.75-0.79 PFLOP/s), with 64 to 1,024 tokens each behind them 159 (658 MB), in long runs at the power limit up
+// to 175; 16 over 2,048 with up to 700 behind them 17.9, of which the merge takes 4.5.
 #include "decode_stream.hpp"
 
 namespace rg {
@@ -634,9 +637,10 @@ SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks, bool f32) {
   // sequences so little behind the prefix that the product (at 0.7 PFLOP/s) outlasts the workers (at 5 TB/s).
   // Splits of fewer than 8 key tiles (2 in fp32, whose tiles take 16 times the time) are not made: each writes
   // 4 D bytes a row for the merge to read.
-  //   Measured (bf16, 32 / 8 heads of 128, us, with one wave to a head in the merge): 256 rows' 16,384 tokens with nothing behind them 113 with one,
-  // 93 with two, with 64 to 1,024 tokens behind them 177 and 189; 16 rows of 16,384 22.2 and 26.7; 16 rows of
-  // 2,048 with up to 700 behind them 18.7 with 8 tiles to a split, 21.7 with 2, 22.7 with 16.
+  //   Measured (bf16, 32 / 8 heads of 128, us, with one wave to a head in the merge): 256 rows' 16,384 tokens with
+  // nothing behind them 113 with one, 93 with two, with 64 to 1,024 tokens behind them 177 and 189; 16 rows of
+  // 16,384 22.2 and 26.7; 16 rows of 2,048 with up to 700 behind them 18.7 with 8 tiles to a split, 21.7 with 2,
+  // 22.7 with 16.
   const double product = 4.0 * sh.B * sh.H * sh.D * (double)prefix / (f32 ? 0.1e15 : 0.7e15);
   const double stream = (f32 ? 8.0 : 4.0) * sh.B * sh.Hkv * sh.D * ((double)sh.MB * sh.bs - (double)prefix) / 5e12;
   const int64_t one = std::max<int64_t>(1, device_cu_count() / ((int64_t)sh.Hkv * p.row_tiles));
