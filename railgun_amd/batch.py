@@ -43,8 +43,10 @@ class DecodeSlot:
 
     ``position`` is the token's place in the text, which its rotation goes by (default: seq_len - 1;
     larger once tokens have been evicted).  ``scored_len``, for a step that gathers attention weights:
-    how many of the cached tokens hold a gathered score (0 after a prefill; seq_len - 1 while every
-    step since gathered)."""
+    how many of the leading cached tokens hold a score.  After such a step all seq_len do, whichever
+    rows it had, so it is 0 after a prefill of fresh blocks and seq_len - 1 while every step since
+    gathered; a sequence that begins with another's blocks, or with copies of them, says how many of
+    the tokens in those hold one."""
 
     last_token_id: int
     seq_len: int
@@ -80,8 +82,11 @@ class StepBatch:
     last_rows: np.ndarray = field(default=None)  # int64 [R]: row of each request's last token
     # Leading block-table entries that all decode rows share (0 unless asked for).
     shared_decode_blocks: int = 0
-    # int32 [decode rows]: cached tokens that hold a score, for a step that gathers attention weights.
+    # int32 [decode rows]: leading cached tokens that hold a score, for a step that gathers attention weights.
     scored_lens: Optional[np.ndarray] = None
+    # int32: slots of the shared prefix that no row's scored_len counts, for such a step.  It does not add
+    # to the prefix, so it sets these to 0: a row that later no longer shares them adds to what they hold.
+    unscored_slots: Optional[np.ndarray] = None
 
     @property
     def num_tokens(self) -> int:
@@ -130,12 +135,22 @@ def _scored_lens(decode_slots: Sequence[DecodeSlot], block_size: int, shared: in
     return np.asarray([d.scored_len for d in decode_slots], np.int32)
 
 
+def _unscored_slots(decode_slots: Sequence[DecodeSlot], block_size: int, shared: int) -> np.ndarray:
+    """Slots of the shared prefix's tokens behind the longest scored length of the rows."""
+    if not shared:
+        return np.zeros(0, np.int32)
+    t = np.arange(max(d.scored_len for d in decode_slots), shared * block_size, dtype=np.int64)
+    blocks = np.asarray([int(b) for b in decode_slots[0].block_table[:shared]], np.int64)
+    return (blocks[t // block_size] * block_size + t % block_size).astype(np.int32)
+
+
 def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[DecodeSlot], block_size: int,
               max_blocks: Optional[int] = None, share_prefix: bool = False, gather_scores: bool = False) -> StepBatch:
     """engine.rs:184-227 plus positions / cu_seqlens; ``max_blocks`` (default: the longest
     table) fixes the padded row length, e.g. to keep one shape across steps.  ``share_prefix`` looks for
     blocks that all decode rows begin with, ``gather_scores`` makes the step add the attention weights of
-    the decode rows' cached tokens, behind such a prefix, to the pool's scores."""
+    the decode rows' cached tokens, behind such a prefix, to the pool's scores (the prefix keeps those it
+    has).  Which rows share a prefix may change from step to step."""
     tokens, positions, slots, ctx, tables = [], [], [], [], []
     cu = [0]
     for c in prefill_chunks:
@@ -177,13 +192,14 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     lens = np.diff(np.asarray(cu))
     last = np.concatenate([np.asarray(cu[1:], np.int64) - 1,
                            cu[-1] + np.arange(len(decode_slots), dtype=np.int64)])
+    scored = _scored_lens(decode_slots, block_size, shared) if gather_scores else None
     return StepBatch(
         tokens=np.asarray(tokens, np.int64), positions=np.asarray(positions, np.int32),
         slot_mapping=np.asarray(slots, np.int32), context_lens=np.asarray(ctx, np.int32), block_table=bt,
         cu_seqlens=np.asarray(cu, np.int32), num_prefill_seqs=len(prefill_chunks), num_prefill_tokens=cu[-1],
         max_context_len=max(ctx, default=0), max_query_len=int(lens.max()) if len(lens) else 0, last_rows=last,
-        shared_decode_blocks=shared,
-        scored_lens=_scored_lens(decode_slots, block_size, shared) if gather_scores else None)
+        shared_decode_blocks=shared, scored_lens=scored,
+        unscored_slots=_unscored_slots(decode_slots, block_size, shared) if gather_scores else None)
 
 
 __all__ = ["CPU_BLOCK_FLAG", "DecodeSlot", "PrefillChunk", "StepBatch", "pack_step", "shared_prefix_blocks", "slot_of"]

@@ -92,6 +92,13 @@ class GpuBlockPool:
             self._scores = torch.zeros((layers, blocks, hkv, bs), device=self.device, dtype=torch.float32)
         return self._scores
 
+    def clear_scores(self, slots: torch.Tensor) -> None:
+        """Sets the scores of the tokens at ``slots`` (block * block_size + offset, on the device) to 0 in
+        every layer: they hold one from then on, of no weight."""
+        at, scores = slots.long(), self.scores
+        # (A zero on the device: a Python one is copied from the host, which a graph's capture refuses.)
+        scores[:, torch.div(at, self.block_size, rounding_mode="floor"), :, at % self.block_size] = scores.new_zeros(())
+
     def evict(self, block_table: torch.Tensor, context_lens: torch.Tensor, budget: int, recent: int,
               protected_len: int = 0, dst_block_table: Optional[torch.Tensor] = None,
               kept_positions: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -193,6 +193,7 @@ class DeviceStep:
     cu_seqlens: torch.Tensor
     last_rows: torch.Tensor
     scored_lens: Optional[torch.Tensor] = None
+    unscored_slots: Optional[torch.Tensor] = None
 
     @staticmethod
     def from_host(b: StepBatch, device) -> "DeviceStep":
@@ -200,7 +201,8 @@ class DeviceStep:
             return torch.from_numpy(np.ascontiguousarray(a)).to(device)
 
         return DeviceStep(b, d(b.tokens), d(b.positions), d(b.slot_mapping), d(b.context_lens), d(b.block_table),
-                          d(b.cu_seqlens), d(b.last_rows), None if b.scored_lens is None else d(b.scored_lens))
+                          d(b.cu_seqlens), d(b.last_rows), None if b.scored_lens is None else d(b.scored_lens),
+                          None if b.unscored_slots is None or not b.unscored_slots.size else d(b.unscored_slots))
 
 
 class RailgunLlama:
@@ -513,6 +515,8 @@ class RailgunLlama:
         T = st.host.num_tokens
         H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
+        if st.unscored_slots is not None:
+            self.pool.clear_scores(st.unscored_slots)
         x = F.embedding(st.tokens, w.embed)                     # residual stream [T, hidden]
         h = torch.empty_like(x)
         q = torch.empty((T, H, D), device=self.device, dtype=self.dtype)
