@@ -15,7 +15,8 @@ no data (crates/vllm-paged-attention/src/allocator.rs:102-153).  Here:
   the attention weight they have gathered (the reference never drops a cached token);
 * :meth:`GpuBlockPool.swap_out`, :meth:`GpuBlockPool.swap_in` and
   :meth:`GpuBlockPool.copy_blocks` are the physical copies behind the allocator's swap and
-  copy-on-write, each one ``rg_copy_blocks`` launch over all layers.
+  copy-on-write, each one ``rg_copy_blocks`` launch over all layers, and one for the scores where the
+  pool has any.
 
 Block ids are pool indices (``BlockId.index()``); which ids are free is the allocator's
 business and stays outside this module.
@@ -40,6 +41,12 @@ def _pairs(src: Sequence[int], dst: Sequence[int], nsrc: int, ndst: int, device)
     return m.to(device) if device is not None else m.pin_memory()
 
 
+def _new_score_rows(storage: torch.Tensor, **where) -> torch.Tensor:
+    """Zeros, fp32 [layers, NB, H_kv * bs and what rounds a row up to the 16 bytes that block copies go by]."""
+    layers, blocks, _, hkv, bs, _ = storage.shape
+    return torch.zeros((layers, blocks, -(-hkv * bs // 4) * 4), dtype=torch.float32, **where)
+
+
 class GpuBlockPool:
     """Per-layer paged KV storage ``[layers, NB, 2, H_kv, bs, D]`` on one GPU."""
 
@@ -58,6 +65,7 @@ class GpuBlockPool:
         self.block_size = block_size
         self.device = self.storage.device
         self._kernels = kernels
+        self._score_rows: Optional[torch.Tensor] = None
         self._scores: Optional[torch.Tensor] = None
 
     @staticmethod
@@ -84,12 +92,13 @@ class GpuBlockPool:
     def scores(self) -> torch.Tensor:
         """fp32 [layers, NB, H_kv, bs]: the attention weight each cached token has gathered
         (launch_v1_scores adds to it, evict goes by it); made, with zeros, when first asked for.
-        copy_blocks, swap_out and swap_in leave it as it is."""
+        copy_blocks, swap_out and swap_in take it along."""
         if self._scores is None:
             if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the pool's scores are first asked for in a graph's capture: ask for them before it")
-            layers, blocks, _, hkv, bs, _ = self.storage.shape
-            self._scores = torch.zeros((layers, blocks, hkv, bs), device=self.device, dtype=torch.float32)
+            self._score_rows = _new_score_rows(self.storage, device=self.device)
+            hkv, bs = self.storage.shape[3:5]
+            self._scores = self._score_rows[..., :hkv * bs].unflatten(-1, (hkv, bs))
         return self._scores
 
     def clear_scores(self, slots: torch.Tensor) -> None:
@@ -119,6 +128,8 @@ class GpuBlockPool:
         if set(int(b) for b in src) & set(int(b) for b in dst):
             raise ValueError("copy_blocks: a block is both a source and a destination")
         self.kernels.launch_copy_blocks(self.storage, self.storage, m, layered=True)
+        if self._scores is not None:
+            self.kernels.launch_copy_blocks(self._score_rows, self._score_rows, m, layered=True)
 
     def swap_out(self, gpu_ids: Sequence[int], cpu_pool: "CpuBlockPool", cpu_ids: Sequence[int]) -> None:
         """allocator.rs:102-131 with the data: GPU block gpu_ids[i] -> host block cpu_ids[i]."""
@@ -127,6 +138,10 @@ class GpuBlockPool:
         cpu_pool.check_compatible(self)
         m = _pairs(gpu_ids, cpu_ids, self.num_blocks, cpu_pool.num_blocks, self.device)
         self.kernels.launch_copy_blocks(self.storage, cpu_pool.storage, m, layered=True)
+        if self._scores is not None:
+            if cpu_pool.score_rows is None:
+                cpu_pool.score_rows = _new_score_rows(cpu_pool.storage, pin_memory=True)
+            self.kernels.launch_copy_blocks(self._score_rows, cpu_pool.score_rows, m, layered=True)
 
     def swap_in(self, cpu_pool: "CpuBlockPool", cpu_ids: Sequence[int], gpu_ids: Sequence[int]) -> None:
         """allocator.rs:133-153 with the data: host block cpu_ids[i] -> GPU block gpu_ids[i]."""
@@ -135,6 +150,9 @@ class GpuBlockPool:
         cpu_pool.check_compatible(self)
         m = _pairs(cpu_ids, gpu_ids, cpu_pool.num_blocks, self.num_blocks, self.device)
         self.kernels.launch_copy_blocks(cpu_pool.storage, self.storage, m, layered=True)
+        if cpu_pool.score_rows is not None:
+            _ = self.scores
+            self.kernels.launch_copy_blocks(cpu_pool.score_rows, self._score_rows, m, layered=True)
 
 
 class CpuBlockPool:
@@ -144,6 +162,8 @@ class CpuBlockPool:
         shape = (like.storage.shape[0], num_blocks) + tuple(like.storage.shape[2:])
         self.storage = torch.zeros(shape, dtype=like.storage.dtype, pin_memory=True)
         self.num_blocks = num_blocks
+        # fp32 [layers, NB, cells]: the blocks' scores, once a pool that has some swaps out to this one.
+        self.score_rows: Optional[torch.Tensor] = None
 
     def check_compatible(self, gpu: GpuBlockPool) -> None:
         g, c = gpu.storage, self.storage
