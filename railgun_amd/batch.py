@@ -29,11 +29,16 @@ CPU_BLOCK_FLAG = 1 << 31  # BlockId bit 31: the block lives in host memory (bloc
 
 @dataclass
 class PrefillChunk:
-    """batch.rs:23-34: a run of prompt tokens starting at ``position_start``."""
+    """batch.rs:23-34: a run of prompt tokens starting at ``position_start``, the number of tokens that
+    are cached before them.
+
+    ``position`` is the first token's place in the text, which the rotation goes by (default:
+    position_start; larger once tokens have been evicted)."""
 
     token_ids: Sequence[int]
     position_start: int
     block_table: Sequence[int]
+    position: Optional[int] = None
 
 
 @dataclass
@@ -161,9 +166,12 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
         end = c.position_start + n
         if (end + block_size - 1) // block_size > len(c.block_table):
             raise ValueError(f"prefill chunk ending at position {end} needs more than {len(c.block_table)} blocks")
+        place = c.position_start if c.position is None else int(c.position)
+        if place < c.position_start:
+            raise ValueError(f"prefill chunk at position {place} with {c.position_start} cached tokens before it")
         tokens.extend(int(t) for t in c.token_ids)
         for i in range(n):
-            positions.append(c.position_start + i)
+            positions.append(place + i)
             slots.append(slot_of(c.block_table, c.position_start + i, block_size))
         ctx.append(end)
         tables.append(list(c.block_table))

@@ -37,11 +37,11 @@ def small_model(device, kernels, blocks=64, dtype=torch.bfloat16, seed=3):
         sd[p + "mlp.gate_proj.weight"] = normal(inter, hid)
         sd[p + "mlp.up_proj.weight"] = normal(inter, hid)
         sd[p + "mlp.down_proj.weight"] = normal(hid, inter)
-    sd = {k: v.to(dtype).float() for k, v in sd.items()}
+    sd = {k: v.bfloat16().float() for k, v in sd.items()}  # (in float16 the same but for the smallest)
     pool = GpuBlockPool.for_model(CFG, blocks, BS, device, dtype=dtype)
     model = RailgunLlama(CFG, LlamaWeights.from_state_dict(CFG, sd, device, dtype=dtype), pool, kernels,
                          max_position=2048, choices="rg")
-    return model, pool, sd
+    return model, pool
 
 
 def prefill(model, device, tables, lens, seed=0):
@@ -73,7 +73,7 @@ SLACK = GROUP * 2.0 ** -12
 def test_a_row_that_outlives_the_others_of_its_prefix(device, kernels):
     """Two rows over eight common blocks gather, one leaves, the other goes on alone: its cells hold the weights
     of its own steps, whatever the blocks held before, and eviction goes by those."""
-    model, pool, _ = small_model(device, kernels)
+    model, pool = small_model(device, kernels)
     prefix = list(range(20, 28))
     a, b = prefix + [1, 2], prefix + [5, 6]
     start = 8 * BS + 9
@@ -106,7 +106,7 @@ def test_a_row_that_outlives_the_others_of_its_prefix(device, kernels):
 
 
 def test_a_row_that_joins_shortens_the_prefix(device, kernels):
-    model, pool, _ = small_model(device, kernels)
+    model, pool = small_model(device, kernels)
     a, b, c = [20, 21, 22, 1, 2], [20, 21, 22, 5, 6], [20, 30, 31, 8, 9]
     prefill(model, device, [a], [60])
     prefill(model, device, [b], [60])
@@ -123,7 +123,7 @@ def test_a_row_that_joins_shortens_the_prefix(device, kernels):
 
 def test_a_captured_step_clears_the_same_cells_each_time(device, kernels):
     """Captured with a prefix that no row counts, replayed with eager steps between."""
-    model, pool, _ = small_model(device, kernels)
+    model, pool = small_model(device, kernels)
     a, b = [20, 21, 1, 2], [20, 21, 5, 6]
     prefill(model, device, [a], [40])
     prefill(model, device, [b], [40])
@@ -141,3 +141,38 @@ def test_a_captured_step_clears_the_same_cells_each_time(device, kernels):
         for t, w in zip((a, b), want):
             np.testing.assert_array_equal(gathered(pool, t, 41), w)
         step(model, device, [(a, 41, 0), (b, 41, 0)])
+
+
+def test_the_next_prompt_of_a_trimmed_chat(device, kernels):
+    """A chunk behind an evicted cache, at its place in the text: the logits of the same tokens fed one at a
+    time as decode steps, whose positions are given too.  Both round their activations to bf16 in an order of
+    their own, so they differ by the drift of that rounding: measured here as the difference between those
+    decode steps and the same ones in float16, which rounds eight times finer (twice it, plus 1e-3)."""
+    n, budget, text = 150, 64, 150
+    table = list(range(30, 42))
+    tokens = np.random.default_rng(1).integers(CFG.vocab_size, size=9).tolist()
+
+    def trimmed(dtype):
+        model, pool = small_model(device, kernels, dtype=dtype)
+        prefill(model, device, [table], [n])
+        pool.scores.copy_(torch.rand(pool.scores.shape, generator=torch.Generator().manual_seed(1)))
+        lens = pool.evict(torch.tensor([table], dtype=torch.int32, device=device),
+                          torch.tensor([n], dtype=torch.int32, device=device), budget, 8, 4)
+        assert lens.tolist() == [budget]
+        return model
+
+    def forward(model, st):
+        return model.forward(DeviceStep.from_host(st, device)).float().cpu()
+
+    def one_at_a_time(dtype):
+        model = trimmed(dtype)
+        for i, t in enumerate(tokens):
+            out = forward(model, pack_step([], [DecodeSlot(t, budget + i + 1, table, position=text + i)], BS))
+        return out
+
+    steps = one_at_a_time(torch.bfloat16)
+    drift = float((steps - one_at_a_time(torch.float16)).abs().max())
+    chunk = forward(trimmed(torch.bfloat16), pack_step([PrefillChunk(tokens, budget, table, position=text)], [], BS))
+    assert float((chunk - steps).abs().max()) <= 2 * drift + 1e-3
+    wrong = forward(trimmed(torch.bfloat16), pack_step([PrefillChunk(tokens, budget, table)], [], BS))
+    assert float((wrong - steps).abs().max()) > 2 * drift + 1e-3
