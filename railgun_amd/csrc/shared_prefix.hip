@@ -623,6 +623,11 @@ void launch_shared(const StreamArgs& sa, const PrefixArgs& pa, int G, int groups
   }
 }
 
+// What the entry refuses, and what the plan's 32-bit counts would not hold.
+bool too_large(const Shape& sh) {
+  return (int64_t)sh.MB * sh.bs > INT32_MAX || sh.B > 65535 || (int64_t)sh.B * (sh.H / sh.Hkv) > INT32_MAX;
+}
+
 struct SharedPlan {
   int32_t rows, row_tiles, tiles, split_tiles, splits, workers, stream_groups;
 };
@@ -703,6 +708,7 @@ extern "C" size_t rg_paged_attention_shared_prefix_workspace_bytes(int32_t batch
     return 0;
   }
   const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  if (too_large(sh)) return 0;
   size_t n = rg_paged_attention_v1_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim, block_size,
                                                    max_blocks_per_seq);
   if (shared_blocks > 0) {
@@ -722,7 +728,7 @@ extern "C" int rg_paged_attention_shared_prefix_pays(int32_t batch_size, int32_t
     return 0;
   }
   const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
-  return shared_applies(sh, dtype, 16, nullptr, nullptr, nullptr, nullptr) &&
+  return !too_large(sh) && shared_applies(sh, dtype, 16, nullptr, nullptr, nullptr, nullptr) &&
                  shared_pays(sh, dtype, plan_shared(sh, shared_blocks, dtype == RG_DTYPE_F32))
              ? 1
              : 0;
@@ -742,8 +748,7 @@ extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* k
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: shared_blocks %d outside 0 .. max_blocks_per_seq %d", op, shared_blocks,
                 max_blocks_per_seq);
   }
-  if ((int64_t)max_blocks_per_seq * block_size > INT32_MAX || batch_size > 65535 ||
-      (int64_t)batch_size * (num_heads / num_kv_heads) > INT32_MAX) {
+  if (too_large(sh)) {
     return fail(RG_ERR_NOT_SUPPORTED, "%s: a block table of %lld tokens, %d sequences", op,
                 (long long)max_blocks_per_seq * block_size, batch_size);
   }

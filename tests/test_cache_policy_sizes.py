@@ -1,0 +1,35 @@
+"""Size queries of the shared-prefix, scoring and eviction entries at sizes that the entries refuse: host
+arithmetic, run without a GPU."""
+from __future__ import annotations
+
+import pytest
+
+import railgun_amd
+from railgun_amd import _lib
+
+BF16 = _lib.RG_DTYPE_BF16
+TOP = 2**31 - 1
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,d,bs,mb,shared", [
+    (2**30, 32, 8, 128, 16, 40, 20),         # rows (batch x heads to a kv-head) past 32 bits: 2^32 of them
+    (TOP, 32, 8, 128, 16, 40, 20),
+    (65535, 2**20, 1, 128, 16, 40, 20),
+    (65536, 32, 8, 128, 16, 40, 20),         # more sequences than a grid has
+    (4, 32, 8, 128, TOP, TOP, TOP),          # prefix tokens past 32 bits
+    (4, 32, 8, 128, 32, 2**27, 2**27),
+    (4, 32, 8, 128, 16, 2**27, 1),
+])
+def test_shared_prefix_sizes_past_the_entry(batch, heads, kv_heads, d, bs, mb, shared):
+    lib = railgun_amd.load_library()
+    shape = (batch, heads, kv_heads, d, bs, mb, shared)
+    assert lib.rg_paged_attention_shared_prefix_workspace_bytes(*shape) == 0
+    assert lib.rg_paged_attention_shared_prefix_pays(*shape, BF16) == 0
+
+
+def test_shared_prefix_sizes_at_the_limits():
+    lib = railgun_amd.load_library()
+    for shape in ((65535, 32, 8, 128, 16, 40, 20), (2, 32, 8, 128, 16, 2**27 - 1, 2**27 - 1),
+                  (1, TOP, 1, 4, 16, 4, 2), (65535, 32767, 1, 4, 16, 4, 2)):
+        assert lib.rg_paged_attention_shared_prefix_workspace_bytes(*shape) > 0
+        assert lib.rg_paged_attention_shared_prefix_pays(*shape, BF16) in (0, 1)
