@@ -507,6 +507,12 @@ size_t generic_bytes(const Shape& sh) {
   return generic_acc_bytes(sh) + align_up((size_t)sh.B * sh.H * generic_partitions(sh) * 8, 256);
 }
 
+// What the entry refuses for its size (the last line: a workspace of more bytes than 64 bits count).
+bool too_large(const Shape& sh) {
+  const int64_t tokens = (int64_t)sh.MB * sh.bs;
+  return tokens > INT32_MAX || sh.B > 65535 || sh.H > 65535 || (int64_t)sh.B * sh.H * tokens > (int64_t)1 << 48;
+}
+
 }  // namespace
 
 int probe_scores_kernels() {
@@ -530,6 +536,7 @@ extern "C" size_t rg_paged_attention_v1_scores_workspace_bytes(int32_t batch_siz
     return 0;
   }
   const Shape sh{num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size};
+  if (too_large(sh)) return 0;
   return logit_bytes(sh) + std::max(generic_bytes(sh), stream_bytes(sh, stream_workers(sh), nullptr, nullptr));
 }
 
@@ -555,7 +562,7 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
                 (long long)score_block_stride);
   }
   const int64_t tokens = (int64_t)max_blocks_per_seq * block_size;
-  if (tokens > INT32_MAX || batch_size > 65535 || num_heads > 65535) {
+  if (too_large(sh)) {
     return fail(RG_ERR_NOT_SUPPORTED, "%s: a block table of %lld tokens, %d sequences, %d heads", op,
                 (long long)tokens, batch_size, num_heads);
   }

@@ -33,3 +33,23 @@ def test_shared_prefix_sizes_at_the_limits():
                   (1, TOP, 1, 4, 16, 4, 2), (65535, 32767, 1, 4, 16, 4, 2)):
         assert lib.rg_paged_attention_shared_prefix_workspace_bytes(*shape) > 0
         assert lib.rg_paged_attention_shared_prefix_pays(*shape, BF16) in (0, 1)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,d,bs,mb", [
+    (65536, 32, 8, 128, 16, 40), (3, 65536, 8, 128, 16, 40), (3, 32, 8, 128, TOP, TOP), (3, 32, 8, 128, 16, 2**27),
+    (65535, 65535, 65535, 128, 16, 2**26),   # raw scores of 2^62 tokens and heads: more bytes than 64 bits count
+    (65535, 65535, 65535, 128, 16, 2**20),
+])
+def test_scores_sizes_past_the_entry(batch, heads, kv_heads, d, bs, mb):
+    lib = railgun_amd.load_library()
+    assert lib.rg_paged_attention_v1_scores_workspace_bytes(batch, heads, kv_heads, d, bs, mb) == 0
+    p = 64  # never followed
+    st = lib.rg_paged_attention_v1_scores(p, p, p, p, p, p, p, None, 0, 0.1, heads, kv_heads, d, bs, mb, batch, BF16, 0,
+                                          0, p, 0, None)
+    assert st == _lib.RG_ERR_NOT_SUPPORTED, _lib.last_error()
+
+
+def test_scores_sizes_at_the_limits():
+    f = railgun_amd.load_library().rg_paged_attention_v1_scores_workspace_bytes
+    assert f(4096, 4096, 4096, 128, 16, 2**20) >= 4 << 48
+    assert f(1, 32, 8, 128, 16, 2**27 - 1) >= 4 * 32 * 16 * (2**27 - 1)
