@@ -576,8 +576,10 @@ extern "C" int rg_paged_attention_v1_scores(const void* query, const void* key_c
                      tiles_take(sh, dtype, kv_stride, query, key_cache, value_cache, output);
   const int32_t workers = stream_workers(sh);
   const size_t logits = logit_bytes(sh);
-  const size_t need = logits + (tiles ? stream_bytes(sh, workers, nullptr, nullptr) : generic_bytes(sh));
-  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) {
+  // (A table of no blocks has no tokens: zeros, from nothing.)
+  const size_t need = max_blocks_per_seq == 0 ? 0
+                      : logits + (tiles ? stream_bytes(sh, workers, nullptr, nullptr) : generic_bytes(sh));
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) {
     return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned), %zu required", op,
                 workspace ? workspace_bytes : (size_t)0, need);
   }

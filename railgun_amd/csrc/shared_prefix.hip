@@ -758,7 +758,7 @@ extern "C" int rg_paged_attention_shared_prefix(const void* query, const void* k
   }
   const size_t need = rg_paged_attention_shared_prefix_workspace_bytes(batch_size, num_heads, num_kv_heads, head_dim,
                                                                        block_size, max_blocks_per_seq, shared_blocks);
-  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) {
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) {
     return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned), %zu required", op,
                 workspace ? workspace_bytes : (size_t)0, need);
   }
