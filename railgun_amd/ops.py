@@ -274,6 +274,7 @@ class PagedAttentionKernels:
     def _shared_prefix(self, query, key_cache, value_cache, block_table, context_lens, output, scale, num_heads,
                        num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size, shared_blocks,
                        workspace) -> None:
+        _require_int32(shared_blocks=shared_blocks)
         check(self.lib.rg_paged_attention_shared_prefix(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
             context_lens.data_ptr(), output.data_ptr(), scale, num_heads, num_kv_heads, head_dim, block_size,
