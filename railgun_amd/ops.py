@@ -77,6 +77,12 @@ def _require_int32(**values: int) -> None:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, f"{name} {v} does not fit 32 bits")
 
 
+def _require_blocks_apart(t: torch.Tensor, dim: int) -> None:
+    """No block stride of 0 (expand): the library takes that for dense blocks."""
+    if t.stride(dim) == 0 and t.shape[dim] > 1:
+        raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "blocks must lie apart, not be one block expanded")
+
+
 def _require_scored_lens(scored_lens: Optional[torch.Tensor], batch: int) -> None:
     if scored_lens is not None:
         _require_i32(scored_lens)
@@ -102,6 +108,7 @@ def cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, i
         raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "cache blocks must be contiguous [H_kv, bs, D]")
     if k_stride[0] != v_stride[0] or k_cache.dtype != v_cache.dtype:
         raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "k and v caches must share dtype and block stride")
+    _require_blocks_apart(k_cache, 0)
     return hkv, bs, d, k_stride[0]
 
 
@@ -112,6 +119,7 @@ def check_scores(scores: torch.Tensor, cache: torch.Tensor) -> None:
         raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
                            f"scores must be float32 {tuple(cache.shape[:-1])} with contiguous blocks, got "
                            f"{scores.dtype} {tuple(scores.shape)}")
+    _require_blocks_apart(scores, -3)
 
 
 def rope_cos_sin_table(max_position: int, head_dim: int, theta: float,
@@ -267,6 +275,7 @@ class PagedAttentionKernels:
         _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, workspace)
         _require_i32(block_table, context_lens)
         _require_table(block_table, context_lens, batch_size, max_blocks_per_seq)
+        _require_blocks_apart(key_cache, 0)
         self._shared_prefix(query, key_cache, value_cache, block_table, context_lens, output, scale, num_heads,
                             num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size, shared_blocks,
                             workspace)
@@ -300,6 +309,7 @@ class PagedAttentionKernels:
         _require_scored_lens(scored_lens, batch_size)
         check_scores(scores, key_cache)
         _require_table(block_table, context_lens, batch_size, max_blocks_per_seq)
+        _require_blocks_apart(key_cache, 0)
         self._v1_scores(query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens,
                         first_scored, scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
                         batch_size, workspace)
@@ -509,6 +519,7 @@ class PagedAttentionKernels:
         nb, hkv, bs, d = (int(x) for x in key_cache.shape[-4:])
         if key_cache.stride()[-3:] != (bs * d, d, 1):
             raise bad("cache blocks must be contiguous [H_kv, bs, D]")
+        _require_blocks_apart(key_cache, -4)
         check_scores(scores, key_cache)
         batch = int(context_lens.numel())
         if block_table.dim() != 2 or int(block_table.shape[0]) != batch:

@@ -34,3 +34,20 @@ def test_shared_blocks_past_32_bits(device, kernels, blocks):
     with pytest.raises(RailgunError, match="32 bits"):
         kernels.launch_shared_prefix(c.q, c.kc, c.vc, c.table, c.lens, torch.empty_like(c.q), 0.125, *c.shape, blocks,
                                      c.ws)
+
+
+def test_one_block_expanded(device, kernels):
+    """A block stride of 0 stands for dense blocks in the library, which would be read and written past the one."""
+    c = Call(device)
+    flat = c.scores[:1].expand_as(c.scores)
+    k, v = c.kc[:1].expand_as(c.kc), c.vc[:1].expand_as(c.vc)
+    out, op = torch.empty_like(c.q), c.op(kernels)
+    for call in (lambda: op.execute_with_scores(c.q, c.kc, c.vc, c.table, c.lens, flat),
+                 lambda: op.execute_with_scores(c.q, k, v, c.table, c.lens, c.scores),
+                 lambda: op.execute_shared_prefix(c.q, k, v, c.table, c.lens, 1),
+                 lambda: kernels.launch_v1_scores(c.q, k, v, c.table, c.lens, out, c.scores, None, 0, 0.125, *c.shape, c.ws),
+                 lambda: kernels.launch_shared_prefix(c.q, k, v, c.table, c.lens, out, 0.125, *c.shape, 1, c.ws),
+                 lambda: kernels.launch_evict(c.kc, c.vc, flat, c.table, None, c.lens, None, None, 32, 4),
+                 lambda: kernels.launch_evict(k, v, c.scores, c.table, None, c.lens, None, None, 32, 4)):
+        with pytest.raises(RailgunError, match="apart"):
+            call()
