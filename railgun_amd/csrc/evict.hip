@@ -387,7 +387,7 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
 constexpr int kMoveMaxTokens = 512;
 constexpr int kInPlacePieces = 8;
 
-// Workgroup (chunk, segment), NT threads: tokens chunk * tok .. of the segment's kept list, tok such that their K
+// Workgroup (segment, chunk), NT threads: tokens chunk * tok .. of the segment's kept list, tok such that their K
 // and V rows fill U pieces V a thread, all of them read before the first is written.  A segment that is evicted in
 // place is walked by its first workgroup alone: the chunk at hand is written once every thread has read its part
 // of it.  That is enough: kept[j] >= j, so rows j .. of the destination never hold a row that a later chunk has
@@ -464,8 +464,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs a, const Segment sg, i
 template <typename V, int NT, int U>
 __global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a, int row_vecs, int tok) {
   const bool in_order = a.in_order[blockIdx.x] != 0;
-  if (in_order && blockIdx.y != 0) return;
-  move_rows<V, NT, U, false>(a, segment_of(a, blockIdx.x), blockIdx.x, row_vecs, tok, (int)blockIdx.y * tok, in_order);
+  // (A grid has no more than 65,535 workgroups in y, and rows in 2-byte pieces make chunks of a single token.)
+  const int64_t chunk = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
+  if ((in_order && chunk != 0) || chunk * tok >= a.budget) return;
+  move_rows<V, NT, U, false>(a, segment_of(a, blockIdx.x), blockIdx.x, row_vecs, tok, (int)(chunk * tok), in_order);
 }
 
 // Both in one launch, a workgroup per segment: where there are segments enough to fill the chip with one each (the
@@ -632,8 +634,8 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   auto move = [&](auto kernel, int threads, int pieces) {
     const int tok = chunk(threads, pieces);
     const int64_t chunks = dst_block_table == nullptr ? 1 : ceil_div(most, tok);
-    if (chunks > 65535) return fail(RG_ERR_NOT_SUPPORTED, "%s: a budget of %lld tokens", op, (long long)most);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)segments, (unsigned)chunks), dim3(threads), 0, s, a, row_vecs, tok);
+    const unsigned y = (unsigned)std::min<int64_t>(chunks, 65535), z = (unsigned)ceil_div(chunks, y);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)segments, y, z), dim3(threads), 0, s, a, row_vecs, tok);
     return check_launch(op);
   };
   // (In place without a second table no segment has use for more than one workgroup.)
