@@ -123,7 +123,8 @@ __device__ __forceinline__ bool select_segment(const EvictArgs a, const Segment 
   const int32_t* row = a.table + (int64_t)sg.seq * a.max_blocks;
   if (a.new_lens != nullptr && sg.layer == 0 && sg.kvh == 0 && tid == 0) a.new_lens[sg.seq] = m;
   if (n <= a.budget) {
-    for (int i = tid; i < a.kept_stride; i += NT) kept[i] = i < n ? i : -1;
+    // (Unsigned: the caller's list may be as long as 32 bits count.)
+    for (unsigned i = tid; i < (unsigned)a.kept_stride; i += NT) kept[i] = (int)i < n ? (int)i : -1;
     return false;
   }
   const int p0 = a.guarded;

@@ -15,3 +15,14 @@ pytestmark = pytest.mark.gpu
 def test_more_chunks_than_a_grid_has_in_y(device, kernels, dst):
     """Rows of 1,000 bytes move in 2-byte pieces, a token a workgroup: 66,000 of them."""
     Case(device, [70100, 300], 66000, dtype="f32", hkv=1, d=250, dst=dst, seed=2).check(kernels, 50, 9)
+
+
+def test_a_list_of_kept_positions_as_long_as_32_bits_count(device, kernels):
+    budget = 2**31 - 1
+    pool = torch.randn((12, 2, 1, 16, 8), device=device).bfloat16()
+    kept = torch.zeros(budget, dtype=torch.int32, device=device)
+    kernels.launch_evict(pool[:, 0], pool[:, 1], torch.rand((12, 1, 16), device=device), i32(np.arange(12)[None], device),
+                         None, i32([190], device), None, kept.view(1, 1, budget), budget, 8)
+    assert kept[:190].tolist() == list(range(190))
+    for part in kept[190:].split(1 << 28):
+        assert int(part.min()) == int(part.max()) == -1
