@@ -193,8 +193,9 @@ int rg_copy_blocks(const void* src_pool, void* dst_pool, const int32_t* block_ma
  * [num_layers, batch, num_kv_heads, budget] the kept positions in order, -1 behind them.
  * key_cache / value_cache / scores point at layer 0, layer l lies layer_stride (score_layer_stride)
  * elements further on.  The workspace (rg_evict_cache_workspace_bytes, 4-byte aligned) needs no
- * clearing; of it the first 4 bytes per (layer, sequence, kv-head), rounded up to 256, suffice with
- * kept_positions.  New entry: the reference never drops a cached token. */
+ * clearing; the bytes for a budget of max_blocks_per_seq * block_size suffice where the budget is
+ * larger, and with kept_positions the first 4 per (layer, sequence, kv-head), rounded up to 256.  New
+ * entry: the reference never drops a cached token. */
 size_t rg_evict_cache_workspace_bytes(int32_t num_layers, int32_t batch_size,
                                       int32_t num_kv_heads, int32_t budget);
 int rg_evict_cache(void* key_cache, void* value_cache, float* scores,

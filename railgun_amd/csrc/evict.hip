@@ -568,7 +568,7 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   if (segments < 0) {
     return fail(RG_ERR_NOT_SUPPORTED, "%s: more than %d (layer, sequence, kv-head) segments", op, INT32_MAX);
   }
-  const size_t need = evict_bytes(segments, budget, kept_positions == nullptr);
+  const size_t need = evict_bytes(segments, most, kept_positions == nullptr);
   if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0) {
     return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (4-byte aligned), %zu required", op,
                 workspace ? workspace_bytes : (size_t)0, need);
@@ -594,7 +594,7 @@ extern "C" int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
   a.kv_stride = kv_stride;
   a.score_layer_stride = num_layers > 1 ? score_layer_stride : 0;
   a.score_stride = score_stride;
-  a.kept_stride = budget;
+  a.kept_stride = kept_positions ? budget : (int32_t)most;
   a.budget = budget;
   a.recent = recent;
   a.guarded = protected_len;

@@ -531,8 +531,9 @@ class PagedAttentionKernels:
         if kept_positions is not None and int(kept_positions.numel()) != layers * batch * hkv * budget:
             raise bad(f"kept_positions must be [{layers}, {batch}, {hkv}, {budget}]")
         if workspace is None:
-            nbytes = self._ask("rg_evict_cache_workspace_bytes", layers, batch, hkv,
-                               budget if kept_positions is None else 1)
+            # (The kept list, where it is the workspace's, is no longer than a table's row of tokens.)
+            held = min(budget, int(block_table.shape[1]) * bs) if kept_positions is None else 1
+            nbytes = self._ask("rg_evict_cache_workspace_bytes", layers, batch, hkv, max(held, 1))
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=key_cache.device)
         check(self.lib.rg_evict_cache(
             key_cache.data_ptr(), value_cache.data_ptr(), scores.data_ptr(), block_table.data_ptr(),

@@ -53,3 +53,14 @@ def test_scores_sizes_at_the_limits():
     f = railgun_amd.load_library().rg_paged_attention_v1_scores_workspace_bytes
     assert f(4096, 4096, 4096, 128, 16, 2**20) >= 4 << 48
     assert f(1, 32, 8, 128, 16, 2**27 - 1) >= 4 * 32 * 16 * (2**27 - 1)
+
+
+@pytest.mark.parametrize("budget,kept,need", [(64, None, 256 + 48 * 64 * 4), (160, None, 256 + 48 * 160 * 4),
+                                              (161, None, 256 + 48 * 160 * 4), (TOP, None, 256 + 48 * 160 * 4),
+                                              (TOP, 64, 256)])
+def test_eviction_asks_for_no_more_than_the_table_holds(budget, kept, need):
+    """Ten blocks of 16 tokens, 48 segments: the call with one byte less says what it needs."""
+    p = 64  # never followed
+    st = railgun_amd.load_library().rg_evict_cache(p, p, p, p, None, p, None, kept, budget, 8, 4, 2, 8, 64, 16, 10, 0, 3,
+                                                   BF16, 1 << 20, 0, 1 << 14, 0, p, need - 1, None)
+    assert st == _lib.RG_ERR_WORKSPACE and f"{need} required" in _lib.last_error()
