@@ -53,6 +53,11 @@ constexpr int kPreRows = 32 * kPreWaves;  // rows of a workgroup, 32 a wave
 constexpr int kTileKeys = 32;
 constexpr int kStages = 3;                // key tiles in the LDS ring
 constexpr float kSlack = 8.f;             // log2 headroom of the lazy maximum: 2^8 a probability at most
+// log2 of what probabilities are held times over.  fp16's normal numbers end at 2^-14: one token's weight beside
+// those of thousands that are 2^-25 of it each would be all that is left.  Times 2^7 they fill the type up to
+// 2^(8 + 7), and the half step of the subnormals, 2^-25, is 2^-32 of the largest weight.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, f16_t> ? 7.f : 0.f;
 
 struct PrefixArgs {
   float* acc;  // [H_kv, splits, rows, D] unnormalised
@@ -227,9 +232,10 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
     // Probabilities, rounded to the operand type of the PV product; the sum takes the rounded ones, so
     // the normaliser weighs what enters the product.
     uint32_t pk[8];
+    const float less = kLift<T> - m_run;
 #pragma unroll
     for (int v = 0; v < 16; v += 2)
-      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, -m_run)), fast_exp2(fmaf(c[v + 1], a.scale_log2, -m_run)));
+      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, less)), fast_exp2(fmaf(c[v + 1], a.scale_log2, less)));
     float s0 = pair_sum<T>(pk[0], l_run), s1 = pair_sum<T>(pk[1], 0.f);
 #pragma unroll
     for (int i = 2; i < 8; i += 2) {
@@ -296,7 +302,7 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
         *reinterpret_cast<float4*>(acc + 32 * db + 8 * p + 4 * hh) =
             make_float4(o[db][4 * p], o[db][4 * p + 1], o[db][4 * p + 2], o[db][4 * p + 3]);
     if (hh == 0) {
-      a.ml[2 * at] = m_run;
+      a.ml[2 * at] = m_run - kLift<T>;
       a.ml[2 * at + 1] = l;
     }
   }
