@@ -1320,11 +1320,15 @@ inline size_t stream_bytes(const Shape& sh, int32_t workers, StreamScratch* carv
 // at 1,024; in fp32 0.92 / 0.98 at 512.
 //   Up to two per CU: 64 tokens, 0.92 at worst (264 to 512 segments); at 128 already 1.33, at 320
 // 1.48.  More: never (1,024 segments of 64 tokens 1.27 to 1.60).
+constexpr int64_t short_widest_tokens(int head_dim, int elem_bytes) {
+  const int64_t kb = (head_dim == 64 ? 224 : 160) + (elem_bytes == 4 ? 32 : 0);  // of K and V
+  return (kb << 10) / (head_dim * 2 * elem_bytes);
+}
+static_assert(short_widest_tokens(64, 2) <= kShortMaxTokens, "the widest of them");
 inline bool short_applies(const Shape& sh, int elem_bytes) {
   const int64_t tokens = (int64_t)sh.MB * sh.bs, segments = (int64_t)sh.B * sh.Hkv;
-  const int64_t widest = (sh.D == 64 ? 224 : 160) + (elem_bytes == 4 ? 32 : 0);  // KB of K and V
-  if ((sh.D != 64 && sh.D != 128) || sh.H / sh.Hkv > 8 || tokens > kShortMaxTokens || sh.B > 65535 ||
-      tokens * sh.D * 2 * elem_bytes > widest << 10) {
+  if ((sh.D != 64 && sh.D != 128) || sh.H / sh.Hkv > 8 || sh.B > 65535 ||
+      tokens > short_widest_tokens(sh.D, elem_bytes)) {
     return false;
   }
   const int64_t cus = device_cu_count();  // (two calls of the runtime: asked for small tables only)

@@ -8,9 +8,10 @@
 // positions 0 .. |K| - 1 of the destination table.
 //
 // evict_select_kernel (one workgroup per segment) finds the threshold: scores become 32-bit keys in
-// the order of the values, and three passes over 11, 11 and 10 bits narrow the key T of the last one
-// to be kept, each with a histogram in LDS over the candidates that agree with the bits found so
-// far (after the first pass mostly few, which are then listed).  A kept candidate's place is then known: before
+// the order of the values, and three passes over 11, 11 and 10 bits (13, 11 and 8 for tables of more
+// than 16,384 tokens) narrow the key T of the last one to be kept, each with a histogram in LDS over
+// the candidates that agree with the bits found so far (after the first pass mostly few, which are
+// then listed).  A kept candidate's place is then known: before
 // position t lie
 //   #{key > T before t} + min(#{key == T before t}, ties to keep)
 // kept candidates.  The kernel leaves the kept positions in order (the caller's array, or workspace).

@@ -25,7 +25,7 @@ constexpr int kFinThreads = 256;
 constexpr int kFinWaves = kFinThreads / 64;
 constexpr int kFinTokens = 1024;   // tokens a workgroup turns into weights at a time
 constexpr int kMaxGroup = 512;     // query heads to a kv-head
-constexpr int kShortMaxScored = 1024;  // tokens of table that the one-launch kernel takes (short_applies admits no more)
+constexpr int kShortMaxScored = 1024;  // tokens of table that the one-launch kernel holds old scores of
 
 struct ScoreArgs {
   void* out;
@@ -411,10 +411,13 @@ __global__ __launch_bounds__(kShortThreads) void scores_short_kernel(
   }
 }
 
-// The one-launch kernel takes what the plain decode's takes, up to kShortMaxScored tokens of table; fp32 at
-// head_dim 128 with 8 heads to a kv-head fills the registers without the scores.
+// The one-launch kernel takes what the plain decode's takes (up to 896 tokens of table at head_dim 64 and 320 at 128
+// in 16 bits, 512 and 192 in fp32); fp32 at head_dim 128 with 8 heads to a kv-head fills the registers without the
+// scores.
+static_assert(short_widest_tokens(64, 2) <= kShortMaxScored && short_widest_tokens(64, 4) <= kShortMaxScored &&
+              short_widest_tokens(128, 2) <= kShortMaxScored && short_widest_tokens(128, 4) <= kShortMaxScored);
 bool scores_short_applies(const Shape& sh, int32_t dtype) {
-  return (int64_t)sh.MB * sh.bs <= kShortMaxScored && short_applies(sh, dtype_bytes(dtype)) &&
+  return short_applies(sh, dtype_bytes(dtype)) &&
          !(dtype == RG_DTYPE_F32 && sh.D == 128 && sh.H / sh.Hkv == 8);
 }
 

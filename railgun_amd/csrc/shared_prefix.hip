@@ -9,12 +9,13 @@
 //   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 //
 // One launch computes both: the product is bound by the matrix cores and LDS, the suffixes by HBM, and
-// workgroups of either kind sit on every CU, so the shorter of the two hides under the longer.  A sequence
+// workgroups of either kind sit on every CU, so the shorter of the two hides under the longer (but for the forms
+// of more than 256 registers, groups_per_cu: there the product's follow the workers').  A sequence
 // whose context ends inside the prefix is not a row of the product (which then needs no mask per row); the
 // stream-K worker takes all of its tokens.
-//   Measured (bf16, 32 / 8 heads of 128): 256 sequences over 16,384 shared tokens alone 87-92 us a call
-// (0.75-0.79 PFLOP/s), with 64 to 1,024 tokens each behind them 159 (658 MB), in long runs at the power limit up
-// to 175; 16 over 2,048 with up to 700 behind them 17.9, of which the merge takes 4.5.
+//   Measured (bf16, 32 / 8 heads of 128): 256 sequences over 16,384 shared tokens alone 88-92 us a call
+// (0.75-0.78 PFLOP/s), with 64 to 1,024 tokens each behind them 158-164 (658 MB; in long runs at the power limit
+// up to 188); 16 over 2,048 with up to 700 behind them 17.3, of which the merge takes 4.4.
 #include "decode_stream.hpp"
 
 namespace rg {
@@ -474,8 +475,14 @@ constexpr int ring_bytes() {
   else return kStages * KeyTile<D>::BYTES;
 }
 
-// Workgroups to a CU that the compiler is held to: two (256 registers a wave) where that costs the worker's tile
-// few of its own.
+// Workgroups to a CU that the compiler is held to: two, 256 registers a wave, where it fits them without scratch
+// memory, which it does not try by itself.  Of the forms that come to more than 256 (or close to it) those are fp32
+// at head_dim 128 with up to 4 heads to a kv-head: 252, 254, 264 and 268 by themselves for 1 to 4, at most 256 held.
+// Held to that, fp32 with more heads (280 to 330), 16 bits at head_dim 64 with 5, 6, 7 and 16 (264 to 281) and at
+// 128 with 16 (280) would spill: those run one workgroup a CU.
+//   Measured (fp32, 8 kv-heads of 128, 64 sequences over 2,048 / 8,192 tokens with up to 200 / 1,500 behind them;
+// left alone -> held, us): G 1 26 -> 26 / 82 -> 82, 2 32 -> 32 / 93 -> 94, 3 44 -> 38 / 140 -> 113, 4 47 -> 40 /
+// 144 -> 118.
 template <typename T, int D, int G>
 constexpr int groups_per_cu() { return std::is_same_v<T, f32_t> && D == 128 && G <= 4 ? 2 : 1; }
 
@@ -648,10 +655,10 @@ SharedPlan plan_shared(const Shape& sh, int32_t shared_blocks, bool f32) {
   // sequences so little behind the prefix that the product (at 0.7 PFLOP/s) outlasts the workers (at 5 TB/s).
   // Splits of fewer than 8 key tiles (2 in fp32, whose tiles take 16 times the time) are not made: each writes
   // 4 D bytes a row for the merge to read.
-  //   Measured (bf16, 32 / 8 heads of 128, us, with one wave to a head in the merge): 256 rows' 16,384 tokens with
-  // nothing behind them 113 with one, 93 with two, with 64 to 1,024 tokens behind them 177 and 189; 16 rows of
-  // 16,384 22.2 and 26.7; 16 rows of 2,048 with up to 700 behind them 18.7 with 8 tiles to a split, 21.7 with 2,
-  // 22.7 with 16.
+  //   Measured (bf16, 32 / 8 heads of 128, us): 256 rows' 16,384 tokens with one token behind them 117 with one,
+  // 109 with two, with 64 to 1,024 tokens behind them 159 and 177; 16 rows of 16,384 22.3 and 29.0; 16 rows of 2,048
+  // with up to 700 behind them 17.4 with 8 tiles to a split, 18.2 with 4, 20.3 with 2, 22.0 with 16.  fp32, 64 rows of
+  // 2,048: 39.8 with 2 tiles, 85 with 16.
   const double product = 4.0 * sh.B * sh.H * sh.D * (double)prefix / (f32 ? 0.1e15 : 0.7e15);
   const double stream = (f32 ? 8.0 : 4.0) * sh.B * sh.Hkv * sh.D * ((double)sh.MB * sh.bs - (double)prefix) / 5e12;
   const int64_t one = std::max<int64_t>(1, device_cu_count() / ((int64_t)sh.Hkv * p.row_tiles));
