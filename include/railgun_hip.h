@@ -189,8 +189,9 @@ int rg_copy_blocks(const void* src_pool, void* dst_pool, const int32_t* block_ma
  * no other entry of either table that the call uses.  Blocks that hold positions below
  * protected_len only, at the same place in both rows, are not written, so sequences may share them.
  *
- * new_context_lens (NULL: not wanted; apart from context_lens) [batch] gets min(n, budget); kept_positions (NULL: not wanted)
- * [num_layers, batch, num_kv_heads, budget] the kept positions in order, -1 behind them.
+ * new_context_lens (NULL: not wanted; apart from context_lens) [batch] gets min(n, budget);
+ * kept_positions (NULL: not wanted) [num_layers, batch, num_kv_heads, budget] the kept positions in
+ * order, -1 behind them.
  * key_cache / value_cache / scores point at layer 0, layer l lies layer_stride (score_layer_stride)
  * elements further on.  The workspace (rg_evict_cache_workspace_bytes, 4-byte aligned) needs no
  * clearing; the bytes for a budget of max_blocks_per_seq * block_size suffice where the budget is
@@ -404,7 +405,7 @@ int rg_paged_attention_v1_plus(const void* query, const void* key_cache,
  * a batch among them) may have other blocks there, and anything behind their own tokens.  The same
  * output up to rounding, with the shared blocks read once for many rows instead of once per sequence, as
  * one product on the matrix cores (in bf16 / f16 with the probabilities of the shared tokens
- * rounded to that type, as in rg_prefill_packed).  Sequences may be shorter than the prefix or
+ * rounded to that type, in f16 times 2^7; rg_paged_attention_v1 keeps them in fp32).  Sequences may be shorter than the prefix or
  * empty (context_lens[s] == 0 gives zeros); shared_blocks == 0 is rg_paged_attention_v1.  Any shape
  * of rg_paged_attention_v1; the shared product runs for more than one sequence with a block_size
  * of 16 * 2^j up to 256 and head_dim 64 or 128, num_heads / num_kv_heads 1 to 8 or 16, the other
@@ -441,7 +442,8 @@ int rg_paged_attention_shared_prefix(const void* query, const void* key_cache,
  * elements between blocks (0: dense).  scored_lens [batch] says how many of a sequence's leading
  * cells hold a score already, so that the cells of new tokens need no clearing; NULL: all of them
  * do; zeros: this step's weights alone are written.  Cells before first_scored (blocks that several
- * sequences share) and from context_lens[s] on keep what they hold.  A block with scored positions
+ * sequences share) and from context_lens[s] on keep what they hold; where first_scored becomes smaller
+ * from call to call, the cells it uncovers have to hold a score by then.  A block with scored positions
  * belongs to one sequence of the call: two that share one would write the same cells in no set order.
  * The workspace (rg_paged_attention_v1_scores_workspace_bytes, 16-byte aligned, needed, no clearing)
  * holds one fp32 per (sequence, query head, token of the table) beside the split-K partials.

@@ -152,10 +152,14 @@ def _unscored_slots(decode_slots: Sequence[DecodeSlot], block_size: int, shared:
 def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[DecodeSlot], block_size: int,
               max_blocks: Optional[int] = None, share_prefix: bool = False, gather_scores: bool = False) -> StepBatch:
     """engine.rs:184-227 plus positions / cu_seqlens; ``max_blocks`` (default: the longest
-    table) fixes the padded row length, e.g. to keep one shape across steps.  ``share_prefix`` looks for
-    blocks that all decode rows begin with, ``gather_scores`` makes the step add the attention weights of
-    the decode rows' cached tokens, behind such a prefix, to the pool's scores (the prefix keeps those it
-    has).  Which rows share a prefix may change from step to step."""
+    table) fixes the padded row length, e.g. to keep one shape across steps.
+
+    ``share_prefix`` looks for blocks that all decode rows begin with (none, once one row begins
+    otherwise); the model reads those once where that pays, and in bf16 / f16 then rounds their tokens'
+    probabilities to that type.  ``gather_scores`` makes the step add the attention weights of the decode
+    rows' cached tokens, behind such a prefix, to the pool's scores; the prefix keeps those it has, and
+    blocks that only some of the rows share are refused.  Which rows share a prefix may change from step
+    to step."""
     tokens, positions, slots, ctx, tables = [], [], [], [], []
     cu = [0]
     for c in prefill_chunks:

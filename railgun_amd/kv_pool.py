@@ -113,7 +113,11 @@ class GpuBlockPool:
               kept_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Trims the sequences of ``block_table`` to ``budget`` tokens by ``scores``, every layer in one
         call (launch_evict); returns the new context lengths, int32 on the device.  In place, the
-        blocks past a sequence's new length hold nothing it needs: the caller frees or refills them."""
+        blocks past a sequence's new length hold nothing it needs: the caller frees or refills them.
+
+        A token whose cell holds no score (cached by a step that did not gather, such as a prefill) ranks
+        by whatever the cell holds: keep such within ``protected_len`` and ``recent``, or clear_scores
+        first.  Few long sequences are trimmed faster into other blocks than in place."""
         new_lens = torch.empty_like(context_lens)
         self.kernels.launch_evict(self.storage[:, :, 0], self.storage[:, :, 1], self.scores, block_table,
                                   dst_block_table, context_lens, new_lens, kept_positions, budget, recent,

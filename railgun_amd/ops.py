@@ -271,7 +271,8 @@ class PagedAttentionKernels:
                              workspace: torch.Tensor) -> None:
         """launch_v1 for a batch whose rows of ``block_table``, as far as their context holds them all,
         begin with the same ``shared_blocks`` entries: those blocks are read once for many rows
-        (rg_paged_attention_shared_prefix)."""
+        (rg_paged_attention_shared_prefix).  In bf16 / f16 the probabilities of the shared tokens are
+        rounded to that type, where launch_v1 keeps them in fp32."""
         _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, workspace)
         _require_i32(block_table, context_lens)
         _require_table(block_table, context_lens, batch_size, max_blocks_per_seq)
@@ -302,8 +303,10 @@ class PagedAttentionKernels:
         """launch_v1 that also adds to ``scores`` (fp32 [NB, H_kv, bs], paged like the caches) the softmax
         weight every cached token from position ``first_scored`` on gets from the kv-head's queries
         (rg_paged_attention_v1_scores).  ``scored_lens`` [batch]: how many of a sequence's leading cells
-        hold a score to add to, the others are overwritten; None: all.  A block with scored positions
-        belongs to one sequence of the call."""
+        hold a score to add to, the others are overwritten; None: all.  Cells before ``first_scored``
+        are left as they are: where it becomes smaller from call to call, they have to hold a score of
+        that sequence (or 0) by then.  A block with scored positions belongs to one sequence of the
+        call."""
         _require_cuda(query, key_cache, value_cache, block_table, context_lens, output, scores, scored_lens, workspace)
         _require_i32(block_table, context_lens)
         _require_scored_lens(scored_lens, batch_size)
@@ -629,8 +632,9 @@ class PagedAttentionOp:
                               block_table: torch.Tensor, context_lens: torch.Tensor, shared_blocks: int,
                               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """execute() for sequences whose block tables begin with the same ``shared_blocks`` entries (all
-        whose context holds those): launch_shared_prefix where it pays, else launch_v1.  The workspace
-        (shared_prefix_workspace_bytes) is allocated here when omitted."""
+        whose context holds those): launch_shared_prefix where it pays, else launch_v1, which in
+        bf16 / f16 is the more precise of the two.  The workspace (shared_prefix_workspace_bytes) is
+        allocated here when omitted."""
         batch, mb = self._check_decode(q, k_cache, v_cache, block_table, context_lens)
         if not 0 <= shared_blocks <= mb:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, f"shared_blocks {shared_blocks} outside 0 .. {mb}")
