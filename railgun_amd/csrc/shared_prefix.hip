@@ -54,11 +54,16 @@ constexpr int kPreRows = 32 * kPreWaves;  // rows of a workgroup, 32 a wave
 constexpr int kTileKeys = 32;
 constexpr int kStages = 3;                // key tiles in the LDS ring
 constexpr float kSlack = 8.f;             // log2 headroom of the lazy maximum: 2^8 a probability at most
-// log2 of what probabilities are held times over.  fp16's normal numbers end at 2^-14: one token's weight beside
-// those of thousands that are 2^-25 of it each would be all that is left.  Times 2^7 they fill the type up to
-// 2^(8 + 7), and the half step of the subnormals, 2^-25, is 2^-32 of the largest weight.
+// What is subtracted from the scores of a row whose lazy maximum is m (log2 units): in fp16 2^7 times the
+// probabilities are held.  Its normal numbers end at 2^-14: one token's weight beside those of thousands that are
+// 2^-25 of it each would be all that is left.  Times 2^7 they fill the type up to 2^(8 + 7), and the half step of
+// the subnormals, 2^-25, is 2^-32 of the largest weight.  Past 2^20 the fp32 scores' own steps grow towards the one
+// factor of two that is left below 2^16; there they are held as they are.
 template <typename T>
-constexpr float kLift = std::is_same_v<T, f16_t> ? 7.f : 0.f;
+__device__ __forceinline__ float reference(float m) {
+  if constexpr (std::is_same_v<T, f16_t>) return m - (fabsf(m) < 0x1p20f ? 7.f : 0.f);
+  else return m;
+}
 
 struct PrefixArgs {
   float* acc;  // [H_kv, splits, rows, D] unnormalised
@@ -163,6 +168,7 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
+  float ref = -INFINITY;    // reference(m_run)
   float m_thr = -INFINITY;  // m_run + kSlack in raw score units, so a tile's test needs no multiply
   const int xor32 = (lane ^ 32) << 2;
   const int k_lane = (j >> 4) * (TL::KB / 2) + hh * 256 + (j & 15) * 16;
@@ -221,8 +227,10 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
       const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)));
       const float both = fmaxf(tmax, other) * a.scale_log2;
       const float m_new = both > m_run + kSlack ? both : m_run;
-      const float alpha = fast_exp2(m_run - m_new);
+      const float ref_new = reference<T>(m_new);
+      const float alpha = fast_exp2(ref - ref_new);
       m_run = m_new;
+      ref = ref_new;
       m_thr = (m_run + kSlack) / a.scale_log2;
       l_run *= alpha;
 #pragma unroll
@@ -233,10 +241,9 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
     // Probabilities, rounded to the operand type of the PV product; the sum takes the rounded ones, so
     // the normaliser weighs what enters the product.
     uint32_t pk[8];
-    const float less = kLift<T> - m_run;
 #pragma unroll
     for (int v = 0; v < 16; v += 2)
-      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, less)), fast_exp2(fmaf(c[v + 1], a.scale_log2, less)));
+      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, -ref)), fast_exp2(fmaf(c[v + 1], a.scale_log2, -ref)));
     float s0 = pair_sum<T>(pk[0], l_run), s1 = pair_sum<T>(pk[1], 0.f);
 #pragma unroll
     for (int i = 2; i < 8; i += 2) {
@@ -303,7 +310,7 @@ __device__ __forceinline__ void prefix_product(const PrefixArgs& a, const uint16
         *reinterpret_cast<float4*>(acc + 32 * db + 8 * p + 4 * hh) =
             make_float4(o[db][4 * p], o[db][4 * p + 1], o[db][4 * p + 2], o[db][4 * p + 3]);
     if (hh == 0) {
-      a.ml[2 * at] = m_run - kLift<T>;
+      a.ml[2 * at] = ref;
       a.ml[2 * at + 1] = l;
     }
   }

@@ -40,3 +40,23 @@ def test_many_small_weights_beside_a_large_one(device, kernels, dtype, gap, at):
         tol = tol + shared * 16 * 2.0 ** -32 * float(v.abs().max())
     assert want.min() > 0.5 * shared * 16 * 2.0 ** -gap
     assert_within(dev_f32(b.run(kernels))[some], want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("power", range(12, 27, 2))
+def test_scores_as_large_as_the_steps_between_them(device, kernels, dtype, power):
+    """Scores around 2^power in log2 units, where fp32 tells them apart by whole powers of two in the end.  All
+    values are 1, so every output is 1 whatever the weights: off by the roundings of the probabilities, which
+    the sum takes too, by the fp32 sums of 16,384 terms (2^-23 each) and by its own rounding."""
+    shared = 1024
+    b = Batch(device, [shared * 16 + 1] * 300, shared, dtype, 32, 32, 64, seed=power)
+    g = torch.Generator(device=device).manual_seed(power)
+    k = torch.randn(b.kc.shape, generator=g, device=device)
+    k[..., 0] = 256.0                                # 2^16 of a raw score; the others' part some hundreds
+    b.kc.copy_(k)
+    b.vc.fill_(1.0)
+    b.q.copy_(32 * torch.randn(b.q.shape, generator=g, device=device))
+    b.q[..., 0] = 256.0
+    b.scale = 2.0 ** (power - 16) / math.log2(math.e)
+    out = dev_f32(b.run(kernels))
+    assert_within(out, 1.0, 16384 * 2.0 ** -23 + {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype])
