@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("gap", [17.0, 25.5, 28.0])
-@pytest.mark.parametrize("at", [0, 7000])
+@pytest.mark.parametrize("gap,at", [(14.5, 0), (15.5, 7000), (17.0, 0), (21.3, 0), (21.8, 7000), (22.5, 0), (25.5, 0),
+                                    (25.5, 7000), (28.0, 0), (28.0, 7000)])
 def test_many_small_weights_beside_a_large_one(device, kernels, dtype, gap, at):
     """Weights of 2^-gap of the largest each, whose value is 0, so the output is theirs alone.  Rows enough that
     the prefix is in two parts, and the large weight stands before half of the others.
