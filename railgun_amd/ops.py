@@ -287,8 +287,8 @@ class PagedAttentionKernels:
         _require_int32(shared_blocks=shared_blocks)
         check(self.lib.rg_paged_attention_shared_prefix(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
-            context_lens.data_ptr(), output.data_ptr(), scale, num_heads, num_kv_heads, head_dim, block_size,
-            max_blocks_per_seq, batch_size, shared_blocks, dtype_code(query), key_cache.stride(0),
+            context_lens.data_ptr(), output.data_ptr(), float(scale), num_heads, num_kv_heads, head_dim,
+            block_size, max_blocks_per_seq, batch_size, shared_blocks, dtype_code(query), key_cache.stride(0),
             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(query)))
 
     def v1_scores_workspace_bytes(self, batch_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -324,7 +324,7 @@ class PagedAttentionKernels:
         check(self.lib.rg_paged_attention_v1_scores(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
             context_lens.data_ptr(), output.data_ptr(), scores.data_ptr(), _ptr(scored_lens), first_scored,
-            scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size,
+            float(scale), num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, batch_size,
             dtype_code(query), key_cache.stride(0), scores.stride(0), workspace.data_ptr(),
             workspace.numel() * workspace.element_size(), _stream(query)))
 

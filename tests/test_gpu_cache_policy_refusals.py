@@ -1,6 +1,7 @@
-"""Calls of the shared-prefix, scoring and eviction bindings that are refused before anything is launched."""
+"""Calls of the shared-prefix, scoring and eviction bindings that are refused before anything is launched, or taken."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -8,11 +9,13 @@ from railgun_amd.ops import PagedAttentionOp, RailgunError
 
 pytestmark = pytest.mark.gpu
 
+BS = 16
+
 
 class Call:
     """Two sequences over a pool of 12 blocks."""
 
-    def __init__(self, device, heads=8, hkv=2, d=64, bs=16):
+    def __init__(self, device, heads=8, hkv=2, d=64, bs=BS):
         self.pool = torch.zeros((12, 2, hkv, bs, d), dtype=torch.bfloat16, device=device)
         self.kc, self.vc = self.pool[:, 0], self.pool[:, 1]
         self.scores = torch.zeros((12, hkv, bs), device=device)
@@ -51,3 +54,17 @@ def test_one_block_expanded(device, kernels):
                  lambda: kernels.launch_evict(k, v, c.scores, c.table, None, c.lens, None, None, 32, 4)):
         with pytest.raises(RailgunError, match="apart"):
             call()
+
+
+@pytest.mark.parametrize("scale", [np.float32(0.125), torch.tensor(0.125), 0.125])
+def test_scales_that_are_no_python_floats(device, kernels, scale):
+    """Taken, as launch_v1 takes them."""
+    c = Call(device)
+    c.q.normal_()
+    c.pool.normal_()
+    outs = [torch.empty_like(c.q) for _ in range(4)]
+    for out, x in zip(outs, (scale, 0.125)):
+        kernels.launch_shared_prefix(c.q, c.kc, c.vc, c.table, c.lens, out, x, *c.shape, 1, c.ws)
+    for out, x in zip(outs[2:], (scale, 0.125)):
+        kernels.launch_v1_scores(c.q, c.kc, c.vc, c.table, c.lens, out, c.scores, None, BS, x, *c.shape, c.ws)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[2], outs[3])
