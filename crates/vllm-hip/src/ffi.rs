@@ -121,6 +121,51 @@ extern "C" {
         score_layer_stride: i64, score_block_stride: i64, workspace: *mut c_void, workspace_bytes: usize,
         stream: *mut c_void,
     ) -> c_int;
+    /// New: ancestors, positions and slots of the nodes of trees of drafted tokens.
+    pub fn rg_tree_layout(
+        parents: *const i32, cu_nodes: *const i32, context_lens: *const i32, block_table: *const i32,
+        text_positions: *const i32, tree_mask: *mut i32, positions: *mut i32, slot_mapping: *mut i32,
+        block_size: i32, max_blocks_per_seq: i32, num_seqs: i32, num_nodes: i32, max_nodes: i32, mask_words:
+        i32, stream: *mut c_void,
+    ) -> c_int;
+    /// New: workspace bytes of rg_paged_attention_tree.
+    pub fn rg_paged_attention_tree_workspace_bytes(
+        num_seqs: i32, max_nodes: i32, num_heads: i32, num_kv_heads: i32, head_dim: i32, block_size: i32,
+        max_blocks_per_seq: i32,
+    ) -> usize;
+    /// New: attention of trees of drafted tokens over the paged cache.
+    pub fn rg_paged_attention_tree(
+        query: *const c_void, key_cache: *const c_void, value_cache: *const c_void, block_table: *const i32,
+        context_lens: *const i32, cu_nodes: *const i32, tree_mask: *const i32, output: *mut c_void, scale: f32,
+        num_heads: i32, num_kv_heads: i32, head_dim: i32, block_size: i32, max_blocks_per_seq: i32, num_seqs:
+        i32, num_nodes: i32, max_nodes: i32, mask_words: i32, dtype: i32, kv_block_stride: i64, workspace: *mut
+        c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> c_int;
+    /// New: workspace bytes of rg_verify_tree.
+    pub fn rg_verify_tree_workspace_bytes(
+        num_nodes: i32, vocab_size: i32,
+    ) -> usize;
+    /// New: the path of each tree that the model's logits agree with.
+    pub fn rg_verify_tree(
+        logits: *const c_void, draft_tokens: *const i32, parents: *const i32, cu_nodes: *const i32,
+        target_tokens: *mut i32, accepted: *mut i32, num_accepted: *mut i32, next_tokens: *mut i32, num_seqs:
+        i32, num_nodes: i32, max_nodes: i32, max_accepted: i32, vocab_size: i32, dtype: i32, logits_row_stride:
+        i64, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> c_int;
+    /// New: rg_verify_tree for target tokens that the caller has.
+    pub fn rg_accept_tree(
+        target_tokens: *const i32, draft_tokens: *const i32, parents: *const i32, cu_nodes: *const i32,
+        accepted: *mut i32, num_accepted: *mut i32, next_tokens: *mut i32, num_seqs: i32, num_nodes: i32,
+        max_nodes: i32, max_accepted: i32, stream: *mut c_void,
+    ) -> c_int;
+    /// New: keeps the accepted nodes' cached tokens, behind those before the tree.
+    pub fn rg_compact_tree(
+        key_cache: *mut c_void, value_cache: *mut c_void, scores: *mut f32, block_table: *const i32,
+        context_lens: *const i32, cu_nodes: *const i32, accepted: *const i32, num_accepted: *const i32,
+        new_context_lens: *mut i32, max_accepted: i32, num_layers: i32, num_kv_heads: i32, head_dim: i32,
+        block_size: i32, max_blocks_per_seq: i32, num_seqs: i32, num_nodes: i32, dtype: i32, layer_stride: i64,
+        kv_block_stride: i64, score_layer_stride: i64, score_block_stride: i64, stream: *mut c_void,
+    ) -> c_int;
     /// Residual add + RMSNorm around each sublayer (architecture.rs:38-59).
     pub fn rg_rms_norm(
         x: *const c_void, residual: *mut c_void, weight: *const c_void, out: *mut c_void, eps: f32,

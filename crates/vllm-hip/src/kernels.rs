@@ -676,6 +676,174 @@ impl PagedAttentionKernels {
             score_block_stride, workspace.as_mut_ptr(), workspace.len(), self.stream))
     }
 
+    /// Steps over drafted tokens: ancestors (`tree_mask`, `mask_words` per node), positions and slots of
+    /// the trees' nodes, from their parents (`text_positions` None: the root stands behind the cached tokens).
+    pub unsafe fn launch_tree_layout(
+        &self,
+        parents: &HipSlice<i32>,
+        cu_nodes: &HipSlice<i32>,
+        context_lens: &HipSlice<i32>,
+        block_table: &HipSlice<i32>,
+        text_positions: Option<&HipSlice<i32>>,
+        tree_mask: &mut HipSlice<i32>,
+        positions: &mut HipSlice<i32>,
+        slot_mapping: &mut HipSlice<i32>,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        num_seqs: i32,
+        num_nodes: i32,
+        max_nodes: i32,
+        mask_words: i32,
+    ) -> CoreResult<()> {
+        let text = text_positions.map_or(std::ptr::null(), |t| t.as_ptr() as *const i32);
+        status(ffi::rg_tree_layout(
+            parents.as_ptr() as *const i32, cu_nodes.as_ptr() as *const i32, context_lens.as_ptr() as *const i32,
+            block_table.as_ptr() as *const i32, text, tree_mask.as_mut_ptr() as *mut i32,
+            positions.as_mut_ptr() as *mut i32, slot_mapping.as_mut_ptr() as *mut i32, block_size,
+            max_blocks_per_seq, num_seqs, num_nodes, max_nodes, mask_words, self.stream))
+    }
+
+    /// Workspace bytes of `launch_tree`.
+    pub fn tree_workspace_bytes(
+        &self,
+        num_seqs: i32,
+        max_nodes: i32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+    ) -> usize {
+        // SAFETY: pure size query.
+        unsafe {
+            ffi::rg_paged_attention_tree_workspace_bytes(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim,
+                                                         block_size, max_blocks_per_seq)
+        }
+    }
+
+    /// Attention of the nodes of trees of drafted tokens over the paged cache: all that lies before a
+    /// node's tree, and within it what its row of `tree_mask` says.
+    pub unsafe fn launch_tree<T: KvElement>(
+        &self,
+        query: &HipSlice<T>,
+        key_cache: &HipSlice<T>,
+        value_cache: &HipSlice<T>,
+        block_table: &HipSlice<i32>,
+        context_lens: &HipSlice<i32>,
+        cu_nodes: &HipSlice<i32>,
+        tree_mask: &HipSlice<i32>,
+        output: &mut HipSlice<T>,
+        scale: f32,
+        num_heads: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        num_seqs: i32,
+        num_nodes: i32,
+        max_nodes: i32,
+        mask_words: i32,
+        workspace: &mut HipSlice<u8>,
+    ) -> CoreResult<()> {
+        status(ffi::rg_paged_attention_tree(
+            query.as_ptr(), key_cache.as_ptr(), value_cache.as_ptr(), block_table.as_ptr() as *const i32,
+            context_lens.as_ptr() as *const i32, cu_nodes.as_ptr() as *const i32, tree_mask.as_ptr() as *const i32,
+            output.as_mut_ptr(), scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_seqs,
+            num_nodes, max_nodes, mask_words, T::DTYPE, self.kv_block_stride, workspace.as_mut_ptr(),
+            workspace.len(), self.stream))
+    }
+
+    /// Workspace bytes of `launch_verify_tree`.
+    pub fn verify_tree_workspace_bytes(&self, num_nodes: i32, vocab_size: i32) -> usize {
+        // SAFETY: pure size query.
+        unsafe { ffi::rg_verify_tree_workspace_bytes(num_nodes, vocab_size) }
+    }
+
+    /// The path of each tree that the model agrees with: `target_tokens` gets the argmax of every
+    /// node's logits, `accepted` the path's nodes (-1 behind them), `next_tokens` the token behind it.
+    pub unsafe fn launch_verify_tree<T: KvElement>(
+        &self,
+        logits: &HipSlice<T>,
+        draft_tokens: &HipSlice<i32>,
+        parents: &HipSlice<i32>,
+        cu_nodes: &HipSlice<i32>,
+        target_tokens: &mut HipSlice<i32>,
+        accepted: &mut HipSlice<i32>,
+        num_accepted: &mut HipSlice<i32>,
+        next_tokens: &mut HipSlice<i32>,
+        num_seqs: i32,
+        num_nodes: i32,
+        max_nodes: i32,
+        max_accepted: i32,
+        vocab_size: i32,
+        logits_row_stride: i64,
+        workspace: &mut HipSlice<u8>,
+    ) -> CoreResult<()> {
+        status(ffi::rg_verify_tree(
+            logits.as_ptr(), draft_tokens.as_ptr() as *const i32, parents.as_ptr() as *const i32,
+            cu_nodes.as_ptr() as *const i32, target_tokens.as_mut_ptr() as *mut i32,
+            accepted.as_mut_ptr() as *mut i32, num_accepted.as_mut_ptr() as *mut i32,
+            next_tokens.as_mut_ptr() as *mut i32, num_seqs, num_nodes, max_nodes, max_accepted, vocab_size, T::DTYPE,
+            logits_row_stride, workspace.as_mut_ptr(), workspace.len(), self.stream))
+    }
+
+    /// `launch_verify_tree` for target tokens that a sampler drew.
+    pub unsafe fn launch_accept_tree(
+        &self,
+        target_tokens: &HipSlice<i32>,
+        draft_tokens: &HipSlice<i32>,
+        parents: &HipSlice<i32>,
+        cu_nodes: &HipSlice<i32>,
+        accepted: &mut HipSlice<i32>,
+        num_accepted: &mut HipSlice<i32>,
+        next_tokens: &mut HipSlice<i32>,
+        num_seqs: i32,
+        num_nodes: i32,
+        max_nodes: i32,
+        max_accepted: i32,
+    ) -> CoreResult<()> {
+        status(ffi::rg_accept_tree(
+            target_tokens.as_ptr() as *const i32, draft_tokens.as_ptr() as *const i32,
+            parents.as_ptr() as *const i32, cu_nodes.as_ptr() as *const i32, accepted.as_mut_ptr() as *mut i32,
+            num_accepted.as_mut_ptr() as *mut i32, next_tokens.as_mut_ptr() as *mut i32, num_seqs, num_nodes,
+            max_nodes, max_accepted, self.stream))
+    }
+
+    /// Keeps the accepted nodes: their K, V and `scores` (None: there are none) move down behind the
+    /// tokens before the tree, in every layer.  The caches and scores point at layer 0; strides in elements.
+    pub unsafe fn launch_compact_tree<T: KvElement>(
+        &self,
+        key_cache: &mut HipSlice<T>,
+        value_cache: &mut HipSlice<T>,
+        scores: Option<&mut HipSlice<f32>>,
+        block_table: &HipSlice<i32>,
+        context_lens: &HipSlice<i32>,
+        cu_nodes: &HipSlice<i32>,
+        accepted: &HipSlice<i32>,
+        num_accepted: &HipSlice<i32>,
+        new_context_lens: Option<&mut HipSlice<i32>>,
+        max_accepted: i32,
+        num_layers: i32,
+        num_kv_heads: i32,
+        head_dim: i32,
+        block_size: i32,
+        max_blocks_per_seq: i32,
+        num_seqs: i32,
+        num_nodes: i32,
+        layer_stride: i64,
+        score_layer_stride: i64,
+        score_block_stride: i64,
+    ) -> CoreResult<()> {
+        let cells = scores.map_or(std::ptr::null_mut(), |t| t.as_mut_ptr() as *mut f32);
+        let lens = new_context_lens.map_or(std::ptr::null_mut(), |t| t.as_mut_ptr() as *mut i32);
+        status(ffi::rg_compact_tree(
+            key_cache.as_mut_ptr(), value_cache.as_mut_ptr(), cells, block_table.as_ptr() as *const i32,
+            context_lens.as_ptr() as *const i32, cu_nodes.as_ptr() as *const i32, accepted.as_ptr() as *const i32,
+            num_accepted.as_ptr() as *const i32, lens, max_accepted, num_layers, num_kv_heads, head_dim, block_size,
+            max_blocks_per_seq, num_seqs, num_nodes, T::DTYPE, layer_stride, self.kv_block_stride,
+            score_layer_stride, score_block_stride, self.stream))
+    }
+
     /// Residual add + RMSNorm over `num_rows` rows (`residual` may be None).
     pub unsafe fn launch_rms_norm<T: KvElement>(
         &self,

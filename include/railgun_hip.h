@@ -210,6 +210,85 @@ int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
                    int64_t score_layer_stride, int64_t score_block_stride,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------- steps over drafted tokens ----- */
+
+/* A step that looks at a tree of drafted tokens per sequence and keeps the path that the model agrees
+ * with.  Sequence s owns nodes [cu_nodes[s], cu_nodes[s + 1]) of the packed arrays, L of them (0: a
+ * row that pads the batch); nodes from cu_nodes[num_seqs] on belong to nobody and are left as they
+ * are.  max_nodes is the largest L, at most 1024.  parents[n] is the index of n's parent in the
+ * sequence's own tree, below n's own; any other value (-1) says that n has none.  Node 0 is the token
+ * decided last.  In the cache a tree lies behind the tokens before it: context_lens[s] counts its
+ * nodes, node j is at position prior + j, prior = max(context_lens[s] - L, 0).  New entries: the
+ * reference decodes one token per sequence and step.
+ *
+ * rg_tree_layout: what the others and the cache write go by, from the parents.
+ *   tree_mask [num_nodes, mask_words]: bit i % 32 of word i / 32 is set where i is the node itself or
+ *     one of its ancestors (mask_words at least max_nodes / 32 rounded up, at most 32; all of a
+ *     node's words are written);
+ *   positions: text_positions[s] (NULL: prior) plus the node's depth, for the rotation;
+ *   slot_mapping: the slot of cache position prior + j, -1 where the context ends before it. */
+int rg_tree_layout(const int32_t* parents, const int32_t* cu_nodes, const int32_t* context_lens,
+                   const int32_t* block_table, const int32_t* text_positions, int32_t* tree_mask,
+                   int32_t* positions, int32_t* slot_mapping, int32_t block_size,
+                   int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_nodes,
+                   int32_t max_nodes, int32_t mask_words, void* stream);
+
+/* Attention of the nodes over the paged cache, their own K and V in it:
+ *   out[n, h] = sum_t softmax_t(scale * q[n, h].K_t) V_t  over the positions t < prior and those
+ *   prior + i < context_lens[s], i < L, whose bit i the node's row of tree_mask has set.
+ * Any mask is taken, a tree's or another's; a node that it leaves nothing (and that has nothing before
+ * it) gets zeros.  What a node does not attend to does not reach it, NaN and infinities included.
+ * query / output [num_nodes, num_heads, head_dim].  Any shape of rg_paged_attention_v1; block sizes of
+ * 16 * 2^j up to 256 and head_dim 64 or 128 run on the matrix cores, in bf16 / f16 with the
+ * probabilities rounded to that type (in f16 times 2^7).  Needs a workspace of
+ * rg_paged_attention_tree_workspace_bytes (16-byte aligned, no clearing) where that is not 0. */
+size_t rg_paged_attention_tree_workspace_bytes(int32_t num_seqs, int32_t max_nodes,
+                                               int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t block_size,
+                                               int32_t max_blocks_per_seq);
+int rg_paged_attention_tree(const void* query, const void* key_cache, const void* value_cache,
+                            const int32_t* block_table, const int32_t* context_lens,
+                            const int32_t* cu_nodes, const int32_t* tree_mask, void* output,
+                            float scale, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                            int32_t block_size, int32_t max_blocks_per_seq, int32_t num_seqs,
+                            int32_t num_nodes, int32_t max_nodes, int32_t mask_words, int32_t dtype,
+                            int64_t kv_block_stride, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* The path that the model agrees with.  target_tokens[n] gets the index of the largest of node n's
+ * logits [num_nodes, vocab_size] (logits_row_stride elements between rows; the lowest index of equal
+ * ones, -0 equals +0, a NaN ranks as -inf).  From node 0 on, the lowest child whose draft_tokens
+ * entry is the target of the last accepted node is accepted, until there is none or max_accepted are:
+ *   accepted [num_seqs, max_accepted]: their indices in the tree, rising, -1 behind them;
+ *   num_accepted [num_seqs]: how many, node 0 among them (0 without nodes);
+ *   next_tokens [num_seqs]: the target of the last one (-1 without nodes), the root of the next tree.
+ * Needs a workspace of rg_verify_tree_workspace_bytes (8-byte aligned, no clearing).
+ * rg_accept_tree: the same for target_tokens that the caller has, from a sampler. */
+size_t rg_verify_tree_workspace_bytes(int32_t num_nodes, int32_t vocab_size);
+int rg_verify_tree(const void* logits, const int32_t* draft_tokens, const int32_t* parents,
+                   const int32_t* cu_nodes, int32_t* target_tokens, int32_t* accepted,
+                   int32_t* num_accepted, int32_t* next_tokens, int32_t num_seqs, int32_t num_nodes,
+                   int32_t max_nodes, int32_t max_accepted, int32_t vocab_size, int32_t dtype,
+                   int64_t logits_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+int rg_accept_tree(const int32_t* target_tokens, const int32_t* draft_tokens, const int32_t* parents,
+                   const int32_t* cu_nodes, int32_t* accepted, int32_t* num_accepted,
+                   int32_t* next_tokens, int32_t num_seqs, int32_t num_nodes, int32_t max_nodes,
+                   int32_t max_accepted, void* stream);
+
+/* Keeps the accepted nodes: in every layer K and V (and with scores, the scores) of position
+ * prior + accepted[s, i] go to prior + i, i < num_accepted[s], and new_context_lens[s] (NULL: not
+ * wanted; apart from context_lens and num_accepted) becomes prior + num_accepted[s].  All other cells
+ * keep what they hold.  accepted rises within a row and lies in [0, L); an entry outside is not
+ * moved.  The blocks from position prior on belong to the sequence alone.  Caches and scores as in
+ * rg_evict_cache, layer l layer_stride (score_layer_stride) elements behind layer 0. */
+int rg_compact_tree(void* key_cache, void* value_cache, float* scores, const int32_t* block_table,
+                    const int32_t* context_lens, const int32_t* cu_nodes, const int32_t* accepted,
+                    const int32_t* num_accepted, int32_t* new_context_lens, int32_t max_accepted,
+                    int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                    int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_nodes, int32_t dtype,
+                    int64_t layer_stride, int64_t kv_block_stride, int64_t score_layer_stride,
+                    int64_t score_block_stride, void* stream);
+
 /* ------------------------------------------------- model element-wise ops -- */
 
 /* Fused residual add + RMSNorm over rows of hidden_size elements:

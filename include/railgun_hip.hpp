@@ -343,6 +343,69 @@ class PagedAttentionKernels {
                          kv_block_stride, score_layer_stride, score_block_stride, workspace, workspace_bytes, stream_),
           "launch_evict");
   }
+  // Steps over drafted tokens (railgun_hip.h): ancestors, positions and slots of the trees' nodes.
+  void launch_tree_layout(const int32_t* parents, const int32_t* cu_nodes, const int32_t* context_lens,
+                          const int32_t* block_table, const int32_t* text_positions, int32_t* tree_mask,
+                          int32_t* positions, int32_t* slot_mapping, int32_t block_size, int32_t max_blocks_per_seq,
+                          int32_t num_seqs, int32_t num_nodes, int32_t max_nodes, int32_t mask_words) const {
+    check(rg_tree_layout(parents, cu_nodes, context_lens, block_table, text_positions, tree_mask, positions,
+                         slot_mapping, block_size, max_blocks_per_seq, num_seqs, num_nodes, max_nodes, mask_words,
+                         stream_),
+          "launch_tree_layout");
+  }
+  size_t tree_workspace_bytes(int32_t num_seqs, int32_t max_nodes, int32_t num_heads, int32_t num_kv_heads,
+                              int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq) const {
+    return rg_paged_attention_tree_workspace_bytes(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size,
+                                                   max_blocks_per_seq);
+  }
+  // Attention of the nodes over the paged cache, under tree_mask within a tree.
+  void launch_tree(const void* query, const void* key_cache, const void* value_cache, const int32_t* block_table,
+                   const int32_t* context_lens, const int32_t* cu_nodes, const int32_t* tree_mask, void* output,
+                   float scale, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                   int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_nodes, int32_t max_nodes,
+                   int32_t mask_words, void* workspace, size_t workspace_bytes, DType dtype = DType::BF16,
+                   int64_t kv_block_stride = 0) const {
+    check(rg_paged_attention_tree(query, key_cache, value_cache, block_table, context_lens, cu_nodes, tree_mask, output,
+                                  scale, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_seqs,
+                                  num_nodes, max_nodes, mask_words, (int32_t)dtype, kv_block_stride, workspace,
+                                  workspace_bytes, stream_),
+          "launch_tree");
+  }
+  size_t verify_tree_workspace_bytes(int32_t num_nodes, int32_t vocab_size) const {
+    return rg_verify_tree_workspace_bytes(num_nodes, vocab_size);
+  }
+  // The path that the model agrees with, from its logits or from tokens that a sampler drew.
+  void launch_verify_tree(const void* logits, const int32_t* draft_tokens, const int32_t* parents,
+                          const int32_t* cu_nodes, int32_t* target_tokens, int32_t* accepted, int32_t* num_accepted,
+                          int32_t* next_tokens, int32_t num_seqs, int32_t num_nodes, int32_t max_nodes,
+                          int32_t max_accepted, int32_t vocab_size, void* workspace, size_t workspace_bytes,
+                          DType dtype = DType::BF16, int64_t logits_row_stride = 0) const {
+    check(rg_verify_tree(logits, draft_tokens, parents, cu_nodes, target_tokens, accepted, num_accepted, next_tokens,
+                         num_seqs, num_nodes, max_nodes, max_accepted, vocab_size, (int32_t)dtype,
+                         logits_row_stride ? logits_row_stride : vocab_size, workspace, workspace_bytes, stream_),
+          "launch_verify_tree");
+  }
+  void launch_accept_tree(const int32_t* target_tokens, const int32_t* draft_tokens, const int32_t* parents,
+                          const int32_t* cu_nodes, int32_t* accepted, int32_t* num_accepted, int32_t* next_tokens,
+                          int32_t num_seqs, int32_t num_nodes, int32_t max_nodes, int32_t max_accepted) const {
+    check(rg_accept_tree(target_tokens, draft_tokens, parents, cu_nodes, accepted, num_accepted, next_tokens, num_seqs,
+                         num_nodes, max_nodes, max_accepted, stream_),
+          "launch_accept_tree");
+  }
+  // Moves the accepted nodes' K, V and scores (nullptr: none) down behind the tokens before the tree.
+  void launch_compact_tree(void* key_cache, void* value_cache, float* scores, const int32_t* block_table,
+                           const int32_t* context_lens, const int32_t* cu_nodes, const int32_t* accepted,
+                           const int32_t* num_accepted, int32_t* new_context_lens, int32_t max_accepted,
+                           int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                           int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_nodes, DType dtype = DType::BF16,
+                           int64_t layer_stride = 0, int64_t kv_block_stride = 0, int64_t score_layer_stride = 0,
+                           int64_t score_block_stride = 0) const {
+    check(rg_compact_tree(key_cache, value_cache, scores, block_table, context_lens, cu_nodes, accepted, num_accepted,
+                          new_context_lens, max_accepted, num_layers, num_kv_heads, head_dim, block_size,
+                          max_blocks_per_seq, num_seqs, num_nodes, (int32_t)dtype, layer_stride, kv_block_stride,
+                          score_layer_stride, score_block_stride, stream_),
+          "launch_compact_tree");
+  }
 
  private:
   int ordinal_;

@@ -76,6 +76,16 @@ SIGNATURES = {
     ),
     "rg_evict_cache_workspace_bytes": (c_size_t, [c_int32] * 4),
     "rg_evict_cache": (c_int, [c_void_p] * 8 + [c_int32] * 11 + [c_int64] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "rg_tree_layout": (c_int, [c_void_p] * 8 + [c_int32] * 6 + [c_void_p]),
+    "rg_paged_attention_tree_workspace_bytes": (c_size_t, [c_int32] * 7),
+    "rg_paged_attention_tree": (
+        c_int,
+        [c_void_p] * 8 + [c_float] + [c_int32] * 10 + [c_int64, c_void_p, c_size_t, c_void_p],
+    ),
+    "rg_verify_tree_workspace_bytes": (c_size_t, [c_int32, c_int32]),
+    "rg_verify_tree": (c_int, [c_void_p] * 8 + [c_int32] * 6 + [c_int64, c_void_p, c_size_t, c_void_p]),
+    "rg_accept_tree": (c_int, [c_void_p] * 7 + [c_int32] * 4 + [c_void_p]),
+    "rg_compact_tree": (c_int, [c_void_p] * 9 + [c_int32] * 9 + [c_int64] * 4 + [c_void_p]),
     "rg_rms_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int32, c_int32, c_int32, c_void_p]),
     "rg_silu_and_mul": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p]),
     "rg_silu_and_mul_interleaved": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p]),

@@ -24,7 +24,7 @@ LIB_OUT = os.path.join(PKG, "librailgun_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_SOURCES = ["rg_status.hip", "cache_ops.hip", "decode.hip", "prefill.hip", "model_ops.hip", "gemm.hip", "validate.hip",
-               "evict.hip", "scores.hip", "shared_prefix.hip"]
+               "evict.hip", "scores.hip", "shared_prefix.hip", "tree.hip", "tree_attention.hip"]
 # -packed-fp32-ops: hipcc must not form v_pk_{add,mul,fma}_f32 on its own.
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++20", f"-I{ROOT}/include",

@@ -62,6 +62,8 @@ int probe_prefill_kernels();
 int probe_evict_kernels();
 int probe_scores_kernels();
 int probe_shared_prefix_kernels();
+int probe_tree_kernels();
+int probe_tree_attention_kernels();
 int setup_no_alloc_scratch();
 }  // namespace rg
 
@@ -96,6 +98,8 @@ extern "C" int rg_init(int device_ordinal) {
   if (st == RG_OK) st = rg::probe_evict_kernels();
   if (st == RG_OK) st = rg::probe_scores_kernels();
   if (st == RG_OK) st = rg::probe_shared_prefix_kernels();
+  if (st == RG_OK) st = rg::probe_tree_kernels();
+  if (st == RG_OK) st = rg::probe_tree_attention_kernels();
   if (st == RG_OK) st = rg::setup_no_alloc_scratch();
   (void)hipSetDevice(cur);
   if (st != RG_OK) return st;

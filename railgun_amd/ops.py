@@ -90,6 +90,38 @@ def _require_scored_lens(scored_lens: Optional[torch.Tensor], batch: int) -> Non
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "scored_lens needs one entry per sequence")
 
 
+def _require_tree_mask(tree_mask: torch.Tensor, nodes: int, max_nodes: int) -> None:
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != nodes or 32 * tree_mask.shape[1] < max_nodes:
+        raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                           f"tree_mask must be [{nodes}, words] with 32 words' bits for {max_nodes} nodes, got "
+                           f"{tuple(tree_mask.shape)}")
+
+
+def _require_rows(block_table: torch.Tensor, context_lens: torch.Tensor, seqs: int) -> None:
+    if block_table.dim() != 2 or block_table.shape[0] != seqs or context_lens.numel() != seqs:
+        raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                           f"block_table must be [{seqs}, max_blocks] and context_lens [{seqs}], got "
+                           f"{tuple(block_table.shape)} and {tuple(context_lens.shape)}")
+
+
+class _on_device:
+    """Makes t's device the current one, if it is not (a launch goes to the current device)."""
+
+    __slots__ = ("wanted", "before")
+
+    def __init__(self, t: torch.Tensor):
+        self.wanted = t.get_device()
+
+    def __enter__(self) -> None:
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.wanted:
+            torch.cuda.set_device(self.wanted)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.wanted:
+            torch.cuda.set_device(self.before)
+
+
 def cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
     """(num_kv_heads, block_size, head_dim, kv_block_stride) of a [NB, H_kv, bs, D] cache view.
 
@@ -547,6 +579,177 @@ class PagedAttentionKernels:
             scores.stride(-3), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
             _stream(key_cache)))
 
+    def launch_tree_layout(self, parents, cu_nodes, context_lens, block_table, tree_mask, positions, slot_mapping,
+                           block_size: int, max_nodes: int, text_positions: Optional[torch.Tensor] = None) -> None:
+        """Ancestor bits, positions and slots of the nodes of trees of drafted tokens (rg_tree_layout).
+
+        ``parents`` [N]: index in the sequence's own tree, -1 without one; ``cu_nodes`` [S + 1]: first node
+        of each sequence; ``context_lens`` [S]: cached tokens, the tree's nodes among them; no tree has more
+        than ``max_nodes`` nodes.  Written: ``tree_mask`` [N, words], ``positions`` [N] (the root's plus the
+        node's depth; the root's is ``text_positions`` [S], or the number of tokens before the tree) and
+        ``slot_mapping`` [N].  All int32."""
+        n, seqs = self._check_tree(max_nodes, cu_nodes, parents, positions, slot_mapping)
+        self._on_one_device(parents, cu_nodes, context_lens, block_table, text_positions, tree_mask, positions,
+                            slot_mapping)
+        _require_i32(parents, context_lens, block_table, tree_mask, positions, slot_mapping)
+        _require_tree_mask(tree_mask, n, max_nodes)
+        _require_rows(block_table, context_lens, seqs)
+        if text_positions is not None:
+            _require_i32(text_positions)
+            if text_positions.numel() != seqs:
+                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "text_positions needs one entry per sequence")
+        _require_int32(block_size=block_size)
+        with _on_device(parents):
+            check(self.lib.rg_tree_layout(
+                parents.data_ptr(), cu_nodes.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
+                _ptr(text_positions), tree_mask.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), block_size,
+                int(block_table.shape[1]), seqs, n, max_nodes, int(tree_mask.shape[1]), _stream(parents)))
+
+    def tree_workspace_bytes(self, num_seqs: int, max_nodes: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                             block_size: int, max_blocks_per_seq: int) -> int:
+        return int(self.lib.rg_paged_attention_tree_workspace_bytes(num_seqs, max_nodes, num_heads, num_kv_heads,
+                                                                    head_dim, block_size, max_blocks_per_seq))
+
+    def launch_tree(self, query, key_cache, value_cache, block_table, context_lens, cu_nodes, tree_mask, output,
+                    scale: float, max_nodes: int, workspace: Optional[torch.Tensor] = None) -> None:
+        """Attention of the nodes of trees of drafted tokens, query / output [N, H, D], over the paged cache
+        that holds their K and V too (rg_paged_attention_tree): a node attends to all positions before its
+        tree and to the nodes that its row of ``tree_mask`` [N, words] has set.  ``workspace``:
+        tree_workspace_bytes, allocated here when omitted."""
+        n, seqs = self._check_tree(max_nodes, cu_nodes)
+        self._on_one_device(query, key_cache, value_cache, block_table, context_lens, cu_nodes, tree_mask, output,
+                            workspace)
+        _require_i32(block_table, context_lens, tree_mask)
+        hkv, bs, d, kv_stride = cache_geometry(key_cache, value_cache)
+        for t in (query, output):
+            if t.dim() != 3 or not t.is_contiguous() or t.shape[2] != d or t.dtype != key_cache.dtype or \
+                    t.shape != query.shape:
+                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                                   f"query and output must be contiguous [nodes, heads, {d}] of {key_cache.dtype}, got "
+                                   f"{tuple(t.shape)} {t.dtype}")
+        n, heads = int(query.shape[0]), int(query.shape[1])
+        _require_tree_mask(tree_mask, n, max_nodes)
+        _require_rows(block_table, context_lens, seqs)
+        mb = int(block_table.shape[1])
+        with _on_device(query):
+            if workspace is None:
+                nbytes = self._ask("rg_paged_attention_tree_workspace_bytes", seqs, max_nodes, heads, hkv, d, bs, mb)
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+            check(self.lib.rg_paged_attention_tree(
+                query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+                context_lens.data_ptr(), cu_nodes.data_ptr(), tree_mask.data_ptr(), output.data_ptr(), float(scale),
+                heads, hkv, d, bs, mb, seqs, n, max_nodes, int(tree_mask.shape[1]), dtype_code(query), kv_stride,
+                _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+                _stream(query)))
+
+    def verify_tree_workspace_bytes(self, num_nodes: int, vocab_size: int) -> int:
+        return int(self.lib.rg_verify_tree_workspace_bytes(num_nodes, vocab_size))
+
+    def launch_verify_tree(self, logits, draft_tokens, parents, cu_nodes, max_nodes: int, target_tokens, accepted,
+                           num_accepted, next_tokens, workspace: Optional[torch.Tensor] = None) -> None:
+        """The path of each tree that the model agrees with (rg_verify_tree): ``target_tokens`` [N] gets the
+        argmax of every node's ``logits`` [N, vocab]; from node 0 on, the lowest child that drafted the
+        target of the last accepted node is accepted.  Written: ``accepted`` [S, most] (indices in the tree,
+        -1 behind them), ``num_accepted`` [S] (node 0 counts) and ``next_tokens`` [S], the last one's target.
+        ``workspace``: verify_tree_workspace_bytes, allocated here when omitted."""
+        n, seqs, most = self._check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted,
+                                           num_accepted, next_tokens)
+        self._on_one_device(draft_tokens, logits, workspace)
+        if logits.dim() != 2 or logits.shape[0] != n or logits.shape[1] < 1 or logits.stride(1) != 1 or \
+                (n > 1 and logits.stride(0) < logits.shape[1]):
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               f"logits must be [{n}, vocab] with unit column stride, got {tuple(logits.shape)}")
+        vocab = int(logits.shape[1])
+        with _on_device(logits):
+            if workspace is None:
+                nbytes = self._ask("rg_verify_tree_workspace_bytes", n, vocab)
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+            check(self.lib.rg_verify_tree(
+                logits.data_ptr(), draft_tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(),
+                target_tokens.data_ptr(), accepted.data_ptr(), num_accepted.data_ptr(), next_tokens.data_ptr(), seqs, n,
+                max_nodes, most, vocab, dtype_code(logits), max(logits.stride(0), vocab), workspace.data_ptr(),
+                workspace.numel() * workspace.element_size(), _stream(logits)))
+
+    def launch_accept_tree(self, target_tokens, draft_tokens, parents, cu_nodes, max_nodes: int, accepted, num_accepted,
+                           next_tokens) -> None:
+        """launch_verify_tree for ``target_tokens`` that a sampler drew (rg_accept_tree)."""
+        n, seqs, most = self._check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted,
+                                           num_accepted, next_tokens)
+        with _on_device(draft_tokens):
+            check(self.lib.rg_accept_tree(
+                target_tokens.data_ptr(), draft_tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(),
+                accepted.data_ptr(), num_accepted.data_ptr(), next_tokens.data_ptr(), seqs, n, max_nodes, most,
+                _stream(draft_tokens)))
+
+    def launch_compact_tree(self, key_cache, value_cache, scores, block_table, context_lens, cu_nodes, accepted,
+                            num_accepted, new_context_lens=None) -> None:
+        """Keeps the accepted nodes of the trees (rg_compact_tree): K, V and ``scores`` (None: there are none)
+        of node ``accepted[s, i]`` move to the i-th place behind the tokens before the tree, in every layer;
+        ``new_context_lens`` [S] (may be None) gets the new lengths.  ``accepted`` rises within a row.
+
+        Caches ``[NB, H_kv, bs, D]`` or ``[layers, NB, H_kv, bs, D]`` with contiguous blocks, scores fp32 of
+        the caches' shape without D."""
+        _, seqs = self._check_tree(0, cu_nodes)
+        self._on_one_device(key_cache, value_cache, scores, block_table, context_lens, cu_nodes, accepted, num_accepted,
+                            new_context_lens)
+        _require_i32(block_table, context_lens, accepted, num_accepted)
+        if key_cache.dim() not in (4, 5) or value_cache.shape != key_cache.shape or \
+                value_cache.dtype != key_cache.dtype or value_cache.stride() != key_cache.stride():
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "caches must be [NB, H_kv, bs, D] or [layers, NB, H_kv, "
+                                                             "bs, D], alike in shape, strides and dtype")
+        layered = key_cache.dim() == 5
+        layers = int(key_cache.shape[0]) if layered else 1
+        hkv, bs, d = (int(x) for x in key_cache.shape[-3:])
+        if key_cache.stride()[-3:] != (bs * d, d, 1):
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "cache blocks must be contiguous [H_kv, bs, D]")
+        _require_blocks_apart(key_cache, -4)
+        if scores is not None:
+            check_scores(scores, key_cache)
+        _require_rows(block_table, context_lens, seqs)
+        if accepted.dim() != 2 or accepted.shape[0] != seqs or num_accepted.numel() != seqs:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               "accepted must be [sequences, most] and num_accepted [sequences]")
+        if new_context_lens is not None:
+            _require_i32(new_context_lens)
+            if new_context_lens.numel() != seqs:
+                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "new_context_lens needs one entry per sequence")
+        with _on_device(key_cache):
+            check(self.lib.rg_compact_tree(
+                key_cache.data_ptr(), value_cache.data_ptr(), _ptr(scores), block_table.data_ptr(),
+                context_lens.data_ptr(), cu_nodes.data_ptr(), accepted.data_ptr(), num_accepted.data_ptr(),
+                _ptr(new_context_lens), int(accepted.shape[1]), layers, hkv, d, bs, int(block_table.shape[1]), seqs,
+                2**31 - 1, dtype_code(key_cache), key_cache.stride(0) if layered else 0, key_cache.stride(-4),
+                0 if scores is None or not layered else scores.stride(0), 0 if scores is None else scores.stride(-3),
+                _stream(key_cache)))
+
+    @staticmethod
+    def _on_one_device(*tensors: Optional[torch.Tensor]) -> None:
+        _require_cuda(*tensors)
+        if len({t.get_device() for t in tensors if t is not None}) > 1:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "tensors must be on one device")
+
+    def _check_tree(self, max_nodes: int, cu_nodes, *per_node) -> tuple:
+        """(nodes, sequences) of one call over trees, as far as its arrays of one entry per node say."""
+        _require_i32(cu_nodes)
+        _require_int32(max_nodes=max_nodes)
+        if cu_nodes.dim() != 1 or cu_nodes.numel() < 1 or len({t.numel() for t in per_node}) > 1:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               "cu_nodes must be [sequences + 1], and arrays of the nodes of one length, got "
+                               f"{tuple(cu_nodes.shape)} and {[tuple(t.shape) for t in per_node]}")
+        return (int(per_node[0].numel()) if per_node else 0), int(cu_nodes.numel()) - 1
+
+    def _check_accept(self, draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted, num_accepted,
+                      next_tokens) -> tuple:
+        """(nodes, sequences, most accepted) of a verification."""
+        n, seqs = self._check_tree(max_nodes, cu_nodes, draft_tokens, parents, target_tokens)
+        self._on_one_device(draft_tokens, parents, cu_nodes, target_tokens, accepted, num_accepted, next_tokens)
+        _require_i32(draft_tokens, parents, target_tokens, accepted, num_accepted, next_tokens)
+        if accepted.dim() != 2 or accepted.shape[0] != seqs or num_accepted.numel() != seqs or \
+                next_tokens.numel() != seqs:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               "accepted must be [sequences, most], num_accepted and next_tokens [sequences]")
+        return n, seqs, int(accepted.shape[1])
+
     def launch_prefill_packed(self, query, key_cache, value_cache, block_table, context_lens, cu_seqlens,
                               output, scale: float, num_heads: int, num_kv_heads: int, head_dim: int,
                               block_size: int, max_blocks_per_seq: int, num_seqs: int, num_tokens: int,
@@ -670,6 +873,24 @@ class PagedAttentionOp:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         k._v1_scores(q, k_cache, v_cache, block_table, context_lens, out, scores, scored_lens, first_scored,
                      self.scale, heads, hkv, d, bs, mb, batch, workspace)
+        return out
+
+    def execute_tree(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                     context_lens: torch.Tensor, cu_nodes: torch.Tensor, tree_mask: torch.Tensor, max_nodes: int,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """execute() for trees of drafted tokens: q [N, H, D] of all nodes -> new output [N, H, D], what belongs
+        to no sequence left unset (launch_tree); the workspace (tree_workspace_bytes) is allocated here when
+        omitted."""
+        if q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or k_cache.dim() != 4 or \
+                tuple(k_cache.shape[1:]) != (self.num_kv_heads, self.block_size, self.head_dim):
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               f"q {tuple(q.shape)} and caches {tuple(k_cache.shape)} do not fit the op's "
+                               f"{self.num_heads} / {self.num_kv_heads} heads of {self.head_dim}, blocks of "
+                               f"{self.block_size}")
+        _require_cuda(q)
+        out = torch.empty_like(q)
+        self.kernels.launch_tree(q, k_cache, v_cache, block_table, context_lens, cu_nodes, tree_mask, out, self.scale,
+                                 max_nodes, workspace)
         return out
 
     def reshape_and_cache(self, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
