@@ -34,7 +34,7 @@ HIPCC_FLAGS = [
 # VGPRs: with the default heuristic they land in AGPRs and are copied to VGPRs around the softmax
 # rescale on every key tile (and in shared_prefix.hip the 80 AGPRs on top of the other half's
 # VGPRs leave room for one workgroup per CU instead of two).
-SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("prefill.hip", "shared_prefix.hip")}
+SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("prefill.hip", "shared_prefix.hip", "tree_attention.hip")}
 CPP_TESTS = ["test_paged_attention_op"]
 
 

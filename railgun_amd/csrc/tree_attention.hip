@@ -3,16 +3,67 @@
 // Node j of sequence s sits in the cache at position prior + j, prior = context_lens[s] - L.  It attends to the
 // positions below prior and to those prior + i whose bit i its mask has set:
 //   out = sum_t p_t V_t,  p = softmax(scale q.K_t) over those t;  zeros where there are none.
-#include <math.h>
-
-#include <algorithm>
-
+//
+// The L G query rows of a sequence that share a kv-head (row r: node r / G, head r % G of the group) stand against the
+// same K and V: an attention product on the matrix cores,
+//   S^T = K Q^T,  running maximum and sum per row,  O^T += V^T P^T,
+// in row tiles of kRows (32 a wave) and key tiles of kTileKeys.  Only the key tiles that reach into the tree are
+// masked.  The (sequence, kv-head, row tile) segments of the batch, end to end, are one line of key tiles, and every
+// workgroup takes an equal piece of it, whatever the lengths.  A segment that lies in one piece is written out at
+// once; of the others the pieces' softmax partials (m, l, unnormalised O) are joined by tree_merge_kernel:
+//   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+//
+// Cells that a row does not attend to must not reach it, and 0 NaN is NaN in a matrix product.  In masked tiles V
+// rows behind the context are cleared in LDS; where a tree's V holds something that is not finite it is cleared too,
+// and added by hand to the rows that attend to it (which it makes that anyway).
+#include "decode_stream.hpp"
 #include "tree.hpp"
 
 namespace rg {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+
+template <typename T> struct mfma32;
+template <> struct mfma32<bf16_t> {
+  __device__ static __forceinline__ f32x16_t run(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+};
+template <> struct mfma32<f16_t> {
+  __device__ static __forceinline__ f32x16_t run(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  }
+};
+// acc + lo + hi of a packed pair.
+template <typename T> __device__ __forceinline__ float pair_sum(uint32_t pair, float acc);
+template <> __device__ __forceinline__ float pair_sum<bf16_t>(uint32_t pair, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), __builtin_bit_cast(bf16x2_t, 0x3F803F80u),
+                                         acc, false);
+}
+template <> __device__ __forceinline__ float pair_sum<f16_t>(uint32_t pair, float acc) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), __builtin_bit_cast(f16x2_t, 0x3C003C00u), acc,
+                                false);
+}
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = 64 * kTreeWaves;
+constexpr int kRows = 32 * kTreeWaves;  // rows of a workgroup's tile, 32 a wave
+constexpr int kTileKeys = 32;
+constexpr float kSlack = 8.f;           // log2 headroom of the lazy maximum: 2^8 a probability at most
+
+// What is subtracted from the scores of a row whose lazy maximum is m (log2 units): in fp16 the probabilities are
+// held times 2^7.  Its normal numbers end at 2^-14, which one token's weight beside those of thousands falls below;
+// times 2^7 they fill the type up to 2^(8 + 7).  Past 2^20 the fp32 scores' own steps grow towards the one factor of
+// two that is left below 2^16; there they are held as they are.
+template <typename T>
+__device__ __forceinline__ float reference(float m) {
+  if constexpr (std::is_same_v<T, f16_t>) return m - (fabsf(m) < 0x1p20f ? 7.f : 0.f);
+  else return m;
+}
 
 struct TreeArgs {
   const void* q;
@@ -26,6 +77,12 @@ struct TreeArgs {
   float scale_log2;
   int32_t num_heads, num_kv_heads, head_dim, block_size, max_blocks, num_seqs, num_nodes, max_nodes, mask_words;
   int64_t kv_stride;
+  // The product's: pieces, their partials, and what the host knows of the line of tiles.
+  float* acc;        // [pieces, kRows, D] unnormalised
+  float* ml;         // [pieces, kRows, 2]: m in log2 units, l
+  int2* segments;    // [num_seqs, row tiles, kv-heads]: first piece's worker, workers
+  uint32_t q_sign;   // bit 0: q is taken (else zeros, a scale of 0), bits 15 and 31: negated (a negative scale)
+  int32_t group, row_tiles, bs_shift, workers, least;  // row_tiles: most of a sequence; least: key tiles to a worker
 };
 
 // Any shape: a wave per (sequence, node, q-head), lane l has dims 4 l .. 4 l + 3, the keys one after the other with
@@ -82,11 +139,811 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs a) {
   }
 }
 
+
+// The arguments, where the kernel has them, read when they are asked for: held in registers from the start, they and
+// the state of the line are more than a wave has scalar ones.
+typedef __attribute__((address_space(4))) TreeArgs Args;
+__device__ __forceinline__ const Args& arguments() {
+  const Args* p = (const Args*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
+// -------------------------------------------------------------- the line ----
+
+// A sequence as the line of tiles has it.
+struct Span {
+  Tree t;
+  int ctx, tiles, row_tiles;
+};
+__device__ __forceinline__ Span span_of(const Args& a, int s) {
+  Span p;
+  p.t = tree_of(a.cu, s, a.num_nodes, a.max_nodes);
+  p.ctx = max(0, min(a.context_lens[s], a.max_blocks * a.block_size));
+  p.row_tiles = (p.t.nodes * a.group + kRows - 1) / kRows;
+  // (A tree whose context is empty has one tile, without keys: its rows are cleared there.)
+  p.tiles = max(1, (p.ctx + kTileKeys - 1) / kTileKeys);
+  return p;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int below = __shfl_up(v, o, 64);
+    if (lane >= o) v += below;
+  }
+  return v;
+}
+
+// The workers' shares of the line: q units each, and one more for the first r.  (plan_tree: a line is counted in
+// 32 bits.)
+struct Line {
+  int q, r;
+  __device__ __forceinline__ Line(int total, int workers) : q(total / workers), r(total - q * workers) {}
+  __device__ __forceinline__ int begin(int w) const { return q * w + min(w, r); }
+  __device__ __forceinline__ int owner(int unit) const {
+    const int longer = r * (q + 1);
+    return unit < longer ? unit / (q + 1) : r + (unit - longer) / q;
+  }
+};
+
+// All sequences, kTreeThreads at a time, scanned by the workgroup.
+struct LineScratch {
+  int32_t wave_sum[kTreeWaves];
+  int32_t total, workers;
+  int32_t seq, seg, tile;  // where the worker's share begins
+};
+__device__ __forceinline__ int units_of(const Args& a, int s) {
+  if (s >= a.num_seqs) return 0;
+  const Span p = span_of(a, s);
+  return p.tiles * p.row_tiles * a.num_kv_heads;
+}
+__device__ __forceinline__ int line_total(const Args& a, LineScratch& sh, int w, int lane) {
+  int sum = 0;
+  for (int s = threadIdx.x; s < a.num_seqs; s += kTreeThreads) sum += units_of(a, s);
+  sum = wave_scan(sum, lane);
+  if (lane == 63) sh.wave_sum[w] = sum;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < kTreeWaves; ++i) total += sh.wave_sum[i];
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(total);
+}
+__device__ __forceinline__ void line_place(const Args& a, LineScratch& sh, int at, int w, int lane) {
+  int before = 0;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += kTreeThreads) {
+    const int s = s0 + threadIdx.x;
+    const int n = units_of(a, s);
+    const int upto = wave_scan(n, lane);
+    if (lane == 63) sh.wave_sum[w] = upto;
+    __syncthreads();
+    int start = before + upto - n;
+#pragma unroll
+    for (int i = 0; i < kTreeWaves; ++i) {
+      start += i < w ? sh.wave_sum[i] : 0;
+      before += sh.wave_sum[i];
+    }
+    if (start <= at && at - start < n) {
+      const int tiles = span_of(a, s).tiles;
+      sh.seq = s;
+      sh.seg = (at - start) / tiles;
+      sh.tile = (at - start) % tiles;
+    }
+    __syncthreads();
+    if (at < before) break;
+  }
+}
+
+// --------------------------------------------------------- the product ------
+
+// One key tile in LDS, two sub-blocks of 16 keys.  K: the 16-byte chunk c of key k of sub-block b at
+// b * KB / 2 + 256 c + 16 k, so that a 1 KB copy reads one sub-block only and the A operand of one MFMA is
+// 256 contiguous bytes per 16 lanes.  V: rows [key][D] with the 16-byte chunks of a row XORed by
+// 2 (key & 3), so that the transposing reads of four rows hit different banks.
+template <int D>
+struct KeyTile {
+  static constexpr int KB = kTileKeys * D * 2;
+  static constexpr int BYTES = 2 * KB;
+  static constexpr int STAGES = 3;
+  static constexpr int VCH = D / 8;          // 16-byte chunks of a V row
+  static constexpr int SUB_COPIES = D / 32;  // 1 KB copies of a sub-block's K, and of its V
+  __device__ static __forceinline__ int vchunk(int key, int c) { return c ^ (2 * (key & 3)); }
+};
+
+// What a piece of a segment is: the rows, the key tiles, where the result goes.
+struct Piece {
+  int seq, kvh, row0, rows;  // the row tile's first row and the rows of the sequence
+  int first, prior, ctx;     // first node; positions
+  int kt0, kt1;
+  int slot;                  // of the partials, -1: the segment is whole
+};
+
+// Tile kt's attended keys for a node, bit k: key k.  All of it lies before the tree (then no row asks), or its bits
+// are shifted out of the node's mask.
+__device__ __forceinline__ uint32_t tile_mask(const Piece& p, int node, int kt) {
+  const Args& a = arguments();
+  const int32_t* bits = a.mask + (int64_t)(p.first + node) * a.mask_words;
+  const int at = kt * kTileKeys - p.prior;  // tree index of key 0
+  uint32_t m;
+  if (at < 0) {
+    m = at > -32 ? ((uint32_t)bits[0] << -at) | ((1u << -at) - 1u) : ~0u;
+  } else {
+    const int w = at >> 5, sh = at & 31;
+    const uint32_t lo = w < a.mask_words ? (uint32_t)bits[w] : 0u;
+    const uint32_t hi = sh != 0 && w + 1 < a.mask_words ? (uint32_t)bits[w + 1] : 0u;
+    m = (uint32_t)(((uint64_t)hi << 32 | lo) >> sh);
+  }
+  const int left = p.ctx - kt * kTileKeys;
+  return left >= 32 ? m : left > 0 ? m & ((1u << left) - 1u) : 0u;
+}
+
+// x where the bit is set, else -inf (by the bit spread over a word: sixteen conditions held as lane masks would take
+// 32 scalar registers).
+__device__ __forceinline__ float if_bit(uint32_t bits, int b, float x) {
+  const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)bits, (uint32_t)b, 1u);
+  return __uint_as_float((__float_as_uint(x) & on) | (0xff800000u & ~on));
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, const f32x16_t (&o)[D / 32], float m,
+                                           float l) {
+  const Args& a = arguments();
+  using S = typename elem<T>::storage;
+  const int in = row - p.row0;
+  if (row >= p.rows) return;
+  if (p.slot >= 0) {
+    const int64_t at = (int64_t)p.slot * kRows + in;
+    float* acc = a.acc + at * D;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(acc + 32 * db + 8 * i + 4 * hh) =
+            make_float4(o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]);
+    if (hh == 0) *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(m, l);
+    return;
+  }
+  const int node = row / a.group, g = row - node * a.group;
+  S* out = static_cast<S*>(a.out) + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D;
+  const float inv = l != 0.f ? 1.f / l : 1.f;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x0 = o[db][4 * i] * inv, x1 = o[db][4 * i + 1] * inv, x2 = o[db][4 * i + 2] * inv,
+                  x3 = o[db][4 * i + 3] * inv;
+      S* to = out + 32 * db + 8 * i + 4 * hh;
+      if constexpr (std::is_same_v<T, f32_t>) *reinterpret_cast<float4*>(to) = make_float4(x0, x1, x2, x3);
+      else *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x0, x1), pack2<T>(x2, x3));
+    }
+}
+
+// Adds to the lane's row what V holds that is not finite, of the keys `sick` that the row attends to (`mine`).  The
+// values come from the cache, 4 dims at a time as the accumulators have them; times any weight they stay what they are.
+template <typename T, int D>
+__device__ __forceinline__ void add_not_finite(const Piece& p, int kt, uint32_t sick, uint32_t mine, int hh,
+                                               f32x16_t (&o)[D / 32]) {
+  const Args& a = arguments();
+  const int32_t* row_table = a.table + (int64_t)p.seq * a.max_blocks;
+  using E = elem<T>;
+  using S = typename E::storage;
+  while (sick != 0) {
+    const int key = __builtin_ctz(sick);
+    sick &= sick - 1;
+    const int at = kt * kTileKeys + key;
+    const S* v = static_cast<const S*>(a.v) + (int64_t)row_table[at / a.block_size] * a.kv_stride +
+                 ((int64_t)p.kvh * a.block_size + at % a.block_size) * D;
+    const bool takes = mine >> key & 1;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = E::to_f32(v[32 * db + 8 * i + 4 * hh + e]);
+          o[db][4 * i + e] += takes && !(fabsf(x) < INFINITY) ? x : 0.f;
+        }
+  }
+}
+
+// Not finite: all exponent bits set, of either half of a packed pair.
+template <typename T> __device__ __forceinline__ bool pair_not_finite(uint32_t w) {
+  constexpr uint32_t e = std::is_same_v<T, bf16_t> ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || (w >> 16 & e) == e;
+}
+template <typename T> __device__ __forceinline__ uint32_t pair_cleared(uint32_t w) {
+  constexpr uint32_t e = std::is_same_v<T, bf16_t> ? 0x7f80u : 0x7c00u;
+  return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
+}
+
+// Lane l of a wave owns query row l % 32 of it; the other half of that row's keys sits in lane l ^ 32.  sick: a word
+// of LDS per stage.
+template <typename T, int D>
+__device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sick, int w, int lane) {
+  const Args& a = arguments();
+  using MF = mfma32<T>;
+  using TL = KeyTile<D>;
+  constexpr int NKC = D / 16, NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF;
+  static_assert(HALF >= 1, "two waves copy a sub-block");
+  const uint16_t* q = static_cast<const uint16_t*>(a.q);
+  const uint16_t* kc = static_cast<const uint16_t*>(a.k);
+  const uint16_t* vc = static_cast<const uint16_t*>(a.v);
+  const int32_t* table = a.table + (int64_t)p.seq * a.max_blocks;
+  const int j = lane & 31, hh = lane >> 5;
+  const int row = p.row0 + w * 32 + j;
+  const bool busy = p.row0 + w * 32 < p.rows;  // (a wave without rows copies and waits with the others)
+  const int node = min(row, p.rows - 1) / a.group, g = min(row, p.rows - 1) - node * a.group;
+  const int subs = (p.ctx + kBS - 1) / kBS;
+
+  // This wave copies half of sub-block cb of every tile.  Lane l of the window holds the entry of tile
+  // wb + l: (physical block << bs_shift) | sub-block within it; past the end the last sub-block's.
+  const int cb = w >> 1, cp = w & 1;
+  int wb = p.kt0, win;
+  auto fill = [&]() {
+    const int sb = min(2 * (wb + lane) + cb, subs - 1);
+    win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
+  };
+  fill();
+  uint4 qb[NKC];
+  {
+    const uint4* qr = reinterpret_cast<const uint4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D);
+#pragma unroll
+    for (int i = 0; i < NKC; ++i) qb[i] = qr[2 * i + hh];
+    // scale_log2 > 0 here: the host passes its magnitude (1 for a scale of 0) and what becomes of q.
+    const uint32_t flip = a.q_sign & 0x80008000u, on = a.q_sign & 1 ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int i = 0; i < NKC; ++i)
+      qb[i] = make_uint4((qb[i].x ^ flip) & on, (qb[i].y ^ flip) & on, (qb[i].z ^ flip) & on, (qb[i].w ^ flip) & on);
+  }
+  // K: copy n of the sub-block takes its chunks 4 n .. 4 n + 3, V: 1024 / (2 D) of its rows; from copy to copy a
+  // lane's place moves by the same bytes.
+  const uint32_t k_off = (uint32_t)(2 * ((lane & 15) * D + 8 * (4 * cp * HALF + (lane >> 4))));
+  constexpr int VROWS = 1024 / (2 * D);
+  static_assert(VROWS % 4 == 0, "copies of V that swizzle alike");
+  const int v_key = cp * HALF * VROWS + lane / TL::VCH;
+  const uint32_t v_off = (uint32_t)(2 * (v_key * D + 8 * TL::vchunk(v_key, lane % TL::VCH)));
+  const uint32_t lds_base = (uint32_t)(uintptr_t)((RG_LDS char*)lds);
+  const int64_t head = (int64_t)p.kvh * (kBS << a.bs_shift) * D;
+  auto issue = [&](int kt, int st) {
+    const int e = __builtin_amdgcn_readlane(win, kt - wb);
+    const int64_t off = (int64_t)(e >> a.bs_shift) * a.kv_stride + head + (int64_t)(e & ((1 << a.bs_shift) - 1)) * (kBS * D);
+    const char* kb = reinterpret_cast<const char*>(kc + off);
+    const char* vb = reinterpret_cast<const char*>(vc + off);
+    const uint32_t at = lds_base + st * TL::BYTES + cb * (TL::KB / 2) + cp * HALF * 1024;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) lds_dma16_s(kb + 64 * i, k_off, at + i * 1024);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) lds_dma16_s(vb + 1024 * i, v_off, at + TL::KB + i * 1024);
+  };
+
+  f32x16_t o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  float ref = -INFINITY;    // reference(m_run)
+  float m_thr = -INFINITY;  // m_run + kSlack in raw score units, so a tile's test needs no multiply
+  const int xor32 = (lane ^ 32) << 2;
+  const int k_lane = (j >> 4) * (TL::KB / 2) + hh * 256 + (j & 15) * 16;
+  const int grp = lane >> 4, e_row = (lane >> 2) & 3, qq = lane & 3;
+
+  // A operand m = n NDB + db of the PV product (keys 16 n .., 32-dim block db) by the transposing LDS read: in
+  // each 16-lane group, lane 4 e + p points at V[key0 + e][d0 + 4 p ..] and lane i receives V[key0 ..][d0 + i].
+  auto v_operand = [&](const char* vbase, int m) {
+    const int n = m / NDB, db = m % NDB;
+    const int d = 32 * db + 16 * (grp & 1) + 4 * qq;
+    uint2 part[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = 16 * n + 8 * half + 4 * (grp >> 1) + e_row;
+      const int off = key * (D * 2) + TL::vchunk(key, d >> 3) * 16 + (d & 7) * 2;
+      part[half] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((RG_LDS v4i16_t*)(vbase + off)));
+    }
+    return make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+  };
+  constexpr int KA = NKC < 4 ? NKC : 4;          // K operands read ahead of their MFMA
+  constexpr int VA = 2 * NDB < 3 ? 2 * NDB : 3;  // V operands, the first of them before the softmax
+  // S^T of a tile in LDS: c[v] is key 8 (v >> 2) + 4 hh + (v & 3) of it for query j.
+  auto scores = [&](const char* tile) __attribute__((always_inline)) -> f32x16_t {
+    const char* kbase = tile + k_lane;
+    uint4 ka[KA];
+#pragma unroll
+    for (int i = 0; i < KA; ++i) ka[i] = *reinterpret_cast<const uint4*>(kbase + i * 512);
+    f32x16_t c;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NKC; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      c = MF::run(ka[i % KA], qb[i], c);
+      if (i + KA < NKC) ka[i % KA] = *reinterpret_cast<const uint4*>(kbase + (i + KA) * 512);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    return c;
+  };
+  auto finish = [&](f32x16_t c, const char* tile) __attribute__((always_inline)) {
+    const char* vbase = tile + TL::KB;
+    uint4 va[VA];
+#pragma unroll
+    for (int m = 0; m < VA; ++m) va[m] = v_operand(vbase, m);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    // The maximum moves only when a tile exceeds it by more than kSlack, for both halves of a row alike.
+    float tmax = c[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, c[v]);
+    if (__ballot(tmax > m_thr)) {
+      const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)));
+      const float both = fmaxf(tmax, other) * a.scale_log2;
+      const bool moves = both > m_run + kSlack;
+      const float m_new = moves ? both : m_run;
+      const float ref_new = reference<T>(m_new);
+      const float alpha = moves ? fast_exp2(ref - ref_new) : 1.f;
+      m_run = m_new;
+      ref = ref_new;
+      m_thr = (m_run + kSlack) / a.scale_log2;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+    }
+    // (A row that has seen no key yet: its scores are -inf, and so are its probabilities' logarithms.)
+    const float sub = ref == -INFINITY ? 0.f : ref;
+    // Probabilities, rounded to the operand type of the PV product; the sum takes the rounded ones, so
+    // the normaliser weighs what enters the product.
+    uint32_t pk[8];
+#pragma unroll
+    for (int v = 0; v < 16; v += 2)
+      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, -sub)), fast_exp2(fmaf(c[v + 1], a.scale_log2, -sub)));
+    float s0 = pair_sum<T>(pk[0], l_run), s1 = pair_sum<T>(pk[1], 0.f);
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) {
+      s0 = pair_sum<T>(pk[i], s0);
+      s1 = pair_sum<T>(pk[i + 1], s1);
+    }
+    l_run = s0 + s1;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int m = 0; m < 2 * NDB; ++m) {
+      const int n = m / NDB, db = m % NDB;
+      __builtin_amdgcn_sched_barrier(0);
+      o[db] = MF::run(va[m % VA], make_uint4(pk[4 * n], pk[4 * n + 1], pk[4 * n + 2], pk[4 * n + 3]), o[db]);
+      if (m + VA < 2 * NDB) va[m % VA] = v_operand(vbase, m + VA);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  // Tile kt reaches into the tree: V rows behind the context and what is not finite are cleared, by the workgroup.
+  auto clean = [&](int kt, int st) {
+    char* vbase = lds + st * TL::BYTES + TL::KB;
+    for (int i = threadIdx.x; i < kTileKeys * TL::VCH; i += kTreeThreads) {
+      const int key = i / TL::VCH;
+      uint4* at = reinterpret_cast<uint4*>(vbase + i * 16);
+      uint4 x = *at;
+      if (kt * kTileKeys + key >= p.ctx) {
+        *at = make_uint4(0u, 0u, 0u, 0u);
+      } else if (pair_not_finite<T>(x.x) || pair_not_finite<T>(x.y) || pair_not_finite<T>(x.z) || pair_not_finite<T>(x.w)) {
+        *at = make_uint4(pair_cleared<T>(x.x), pair_cleared<T>(x.y), pair_cleared<T>(x.z), pair_cleared<T>(x.w));
+        atomicOr(&sick[st], 1u << key);
+      }
+    }
+    __syncthreads();
+  };
+
+  // The window and Q have landed (the builtin, which the compiler's own counting follows: behind an asm
+  // wait it would wait for Q again in every tile, and with it for every copy in flight).
+  __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0)
+#pragma unroll
+  for (int i = 0; i < TL::STAGES - 1; ++i)
+    if (p.kt0 + i < p.kt1) issue(p.kt0 + i, i);
+  static_assert(TL::STAGES == 3 && COPIES < 16, "one tile newer than the awaited one; low bits of vmcnt");
+  int st = 0;
+#pragma clang loop unroll(disable)
+  for (int kt = p.kt0; kt < p.kt1; ++kt) {
+    // Tile kt has landed (a newer one may not have), for every wave; all are done with tile kt - 1, whose
+    // stage takes tile kt + STAGES - 1.
+    asm volatile("" ::: "memory");
+    if (kt + 1 < p.kt1) __builtin_amdgcn_s_waitcnt(COPIES | 0x70 | 0xF00);
+    else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+    tile_barrier();
+    const int next = kt + TL::STAGES - 1, next_st = st == 0 ? TL::STAGES - 1 : st - 1;
+    if (next - wb >= 64) {
+      wb = next;
+      fill();
+      __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+    }
+    const bool masked = (kt + 1) * kTileKeys > p.prior;
+    if (masked) {
+      // (The word is this tile's: the last use of the stage ended before the barrier above.)
+      if (threadIdx.x == 0) sick[st] = 0;
+      __syncthreads();
+      clean(kt, st);
+    }
+    const char* tile = lds + st * TL::BYTES;
+    if (busy) {
+      __builtin_amdgcn_s_setprio(1);
+      f32x16_t c = scores(tile);
+      if (next < p.kt1) issue(next, next_st);  // while the QK MFMAs run
+      uint32_t mine = 0;
+      if (masked) {
+        mine = tile_mask(p, node, kt);
+        const uint32_t shifted = mine >> (4 * hh);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) c[v] = if_bit(shifted, 8 * (v >> 2) + (v & 3), c[v]);
+      }
+      finish(c, tile);
+      if (masked && sick[st] != 0) add_not_finite<T, D>(p, kt, sick[st], mine, hh, o);
+    } else if (next < p.kt1) {
+      issue(next, next_st);
+    }
+    st = st == TL::STAGES - 1 ? 0 : st + 1;
+  }
+  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  if (busy) store_rows<T, D>(p, row, hh, o, ref, l);
+}
+
+
+// The fp32 product, on v_mfma_f32_32x32x2: step m of S^T = K Q^T takes the k-slot of lane half hh from dim
+// hh D/2 + m, so a lane reads its K row in 16-byte pieces; step v of O^T += V^T P^T takes the keys
+// 8 (v >> 2) + 4 hh + (v & 3), which is where S^T leaves them, so the probabilities stay in fp32 and in their
+// registers.  A key tile is twice as long as in 16 bits and its product 16 times, so one tile in flight ahead of the
+// one at hand is enough: two stages.
+// K in LDS: rows [key][D], the 16-byte chunk c of a row at c ^ (key & 7) (rows of 256 or 512 bytes would put all
+// keys of a read on the same banks); V: rows [key][D] as they are (a read takes 32 neighbours of one row).
+template <int D>
+struct KeyTileF32 {
+  static constexpr int KB = kTileKeys * D * 4;
+  static constexpr int BYTES = 2 * KB;
+  static constexpr int STAGES = 2;
+  static constexpr int CH = D / 4;           // 16-byte chunks of a row
+  static constexpr int SUB_COPIES = D / 16;  // 1 KB copies of a sub-block's K, and of its V
+};
+
+template <int D>
+__device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t* sick, int w, int lane) {
+  const Args& a = arguments();
+  using TL = KeyTileF32<D>;
+  constexpr int NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF, HD = D / 2;
+  const float* q = static_cast<const float*>(a.q);
+  const float* kc = static_cast<const float*>(a.k);
+  const float* vc = static_cast<const float*>(a.v);
+  const int32_t* table = a.table + (int64_t)p.seq * a.max_blocks;
+  const int j = lane & 31, hh = lane >> 5;
+  const int row = p.row0 + w * 32 + j;
+  const bool busy = p.row0 + w * 32 < p.rows;
+  const int node = min(row, p.rows - 1) / a.group, g = min(row, p.rows - 1) - node * a.group;
+  const int subs = (p.ctx + kBS - 1) / kBS;
+  const int cb = w >> 1, cp = w & 1;
+  int wb = p.kt0, win;
+  auto fill = [&]() {
+    const int sb = min(2 * (wb + lane) + cb, subs - 1);
+    win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
+  };
+  fill();
+  float qf[HD];
+  {
+    const float4* qr = reinterpret_cast<const float4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D + hh * HD);
+    const float on = a.q_sign == 0 ? 0.f : a.q_sign & 0x8000u ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) {
+      const float4 x = qr[i];
+      qf[4 * i] = on != 0.f ? x.x * on : 0.f;
+      qf[4 * i + 1] = on != 0.f ? x.y * on : 0.f;
+      qf[4 * i + 2] = on != 0.f ? x.z * on : 0.f;
+      qf[4 * i + 3] = on != 0.f ? x.w * on : 0.f;
+    }
+  }
+  // Copy n of a sub-block's K or V (1 KB): chunk positions 64 n + lane of its rows.
+  uint32_t k_off[HALF], v_off[HALF];  // bytes within the sub-block
+#pragma unroll
+  for (int i = 0; i < HALF; ++i) {
+    const int at = (cp * HALF + i) * 64 + lane, key = at / TL::CH, c = at % TL::CH;
+    k_off[i] = (uint32_t)(key * D * 4 + 16 * (c ^ (key & 7)));
+    v_off[i] = (uint32_t)(at * 16);
+  }
+  const uint32_t lds_base = (uint32_t)(uintptr_t)((RG_LDS char*)lds);
+  const int64_t head = (int64_t)p.kvh * (kBS << a.bs_shift) * D;
+  auto issue = [&](int kt, int st) {
+    const int e = __builtin_amdgcn_readlane(win, kt - wb);
+    const int64_t off = (int64_t)(e >> a.bs_shift) * a.kv_stride + head + (int64_t)(e & ((1 << a.bs_shift) - 1)) * (kBS * D);
+    const uint32_t at = lds_base + st * TL::BYTES + cb * (TL::KB / 2) + cp * HALF * 1024;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) lds_dma16_s(reinterpret_cast<const char*>(kc + off), k_off[i], at + i * 1024);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) lds_dma16_s(reinterpret_cast<const char*>(vc + off), v_off[i], at + TL::KB + i * 1024);
+  };
+  f32x16_t o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  const int xor32 = (lane ^ 32) << 2;
+  auto clean = [&](int kt, int st) {
+    char* vbase = lds + st * TL::BYTES + TL::KB;
+    for (int i = threadIdx.x; i < kTileKeys * TL::CH; i += kTreeThreads) {
+      const int key = i / TL::CH;
+      float4* at = reinterpret_cast<float4*>(vbase + i * 16);
+      const float4 x = *at;
+      auto fine = [](float v) { return fabsf(v) < INFINITY; };
+      if (kt * kTileKeys + key >= p.ctx) {
+        *at = make_float4(0.f, 0.f, 0.f, 0.f);
+      } else if (!(fine(x.x) && fine(x.y) && fine(x.z) && fine(x.w))) {
+        *at = make_float4(fine(x.x) ? x.x : 0.f, fine(x.y) ? x.y : 0.f, fine(x.z) ? x.z : 0.f, fine(x.w) ? x.w : 0.f);
+        atomicOr(&sick[st], 1u << key);
+      }
+    }
+    __syncthreads();
+  };
+  auto compute = [&](int kt, int st, bool masked) __attribute__((always_inline)) {
+    const char* krow = lds + st * TL::BYTES + j * (D * 4);
+    f32x16_t c;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) c[v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) {
+      const float4 k4 = *reinterpret_cast<const float4*>(krow + 16 * ((hh * (HD / 4) + i) ^ (j & 7)));
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.x, qf[4 * i], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.y, qf[4 * i + 1], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.z, qf[4 * i + 2], c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.w, qf[4 * i + 3], c, 0, 0, 0);
+    }
+    uint32_t mine = ~0u;
+    if (masked) {
+      mine = tile_mask(p, node, kt);
+      const uint32_t shifted = mine >> (4 * hh);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) c[v] = if_bit(shifted, 8 * (v >> 2) + (v & 3), c[v]);
+    }
+    float tmax = c[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, c[v]);
+    tmax = fmaxf(tmax, __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)))) * a.scale_log2;
+    if (__ballot(tmax > m_run)) {
+      const bool moves = tmax > m_run;
+      const float alpha = moves ? fast_exp2(m_run - tmax) : 1.f;
+      m_run = moves ? tmax : m_run;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+    }
+    const float sub = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      c[v] = fast_exp2(fmaf(c[v], a.scale_log2, -sub));
+      l_run += c[v];
+    }
+    const float* vrow = reinterpret_cast<const float*>(lds + st * TL::BYTES + TL::KB) + 4 * hh * D + j;
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[(8 * (v >> 2) + (v & 3)) * D + 32 * db], c[v], o[db], 0, 0, 0);
+    if (masked && sick[st] != 0) add_not_finite<f32_t, D>(p, kt, sick[st], mine, hh, o);
+  };
+  __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0): the window and Q
+  issue(p.kt0, 0);
+  if (p.kt0 + 1 < p.kt1) issue(p.kt0 + 1, 1);
+  static_assert(COPIES < 16, "low bits of vmcnt");
+#pragma clang loop unroll(disable)
+  for (int kt = p.kt0; kt < p.kt1; ++kt) {
+    const int st = (kt - p.kt0) & 1;
+    asm volatile("" ::: "memory");
+    if (kt + 1 < p.kt1) __builtin_amdgcn_s_waitcnt(COPIES | 0x70 | 0xF00);
+    else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+    tile_barrier();  // tile kt has landed for every wave
+    const bool masked = (kt + 1) * kTileKeys > p.prior;
+    if (masked) {
+      if (threadIdx.x == 0) sick[st] = 0;
+      __syncthreads();
+      clean(kt, st);
+    }
+    if (busy) compute(kt, st, masked);
+    if (kt + 2 < p.kt1) {
+      if (kt + 2 - wb >= 64) {
+        wb = kt + 2;
+        fill();
+        __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+      }
+      tile_barrier();  // every wave is done with the stage
+      issue(kt + 2, st);
+    }
+  }
+  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  if (busy) store_rows<f32_t, D>(p, row, hh, o, m_run, l);
+}
+
+template <typename T, int D>
+constexpr int ring_bytes() {
+  if constexpr (std::is_same_v<T, f32_t>) return KeyTileF32<D>::STAGES * KeyTileF32<D>::BYTES;
+  else return KeyTile<D>::STAGES * KeyTile<D>::BYTES;
+}
+template <typename T, int D>
+constexpr int groups_per_cu() { return std::is_same_v<T, f32_t> ? 2 : D == 128 ? 3 : 4; }
+
+// One worker: its piece of the line, segment by segment.
+template <typename T, int D>
+__global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_kernel(TreeArgs) {
+  __shared__ __attribute__((aligned(16))) char ring[ring_bytes<T, D>()];
+  __shared__ LineScratch scratch;
+  __shared__ uint32_t sick[4];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int s, seg, kt, left;
+  int me;
+  {
+    const Args& a = arguments();
+    const int total = line_total(a, scratch, w, lane);
+    if (total == 0) return;
+    // Shares of `least` key tiles and more.  Neighbours on the line go to the same XCD (workgroups are dealt to the
+    // eight in turn), whose L2 the row tiles of a kv-head share.
+    const int workers = min(a.workers, max(1, total / a.least)), per = (workers + 7) / 8;
+    me = (int)(blockIdx.x % 8) * per + (int)blockIdx.x / 8;
+    if ((int)blockIdx.x / 8 >= per || me >= workers) return;
+    const Line line(total, workers);
+    line_place(a, scratch, line.begin(me), w, lane);
+    if (threadIdx.x == 0) {
+      scratch.total = total;
+      scratch.workers = workers;
+    }
+    left = line.begin(me + 1) - line.begin(me);
+    s = __builtin_amdgcn_readfirstlane(scratch.seq);
+    seg = __builtin_amdgcn_readfirstlane(scratch.seg);
+    kt = __builtin_amdgcn_readfirstlane(scratch.tile);
+  }
+  while (left > 0) {
+    Piece p;
+    {
+      const Args& a = arguments();
+      const Span sp = span_of(a, s);
+      if (seg >= sp.row_tiles * a.num_kv_heads) {  // on to the next sequence that has any
+        ++s;
+        seg = 0;
+        continue;
+      }
+      const int n = min(sp.tiles - kt, left);
+      p.kvh = seg / sp.row_tiles;
+      const int rt = seg - p.kvh * sp.row_tiles;
+      p.seq = s;
+      p.row0 = rt * kRows;
+      p.rows = sp.t.nodes * a.group;
+      p.first = sp.t.first;
+      p.ctx = sp.ctx;
+      p.prior = max(sp.ctx - sp.t.len, 0);
+      p.kt0 = kt;
+      p.kt1 = kt + n;
+      const bool starts = kt == 0, ends = p.kt1 == sp.tiles;
+      p.slot = starts && ends ? -1 : 2 * me + (starts ? 1 : 0);
+      if (starts && threadIdx.x == 0) {
+        int pieces = 1;
+        if (!ends) {
+          const Line line(scratch.total, scratch.workers);
+          pieces = line.owner(line.begin(me + 1) - left + sp.tiles - 1) - me + 1;
+        }
+        a.segments[((int64_t)s * a.row_tiles + rt) * a.num_kv_heads + p.kvh] = make_int2(me, pieces);
+      }
+      left -= n;
+      kt = ends ? 0 : p.kt1;
+      seg += ends;
+    }
+    if (p.ctx == 0) {
+      const int row = p.row0 + w * 32 + (lane & 31);
+      f32x16_t o[D / 32];
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+      store_rows<T, D>(p, row, lane >> 5, o, -INFINITY, 0.f);
+    } else if constexpr (std::is_same_v<T, f32_t>) {
+      product_f32<D>(p, ring, sick, w, lane);
+    } else {
+      product<T, D>(p, ring, sick, w, lane);
+    }
+    __syncthreads();  // the ring is free
+  }
+}
+
+// A wave per row of a segment that lies in several pieces; lane l folds dims [l PER, (l + 1) PER) of them.
+constexpr int kMergeRows = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kMergeRows) void tree_merge_kernel(TreeArgs a) {
+  using S = typename elem<T>::storage;
+  constexpr int PER = D / 64;
+  const int s = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63;
+  const int row = (int)blockIdx.x * kMergeRows + (threadIdx.x >> 6);
+  const int rt = row / kRows, in = row - rt * kRows;
+  const int2 seg = a.segments[((int64_t)s * a.row_tiles + rt) * a.num_kv_heads + kvh];  // (not used where there is none)
+  const Span sp = span_of(arguments(), s);
+  if (row >= sp.t.nodes * a.group || seg.y <= 1) return;
+  struct Part {
+    float2 ml;
+    float v[PER];
+  };
+  auto load = [&](int i) __attribute__((always_inline)) {
+    const int64_t at = ((int64_t)2 * (seg.x + i) + (i == 0 ? 1 : 0)) * kRows + in;
+    Part p;
+    p.ml = *reinterpret_cast<const float2*>(a.ml + 2 * at);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) p.v[e] = a.acc[at * D + lane * PER + e];
+    return p;
+  };
+  float m = -INFINITY, l = 0.f;
+  float acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  auto fold = [&](const Part& p) __attribute__((always_inline)) {
+    // (A piece without keys for the row has m = -inf and nothing to add.)
+    const float mn = fmaxf(m, p.ml.x);
+    const float fo = m == mn ? 1.f : exp2f(m - mn), fq = p.ml.x == -INFINITY ? 0.f : exp2f(p.ml.x - mn);
+    l = l * fo + p.ml.y * fq;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = acc[e] * fo + p.v[e] * fq;
+    m = mn;
+  };
+  constexpr int AHEAD = 4;
+  int i = 0;
+  for (; i + AHEAD <= seg.y; i += AHEAD) {
+    Part part[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) part[u] = load(i + u);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) fold(part[u]);
+  }
+  for (; i < seg.y; ++i) fold(load(i));
+  const int node = row / a.group, g = row - node * a.group;
+  S* out = static_cast<S*>(a.out) + ((int64_t)(sp.t.first + node) * a.num_heads + kvh * a.group + g) * D + lane * PER;
+  const float inv = l != 0.f ? 1.f / l : 1.f;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) out[e] = elem<T>::from_f32(acc[e] * inv);
+}
+
+// ---------------------------------------------------------------- the plan --
+
+constexpr int kWorkersPerCu = 2;
+
+// Key tiles on the line of the longest sequences and largest trees.
+double most_units(int32_t num_seqs, int32_t row_tiles, int32_t Hkv, int32_t bs, int32_t MB) {
+  return (double)num_seqs * Hkv * row_tiles * std::max<int64_t>(1, ceil_div((int64_t)MB * bs, kTileKeys));
+}
+
+struct TreePlan {
+  int32_t row_tiles, workers;
+  size_t ml_at, segments_at, bytes;
+};
+TreePlan plan_tree(int32_t num_seqs, int32_t max_nodes, int32_t H, int32_t Hkv, int32_t D, int32_t bs, int32_t MB) {
+  TreePlan p;
+  p.row_tiles = (int32_t)ceil_div((int64_t)max_nodes * (H / Hkv), kRows);
+  // (What the product does not take runs on the generic kernel.)
+  const double most = most_units(num_seqs, p.row_tiles, Hkv, bs, MB);
+  if ((D != 64 && D != 128) || block_shift(bs) < 0 || most > INT32_MAX) return TreePlan{};
+  p.workers = (int32_t)std::min<double>((double)device_cu_count() * kWorkersPerCu, most);
+  const size_t pieces = 2 * (size_t)p.workers;
+  p.ml_at = align_up(pieces * kRows * D * 4, 256);
+  p.segments_at = p.ml_at + align_up(pieces * kRows * 8, 256);
+  p.bytes = p.segments_at + align_up((size_t)num_seqs * p.row_tiles * Hkv * 8, 256);
+  return p;
+}
+
+template <typename T, int D>
+void launch_product(const TreeArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((tree_kernel<T, D>), dim3((unsigned)ceil_div(a.workers, 8) * 8), dim3(kTreeThreads), 0, s, a);
+  const unsigned rows = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, kMergeRows);
+  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3(rows, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs),
+                     dim3(64 * kMergeRows), 0, s, a);
+}
+
 }  // namespace
 
 int probe_tree_attention_kernels() {
   hipFuncAttributes at;
-  if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_generic_kernel<bf16_t>)) != hipSuccess) {
+  if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_generic_kernel<bf16_t>)) != hipSuccess ||
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_kernel<bf16_t, 128>)) != hipSuccess ||
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_merge_kernel<bf16_t, 128>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the tree attention kernels: %s", hipGetErrorString(hipGetLastError()));
   }
   return RG_OK;
@@ -99,7 +956,12 @@ using namespace rg;
 extern "C" size_t rg_paged_attention_tree_workspace_bytes(int32_t num_seqs, int32_t max_nodes, int32_t num_heads,
                                                           int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                                           int32_t max_blocks_per_seq) {
-  return 0;
+  if (num_seqs <= 0 || max_nodes <= 0 || max_nodes > kMaxTreeNodes || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads != 0 || block_size <= 0 || max_blocks_per_seq < 0 ||
+      (int64_t)max_blocks_per_seq * block_size > INT32_MAX - 65536 || num_seqs > 65535 || num_heads > 65535) {
+    return 0;
+  }
+  return plan_tree(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq).bytes;
 }
 
 extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache, const void* value_cache,
@@ -140,9 +1002,54 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
   if (!query || !key_cache || !value_cache || !block_table || !context_lens || !cu_nodes || !tree_mask || !output) {
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
   }
-  const TreeArgs a{query, key_cache, value_cache, output, block_table, context_lens, cu_nodes, tree_mask,
-                   scale * kLog2e, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_seqs,
-                   num_nodes, max_nodes, mask_words, kv_block_stride ? kv_block_stride : block};
+  const size_t need = rg_paged_attention_tree_workspace_bytes(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim,
+                                                              block_size, max_blocks_per_seq);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) {
+    return fail(RG_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned), %zu required", op,
+                workspace ? workspace_bytes : (size_t)0, need);
+  }
+  TreeArgs a{};
+  a.q = query;
+  a.k = key_cache;
+  a.v = value_cache;
+  a.out = output;
+  a.table = block_table;
+  a.context_lens = context_lens;
+  a.cu = cu_nodes;
+  a.mask = tree_mask;
+  a.scale_log2 = scale * kLog2e;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  a.block_size = block_size;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_seqs = num_seqs;
+  a.num_nodes = num_nodes;
+  a.max_nodes = max_nodes;
+  a.mask_words = mask_words;
+  a.kv_stride = kv_block_stride ? kv_block_stride : block;
+  if (need > 0 && aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(output) &&
+      a.kv_stride * dtype_bytes(dtype) % 16 == 0) {
+    const TreePlan p = plan_tree(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq);
+    char* const ws = static_cast<char*>(workspace);
+    a.acc = reinterpret_cast<float*>(ws);
+    a.ml = reinterpret_cast<float*>(ws + p.ml_at);
+    a.segments = reinterpret_cast<int2*>(ws + p.segments_at);
+    // The product works with a positive scale: a negative one turns q's signs, 0 takes zeros for q.
+    a.q_sign = scale == 0.f ? 0u : scale < 0.f ? 0x80008001u : 1u;
+    a.scale_log2 = scale != 0.f ? fabsf(a.scale_log2) : 1.f;
+    a.group = num_heads / num_kv_heads;
+    a.row_tiles = p.row_tiles;
+    a.bs_shift = block_shift(block_size);
+    a.workers = p.workers;
+    a.least = dtype == RG_DTYPE_F32 ? 1 : 8;
+    return dispatch_dtype(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      if (head_dim == 128) launch_product<T, 128>(a, as_stream(stream));
+      else launch_product<T, 64>(a, as_stream(stream));
+      return check_launch(op);
+    });
+  }
   const dim3 grid((unsigned)max_nodes, (unsigned)num_heads, (unsigned)num_seqs);
   return dispatch_dtype(dtype, [&](auto tag) {
     hipLaunchKernelGGL(tree_generic_kernel<decltype(tag)>, grid, dim3(64), 0, as_stream(stream), a);
