@@ -60,6 +60,27 @@ class DecodeSlot:
     scored_len: Optional[int] = None
 
 
+@dataclass
+class DraftTree:
+    """Drafted tokens of a sequence, checked in one step: ``token_ids[0]`` is the token decided last (not cached
+    yet), the others are drafts; ``parents[i]`` is the index of the token that draft i follows (-1 for the
+    first).  ``seq_len`` counts them all (cached tokens before the tree + tree), as DecodeSlot counts its token,
+    and the block table holds room for them.
+
+    ``position`` is the first token's place in the text (default: the number of tokens before the tree; larger
+    once tokens have been evicted).  The reference decodes one token per step."""
+
+    token_ids: Sequence[int]
+    parents: Sequence[int]
+    seq_len: int
+    block_table: Sequence[int]
+    position: Optional[int] = None
+
+
+# Most tokens of a DraftTree (rg_paged_attention_tree).
+MAX_TREE_NODES = 1024
+
+
 def slot_of(block_table: Sequence[int], pos: int, block_size: int) -> int:
     """scheduler.rs:230-235 / :258-263: block_table[pos / bs] * bs + pos % bs."""
     return int(block_table[pos // block_size]) * block_size + pos % block_size
@@ -70,8 +91,9 @@ class StepBatch:
     """Packed host metadata of one step (int32 numpy arrays, ready to copy to the device).
 
     Rows ``[0, num_prefill_tokens)`` are the prefill tokens of ``num_prefill_seqs``
-    sequences (``cu_seqlens`` over them), rows after that one decode token each.  Request r
-    (prefill chunks first) owns ``block_table[r]`` and ``context_lens[r]``.
+    sequences (``cu_seqlens`` over them), rows after that one decode token each, and behind
+    those the tokens of the draft trees (``tree_cu`` over them).  Request r (prefill chunks
+    first, draft trees last) owns ``block_table[r]`` and ``context_lens[r]``.
     """
 
     tokens: np.ndarray          # int64 [T]
@@ -84,7 +106,8 @@ class StepBatch:
     num_prefill_tokens: int
     max_context_len: int
     max_query_len: int
-    last_rows: np.ndarray = field(default=None)  # int64 [R]: row of each request's last token
+    # int64: rows whose logits are asked for, each request's last token, and every token of a tree
+    last_rows: np.ndarray = field(default=None)
     # Leading block-table entries that all decode rows share (0 unless asked for).
     shared_decode_blocks: int = 0
     # int32 [decode rows]: leading cached tokens that hold a score, for a step that gathers attention weights.
@@ -92,6 +115,12 @@ class StepBatch:
     # int32: slots of the shared prefix that no row's scored_len counts, for such a step.  It does not add
     # to the prefix, so it sets these to 0: a row that later no longer shares them adds to what they hold.
     unscored_slots: Optional[np.ndarray] = None
+    num_trees: int = 0
+    max_tree_nodes: int = 0
+    max_tree_depth: int = 0                     # tokens on the longest path of a tree
+    tree_cu: Optional[np.ndarray] = None        # int32 [num_trees + 1], from the trees' first row on
+    tree_parents: Optional[np.ndarray] = None   # int32 [tokens of the trees]
+    tree_places: Optional[np.ndarray] = None    # int32 [num_trees]: first token's place in the text
 
     @property
     def num_tokens(self) -> int:
@@ -103,7 +132,11 @@ class StepBatch:
 
     @property
     def num_decode(self) -> int:
-        return self.num_requests - self.num_prefill_seqs
+        return self.num_requests - self.num_prefill_seqs - self.num_trees
+
+    @property
+    def first_tree_row(self) -> int:
+        return self.num_prefill_tokens + self.num_decode
 
 
 def _check_ids(table: Sequence[int]) -> None:
@@ -149,8 +182,23 @@ def _unscored_slots(decode_slots: Sequence[DecodeSlot], block_size: int, shared:
     return (blocks[t // block_size] * block_size + t % block_size).astype(np.int32)
 
 
+def _tree_depths(tree: DraftTree) -> list:
+    """The drafts' distances from the first token; every one of them follows an earlier token."""
+    n = len(tree.token_ids)
+    if not 0 < n <= MAX_TREE_NODES or len(tree.parents) != n:
+        raise ValueError(f"draft tree of {n} tokens with {len(tree.parents)} parents (1 to {MAX_TREE_NODES})")
+    depths = [0]
+    for i, p in enumerate(tree.parents):
+        if i == 0 and int(p) != -1 or i > 0 and not 0 <= int(p) < i:
+            raise ValueError(f"token {i} of a draft tree follows token {int(p)}")
+        if i > 0:
+            depths.append(depths[int(p)] + 1)
+    return depths
+
+
 def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[DecodeSlot], block_size: int,
-              max_blocks: Optional[int] = None, share_prefix: bool = False, gather_scores: bool = False) -> StepBatch:
+              max_blocks: Optional[int] = None, share_prefix: bool = False, gather_scores: bool = False,
+              draft_trees: Sequence[DraftTree] = ()) -> StepBatch:
     """engine.rs:184-227 plus positions / cu_seqlens; ``max_blocks`` (default: the longest
     table) fixes the padded row length, e.g. to keep one shape across steps.
 
@@ -159,7 +207,10 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     probabilities to that type.  ``gather_scores`` makes the step add the attention weights of the decode
     rows' cached tokens, behind such a prefix, to the pool's scores; the prefix keeps those it has, and
     blocks that only some of the rows share are refused.  Which rows share a prefix may change from step
-    to step."""
+    to step.
+
+    ``draft_trees``: sequences that check drafted tokens in this step; they neither share a prefix nor
+    gather scores."""
     tokens, positions, slots, ctx, tables = [], [], [], [], []
     cu = [0]
     for c in prefill_chunks:
@@ -193,6 +244,27 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
         slots.append(slot_of(d.block_table, d.seq_len - 1, block_size))
         ctx.append(d.seq_len)
         tables.append(list(d.block_table))
+    tree_cu, parents, places, deepest = [0], [], [], 0
+    for d in draft_trees:
+        depths, n = _tree_depths(d), len(d.token_ids)
+        before = d.seq_len - n
+        if before < 0:
+            raise ValueError(f"draft tree of {n} tokens with seq_len {d.seq_len}")
+        _check_ids(d.block_table)
+        if (d.seq_len + block_size - 1) // block_size > len(d.block_table):
+            raise ValueError(f"draft tree ending at length {d.seq_len} needs more than {len(d.block_table)} blocks")
+        place = before if d.position is None else int(d.position)
+        if place < before:
+            raise ValueError(f"draft tree at position {place} with {before} cached tokens before it")
+        tokens.extend(int(t) for t in d.token_ids)
+        positions.extend(place + depth for depth in depths)
+        slots.extend(slot_of(d.block_table, before + i, block_size) for i in range(n))
+        ctx.append(d.seq_len)
+        tables.append(list(d.block_table))
+        tree_cu.append(tree_cu[-1] + n)
+        parents.extend(int(p) for p in d.parents)
+        places.append(place)
+        deepest = max(deepest, max(depths) + 1)
     widest = max((len(t) for t in tables), default=0)
     mb = widest if max_blocks is None else int(max_blocks)
     if mb < widest:
@@ -203,7 +275,7 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     shared = shared_prefix_blocks(decode_slots, block_size) if share_prefix else 0
     lens = np.diff(np.asarray(cu))
     last = np.concatenate([np.asarray(cu[1:], np.int64) - 1,
-                           cu[-1] + np.arange(len(decode_slots), dtype=np.int64)])
+                           cu[-1] + np.arange(len(decode_slots) + tree_cu[-1], dtype=np.int64)])
     scored = _scored_lens(decode_slots, block_size, shared) if gather_scores else None
     return StepBatch(
         tokens=np.asarray(tokens, np.int64), positions=np.asarray(positions, np.int32),
@@ -211,7 +283,10 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
         cu_seqlens=np.asarray(cu, np.int32), num_prefill_seqs=len(prefill_chunks), num_prefill_tokens=cu[-1],
         max_context_len=max(ctx, default=0), max_query_len=int(lens.max()) if len(lens) else 0, last_rows=last,
         shared_decode_blocks=shared, scored_lens=scored,
-        unscored_slots=_unscored_slots(decode_slots, block_size, shared) if gather_scores else None)
+        unscored_slots=_unscored_slots(decode_slots, block_size, shared) if gather_scores else None,
+        num_trees=len(draft_trees), max_tree_nodes=max((len(d.token_ids) for d in draft_trees), default=0),
+        max_tree_depth=deepest, tree_cu=np.asarray(tree_cu, np.int32), tree_parents=np.asarray(parents, np.int32),
+        tree_places=np.asarray(places, np.int32))
 
 
-__all__ = ["CPU_BLOCK_FLAG", "DecodeSlot", "PrefillChunk", "StepBatch", "pack_step", "shared_prefix_blocks", "slot_of"]
+__all__ = ["CPU_BLOCK_FLAG", "DecodeSlot", "DraftTree", "MAX_TREE_NODES", "PrefillChunk", "StepBatch", "pack_step", "shared_prefix_blocks", "slot_of"]

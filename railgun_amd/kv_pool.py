@@ -13,6 +13,7 @@ no data (crates/vllm-paged-attention/src/allocator.rs:102-153).  Here:
   directly;
 * :attr:`GpuBlockPool.scores` and :meth:`GpuBlockPool.evict` trim sequences to a budget of tokens by
   the attention weight they have gathered (the reference never drops a cached token);
+* :meth:`GpuBlockPool.keep_accepted` keeps what a step's model agreed with of drafted tokens;
 * :meth:`GpuBlockPool.swap_out`, :meth:`GpuBlockPool.swap_in` and
   :meth:`GpuBlockPool.copy_blocks` are the physical copies behind the allocator's swap and
   copy-on-write, each one ``rg_copy_blocks`` launch over all layers, and one for the scores where the
@@ -122,6 +123,17 @@ class GpuBlockPool:
         self.kernels.launch_evict(self.storage[:, :, 0], self.storage[:, :, 1], self.scores, block_table,
                                   dst_block_table, context_lens, new_lens, kept_positions, budget, recent,
                                   protected_len)
+        return new_lens
+
+    def keep_accepted(self, block_table: torch.Tensor, context_lens: torch.Tensor, cu_nodes: torch.Tensor,
+                      accepted: torch.Tensor, num_accepted: torch.Tensor) -> torch.Tensor:
+        """Keeps the accepted nodes of trees of drafted tokens, cached at the ends of the sequences of
+        ``block_table``: they move down directly behind the tokens before their tree, with their scores if the
+        pool has any, every layer in one call (launch_compact_tree); returns the new context lengths, int32 on
+        the device.  The blocks past a sequence's new length hold nothing it needs."""
+        new_lens = torch.empty_like(context_lens)
+        self.kernels.launch_compact_tree(self.storage[:, :, 0], self.storage[:, :, 1], self._scores, block_table,
+                                         context_lens, cu_nodes, accepted, num_accepted, new_lens)
         return new_lens
 
     def copy_blocks(self, src: Sequence[int], dst: Sequence[int]) -> None:

@@ -14,6 +14,9 @@ then decode slots, :mod:`railgun_amd.batch`) runs as:
   the decode op, D7); decode rows that begin with the same blocks read those once
   (``rg_paged_attention_shared_prefix``) where the step was packed so and it pays, and a step packed
   to gather attention weights adds them to the pool's scores (``rg_paged_attention_v1_scores``);
+  trees of drafted tokens attend to the cache and their own ancestors (``rg_tree_layout``,
+  ``rg_paged_attention_tree``), ``verify_trees`` says which of them the logits agree with
+  (``rg_verify_tree``) and ``GpuBlockPool.keep_accepted`` keeps those cached;
 * ``rg_rms_norm`` fuses each residual add with the next RMSNorm; ``rg_silu_and_mul`` is the
   SwiGLU gate;
 * the projections of decode-sized steps (at most 128 rows) run on ``rg_linear``, the skinny
@@ -194,21 +197,55 @@ class DeviceStep:
     last_rows: torch.Tensor
     scored_lens: Optional[torch.Tensor] = None
     unscored_slots: Optional[torch.Tensor] = None
+    # The draft trees: first tokens [trees + 1], parents and drafts [tokens], places in the text, and the mask
+    # that a step's layout writes.
+    tree_cu: Optional[torch.Tensor] = None
+    tree_parents: Optional[torch.Tensor] = None
+    tree_places: Optional[torch.Tensor] = None
+    draft_tokens: Optional[torch.Tensor] = None
+    tree_mask: Optional[torch.Tensor] = None
+
+    @property
+    def tree_lens(self) -> torch.Tensor:
+        """Context lengths of the sequences with draft trees."""
+        return self.context_lens[self.host.num_requests - self.host.num_trees:]
+
+    @property
+    def tree_table(self) -> torch.Tensor:
+        """Their block tables."""
+        return self.block_table[self.host.num_requests - self.host.num_trees:]
 
     @staticmethod
     def from_host(b: StepBatch, device) -> "DeviceStep":
         def d(a):
             return torch.from_numpy(np.ascontiguousarray(a)).to(device)
 
-        return DeviceStep(b, d(b.tokens), d(b.positions), d(b.slot_mapping), d(b.context_lens), d(b.block_table),
-                          d(b.cu_seqlens), d(b.last_rows), None if b.scored_lens is None else d(b.scored_lens),
-                          None if b.unscored_slots is None or not b.unscored_slots.size else d(b.unscored_slots))
+        st = DeviceStep(b, d(b.tokens), d(b.positions), d(b.slot_mapping), d(b.context_lens), d(b.block_table),
+                        d(b.cu_seqlens), d(b.last_rows), None if b.scored_lens is None else d(b.scored_lens),
+                        None if b.unscored_slots is None or not b.unscored_slots.size else d(b.unscored_slots))
+        if b.num_trees:
+            st.tree_cu, st.tree_parents, st.tree_places = d(b.tree_cu), d(b.tree_parents), d(b.tree_places)
+            st.draft_tokens = d(b.tokens[b.first_tree_row:].astype(np.int32))
+            st.tree_mask = torch.zeros((len(b.tree_parents), (b.max_tree_nodes + 31) // 32), dtype=torch.int32,
+                                       device=device)
+        return st
+
+
+@dataclass
+class TreeVerdict:
+    """What a step's logits say of its draft trees (rg_verify_tree), int32 on the device."""
+
+    target_tokens: torch.Tensor  # [tokens of the trees]: what follows each of them
+    accepted: torch.Tensor       # [trees, most]: accepted tokens, indices in the tree, -1 behind them
+    num_accepted: torch.Tensor   # [trees]: how many, the first token among them
+    next_tokens: torch.Tensor    # [trees]: what follows the last accepted one
 
 
 class RailgunLlama:
     """architecture.rs:86-165 on the gfx950 kernels.  ``forward`` runs one packed engine
     step and returns the logits of each request's last token ``[requests, vocab]``
-    (engine.rs:238-245 samples from those)."""
+    (engine.rs:238-245 samples from those), and behind them those of every token of the draft
+    trees."""
 
     def __init__(self, cfg: LlamaConfig, weights: LlamaWeights, pool: GpuBlockPool,
                  kernels: Optional[PagedAttentionKernels] = None, max_position: Optional[int] = None,
@@ -267,21 +304,26 @@ class RailgunLlama:
             k.launch_prefill_packed(q[:TP], kc, vc, st.block_table[:P], st.context_lens[:P], st.cu_seqlens,
                                     out[:TP], self.scale, H, Hkv, D, bs, mb, P, TP, b.max_query_len)
         nd = b.num_decode
-        if nd and st.scored_lens is not None:
+        if b.num_trees:
+            # (Its workspace is the call's own: one that grows with the trees would leave a captured decode's behind.)
+            k.launch_tree(q[TP + nd:], kc, vc, st.tree_table, st.tree_lens, st.tree_cu, st.tree_mask, out[TP + nd:],
+                          self.scale, b.max_tree_nodes)
+        if not nd:
+            return
+        qd, od, table, lens = q[TP:TP + nd], out[TP:TP + nd], st.block_table[P:P + nd], st.context_lens[P:P + nd]
+        if st.scored_lens is not None:
             # A step that gathers attention weights, of the tokens behind a prefix that the rows share.
             ws = self._workspace(k.v1_scores_workspace_bytes(nd, H, Hkv, D, bs, mb))
-            k.launch_v1_scores(q[TP:], kc, vc, st.block_table[P:], st.context_lens[P:], out[TP:],
-                               self.pool.scores[layer], st.scored_lens, b.shared_decode_blocks * bs, self.scale, H, Hkv,
-                               D, bs, mb, nd, ws)
-        elif nd and b.shared_decode_blocks and k.shared_prefix_pays(nd, H, Hkv, D, bs, mb, b.shared_decode_blocks,
-                                                                    self.dtype):
+            k.launch_v1_scores(qd, kc, vc, table, lens, od, self.pool.scores[layer], st.scored_lens,
+                               b.shared_decode_blocks * bs, self.scale, H, Hkv, D, bs, mb, nd, ws)
+        elif b.shared_decode_blocks and k.shared_prefix_pays(nd, H, Hkv, D, bs, mb, b.shared_decode_blocks, self.dtype):
             ws = self._workspace(k.shared_prefix_workspace_bytes(nd, H, Hkv, D, bs, mb, b.shared_decode_blocks))
-            k.launch_shared_prefix(q[TP:], kc, vc, st.block_table[P:], st.context_lens[P:], out[TP:], self.scale, H,
-                                   Hkv, D, bs, mb, nd, b.shared_decode_blocks, ws)
-        elif nd:
+            k.launch_shared_prefix(qd, kc, vc, table, lens, od, self.scale, H, Hkv, D, bs, mb, nd,
+                                   b.shared_decode_blocks, ws)
+        else:
             ws = self._workspace(k.v1_workspace_bytes(nd, H, Hkv, D, bs, mb))
-            k.launch_v1(q[TP:], kc, vc, st.block_table[P:], st.context_lens[P:], out[TP:], self.scale, H, Hkv, D,
-                        bs, mb, nd, workspace=ws if ws.numel() else None)
+            k.launch_v1(qd, kc, vc, table, lens, od, self.scale, H, Hkv, D, bs, mb, nd,
+                        workspace=ws if ws.numel() else None)
 
     def _rg_linear_fits(self, x: torch.Tensor, weight: torch.Tensor) -> bool:
         rows, k = (int(d) for d in x.shape)
@@ -508,11 +550,43 @@ class RailgunLlama:
         self.norm_chain[rows] = use
         return use
 
+    def verify_trees(self, logits: torch.Tensor, st: DeviceStep,
+                     sampled: Optional[torch.Tensor] = None) -> TreeVerdict:
+        """Which drafts of a step's trees its ``logits`` (forward's) agree with: a token's target is the argmax
+        of its logits, or what a sampler drew for it (``sampled``, int32 [tokens of the trees])."""
+        b = st.host
+        if not b.num_trees:
+            raise ValueError("the step has no draft trees")
+
+        def new(*shape):
+            return torch.empty(shape, dtype=torch.int32, device=self.device)
+
+        v = TreeVerdict(new(len(b.tree_parents)) if sampled is None else sampled, new(b.num_trees, b.max_tree_depth),
+                        new(b.num_trees), new(b.num_trees))
+        if sampled is None:
+            self.kernels.launch_verify_tree(logits[b.num_requests - b.num_trees:], st.draft_tokens, st.tree_parents,
+                                            st.tree_cu, b.max_tree_nodes, v.target_tokens, v.accepted, v.num_accepted,
+                                            v.next_tokens)
+        else:
+            self.kernels.launch_accept_tree(sampled, st.draft_tokens, st.tree_parents, st.tree_cu, b.max_tree_nodes,
+                                            v.accepted, v.num_accepted, v.next_tokens)
+        return v
+
+    def keep_accepted(self, st: DeviceStep, verdict: TreeVerdict) -> torch.Tensor:
+        """Keeps the accepted tokens of a step's trees cached, and nothing else of the trees
+        (GpuBlockPool.keep_accepted); returns the sequences' new lengths, int32 on the device."""
+        return self.pool.keep_accepted(st.tree_table, st.tree_lens, st.tree_cu, verdict.accepted, verdict.num_accepted)
+
     @torch.no_grad()
     def forward(self, st: DeviceStep) -> torch.Tensor:
         cfg, w = self.cfg, self.w
         self.check_step(st.host)
         T = st.host.num_tokens
+        if st.host.num_trees:
+            r = st.host.first_tree_row
+            self.kernels.launch_tree_layout(st.tree_parents, st.tree_cu, st.tree_lens, st.tree_table, st.tree_mask,
+                                            st.positions[r:], st.slot_mapping[r:], self.pool.block_size,
+                                            st.host.max_tree_nodes, st.tree_places)
         H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
         if st.unscored_slots is not None:
@@ -564,4 +638,4 @@ class RailgunLlama:
 
 
 __all__ = ["DeviceStep", "LLAMA_3_2_1B", "LayerWeights", "LlamaConfig", "LlamaWeights",
-           "RailgunLlama", "graph_us"]
+           "RailgunLlama", "TreeVerdict", "graph_us"]
