@@ -8,9 +8,11 @@
 // same K and V: an attention product on the matrix cores,
 //   S^T = K Q^T,  running maximum and sum per row,  O^T += V^T P^T,
 // in row tiles of kRows (32 a wave) and key tiles of kTileKeys.  Only the key tiles that reach into the tree are
-// masked.  The (sequence, kv-head, row tile) segments of the batch, end to end, are one line of key tiles, and every
-// workgroup takes an equal piece of it, whatever the lengths.  A segment that lies in one piece is written out at
-// once; of the others the pieces' softmax partials (m, l, unnormalised O) are joined by tree_merge_kernel:
+// masked.  A (sequence, kv-head, row tile) segment is cut into equal pieces, as many as its length asks for so that the
+// batch's pieces fill the chip, whatever the lengths: a workgroup each.  The row tiles of the same keys are neighbours,
+// on one XCD at one time: the first to read a key tile brings it to the L2 for the others.  A segment of one piece is
+// written out at once; of the others the pieces' softmax partials (m, l, unnormalised O) are joined by
+// tree_merge_kernel:
 //   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 //
 // Cells that a row does not attend to must not reach it, and 0 NaN is NaN in a matrix product.  In masked tiles V
@@ -77,12 +79,14 @@ struct TreeArgs {
   float scale_log2;
   int32_t num_heads, num_kv_heads, head_dim, block_size, max_blocks, num_seqs, num_nodes, max_nodes, mask_words;
   int64_t kv_stride;
-  // The product's: pieces, their partials, and what the host knows of the line of tiles.
-  float* acc;        // [pieces, kRows, D] unnormalised
-  float* ml;         // [pieces, kRows, 2]: m in log2 units, l
-  int2* segments;    // [num_seqs, row tiles, kv-heads]: first piece's worker, workers
+  // The product's.
+  float* acc;        // [parts, kRows, D] unnormalised
+  float* ml;         // [parts, kRows, 2]: m in log2 units, l
+  int2* cuts;        // [num_seqs]: the first of its parts, pieces of a segment
   uint32_t q_sign;   // bit 0: q is taken (else zeros, a scale of 0), bits 15 and 31: negated (a negative scale)
-  int32_t group, row_tiles, bs_shift, workers, least;  // row_tiles: most of a sequence; least: key tiles to a worker
+  int32_t group, bs_shift;
+  int32_t slots;     // pieces that are at work together
+  int32_t least;     // key tiles of a piece that is worth its partials
 };
 
 // Any shape: a wave per (sequence, node, q-head), lane l has dims 4 l .. 4 l + 3, the keys one after the other with
@@ -149,9 +153,9 @@ __device__ __forceinline__ const Args& arguments() {
   return *p;
 }
 
-// -------------------------------------------------------------- the line ----
+// --------------------------------------------------------------- the cuts ---
 
-// A sequence as the line of tiles has it.
+// A sequence as the cuts see it.
 struct Span {
   Tree t;
   int ctx, tiles, row_tiles;
@@ -174,63 +178,117 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
   return v;
 }
 
-// The workers' shares of the line: q units each, and one more for the first r.  (plan_tree: a line is counted in
-// 32 bits.)
-struct Line {
-  int q, r;
-  __device__ __forceinline__ Line(int total, int workers) : q(total / workers), r(total - q * workers) {}
-  __device__ __forceinline__ int begin(int w) const { return q * w + min(w, r); }
-  __device__ __forceinline__ int owner(int unit) const {
-    const int longer = r * (q + 1);
-    return unit < longer ? unit / (q + 1) : r + (unit - longer) / q;
-  }
+// Pieces that a batch of so many segments is cut into at most: a round of the chip's, or where the segments alone come
+// near that or past it, half a round more than they are.  At most `slots` of them are parts of a segment: n cuts make
+// 2 n parts at most.
+__host__ __device__ inline int64_t most_pieces(int64_t segments, int64_t slots) {
+  return segments <= slots * 3 / 4 ? slots : segments + slots / 2;
+}
+struct CutScratch {
+  uint32_t spans[kTreeThreads];  // tiles, row tiles of up to so many sequences
+  int32_t sums[kTreeWaves][64];
+  int32_t wave_sum[2][kTreeWaves];
+  int32_t seq, local, pieces, base;  // the workgroup's: its sequence; of that, the piece, pieces of a segment, first part
 };
 
-// All sequences, kTreeThreads at a time, scanned by the workgroup.
-struct LineScratch {
-  int32_t wave_sum[kTreeWaves];
-  int32_t total, workers;
-  int32_t seq, seg, tile;  // where the worker's share begins
-};
-__device__ __forceinline__ int units_of(const Args& a, int s) {
-  if (s >= a.num_seqs) return 0;
-  const Span p = span_of(a, s);
-  return p.tiles * p.row_tiles * a.num_kv_heads;
+// x / d rounded up, 0 < x, d < 2^22: the quotient in fp32 is off by less than one either way.
+__device__ __forceinline__ int ceil_quotient(int x, int d) {
+  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+  q += q * d < x;
+  q += q * d < x;
+  return q - ((q - 1) * d >= x);
 }
-__device__ __forceinline__ int line_total(const Args& a, LineScratch& sh, int w, int lane) {
-  int sum = 0;
-  for (int s = threadIdx.x; s < a.num_seqs; s += kTreeThreads) sum += units_of(a, s);
-  sum = wave_scan(sum, lane);
-  if (lane == 63) sh.wave_sum[w] = sum;
-  __syncthreads();
-  int total = 0;
+
+// Key tiles to a piece: the least length (a.least and more) that makes no more pieces than most_pieces.  Between
+// total / pieces and total / (pieces - segments), where every segment's last piece may be short, a lane each tries 64
+// lengths; the waves share the sequences.  Returns that length (0 if there is nothing to do) and the number of pieces.
+__device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, int w, int lane) {
+  int tiles = 0, segments = 0, longest = 1;  // tiles: of all segments
+  for (int s = threadIdx.x; s < a.num_seqs; s += kTreeThreads) {
+    const Span p = span_of(a, s);
+    const int n = p.row_tiles * a.num_kv_heads;
+    tiles += n * p.tiles;
+    segments += n;
+    if (n > 0) longest = max(longest, p.tiles);
+    if (s < kTreeThreads) sh.spans[s] = (uint32_t)p.row_tiles << 24 | (uint32_t)p.tiles;
+  }
+  tiles = wave_scan(tiles, lane);
+  segments = wave_scan(segments, lane);
 #pragma unroll
-  for (int i = 0; i < kTreeWaves; ++i) total += sh.wave_sum[i];
+  for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+  if (lane == 63) {
+    sh.sums[w][0] = tiles;
+    sh.sums[w][1] = segments;
+    sh.sums[w][2] = longest;
+  }
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(total);
+  tiles = segments = 0;
+#pragma unroll
+  for (int i = 0; i < kTreeWaves; ++i) {
+    tiles += sh.sums[i][0];
+    segments += sh.sums[i][1];
+    longest = max(longest, sh.sums[i][2]);
+  }
+  __syncthreads();
+  if (segments == 0) return make_int2(0, 0);
+  const int most = (int)most_pieces(segments, a.slots);
+  const int lo = max(a.least, tiles / most), hi = max(lo, min(longest, tiles / (most - segments) + 1));
+  if (lo >= longest) return make_int2(longest, segments);
+  const int mine = lo + (int)((int64_t)(hi - lo) * lane / 63);
+  int pieces = 0;
+  for (int s = w; s < a.num_seqs; s += kTreeWaves) {
+    uint32_t span;
+    if (s < kTreeThreads) {
+      span = sh.spans[s];
+    } else {
+      const Span p = span_of(a, s);
+      span = (uint32_t)p.row_tiles << 24 | (uint32_t)p.tiles;
+    }
+    pieces += (int)(span >> 24) * a.num_kv_heads * ceil_quotient((int)(span & 0xffffffu), mine);
+  }
+  sh.sums[w][lane] = pieces;
+  __syncthreads();
+  pieces = 0;
+#pragma unroll
+  for (int i = 0; i < kTreeWaves; ++i) pieces += sh.sums[i][lane];
+  const int first = __builtin_ctzll(__ballot(pieces <= most));  // (hi fits)
+  return make_int2(__builtin_amdgcn_readlane(mine, first), __builtin_amdgcn_readlane(pieces, first));
 }
-__device__ __forceinline__ void line_place(const Args& a, LineScratch& sh, int at, int w, int lane) {
-  int before = 0;
+
+// The piece that workgroup `me` has: its sequence, its place among that one's, and the cuts of those.
+__device__ __forceinline__ void find_piece(const Args& a, CutScratch& sh, int tiles, int me, int w, int lane) {
+  int before = 0, parts_before = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += kTreeThreads) {
     const int s = s0 + threadIdx.x;
-    const int n = units_of(a, s);
-    const int upto = wave_scan(n, lane);
-    if (lane == 63) sh.wave_sum[w] = upto;
+    int n = 0, cuts = 0;
+    if (s < a.num_seqs) {
+      const Span p = span_of(a, s);
+      cuts = (p.tiles + tiles - 1) / tiles;
+      n = p.row_tiles * a.num_kv_heads * cuts;
+    }
+    const int parts = cuts > 1 ? n : 0;
+    const int upto = wave_scan(n, lane), parts_upto = wave_scan(parts, lane);
+    if (lane == 63) {
+      sh.wave_sum[0][w] = upto;
+      sh.wave_sum[1][w] = parts_upto;
+    }
     __syncthreads();
-    int start = before + upto - n;
+    int start = before + upto - n, base = parts_before + parts_upto - parts;
 #pragma unroll
     for (int i = 0; i < kTreeWaves; ++i) {
-      start += i < w ? sh.wave_sum[i] : 0;
-      before += sh.wave_sum[i];
+      start += i < w ? sh.wave_sum[0][i] : 0;
+      base += i < w ? sh.wave_sum[1][i] : 0;
+      before += sh.wave_sum[0][i];
+      parts_before += sh.wave_sum[1][i];
     }
-    if (start <= at && at - start < n) {
-      const int tiles = span_of(a, s).tiles;
+    if (start <= me && me - start < n) {
       sh.seq = s;
-      sh.seg = (at - start) / tiles;
-      sh.tile = (at - start) % tiles;
+      sh.local = me - start;
+      sh.pieces = cuts;
+      sh.base = base;
     }
     __syncthreads();
-    if (at < before) break;
+    if (me < before) break;
   }
 }
 
@@ -256,6 +314,7 @@ struct Piece {
   int first, prior, ctx;     // first node; positions
   int kt0, kt1;
   int slot;                  // of the partials, -1: the segment is whole
+  bool once;                 // no other row tile reads these keys
 };
 
 // Tile kt's attended keys for a node, bit k: key k.  All of it lies before the tree (then no row asks), or its bits
@@ -358,6 +417,12 @@ template <typename T> __device__ __forceinline__ uint32_t pair_cleared(uint32_t 
 
 // Lane l of a wave owns query row l % 32 of it; the other half of that row's keys sits in lane l ^ 32.  sick: a word
 // of LDS per stage.
+// 1 KB to LDS, non-temporal where it is read once.
+__device__ __forceinline__ void copy(const char* base, uint32_t lane_bytes, uint32_t lds_addr, bool once) {
+  if (once) lds_dma16_s_nt(base, lane_bytes, lds_addr);
+  else lds_dma16_s(base, lane_bytes, lds_addr);
+}
+
 template <typename T, int D>
 __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sick, int w, int lane) {
   const Args& a = arguments();
@@ -411,9 +476,9 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
     const char* vb = reinterpret_cast<const char*>(vc + off);
     const uint32_t at = lds_base + st * TL::BYTES + cb * (TL::KB / 2) + cp * HALF * 1024;
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) lds_dma16_s(kb + 64 * i, k_off, at + i * 1024);
+    for (int i = 0; i < HALF; ++i) copy(kb + 64 * i, k_off, at + i * 1024, p.once);
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) lds_dma16_s(vb + 1024 * i, v_off, at + TL::KB + i * 1024);
+    for (int i = 0; i < HALF; ++i) copy(vb + 1024 * i, v_off, at + TL::KB + i * 1024, p.once);
   };
 
   f32x16_t o[NDB];
@@ -766,175 +831,151 @@ constexpr int ring_bytes() {
 template <typename T, int D>
 constexpr int groups_per_cu() { return std::is_same_v<T, f32_t> ? 2 : D == 128 ? 3 : 4; }
 
-// One worker: its piece of the line, segment by segment.
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_kernel(TreeArgs) {
   __shared__ __attribute__((aligned(16))) char ring[ring_bytes<T, D>()];
-  __shared__ LineScratch scratch;
   __shared__ uint32_t sick[4];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int s, seg, kt, left;
-  int me;
+  Piece p;
   {
     const Args& a = arguments();
-    const int total = line_total(a, scratch, w, lane);
-    if (total == 0) return;
-    // Shares of `least` key tiles and more.  Neighbours on the line go to the same XCD (workgroups are dealt to the
-    // eight in turn), whose L2 the row tiles of a kv-head share.
-    const int workers = min(a.workers, max(1, total / a.least)), per = (workers + 7) / 8;
-    me = (int)(blockIdx.x % 8) * per + (int)blockIdx.x / 8;
-    if ((int)blockIdx.x / 8 >= per || me >= workers) return;
-    const Line line(total, workers);
-    line_place(a, scratch, line.begin(me), w, lane);
-    if (threadIdx.x == 0) {
-      scratch.total = total;
-      scratch.workers = workers;
-    }
-    left = line.begin(me + 1) - line.begin(me);
-    s = __builtin_amdgcn_readfirstlane(scratch.seq);
-    seg = __builtin_amdgcn_readfirstlane(scratch.seg);
-    kt = __builtin_amdgcn_readfirstlane(scratch.tile);
+    CutScratch& sh = *reinterpret_cast<CutScratch*>(ring);  // (before the first key tile)
+    static_assert(sizeof(CutScratch) <= sizeof(ring), "the cuts' scratch lies in the ring");
+    const int2 cut_to = piece_tiles(a, sh, w, lane);
+    // Neighbours go to the same XCD (workgroups are dealt to the eight in turn).
+    const int per = (cut_to.y + 7) / 8, me = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    if ((int)(blockIdx.x / 8) >= per || me >= cut_to.y) return;
+    find_piece(a, sh, cut_to.x, me, w, lane);
+    const int s = __builtin_amdgcn_readfirstlane(sh.seq);
+    const int local = __builtin_amdgcn_readfirstlane(sh.local), n = __builtin_amdgcn_readfirstlane(sh.pieces);
+    const int base = __builtin_amdgcn_readfirstlane(sh.base);
+    __syncthreads();  // the scratch is free
+    const Span sp = span_of(a, s);
+    const int rt = local % sp.row_tiles, cut = local / sp.row_tiles % n;
+    p.seq = s;
+    p.kvh = local / sp.row_tiles / n;
+    p.row0 = rt * kRows;
+    p.rows = sp.t.nodes * a.group;
+    p.first = sp.t.first;
+    p.ctx = sp.ctx;
+    p.prior = max(sp.ctx - sp.t.len, 0);
+    p.kt0 = (int)((int64_t)sp.tiles * cut / n);
+    p.kt1 = (int)((int64_t)sp.tiles * (cut + 1) / n);
+    p.slot = n > 1 ? base + local : -1;
+    p.once = sp.row_tiles == 1;
+    if (local == 0 && threadIdx.x == 0) a.cuts[s] = make_int2(base, n);
   }
-  while (left > 0) {
-    Piece p;
-    {
-      const Args& a = arguments();
-      const Span sp = span_of(a, s);
-      if (seg >= sp.row_tiles * a.num_kv_heads) {  // on to the next sequence that has any
-        ++s;
-        seg = 0;
-        continue;
-      }
-      const int n = min(sp.tiles - kt, left);
-      p.kvh = seg / sp.row_tiles;
-      const int rt = seg - p.kvh * sp.row_tiles;
-      p.seq = s;
-      p.row0 = rt * kRows;
-      p.rows = sp.t.nodes * a.group;
-      p.first = sp.t.first;
-      p.ctx = sp.ctx;
-      p.prior = max(sp.ctx - sp.t.len, 0);
-      p.kt0 = kt;
-      p.kt1 = kt + n;
-      const bool starts = kt == 0, ends = p.kt1 == sp.tiles;
-      p.slot = starts && ends ? -1 : 2 * me + (starts ? 1 : 0);
-      if (starts && threadIdx.x == 0) {
-        int pieces = 1;
-        if (!ends) {
-          const Line line(scratch.total, scratch.workers);
-          pieces = line.owner(line.begin(me + 1) - left + sp.tiles - 1) - me + 1;
-        }
-        a.segments[((int64_t)s * a.row_tiles + rt) * a.num_kv_heads + p.kvh] = make_int2(me, pieces);
-      }
-      left -= n;
-      kt = ends ? 0 : p.kt1;
-      seg += ends;
-    }
-    if (p.ctx == 0) {
-      const int row = p.row0 + w * 32 + (lane & 31);
-      f32x16_t o[D / 32];
+  if (p.ctx == 0) {
+    const int row = p.row0 + w * 32 + (lane & 31);
+    f32x16_t o[D / 32];
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
-      store_rows<T, D>(p, row, lane >> 5, o, -INFINITY, 0.f);
-    } else if constexpr (std::is_same_v<T, f32_t>) {
-      product_f32<D>(p, ring, sick, w, lane);
-    } else {
-      product<T, D>(p, ring, sick, w, lane);
-    }
-    __syncthreads();  // the ring is free
+      for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+    store_rows<T, D>(p, row, lane >> 5, o, -INFINITY, 0.f);
+  } else if constexpr (std::is_same_v<T, f32_t>) {
+    product_f32<D>(p, ring, sick, w, lane);
+  } else {
+    product<T, D>(p, ring, sick, w, lane);
   }
 }
 
-// A wave per row of a segment that lies in several pieces; lane l folds dims [l PER, (l + 1) PER) of them.
-constexpr int kMergeRows = 4;
+// The rows of a cut segment: D / 4 lanes have 4 dims each of a row, a wave kMergeRows of them, the AHEAD next pieces'
+// in flight.
+constexpr int kMergeWaves = 4;
+template <int D> constexpr int merge_rows() { return 256 / D; }
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kMergeRows) void tree_merge_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a) {
   using S = typename elem<T>::storage;
-  constexpr int PER = D / 64;
+  constexpr int LANES = D / 4, ROWS = merge_rows<D>(), AHEAD = 8;
   const int s = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63;
-  const int row = (int)blockIdx.x * kMergeRows + (threadIdx.x >> 6);
-  const int rt = row / kRows, in = row - rt * kRows;
-  const int2 seg = a.segments[((int64_t)s * a.row_tiles + rt) * a.num_kv_heads + kvh];  // (not used where there is none)
+  const int row0 = ((int)blockIdx.x * kMergeWaves + (threadIdx.x >> 6)) * ROWS;
+  const int2 cuts = a.cuts[s];  // (not used where the sequence has no tree)
   const Span sp = span_of(arguments(), s);
-  if (row >= sp.t.nodes * a.group || seg.y <= 1) return;
-  struct Part {
-    float2 ml;
-    float v[PER];
-  };
-  auto load = [&](int i) __attribute__((always_inline)) {
-    const int64_t at = ((int64_t)2 * (seg.x + i) + (i == 0 ? 1 : 0)) * kRows + in;
-    Part p;
-    p.ml = *reinterpret_cast<const float2*>(a.ml + 2 * at);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) p.v[e] = a.acc[at * D + lane * PER + e];
-    return p;
-  };
+  const int rows = sp.t.nodes * a.group, n = cuts.y;
+  if (row0 >= rows || n <= 1) return;
+  const int rt = row0 / kRows, d = lane % LANES * 4;
+  const int row = row0 + lane / LANES, in = min(row, rows - 1) - rt * kRows;  // (a row tile's rows are written so far)
+  static_assert(kRows % ROWS == 0, "a wave's rows lie in one row tile");
+  const int64_t first = (int64_t)(cuts.x + kvh * n * sp.row_tiles + rt) * kRows + in;
+  const int64_t step = (int64_t)sp.row_tiles * kRows;
   float m = -INFINITY, l = 0.f;
-  float acc[PER];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < n; i += AHEAD) {
+    float2 ml[AHEAD];
+    float4 v[AHEAD];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-  auto fold = [&](const Part& p) __attribute__((always_inline)) {
-    // (A piece without keys for the row has m = -inf and nothing to add.)
-    const float mn = fmaxf(m, p.ml.x);
-    const float fo = m == mn ? 1.f : exp2f(m - mn), fq = p.ml.x == -INFINITY ? 0.f : exp2f(p.ml.x - mn);
-    l = l * fo + p.ml.y * fq;
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t at = first + min(i + u, n - 1) * step;
+      ml[u] = *reinterpret_cast<const float2*>(a.ml + 2 * at);
+      v[u] = *reinterpret_cast<const float4*>(a.acc + at * D + d);
+    }
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = acc[e] * fo + p.v[e] * fq;
-    m = mn;
-  };
-  constexpr int AHEAD = 4;
-  int i = 0;
-  for (; i + AHEAD <= seg.y; i += AHEAD) {
-    Part part[AHEAD];
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) part[u] = load(i + u);
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) fold(part[u]);
+    for (int u = 0; u < AHEAD; ++u) {
+      // (A piece without keys for the row has m = -inf and nothing to add; one whose scores are all NaN has m = -inf too.)
+      const bool counts = i + u < n && !(ml[u].x == -INFINITY && ml[u].y == 0.f);
+      const float mn = counts ? fmaxf(m, ml[u].x) : m;
+      const float fo = m == mn ? 1.f : exp2f(m - mn), fq = !counts ? 0.f : ml[u].x == mn ? 1.f : exp2f(ml[u].x - mn);
+      l = l * fo + (counts ? ml[u].y * fq : 0.f);
+      acc.x = acc.x * fo + (counts ? v[u].x * fq : 0.f);
+      acc.y = acc.y * fo + (counts ? v[u].y * fq : 0.f);
+      acc.z = acc.z * fo + (counts ? v[u].z * fq : 0.f);
+      acc.w = acc.w * fo + (counts ? v[u].w * fq : 0.f);
+      m = mn;
+    }
   }
-  for (; i < seg.y; ++i) fold(load(i));
+  if (row >= rows) return;
   const int node = row / a.group, g = row - node * a.group;
-  S* out = static_cast<S*>(a.out) + ((int64_t)(sp.t.first + node) * a.num_heads + kvh * a.group + g) * D + lane * PER;
+  S* out = static_cast<S*>(a.out) + ((int64_t)(sp.t.first + node) * a.num_heads + kvh * a.group + g) * D + d;
   const float inv = l != 0.f ? 1.f / l : 1.f;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) out[e] = elem<T>::from_f32(acc[e] * inv);
+  const float x0 = acc.x * inv, x1 = acc.y * inv, x2 = acc.z * inv, x3 = acc.w * inv;
+  if constexpr (std::is_same_v<T, f32_t>) *reinterpret_cast<float4*>(out) = make_float4(x0, x1, x2, x3);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x0, x1), pack2<T>(x2, x3));
 }
 
 // ---------------------------------------------------------------- the plan --
 
-constexpr int kWorkersPerCu = 2;
-
-// Key tiles on the line of the longest sequences and largest trees.
-double most_units(int32_t num_seqs, int32_t row_tiles, int32_t Hkv, int32_t bs, int32_t MB) {
-  return (double)num_seqs * Hkv * row_tiles * std::max<int64_t>(1, ceil_div((int64_t)MB * bs, kTileKeys));
-}
+#ifndef RG_TREE_WPC
+#define RG_TREE_WPC 2
+#endif
+#ifndef RG_TREE_LEAST
+#define RG_TREE_LEAST 8
+#endif
+constexpr int kPiecesPerCu = RG_TREE_WPC;
 
 struct TreePlan {
-  int32_t row_tiles, workers;
-  size_t ml_at, segments_at, bytes;
+  int32_t slots, groups, tiles;  // tiles: of the longest sequence
+  size_t ml_at, cuts_at, bytes;
 };
 TreePlan plan_tree(int32_t num_seqs, int32_t max_nodes, int32_t H, int32_t Hkv, int32_t D, int32_t bs, int32_t MB) {
-  TreePlan p;
-  p.row_tiles = (int32_t)ceil_div((int64_t)max_nodes * (H / Hkv), kRows);
-  // (What the product does not take runs on the generic kernel.)
-  const double most = most_units(num_seqs, p.row_tiles, Hkv, bs, MB);
-  if ((D != 64 && D != 128) || block_shift(bs) < 0 || most > INT32_MAX) return TreePlan{};
-  p.workers = (int32_t)std::min<double>((double)device_cu_count() * kWorkersPerCu, most);
-  const size_t pieces = 2 * (size_t)p.workers;
-  p.ml_at = align_up(pieces * kRows * D * 4, 256);
-  p.segments_at = p.ml_at + align_up(pieces * kRows * 8, 256);
-  p.bytes = p.segments_at + align_up((size_t)num_seqs * p.row_tiles * Hkv * 8, 256);
+  TreePlan p{};
+  const int64_t row_tiles = ceil_div((int64_t)max_nodes * (H / Hkv), kRows), segments = num_seqs * row_tiles * Hkv;
+  const int64_t tiles = std::max<int64_t>(1, ceil_div((int64_t)MB * bs, kTileKeys));
+  p.tiles = (int32_t)std::min<int64_t>(tiles, INT32_MAX);
+  p.slots = device_cu_count() * kPiecesPerCu;
+  const int64_t pieces = most_pieces(segments, p.slots);
+  // (What the product does not take runs on the generic kernel.  The cuts count in 32 bits, a sequence's tiles in 22,
+  // its row tiles in 8.)
+  if ((D != 64 && D != 128) || block_shift(bs) < 0 || tiles >= 1 << 22 || row_tiles > 255 ||
+      (double)segments * tiles > INT32_MAX || pieces > INT32_MAX - 8) {
+    return p;
+  }
+  p.groups = (int32_t)(ceil_div(std::min(pieces, segments * tiles), 8) * 8);
+  const int64_t parts = std::min<int64_t>(p.slots, segments * tiles);
+  p.ml_at = align_up((size_t)parts * kRows * D * 4, 256);
+  p.cuts_at = p.ml_at + align_up((size_t)parts * kRows * 8, 256);
+  p.bytes = p.cuts_at + align_up((size_t)num_seqs * 8, 256);
   return p;
 }
 
 template <typename T, int D>
-void launch_product(const TreeArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((tree_kernel<T, D>), dim3((unsigned)ceil_div(a.workers, 8) * 8), dim3(kTreeThreads), 0, s, a);
-  const unsigned rows = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, kMergeRows);
+void launch_product(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((tree_kernel<T, D>), dim3((unsigned)p.groups), dim3(kTreeThreads), 0, s, a);
+  if (p.tiles <= a.least) return;  // nothing is cut
+  const unsigned rows = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, merge_rows<D>() * kMergeWaves);
   hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3(rows, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs),
-                     dim3(64 * kMergeRows), 0, s, a);
+                     dim3(64 * kMergeWaves), 0, s, a);
 }
 
 }  // namespace
@@ -1034,19 +1075,18 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
     char* const ws = static_cast<char*>(workspace);
     a.acc = reinterpret_cast<float*>(ws);
     a.ml = reinterpret_cast<float*>(ws + p.ml_at);
-    a.segments = reinterpret_cast<int2*>(ws + p.segments_at);
+    a.cuts = reinterpret_cast<int2*>(ws + p.cuts_at);
     // The product works with a positive scale: a negative one turns q's signs, 0 takes zeros for q.
     a.q_sign = scale == 0.f ? 0u : scale < 0.f ? 0x80008001u : 1u;
     a.scale_log2 = scale != 0.f ? fabsf(a.scale_log2) : 1.f;
     a.group = num_heads / num_kv_heads;
-    a.row_tiles = p.row_tiles;
     a.bs_shift = block_shift(block_size);
-    a.workers = p.workers;
-    a.least = dtype == RG_DTYPE_F32 ? 1 : 8;
+    a.slots = p.slots;
+    a.least = dtype == RG_DTYPE_F32 ? 1 : RG_TREE_LEAST;
     return dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
-      if (head_dim == 128) launch_product<T, 128>(a, as_stream(stream));
-      else launch_product<T, 64>(a, as_stream(stream));
+      if (head_dim == 128) launch_product<T, 128>(a, p, as_stream(stream));
+      else launch_product<T, 64>(a, p, as_stream(stream));
       return check_launch(op);
     });
   }
