@@ -169,12 +169,25 @@ __device__ __forceinline__ Span span_of(const Args& a, int s) {
   p.tiles = max(1, (p.ctx + kTileKeys - 1) / kTileKeys);
   return p;
 }
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int below = __shfl_up(v, o, 64);
-    if (lane >= o) v += below;
-  }
+// Inclusive prefix sum over the 64 lanes: within each row of 16 lanes by shifts of 1, 2, 4 and 8, then lane 15 of rows
+// 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.  Lanes whose source falls outside the row receive 0.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
+// Maximum over the 64 lanes of values not below 0, in lane 63.
+__device__ __forceinline__ int wave_top(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
   return v;
 }
 
@@ -188,34 +201,36 @@ struct CutScratch {
   uint32_t spans[kTreeThreads];  // tiles, row tiles of up to so many sequences
   int32_t sums[kTreeWaves][64];
   int32_t wave_sum[2][kTreeWaves];
-  int32_t seq, local, pieces, base;  // the workgroup's: its sequence; of that, the piece, pieces of a segment, first part
+  // The workgroup's: its sequence; of that, the piece, pieces of a segment, the first part.
+  int32_t seq, local, pieces, base;
+  Span span;
 };
 
-// x / d rounded up, 0 < x, d < 2^22: the quotient in fp32 is off by less than one either way.
-__device__ __forceinline__ int ceil_quotient(int x, int d) {
-  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
-  q += q * d < x;
-  q += q * d < x;
-  return q - ((q - 1) * d >= x);
+// x / d rounded up, 0 < x, d < 2^22, by = 1 / d: the quotient in fp32 is off by less than one either way.
+__device__ __forceinline__ int ceil_quotient(int x, int d, float by) {
+  int q = (int)((float)x * by);
+  q += (int)__umul24(q, d) < x;
+  q += (int)__umul24(q, d) < x;
+  return q - ((int)__umul24(q - 1, d) >= x);
 }
 
 // Key tiles to a piece: the least length (a.least and more) that makes no more pieces than most_pieces.  Between
 // total / pieces and total / (pieces - segments), where every segment's last piece may be short, a lane each tries 64
 // lengths; the waves share the sequences.  Returns that length (0 if there is nothing to do) and the number of pieces.
-__device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, int w, int lane) {
+// `own`: the thread's sequence of the first kTreeThreads.
+__device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, const Span& own, int w, int lane) {
   int tiles = 0, segments = 0, longest = 1;  // tiles: of all segments
   for (int s = threadIdx.x; s < a.num_seqs; s += kTreeThreads) {
-    const Span p = span_of(a, s);
+    const Span p = s < kTreeThreads ? own : span_of(a, s);
     const int n = p.row_tiles * a.num_kv_heads;
     tiles += n * p.tiles;
     segments += n;
     if (n > 0) longest = max(longest, p.tiles);
     if (s < kTreeThreads) sh.spans[s] = (uint32_t)p.row_tiles << 24 | (uint32_t)p.tiles;
   }
-  tiles = wave_scan(tiles, lane);
-  segments = wave_scan(segments, lane);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+  tiles = wave_scan(tiles);
+  segments = wave_scan(segments);
+  longest = wave_top(longest);
   if (lane == 63) {
     sh.sums[w][0] = tiles;
     sh.sums[w][1] = segments;
@@ -229,23 +244,25 @@ __device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, int w
     segments += sh.sums[i][1];
     longest = max(longest, sh.sums[i][2]);
   }
-  __syncthreads();
   if (segments == 0) return make_int2(0, 0);
   const int most = (int)most_pieces(segments, a.slots);
   const int lo = max(a.least, tiles / most), hi = max(lo, min(longest, tiles / (most - segments) + 1));
   if (lo >= longest) return make_int2(longest, segments);
   const int mine = lo + (int)((int64_t)(hi - lo) * lane / 63);
+  const float by = __builtin_amdgcn_rcpf((float)mine);
   int pieces = 0;
-  for (int s = w; s < a.num_seqs; s += kTreeWaves) {
-    uint32_t span;
-    if (s < kTreeThreads) {
-      span = sh.spans[s];
-    } else {
-      const Span p = span_of(a, s);
-      span = (uint32_t)p.row_tiles << 24 | (uint32_t)p.tiles;
-    }
-    pieces += (int)(span >> 24) * a.num_kv_heads * ceil_quotient((int)(span & 0xffffffu), mine);
+  const int near = min(a.num_seqs, kTreeThreads);
+#pragma unroll 4
+  for (int s = w; s < near; s += kTreeWaves) {
+    const uint32_t span = sh.spans[s];
+    pieces += (int)__umul24(span >> 24, ceil_quotient((int)(span & 0xffffffu), mine, by));
   }
+  for (int s = kTreeThreads + w; s < a.num_seqs; s += kTreeWaves) {
+    const Span p = span_of(a, s);
+    pieces += p.row_tiles * ceil_quotient(p.tiles, mine, by);
+  }
+  pieces *= a.num_kv_heads;
+  __syncthreads();  // sums are read
   sh.sums[w][lane] = pieces;
   __syncthreads();
   pieces = 0;
@@ -256,18 +273,20 @@ __device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, int w
 }
 
 // The piece that workgroup `me` has: its sequence, its place among that one's, and the cuts of those.
-__device__ __forceinline__ void find_piece(const Args& a, CutScratch& sh, int tiles, int me, int w, int lane) {
+__device__ __forceinline__ void find_piece(const Args& a, CutScratch& sh, const Span& own, int tiles, int me, int w,
+                                           int lane) {
   int before = 0, parts_before = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += kTreeThreads) {
     const int s = s0 + threadIdx.x;
     int n = 0, cuts = 0;
+    Span p = own;
     if (s < a.num_seqs) {
-      const Span p = span_of(a, s);
+      if (s0 > 0) p = span_of(a, s);
       cuts = (p.tiles + tiles - 1) / tiles;
       n = p.row_tiles * a.num_kv_heads * cuts;
     }
     const int parts = cuts > 1 ? n : 0;
-    const int upto = wave_scan(n, lane), parts_upto = wave_scan(parts, lane);
+    const int upto = wave_scan(n), parts_upto = wave_scan(parts);
     if (lane == 63) {
       sh.wave_sum[0][w] = upto;
       sh.wave_sum[1][w] = parts_upto;
@@ -286,6 +305,7 @@ __device__ __forceinline__ void find_piece(const Args& a, CutScratch& sh, int ti
       sh.local = me - start;
       sh.pieces = cuts;
       sh.base = base;
+      sh.span = p;
     }
     __syncthreads();
     if (me < before) break;
@@ -334,6 +354,22 @@ __device__ __forceinline__ uint32_t tile_mask(const Piece& p, int node, int kt) 
   }
   const int left = p.ctx - kt * kTileKeys;
   return left >= 32 ? m : left > 0 ? m & ((1u << left) - 1u) : 0u;
+}
+
+// Which keys of a tile hold a value that is not finite: a word for every tile that reaches into the tree.  (A tree of
+// more nodes than max_nodes says shares the last one.)
+constexpr int kSickWords = kMaxTreeNodes / kTileKeys + 2;
+__device__ __forceinline__ int sick_word(const Piece& p, int kt) { return min(kt - p.prior / kTileKeys, kSickWords - 1); }
+
+// A row's masks of kMaskTiles key tiles from tile `from` on, into LDS; a row's lanes l and l + 32 do half each.  Read
+// by their wave alone.
+constexpr int kMaskTiles = 4;
+__device__ __forceinline__ void fill_masks(const Piece& p, int node, int from, int in, int hh, uint32_t (&masks)[kMaskTiles][kRows]) {
+#pragma unroll
+  for (int i = 0; i < kMaskTiles / 2; ++i) {
+    const int n = hh * (kMaskTiles / 2) + i;
+    masks[n][in] = tile_mask(p, node, from + n);
+  }
 }
 
 // x where the bit is set, else -inf (by the bit spread over a word: sixteen conditions held as lane masks would take
@@ -424,7 +460,8 @@ __device__ __forceinline__ void copy(const char* base, uint32_t lane_bytes, uint
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sick, int w, int lane) {
+__device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sick,
+                                        uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
   const Args& a = arguments();
   using MF = mfma32<T>;
   using TL = KeyTile<D>;
@@ -449,6 +486,8 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
     win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
   };
   fill();
+  int masks_from = max(p.kt0, p.prior / kTileKeys);
+  if (masks_from < p.kt1) fill_masks(p, node, masks_from, w * 32 + j, hh, masks);
   uint4 qb[NKC];
   {
     const uint4* qr = reinterpret_cast<const uint4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D);
@@ -592,10 +631,11 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
         *at = make_uint4(0u, 0u, 0u, 0u);
       } else if (pair_not_finite<T>(x.x) || pair_not_finite<T>(x.y) || pair_not_finite<T>(x.z) || pair_not_finite<T>(x.w)) {
         *at = make_uint4(pair_cleared<T>(x.x), pair_cleared<T>(x.y), pair_cleared<T>(x.z), pair_cleared<T>(x.w));
-        atomicOr(&sick[st], 1u << key);
+        atomicOr(&sick[sick_word(p, kt)], 1u << key);
       }
     }
-    __syncthreads();
+    wave_lds_sync();  // (the copies in flight stay in flight)
+    tile_barrier();
   };
 
   // The window and Q have landed (the builtin, which the compiler's own counting follows: behind an asm
@@ -621,12 +661,7 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
       __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
     }
     const bool masked = (kt + 1) * kTileKeys > p.prior;
-    if (masked) {
-      // (The word is this tile's: the last use of the stage ended before the barrier above.)
-      if (threadIdx.x == 0) sick[st] = 0;
-      __syncthreads();
-      clean(kt, st);
-    }
+    if (masked) clean(kt, st);
     const char* tile = lds + st * TL::BYTES;
     if (busy) {
       __builtin_amdgcn_s_setprio(1);
@@ -634,13 +669,14 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
       if (next < p.kt1) issue(next, next_st);  // while the QK MFMAs run
       uint32_t mine = 0;
       if (masked) {
-        mine = tile_mask(p, node, kt);
+        if (kt - masks_from >= kMaskTiles) fill_masks(p, node, masks_from = kt, w * 32 + j, hh, masks);
+        mine = masks[kt - masks_from][w * 32 + j];
         const uint32_t shifted = mine >> (4 * hh);
 #pragma unroll
         for (int v = 0; v < 16; ++v) c[v] = if_bit(shifted, 8 * (v >> 2) + (v & 3), c[v]);
       }
       finish(c, tile);
-      if (masked && sick[st] != 0) add_not_finite<T, D>(p, kt, sick[st], mine, hh, o);
+      if (masked && sick[sick_word(p, kt)] != 0) add_not_finite<T, D>(p, kt, sick[sick_word(p, kt)], mine, hh, o);
     } else if (next < p.kt1) {
       issue(next, next_st);
     }
@@ -668,7 +704,8 @@ struct KeyTileF32 {
 };
 
 template <int D>
-__device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t* sick, int w, int lane) {
+__device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t* sick,
+                                        uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
   const Args& a = arguments();
   using TL = KeyTileF32<D>;
   constexpr int NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF, HD = D / 2;
@@ -688,6 +725,8 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
     win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
   };
   fill();
+  int masks_from = max(p.kt0, p.prior / kTileKeys);
+  if (masks_from < p.kt1) fill_masks(p, node, masks_from, w * 32 + j, hh, masks);
   float qf[HD];
   {
     const float4* qr = reinterpret_cast<const float4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D + hh * HD);
@@ -738,10 +777,11 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
         *at = make_float4(0.f, 0.f, 0.f, 0.f);
       } else if (!(fine(x.x) && fine(x.y) && fine(x.z) && fine(x.w))) {
         *at = make_float4(fine(x.x) ? x.x : 0.f, fine(x.y) ? x.y : 0.f, fine(x.z) ? x.z : 0.f, fine(x.w) ? x.w : 0.f);
-        atomicOr(&sick[st], 1u << key);
+        atomicOr(&sick[sick_word(p, kt)], 1u << key);
       }
     }
-    __syncthreads();
+    wave_lds_sync();  // (the copies in flight stay in flight)
+    tile_barrier();
   };
   auto compute = [&](int kt, int st, bool masked) __attribute__((always_inline)) {
     const char* krow = lds + st * TL::BYTES + j * (D * 4);
@@ -758,7 +798,8 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
     }
     uint32_t mine = ~0u;
     if (masked) {
-      mine = tile_mask(p, node, kt);
+      if (kt - masks_from >= kMaskTiles) fill_masks(p, node, masks_from = kt, w * 32 + j, hh, masks);
+      mine = masks[kt - masks_from][w * 32 + j];
       const uint32_t shifted = mine >> (4 * hh);
 #pragma unroll
       for (int v = 0; v < 16; ++v) c[v] = if_bit(shifted, 8 * (v >> 2) + (v & 3), c[v]);
@@ -789,7 +830,7 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
         o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[(8 * (v >> 2) + (v & 3)) * D + 32 * db], c[v], o[db], 0, 0, 0);
-    if (masked && sick[st] != 0) add_not_finite<f32_t, D>(p, kt, sick[st], mine, hh, o);
+    if (masked && sick[sick_word(p, kt)] != 0) add_not_finite<f32_t, D>(p, kt, sick[sick_word(p, kt)], mine, hh, o);
   };
   __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0): the window and Q
   issue(p.kt0, 0);
@@ -803,11 +844,7 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
     else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
     tile_barrier();  // tile kt has landed for every wave
     const bool masked = (kt + 1) * kTileKeys > p.prior;
-    if (masked) {
-      if (threadIdx.x == 0) sick[st] = 0;
-      __syncthreads();
-      clean(kt, st);
-    }
+    if (masked) clean(kt, st);
     if (busy) compute(kt, st, masked);
     if (kt + 2 < p.kt1) {
       if (kt + 2 - wb >= 64) {
@@ -834,7 +871,9 @@ constexpr int groups_per_cu() { return std::is_same_v<T, f32_t> ? 2 : D == 128 ?
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_kernel(TreeArgs) {
   __shared__ __attribute__((aligned(16))) char ring[ring_bytes<T, D>()];
-  __shared__ uint32_t sick[4];
+  __shared__ uint32_t sick[kSickWords];
+  __shared__ uint32_t masks[kMaskTiles][kRows];
+  if (threadIdx.x < kSickWords) sick[threadIdx.x] = 0;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Piece p;
@@ -842,16 +881,24 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
     const Args& a = arguments();
     CutScratch& sh = *reinterpret_cast<CutScratch*>(ring);  // (before the first key tile)
     static_assert(sizeof(CutScratch) <= sizeof(ring), "the cuts' scratch lies in the ring");
-    const int2 cut_to = piece_tiles(a, sh, w, lane);
+    Span own{};
+    if (threadIdx.x < (unsigned)a.num_seqs) own = span_of(a, threadIdx.x);
+    const int2 cut_to = piece_tiles(a, sh, own, w, lane);
     // Neighbours go to the same XCD (workgroups are dealt to the eight in turn).
     const int per = (cut_to.y + 7) / 8, me = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     if ((int)(blockIdx.x / 8) >= per || me >= cut_to.y) return;
-    find_piece(a, sh, cut_to.x, me, w, lane);
+    find_piece(a, sh, own, cut_to.x, me, w, lane);
     const int s = __builtin_amdgcn_readfirstlane(sh.seq);
     const int local = __builtin_amdgcn_readfirstlane(sh.local), n = __builtin_amdgcn_readfirstlane(sh.pieces);
     const int base = __builtin_amdgcn_readfirstlane(sh.base);
+    Span sp;
+    sp.t.first = __builtin_amdgcn_readfirstlane(sh.span.t.first);
+    sp.t.len = __builtin_amdgcn_readfirstlane(sh.span.t.len);
+    sp.t.nodes = __builtin_amdgcn_readfirstlane(sh.span.t.nodes);
+    sp.ctx = __builtin_amdgcn_readfirstlane(sh.span.ctx);
+    sp.tiles = __builtin_amdgcn_readfirstlane(sh.span.tiles);
+    sp.row_tiles = __builtin_amdgcn_readfirstlane(sh.span.row_tiles);
     __syncthreads();  // the scratch is free
-    const Span sp = span_of(a, s);
     const int rt = local % sp.row_tiles, cut = local / sp.row_tiles % n;
     p.seq = s;
     p.kvh = local / sp.row_tiles / n;
@@ -875,9 +922,9 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
       for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
     store_rows<T, D>(p, row, lane >> 5, o, -INFINITY, 0.f);
   } else if constexpr (std::is_same_v<T, f32_t>) {
-    product_f32<D>(p, ring, sick, w, lane);
+    product_f32<D>(p, ring, sick, masks, w, lane);
   } else {
-    product<T, D>(p, ring, sick, w, lane);
+    product<T, D>(p, ring, sick, masks, w, lane);
   }
 }
 
