@@ -248,7 +248,7 @@ __device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, const
   const int most = (int)most_pieces(segments, a.slots);
   const int lo = max(a.least, tiles / most), hi = max(lo, min(longest, tiles / (most - segments) + 1));
   if (lo >= longest) return make_int2(longest, segments);
-  const int mine = lo + (int)((int64_t)(hi - lo) * lane / 63);
+  const int mine = lo + (hi - lo) * lane / 63;
   const float by = __builtin_amdgcn_rcpf((float)mine);
   int pieces = 0;
   const int near = min(a.num_seqs, kTreeThreads);
@@ -453,52 +453,54 @@ template <typename T> __device__ __forceinline__ uint32_t pair_cleared(uint32_t 
 
 // Lane l of a wave owns query row l % 32 of it; the other half of that row's keys sits in lane l ^ 32.  sick: a word
 // of LDS per stage.
-// 1 KB to LDS, non-temporal where it is read once.
-__device__ __forceinline__ void copy(const char* base, uint32_t lane_bytes, uint32_t lds_addr, bool once) {
-  if (once) lds_dma16_s_nt(base, lane_bytes, lds_addr);
-  else lds_dma16_s(base, lane_bytes, lds_addr);
+// N copies of 1 KB to LDS, `step` bytes apart, non-temporal where they are read once.
+template <int N>
+__device__ __forceinline__ void copy(const char* base, uint32_t step, uint32_t lane_bytes, uint32_t lds_addr, bool once) {
+  if (once) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds_dma16_s_nt(base + step * i, lane_bytes, lds_addr + i * 1024);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds_dma16_s(base + step * i, lane_bytes, lds_addr + i * 1024);
+  }
 }
 
 template <typename T, int D>
 __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sick,
                                         uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
-  const Args& a = arguments();
   using MF = mfma32<T>;
   using TL = KeyTile<D>;
   constexpr int NKC = D / 16, NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF;
   static_assert(HALF >= 1, "two waves copy a sub-block");
-  const uint16_t* q = static_cast<const uint16_t*>(a.q);
-  const uint16_t* kc = static_cast<const uint16_t*>(a.k);
-  const uint16_t* vc = static_cast<const uint16_t*>(a.v);
-  const int32_t* table = a.table + (int64_t)p.seq * a.max_blocks;
+  const Args& a = arguments();
   const int j = lane & 31, hh = lane >> 5;
   const int row = p.row0 + w * 32 + j;
   const bool busy = p.row0 + w * 32 < p.rows;  // (a wave without rows copies and waits with the others)
   const int node = min(row, p.rows - 1) / a.group, g = min(row, p.rows - 1) - node * a.group;
-  const int subs = (p.ctx + kBS - 1) / kBS;
 
-  // This wave copies half of sub-block cb of every tile.  Lane l of the window holds the entry of tile
-  // wb + l: (physical block << bs_shift) | sub-block within it; past the end the last sub-block's.
+  // This wave copies half of sub-block cb of every tile.  Lane l of the window holds where that of tile wb + l lies in
+  // the caches, in bytes; past the end the last sub-block.
   const int cb = w >> 1, cp = w & 1;
-  int wb = p.kt0, win;
+  int wb = p.kt0;
+  uint32_t win_lo, win_hi;
   auto fill = [&]() {
-    const int sb = min(2 * (wb + lane) + cb, subs - 1);
-    win = (table[sb >> a.bs_shift] << a.bs_shift) | (sb & ((1 << a.bs_shift) - 1));
+    const Args& a = arguments();
+    const int subs = (p.ctx + kBS - 1) / kBS, sb = min(2 * (wb + lane) + cb, subs - 1);
+    const int64_t block = a.table[(int64_t)p.seq * a.max_blocks + (sb >> a.bs_shift)];
+    const int64_t at = 2 * (block * a.kv_stride + ((int64_t)(p.kvh << a.bs_shift) + (sb & ((1 << a.bs_shift) - 1))) * (kBS * D));
+    win_lo = (uint32_t)at;
+    win_hi = (uint32_t)((uint64_t)at >> 32);
   };
   fill();
-  int masks_from = max(p.kt0, p.prior / kTileKeys);
-  if (masks_from < p.kt1) fill_masks(p, node, masks_from, w * 32 + j, hh, masks);
   uint4 qb[NKC];
   {
-    const uint4* qr = reinterpret_cast<const uint4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D);
+    const uint4* qr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                     ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D);
 #pragma unroll
     for (int i = 0; i < NKC; ++i) qb[i] = qr[2 * i + hh];
-    // scale_log2 > 0 here: the host passes its magnitude (1 for a scale of 0) and what becomes of q.
-    const uint32_t flip = a.q_sign & 0x80008000u, on = a.q_sign & 1 ? 0xffffffffu : 0u;
-#pragma unroll
-    for (int i = 0; i < NKC; ++i)
-      qb[i] = make_uint4((qb[i].x ^ flip) & on, (qb[i].y ^ flip) & on, (qb[i].z ^ flip) & on, (qb[i].w ^ flip) & on);
   }
+  int masks_from = max(p.kt0, p.prior / kTileKeys);
+  if (masks_from < p.kt1) fill_masks(p, node, masks_from, w * 32 + j, hh, masks);
   // K: copy n of the sub-block takes its chunks 4 n .. 4 n + 3, V: 1024 / (2 D) of its rows; from copy to copy a
   // lane's place moves by the same bytes.
   const uint32_t k_off = (uint32_t)(2 * ((lane & 15) * D + 8 * (4 * cp * HALF + (lane >> 4))));
@@ -506,18 +508,14 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
   static_assert(VROWS % 4 == 0, "copies of V that swizzle alike");
   const int v_key = cp * HALF * VROWS + lane / TL::VCH;
   const uint32_t v_off = (uint32_t)(2 * (v_key * D + 8 * TL::vchunk(v_key, lane % TL::VCH)));
-  const uint32_t lds_base = (uint32_t)(uintptr_t)((RG_LDS char*)lds);
-  const int64_t head = (int64_t)p.kvh * (kBS << a.bs_shift) * D;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)((RG_LDS char*)lds) + cb * (TL::KB / 2) + cp * HALF * 1024;
+  const char* const kc = static_cast<const char*>(a.k);
+  const char* const vc = static_cast<const char*>(a.v);
   auto issue = [&](int kt, int st) {
-    const int e = __builtin_amdgcn_readlane(win, kt - wb);
-    const int64_t off = (int64_t)(e >> a.bs_shift) * a.kv_stride + head + (int64_t)(e & ((1 << a.bs_shift) - 1)) * (kBS * D);
-    const char* kb = reinterpret_cast<const char*>(kc + off);
-    const char* vb = reinterpret_cast<const char*>(vc + off);
-    const uint32_t at = lds_base + st * TL::BYTES + cb * (TL::KB / 2) + cp * HALF * 1024;
-#pragma unroll
-    for (int i = 0; i < HALF; ++i) copy(kb + 64 * i, k_off, at + i * 1024, p.once);
-#pragma unroll
-    for (int i = 0; i < HALF; ++i) copy(vb + 1024 * i, v_off, at + TL::KB + i * 1024, p.once);
+    const int64_t at = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)win_hi, kt - wb) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)win_lo, kt - wb));
+    copy<HALF>(kc + at, 64, k_off, lds_at + st * TL::BYTES, p.once);
+    copy<HALF>(vc + at, 1024, v_off, lds_at + st * TL::BYTES + TL::KB, p.once);
   };
 
   f32x16_t o[NDB];
@@ -528,6 +526,7 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
   float m_run = -INFINITY, l_run = 0.f;
   float ref = -INFINITY;    // reference(m_run)
   float m_thr = -INFINITY;  // m_run + kSlack in raw score units, so a tile's test needs no multiply
+  const float scale = a.scale_log2;
   const int xor32 = (lane ^ 32) << 2;
   const int k_lane = (j >> 4) * (TL::KB / 2) + hh * 256 + (j & 15) * 16;
   const int grp = lane >> 4, e_row = (lane >> 2) & 3, qq = lane & 3;
@@ -579,14 +578,14 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
     for (int v = 1; v < 16; ++v) tmax = fmaxf(tmax, c[v]);
     if (__ballot(tmax > m_thr)) {
       const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(xor32, __float_as_int(tmax)));
-      const float both = fmaxf(tmax, other) * a.scale_log2;
+      const float both = fmaxf(tmax, other) * scale;
       const bool moves = both > m_run + kSlack;
       const float m_new = moves ? both : m_run;
       const float ref_new = reference<T>(m_new);
       const float alpha = moves ? fast_exp2(ref - ref_new) : 1.f;
       m_run = m_new;
       ref = ref_new;
-      m_thr = (m_run + kSlack) / a.scale_log2;
+      m_thr = (m_run + kSlack) / scale;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -600,7 +599,7 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
     uint32_t pk[8];
 #pragma unroll
     for (int v = 0; v < 16; v += 2)
-      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], a.scale_log2, -sub)), fast_exp2(fmaf(c[v + 1], a.scale_log2, -sub)));
+      pk[v / 2] = pack2<T>(fast_exp2(fmaf(c[v], scale, -sub)), fast_exp2(fmaf(c[v + 1], scale, -sub)));
     float s0 = pair_sum<T>(pk[0], l_run), s1 = pair_sum<T>(pk[1], 0.f);
 #pragma unroll
     for (int i = 2; i < 8; i += 2) {
@@ -638,35 +637,65 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
     tile_barrier();
   };
 
-  // The window and Q have landed (the builtin, which the compiler's own counting follows: behind an asm
+  static_assert(TL::STAGES == 3 && COPIES < 16, "one tile newer than the awaited one; low bits of vmcnt");
+  issue(p.kt0, 0);
+  if (p.kt0 + 1 < p.kt1) issue(p.kt0 + 1, 1);
+  // Q, the masks and the first tiles have landed (the builtin, which the compiler's own counting follows: behind an asm
   // wait it would wait for Q again in every tile, and with it for every copy in flight).
   __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0)
+  // scale_log2 > 0 here: the host passes its magnitude (1 for a scale of 0) and what becomes of q.
+  {
+    const uint32_t flip = a.q_sign & 0x80008000u, on = a.q_sign & 1 ? 0xffffffffu : 0u;
 #pragma unroll
-  for (int i = 0; i < TL::STAGES - 1; ++i)
-    if (p.kt0 + i < p.kt1) issue(p.kt0 + i, i);
-  static_assert(TL::STAGES == 3 && COPIES < 16, "one tile newer than the awaited one; low bits of vmcnt");
-  int st = 0;
-#pragma clang loop unroll(disable)
-  for (int kt = p.kt0; kt < p.kt1; ++kt) {
-    // Tile kt has landed (a newer one may not have), for every wave; all are done with tile kt - 1, whose
-    // stage takes tile kt + STAGES - 1.
+    for (int i = 0; i < NKC; ++i)
+      qb[i] = make_uint4((qb[i].x ^ flip) & on, (qb[i].y ^ flip) & on, (qb[i].z ^ flip) & on, (qb[i].w ^ flip) & on);
+  }
+  // Tile kt has landed (a newer one may not have), for every wave; all are done with tile kt - 1, whose stage takes
+  // tile kt + STAGES - 1.  Returns whether there is one.
+  auto ready = [&](int kt) __attribute__((always_inline)) {
     asm volatile("" ::: "memory");
     if (kt + 1 < p.kt1) __builtin_amdgcn_s_waitcnt(COPIES | 0x70 | 0xF00);
     else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
     tile_barrier();
-    const int next = kt + TL::STAGES - 1, next_st = st == 0 ? TL::STAGES - 1 : st - 1;
+    const int next = kt + TL::STAGES - 1;
     if (next - wb >= 64) {
       wb = next;
       fill();
       __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
     }
-    const bool masked = (kt + 1) * kTileKeys > p.prior;
+    return next < p.kt1;
+  };
+  int kt = p.kt0;
+  // The tiles that every row attends to, as far as STAGES of them follow each other.
+  const int whole = min(p.kt1, p.prior / kTileKeys);
+  for (; kt + TL::STAGES <= whole; kt += TL::STAGES) {
+#pragma unroll
+    for (int st = 0; st < TL::STAGES; ++st) {
+      const bool more = ready(kt + st);
+      const char* tile = lds + st * TL::BYTES;
+      const int next_st = st == 0 ? TL::STAGES - 1 : st - 1;
+      if (busy) {
+        __builtin_amdgcn_s_setprio(1);
+        const f32x16_t c = scores(tile);
+        if (more) issue(kt + st + TL::STAGES - 1, next_st);  // while the QK MFMAs run
+        finish(c, tile);
+      } else if (more) {
+        issue(kt + st + TL::STAGES - 1, next_st);
+      }
+    }
+  }
+  int st = 0;
+#pragma clang loop unroll(disable)
+  for (; kt < p.kt1; ++kt) {
+    const bool more = ready(kt);
+    const bool masked = kt >= whole;
     if (masked) clean(kt, st);
     const char* tile = lds + st * TL::BYTES;
+    const int next_st = st == 0 ? TL::STAGES - 1 : st - 1;
     if (busy) {
       __builtin_amdgcn_s_setprio(1);
       f32x16_t c = scores(tile);
-      if (next < p.kt1) issue(next, next_st);  // while the QK MFMAs run
+      if (more) issue(kt + TL::STAGES - 1, next_st);
       uint32_t mine = 0;
       if (masked) {
         if (kt - masks_from >= kMaskTiles) fill_masks(p, node, masks_from = kt, w * 32 + j, hh, masks);
@@ -677,8 +706,8 @@ __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sic
       }
       finish(c, tile);
       if (masked && sick[sick_word(p, kt)] != 0) add_not_finite<T, D>(p, kt, sick[sick_word(p, kt)], mine, hh, o);
-    } else if (next < p.kt1) {
-      issue(next, next_st);
+    } else if (more) {
+      issue(kt + TL::STAGES - 1, next_st);
     }
     st = st == TL::STAGES - 1 ? 0 : st + 1;
   }
@@ -907,8 +936,9 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
     p.first = sp.t.first;
     p.ctx = sp.ctx;
     p.prior = max(sp.ctx - sp.t.len, 0);
-    p.kt0 = (int)((int64_t)sp.tiles * cut / n);
-    p.kt1 = (int)((int64_t)sp.tiles * (cut + 1) / n);
+    const int each = sp.tiles / n, longer = sp.tiles - each * n;  // the first few are a tile longer
+    p.kt0 = each * cut + min(cut, longer);
+    p.kt1 = each * (cut + 1) + min(cut + 1, longer);
     p.slot = n > 1 ? base + local : -1;
     p.once = sp.row_tiles == 1;
     if (local == 0 && threadIdx.x == 0) a.cuts[s] = make_int2(base, n);
