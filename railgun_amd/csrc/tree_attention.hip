@@ -85,7 +85,7 @@ struct TreeArgs {
   int2* cuts;        // [num_seqs]: the first of its parts, pieces of a segment
   uint32_t q_sign;   // bit 0: q is taken (else zeros, a scale of 0), bits 15 and 31: negated (a negative scale)
   int32_t group, bs_shift;
-  int32_t slots;     // pieces that are at work together
+  int32_t slots, slots_full;  // pieces that a batch is cut into: as many as are at work together if they are long
   int32_t least;     // key tiles of a piece that is worth its partials
 };
 
@@ -191,16 +191,19 @@ __device__ __forceinline__ int wave_top(int v) {
   return v;
 }
 
-// Pieces that a batch of so many segments is cut into at most: a round of the chip's, or where the segments alone come
-// near that or past it, half a round more than they are.  At most `slots` of them are parts of a segment: n cuts make
-// 2 n parts at most.
+// Pieces that a batch of so many segments is cut into at most: `slots`, or where the segments alone come near that or
+// past it, half of it more than they are.  As many at most are parts of a segment: n cuts make 2 n parts.
 __host__ __device__ inline int64_t most_pieces(int64_t segments, int64_t slots) {
   return segments <= slots * 3 / 4 ? slots : segments + slots / 2;
 }
+
+// Lengths of pieces, by quarters of the longest: where no two workgroups read the same keys, the long ones come first.
+constexpr int kLengths = 4;
+
 struct CutScratch {
   uint32_t spans[kTreeThreads];  // tiles, row tiles of up to so many sequences
   int32_t sums[kTreeWaves][64];
-  int32_t wave_sum[2][kTreeWaves];
+  int32_t wave_sum[1 + kLengths][kTreeWaves];
   // The workgroup's: its sequence; of that, the piece, pieces of a segment, the first part.
   int32_t seq, local, pieces, base;
   Span span;
@@ -216,25 +219,37 @@ __device__ __forceinline__ int ceil_quotient(int x, int d, float by) {
 
 // Key tiles to a piece: the least length (a.least and more) that makes no more pieces than most_pieces.  Between
 // total / pieces and total / (pieces - segments), where every segment's last piece may be short, a lane each tries 64
-// lengths; the waves share the sequences.  Returns that length (0 if there is nothing to do) and the number of pieces.
+// lengths; the waves share the sequences.
 // `own`: the thread's sequence of the first kTreeThreads.
-__device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, const Span& own, int w, int lane) {
-  int tiles = 0, segments = 0, longest = 1;  // tiles: of all segments
+// Key tiles of a piece from which on the chip is filled with them; of shorter ones two go to a CU, whose start and
+// partials cost less than a third hides.  Measured (us, two / three a CU; bf16, 32 / 8 heads of 128): 4 sequences of
+// 32,768 with 128 nodes, 160 to 250 tiles a piece 291 / 279; 17 of up to 3,900 with up to 37 (fp16, 28 / 4 heads), 4 to 15
+// tiles 39 / 45.
+constexpr int kLongPiece = 24;
+struct Cut {
+  int tiles, pieces;  // a piece's length; how many there are
+  bool alone;         // no sequence has more than one row tile
+};
+__device__ __forceinline__ Cut piece_tiles(const Args& a, CutScratch& sh, const Span& own, int w, int lane) {
+  int tiles = 0, segments = 0, longest = 1, widest = 0;  // tiles: of all segments
   for (int s = threadIdx.x; s < a.num_seqs; s += kTreeThreads) {
     const Span p = s < kTreeThreads ? own : span_of(a, s);
     const int n = p.row_tiles * a.num_kv_heads;
     tiles += n * p.tiles;
     segments += n;
     if (n > 0) longest = max(longest, p.tiles);
+    widest = max(widest, p.row_tiles);
     if (s < kTreeThreads) sh.spans[s] = (uint32_t)p.row_tiles << 24 | (uint32_t)p.tiles;
   }
   tiles = wave_scan(tiles);
   segments = wave_scan(segments);
   longest = wave_top(longest);
+  widest = wave_top(widest);
   if (lane == 63) {
     sh.sums[w][0] = tiles;
     sh.sums[w][1] = segments;
     sh.sums[w][2] = longest;
+    sh.sums[w][3] = widest;
   }
   __syncthreads();
   tiles = segments = 0;
@@ -243,11 +258,13 @@ __device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, const
     tiles += sh.sums[i][0];
     segments += sh.sums[i][1];
     longest = max(longest, sh.sums[i][2]);
+    widest = max(widest, sh.sums[i][3]);
   }
-  if (segments == 0) return make_int2(0, 0);
-  const int most = (int)most_pieces(segments, a.slots);
+  Cut cut{longest, segments, widest == 1};
+  if (segments == 0) return cut;
+  const int most = (int)most_pieces(segments, tiles >= kLongPiece * a.slots_full ? a.slots_full : a.slots);
   const int lo = max(a.least, tiles / most), hi = max(lo, min(longest, tiles / (most - segments) + 1));
-  if (lo >= longest) return make_int2(longest, segments);
+  if (lo >= longest) return cut;
   const int mine = lo + (hi - lo) * lane / 63;
   const float by = __builtin_amdgcn_rcpf((float)mine);
   int pieces = 0;
@@ -269,37 +286,49 @@ __device__ __forceinline__ int2 piece_tiles(const Args& a, CutScratch& sh, const
 #pragma unroll
   for (int i = 0; i < kTreeWaves; ++i) pieces += sh.sums[i][lane];
   const int first = __builtin_ctzll(__ballot(pieces <= most));  // (hi fits)
-  return make_int2(__builtin_amdgcn_readlane(mine, first), __builtin_amdgcn_readlane(pieces, first));
+  cut.tiles = __builtin_amdgcn_readlane(mine, first);
+  cut.pieces = __builtin_amdgcn_readlane(pieces, first);
+  return cut;
 }
 
 // The piece that workgroup `me` has: its sequence, its place among that one's, and the cuts of those.
-__device__ __forceinline__ void find_piece(const Args& a, CutScratch& sh, const Span& own, int tiles, int me, int w,
+__device__ __forceinline__ void find_piece(const Args& a, CutScratch& sh, const Span& own, const Cut& cut, int me, int w,
                                            int lane) {
+  // (A batch of more sequences has enough pieces for their order not to matter.)
+  const bool sorted = cut.alone && a.num_seqs <= kTreeThreads;
   int before = 0, parts_before = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += kTreeThreads) {
     const int s = s0 + threadIdx.x;
-    int n = 0, cuts = 0;
+    int n = 0, cuts = 0, length = 0;
     Span p = own;
     if (s < a.num_seqs) {
       if (s0 > 0) p = span_of(a, s);
-      cuts = (p.tiles + tiles - 1) / tiles;
+      cuts = (p.tiles + cut.tiles - 1) / cut.tiles;
       n = p.row_tiles * a.num_kv_heads * cuts;
+      if (sorted) length = min(kLengths - 1, kLengths - kLengths * ((p.tiles + cuts - 1) / cuts) / cut.tiles);
     }
-    const int parts = cuts > 1 ? n : 0;
-    const int upto = wave_scan(n), parts_upto = wave_scan(parts);
-    if (lane == 63) {
-      sh.wave_sum[0][w] = upto;
-      sh.wave_sum[1][w] = parts_upto;
-    }
-    __syncthreads();
-    int start = before + upto - n, base = parts_before + parts_upto - parts;
+    const int parts = cuts > 1 ? n : 0, parts_upto = wave_scan(parts);
+    int upto[kLengths];
 #pragma unroll
-    for (int i = 0; i < kTreeWaves; ++i) {
-      start += i < w ? sh.wave_sum[0][i] : 0;
-      base += i < w ? sh.wave_sum[1][i] : 0;
-      before += sh.wave_sum[0][i];
-      parts_before += sh.wave_sum[1][i];
+    for (int i = 0; i < kLengths; ++i) {
+      upto[i] = wave_scan(length == i ? n : 0);
+      if (lane == 63) sh.wave_sum[i][w] = upto[i];
     }
+    if (lane == 63) sh.wave_sum[kLengths][w] = parts_upto;
+    __syncthreads();
+    int start = before - n, base = parts_before + parts_upto - parts;
+#pragma unroll
+    for (int k = 0; k < kTreeWaves; ++k) {
+      base += k < w ? sh.wave_sum[kLengths][k] : 0;
+      parts_before += sh.wave_sum[kLengths][k];
+#pragma unroll
+      for (int i = 0; i < kLengths; ++i) {
+        start += i < length || (i == length && k < w) ? sh.wave_sum[i][k] : 0;
+        before += sh.wave_sum[i][k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kLengths; ++i) start += i == length ? upto[i] : 0;
     if (start <= me && me - start < n) {
       sh.seq = s;
       sh.local = me - start;
@@ -894,8 +923,10 @@ constexpr int ring_bytes() {
   if constexpr (std::is_same_v<T, f32_t>) return KeyTileF32<D>::STAGES * KeyTileF32<D>::BYTES;
   else return KeyTile<D>::STAGES * KeyTile<D>::BYTES;
 }
+// Workgroups to a CU: what their registers allow (168 a wave for three) and the rings, 64 KB in fp32 at head_dim 128.
+constexpr int pieces_per_cu(int32_t dtype, int D) { return dtype == RG_DTYPE_F32 ? 2 : D == 128 ? 3 : 4; }
 template <typename T, int D>
-constexpr int groups_per_cu() { return std::is_same_v<T, f32_t> ? 2 : D == 128 ? 3 : 4; }
+constexpr int groups_per_cu() { return pieces_per_cu(std::is_same_v<T, f32_t> ? RG_DTYPE_F32 : RG_DTYPE_BF16, D); }
 
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_kernel(TreeArgs) {
@@ -912,11 +943,13 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
     static_assert(sizeof(CutScratch) <= sizeof(ring), "the cuts' scratch lies in the ring");
     Span own{};
     if (threadIdx.x < (unsigned)a.num_seqs) own = span_of(a, threadIdx.x);
-    const int2 cut_to = piece_tiles(a, sh, own, w, lane);
-    // Neighbours go to the same XCD (workgroups are dealt to the eight in turn).
-    const int per = (cut_to.y + 7) / 8, me = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if ((int)(blockIdx.x / 8) >= per || me >= cut_to.y) return;
-    find_piece(a, sh, own, cut_to.x, me, w, lane);
+    const Cut cut_to = piece_tiles(a, sh, own, w, lane);
+    // Workgroups are dealt to the XCDs in turn.  The row tiles of the same keys go to the same one; where there are none,
+    // the order of the pieces is that of their dispatch.
+    const int per = (cut_to.pieces + 7) / 8, on_xcd = (int)blockIdx.x / 8;
+    const int me = cut_to.alone ? (int)blockIdx.x : on_xcd < per ? (int)(blockIdx.x % 8) * per + on_xcd : cut_to.pieces;
+    if (me >= cut_to.pieces) return;
+    find_piece(a, sh, own, cut_to, me, w, lane);
     const int s = __builtin_amdgcn_readfirstlane(sh.seq);
     const int local = __builtin_amdgcn_readfirstlane(sh.local), n = __builtin_amdgcn_readfirstlane(sh.pieces);
     const int base = __builtin_amdgcn_readfirstlane(sh.base);
@@ -958,88 +991,105 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
   }
 }
 
-// The rows of a cut segment: D / 4 lanes have 4 dims each of a row, a wave kMergeRows of them, the AHEAD next pieces'
-// in flight.
+// The rows of a cut segment: D / 4 lanes have 4 dims each of a row, a wave N times 256 / D rows, the AHEAD next pieces'
+// in flight: a batch of few segments has them in many pieces (N = 1, AHEAD = 8), one of many in two or three (4, 2).
 constexpr int kMergeWaves = 4;
 template <int D> constexpr int merge_rows() { return 256 / D; }
-template <typename T, int D>
+template <typename T, int D, int N, int AHEAD>
 __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a) {
   using S = typename elem<T>::storage;
-  constexpr int LANES = D / 4, ROWS = merge_rows<D>(), AHEAD = 8;
+  constexpr int LANES = D / 4, ROWS = merge_rows<D>();
   const int s = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63;
-  const int row0 = ((int)blockIdx.x * kMergeWaves + (threadIdx.x >> 6)) * ROWS;
+  const int row0 = ((int)blockIdx.x * kMergeWaves + (threadIdx.x >> 6)) * (N * ROWS);
   const int2 cuts = a.cuts[s];  // (not used where the sequence has no tree)
   const Span sp = span_of(arguments(), s);
   const int rows = sp.t.nodes * a.group, n = cuts.y;
   if (row0 >= rows || n <= 1) return;
   const int rt = row0 / kRows, d = lane % LANES * 4;
-  const int row = row0 + lane / LANES, in = min(row, rows - 1) - rt * kRows;  // (a row tile's rows are written so far)
-  static_assert(kRows % ROWS == 0, "a wave's rows lie in one row tile");
-  const int64_t first = (int64_t)(cuts.x + kvh * n * sp.row_tiles + rt) * kRows + in;
+  static_assert(kRows % (N * ROWS) == 0, "a wave's rows lie in one row tile");
+  const int64_t first = (int64_t)(cuts.x + kvh * n * sp.row_tiles + rt) * kRows - rt * kRows;
   const int64_t step = (int64_t)sp.row_tiles * kRows;
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  int row[N];
+  float m[N], l[N];
+  float4 acc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    row[k] = min(row0 + k * ROWS + lane / LANES, rows - 1);  // (a row tile's rows are written so far)
+    m[k] = -INFINITY;
+    l[k] = 0.f;
+    acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   for (int i = 0; i < n; i += AHEAD) {
-    float2 ml[AHEAD];
-    float4 v[AHEAD];
+    float2 ml[AHEAD][N];
+    float4 v[AHEAD][N];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int64_t at = first + min(i + u, n - 1) * step;
-      ml[u] = *reinterpret_cast<const float2*>(a.ml + 2 * at);
-      v[u] = *reinterpret_cast<const float4*>(a.acc + at * D + d);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        ml[u][k] = *reinterpret_cast<const float2*>(a.ml + 2 * (at + row[k]));
+        v[u][k] = *reinterpret_cast<const float4*>(a.acc + (at + row[k]) * D + d);
+      }
     }
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      // (A piece without keys for the row has m = -inf and nothing to add; one whose scores are all NaN has m = -inf too.)
-      const bool counts = i + u < n && !(ml[u].x == -INFINITY && ml[u].y == 0.f);
-      const float mn = counts ? fmaxf(m, ml[u].x) : m;
-      const float fo = m == mn ? 1.f : exp2f(m - mn), fq = !counts ? 0.f : ml[u].x == mn ? 1.f : exp2f(ml[u].x - mn);
-      l = l * fo + (counts ? ml[u].y * fq : 0.f);
-      acc.x = acc.x * fo + (counts ? v[u].x * fq : 0.f);
-      acc.y = acc.y * fo + (counts ? v[u].y * fq : 0.f);
-      acc.z = acc.z * fo + (counts ? v[u].z * fq : 0.f);
-      acc.w = acc.w * fo + (counts ? v[u].w * fq : 0.f);
-      m = mn;
-    }
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        // (A piece without keys for the row has m = -inf and nothing to add; one whose scores are all NaN has m = -inf
+        // too.)
+        const float2 x = ml[u][k];
+        const bool counts = i + u < n && !(x.x == -INFINITY && x.y == 0.f);
+        const float mn = counts ? fmaxf(m[k], x.x) : m[k];
+        const float fo = m[k] == mn ? 1.f : exp2f(m[k] - mn), fq = !counts ? 0.f : x.x == mn ? 1.f : exp2f(x.x - mn);
+        l[k] = l[k] * fo + (counts ? x.y * fq : 0.f);
+        acc[k].x = acc[k].x * fo + (counts ? v[u][k].x * fq : 0.f);
+        acc[k].y = acc[k].y * fo + (counts ? v[u][k].y * fq : 0.f);
+        acc[k].z = acc[k].z * fo + (counts ? v[u][k].z * fq : 0.f);
+        acc[k].w = acc[k].w * fo + (counts ? v[u][k].w * fq : 0.f);
+        m[k] = mn;
+      }
   }
-  if (row >= rows) return;
-  const int node = row / a.group, g = row - node * a.group;
-  S* out = static_cast<S*>(a.out) + ((int64_t)(sp.t.first + node) * a.num_heads + kvh * a.group + g) * D + d;
-  const float inv = l != 0.f ? 1.f / l : 1.f;
-  const float x0 = acc.x * inv, x1 = acc.y * inv, x2 = acc.z * inv, x3 = acc.w * inv;
-  if constexpr (std::is_same_v<T, f32_t>) *reinterpret_cast<float4*>(out) = make_float4(x0, x1, x2, x3);
-  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x0, x1), pack2<T>(x2, x3));
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (row0 + k * ROWS + lane / LANES >= rows) continue;
+    const int node = row[k] / a.group, g = row[k] - node * a.group;
+    S* out = static_cast<S*>(a.out) + ((int64_t)(sp.t.first + node) * a.num_heads + kvh * a.group + g) * D + d;
+    const float inv = l[k] != 0.f ? 1.f / l[k] : 1.f;
+    const float x0 = acc[k].x * inv, x1 = acc[k].y * inv, x2 = acc[k].z * inv, x3 = acc[k].w * inv;
+    if constexpr (std::is_same_v<T, f32_t>) *reinterpret_cast<float4*>(out) = make_float4(x0, x1, x2, x3);
+    else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x0, x1), pack2<T>(x2, x3));
+  }
 }
 
 // ---------------------------------------------------------------- the plan --
 
-#ifndef RG_TREE_WPC
-#define RG_TREE_WPC 2
-#endif
-#ifndef RG_TREE_LEAST
-#define RG_TREE_LEAST 8
-#endif
-constexpr int kPiecesPerCu = RG_TREE_WPC;
+// Key tiles of a piece that is worth its partials, 16 bits and fp32 (whose tiles take 16 times the time).
+constexpr int kLeast = 8, kLeastF32 = 1;
 
 struct TreePlan {
-  int32_t slots, groups, tiles;  // tiles: of the longest sequence
+  int32_t slots, slots_full, groups, tiles;  // tiles: of the longest sequence
+  int32_t cut_in;                                // pieces of a segment that the merge is made for
   size_t ml_at, cuts_at, bytes;
 };
-TreePlan plan_tree(int32_t num_seqs, int32_t max_nodes, int32_t H, int32_t Hkv, int32_t D, int32_t bs, int32_t MB) {
+TreePlan plan_tree(int32_t num_seqs, int32_t max_nodes, int32_t H, int32_t Hkv, int32_t D, int32_t bs, int32_t MB,
+                   int32_t dtype) {
   TreePlan p{};
   const int64_t row_tiles = ceil_div((int64_t)max_nodes * (H / Hkv), kRows), segments = num_seqs * row_tiles * Hkv;
   const int64_t tiles = std::max<int64_t>(1, ceil_div((int64_t)MB * bs, kTileKeys));
   p.tiles = (int32_t)std::min<int64_t>(tiles, INT32_MAX);
-  p.slots = device_cu_count() * kPiecesPerCu;
-  const int64_t pieces = most_pieces(segments, p.slots);
+  p.slots = device_cu_count() * 2;
+  p.slots_full = device_cu_count() * pieces_per_cu(dtype, D);
+  // (The kernel goes by either.)
+  const int64_t pieces = std::max(most_pieces(segments, p.slots), most_pieces(segments, p.slots_full));
   // (What the product does not take runs on the generic kernel.  The cuts count in 32 bits, a sequence's tiles in 22,
   // its row tiles in 8.)
   if ((D != 64 && D != 128) || block_shift(bs) < 0 || tiles >= 1 << 22 || row_tiles > 255 ||
       (double)segments * tiles > INT32_MAX || pieces > INT32_MAX - 8) {
     return p;
   }
+  p.cut_in = (int32_t)std::min<int64_t>(p.slots_full / segments, 8);
   p.groups = (int32_t)(ceil_div(std::min(pieces, segments * tiles), 8) * 8);
-  const int64_t parts = std::min<int64_t>(p.slots, segments * tiles);
+  const int64_t parts = std::min<int64_t>(std::max(p.slots, p.slots_full), segments * tiles);
   p.ml_at = align_up((size_t)parts * kRows * D * 4, 256);
   p.cuts_at = p.ml_at + align_up((size_t)parts * kRows * 8, 256);
   p.bytes = p.cuts_at + align_up((size_t)num_seqs * 8, 256);
@@ -1050,9 +1100,13 @@ template <typename T, int D>
 void launch_product(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
   hipLaunchKernelGGL((tree_kernel<T, D>), dim3((unsigned)p.groups), dim3(kTreeThreads), 0, s, a);
   if (p.tiles <= a.least) return;  // nothing is cut
-  const unsigned rows = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, merge_rows<D>() * kMergeWaves);
-  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3(rows, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs),
-                     dim3(64 * kMergeWaves), 0, s, a);
+  auto merge = [&](auto kernel, int n) {
+    const unsigned rows = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, n * merge_rows<D>() * kMergeWaves);
+    hipLaunchKernelGGL(kernel, dim3(rows, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), dim3(64 * kMergeWaves), 0, s, a);
+  };
+  if (p.cut_in >= 8) merge(tree_merge_kernel<T, D, 1, 8>, 1);
+  else if (p.cut_in >= 2) merge(tree_merge_kernel<T, D, 2, 4>, 2);
+  else merge(tree_merge_kernel<T, D, 4, 2>, 4);
 }
 
 }  // namespace
@@ -1061,7 +1115,7 @@ int probe_tree_attention_kernels() {
   hipFuncAttributes at;
   if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_generic_kernel<bf16_t>)) != hipSuccess ||
       hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_kernel<bf16_t, 128>)) != hipSuccess ||
-      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_merge_kernel<bf16_t, 128>)) != hipSuccess) {
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_merge_kernel<bf16_t, 128, 1, 8>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the tree attention kernels: %s", hipGetErrorString(hipGetLastError()));
   }
   return RG_OK;
@@ -1079,7 +1133,9 @@ extern "C" size_t rg_paged_attention_tree_workspace_bytes(int32_t num_seqs, int3
       (int64_t)max_blocks_per_seq * block_size > INT32_MAX - 65536 || num_seqs > 65535 || num_heads > 65535) {
     return 0;
   }
-  return plan_tree(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq).bytes;
+  // (A batch of 16 bits is cut into more pieces.)
+  return plan_tree(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, RG_DTYPE_BF16)
+      .bytes;
 }
 
 extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache, const void* value_cache,
@@ -1148,7 +1204,7 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
   a.kv_stride = kv_block_stride ? kv_block_stride : block;
   if (need > 0 && aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(output) &&
       a.kv_stride * dtype_bytes(dtype) % 16 == 0) {
-    const TreePlan p = plan_tree(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq);
+    const TreePlan p = plan_tree(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, dtype);
     char* const ws = static_cast<char*>(workspace);
     a.acc = reinterpret_cast<float*>(ws);
     a.ml = reinterpret_cast<float*>(ws + p.ml_at);
@@ -1159,7 +1215,8 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
     a.group = num_heads / num_kv_heads;
     a.bs_shift = block_shift(block_size);
     a.slots = p.slots;
-    a.least = dtype == RG_DTYPE_F32 ? 1 : RG_TREE_LEAST;
+    a.slots_full = p.slots_full;
+    a.least = dtype == RG_DTYPE_F32 ? kLeastF32 : kLeast;
     return dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
       if (head_dim == 128) launch_product<T, 128>(a, p, as_stream(stream));

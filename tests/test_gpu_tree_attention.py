@@ -78,6 +78,15 @@ def test_batches(device, kernels, batch):
     TreeBatch(device, prior, trees(rng, sizes), heads=4, hkv=2, seed=batch, wide=3).check(kernels)
 
 
+@pytest.mark.parametrize("long,short,d", [(32, 38, 128), (48, 64, 64), (20, 75, 128)])
+def test_segments_near_a_round(device, kernels, long, short, d):
+    """Segments that are nearly as many as the workgroups that are at work together, some of them cut: more pieces
+    than those."""
+    rng = np.random.default_rng(long)
+    prior = rng.permutation([20 * 32 - 3] * long + [12 * 32 - 3] * short)
+    TreeBatch(device, prior, trees(rng, [3] * (long + short)), heads=8, hkv=8, d=d, seed=long).check(kernels)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_any_mask(device, kernels, dtype):
     """Masks that are no tree's: dense, empty rows (zeros where nothing lies before), later nodes seen, oneself
