@@ -34,16 +34,30 @@ struct LayoutArgs {
 };
 
 __global__ __launch_bounds__(kLayoutThreads) void tree_layout_kernel(LayoutArgs a) {
-  __shared__ uint32_t seen[kMaxTreeNodes * kLayoutWords];
+  __shared__ uint4 seen[kMaxTreeNodes * kLayoutWords / 4];
   __shared__ int16_t up[2][kMaxTreeNodes], depth[2][kMaxTreeNodes];
+  static_assert(kLayoutWords == 8, "two 16-byte pieces to a node");
   const int s = blockIdx.x, w0 = blockIdx.y * kLayoutWords, tid = threadIdx.x;
   const Tree t = tree_of(a.cu, s, a.num_nodes, a.max_nodes);
   const int words = min(kLayoutWords, a.mask_words - w0);
+  const int ctx = max(0, min(a.context_lens[s], a.max_blocks * a.block_size)), prior = max(ctx - t.len, 0);
+  const int root = a.text ? a.text[s] : prior;
   for (int j = tid; j < t.nodes; j += kLayoutThreads) {
     const int p = a.parents[t.first + j];
+    if (blockIdx.y == 0) {
+      const int at = prior + j;
+      int slot = -1;
+      if (at < ctx) {
+        slot = a.table[(int64_t)s * a.max_blocks + at / a.block_size] * a.block_size + at % a.block_size;
+      }
+      a.slots[t.first + j] = slot;
+    }
     up[0][j] = (int16_t)(p >= 0 && p < j ? p : -1);
     depth[0][j] = (int16_t)(p >= 0 && p < j);
-    for (int w = 0; w < words; ++w) seen[j * kLayoutWords + w] = w0 + w == j >> 5 ? 1u << (j & 31) : 0u;
+    const uint32_t bit = 1u << (j & 31);
+    const int w = (j >> 5) - w0;
+    seen[2 * j] = make_uint4(w == 0 ? bit : 0u, w == 1 ? bit : 0u, w == 2 ? bit : 0u, w == 3 ? bit : 0u);
+    seen[2 * j + 1] = make_uint4(w == 4 ? bit : 0u, w == 5 ? bit : 0u, w == 6 ? bit : 0u, w == 7 ? bit : 0u);
   }
   __syncthreads();
   int cur = 0;
@@ -51,32 +65,29 @@ __global__ __launch_bounds__(kLayoutThreads) void tree_layout_kernel(LayoutArgs 
     int more = 0;
     for (int j = tid; j < t.nodes; j += kLayoutThreads) {
       const int p = up[cur][j];
-      const int q = p < 0 ? -1 : up[cur][p];
-      depth[cur ^ 1][j] = (int16_t)(depth[cur][j] + (p < 0 ? 0 : depth[cur][p]));
-      up[cur ^ 1][j] = (int16_t)q;
+      int q = -1, d = depth[cur][j];
       if (p >= 0) {
-        for (int w = 0; w < words; ++w) seen[j * kLayoutWords + w] |= seen[p * kLayoutWords + w];
+        uint4 x = seen[2 * j], y = seen[2 * j + 1];
+        const uint4 u = seen[2 * p], v = seen[2 * p + 1];
+        q = up[cur][p];
+        d += depth[cur][p];
+        x = make_uint4(x.x | u.x, x.y | u.y, x.z | u.z, x.w | u.w);
+        y = make_uint4(y.x | v.x, y.y | v.y, y.z | v.z, y.w | v.w);
+        seen[2 * j] = x;
+        seen[2 * j + 1] = y;
       }
+      depth[cur ^ 1][j] = (int16_t)d;
+      up[cur ^ 1][j] = (int16_t)q;
       more |= q >= 0;
     }
     cur ^= 1;
     if (!__syncthreads_or(more)) break;
   }
-  for (int i = tid; i < t.nodes * words; i += kLayoutThreads) {
-    const int j = i / words, w = i - j * words;
-    a.mask[(int64_t)(t.first + j) * a.mask_words + w0 + w] = (int32_t)seen[j * kLayoutWords + w];
-  }
-  if (blockIdx.y != 0) return;
-  const int ctx = min(a.context_lens[s], a.max_blocks * a.block_size), prior = max(ctx - t.len, 0);
-  const int root = a.text ? a.text[s] : prior;
+  const uint32_t* bits = reinterpret_cast<const uint32_t*>(seen);
   for (int j = tid; j < t.nodes; j += kLayoutThreads) {
-    const int at = prior + j;
-    a.positions[t.first + j] = root + depth[cur][j];
-    int slot = -1;
-    if (at < ctx) {
-      slot = a.table[(int64_t)s * a.max_blocks + at / a.block_size] * a.block_size + at % a.block_size;
-    }
-    a.slots[t.first + j] = slot;
+    int32_t* to = a.mask + (int64_t)(t.first + j) * a.mask_words + w0;
+    for (int w = 0; w < words; ++w) to[w] = (int32_t)bits[j * kLayoutWords + w];
+    if (blockIdx.y == 0) a.positions[t.first + j] = root + depth[cur][j];
   }
 }
 
@@ -88,6 +99,8 @@ __device__ __forceinline__ uint64_t rank_of(float v, uint32_t index) {
   const uint32_t u = __float_as_uint(v + 0.f);  // -0 + 0 = +0
   return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~index;
 }
+// The index in it (nothing above -inf: the first).
+__device__ __forceinline__ int32_t token_of(uint64_t key) { return key ? (int32_t)~(uint32_t)key : 0; }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -124,8 +137,8 @@ template <typename T> struct Piece {
 
 // Workgroup (row, split): the best of one piece of a row of logits.  The row's 16-byte pieces are dealt to the
 // splits; what lies before the first and behind the last goes to the first and the last split.  A thread keeps the
-// largest value and the piece it was in (of equal ones the first, it goes through them in order) and looks the place
-// up at the end.  Bound by HBM.
+// largest value and the piece it was in (of equal ones the first, it goes through them in order) and looks for the
+// place in that at the end.  Bound by HBM.
 template <typename T>
 __global__ __launch_bounds__(kArgmaxThreads) void argmax_kernel(const typename elem<T>::storage* __restrict__ logits,
                                                                 int64_t row_stride, int32_t vocab, int32_t splits,
@@ -143,6 +156,7 @@ __global__ __launch_bounds__(kArgmaxThreads) void argmax_kernel(const typename e
   const int p0 = (int)((int64_t)pieces * split / splits), p1 = (int)((int64_t)pieces * (split + 1) / splits);
   float top = -INFINITY;
   int at = -1;
+  uint4 held = make_uint4(0u, 0u, 0u, 0u);
   for (int p = p0 + tid; p < p1; p += kArgmaxThreads * kArgmaxAhead) {
     uint4 u[kArgmaxAhead];
 #pragma unroll
@@ -153,15 +167,16 @@ __global__ __launch_bounds__(kArgmaxThreads) void argmax_kernel(const typename e
 #pragma unroll
     for (int i = 0; i < kArgmaxAhead; ++i) {
       const float m = Piece<T>(u[i]).largest();
-      if (m > top && p + i * kArgmaxThreads < p1) {
-        top = m;
-        at = p + i * kArgmaxThreads;
-      }
+      const bool better = m > top && p + i * kArgmaxThreads < p1;
+      top = better ? m : top;
+      at = better ? p + i * kArgmaxThreads : at;
+      held = make_uint4(better ? u[i].x : held.x, better ? u[i].y : held.y, better ? u[i].z : held.z,
+                        better ? u[i].w : held.w);
     }
   }
   uint64_t key = 0;
   if (at >= 0) {
-    const Piece<T> piece(body[at]);
+    const Piece<T> piece(held);
     int e = 0;
 #pragma unroll
     for (int i = N - 1; i >= 0; --i) e = piece.v[i] == top ? i : e;
@@ -197,17 +212,21 @@ struct AcceptArgs {
 };
 
 // One workgroup per sequence.  child[p] is the lowest node below p that drafted p's target, found by all nodes at
-// once; the path from the root is then a walk through LDS.
-constexpr int kAcceptThreads = 256;
-__global__ __launch_bounds__(kAcceptThreads) void accept_tree_kernel(AcceptArgs a) {
+// once; the path from the root is then a walk through LDS.  With the rows in many splits (few sequences, then) the
+// workgroups are large, so that all of a tree's are read at once.
+constexpr int kAcceptThreads = 256, kAcceptMost = 1024;
+__global__ __launch_bounds__(kAcceptMost) void accept_tree_kernel(AcceptArgs a) {
   __shared__ int32_t target[kMaxTreeNodes], child[kMaxTreeNodes], path[kMaxTreeNodes];
   __shared__ int32_t length;
-  const int s = blockIdx.x, tid = threadIdx.x;
+  const int s = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
   const Tree t = tree_of(a.cu, s, a.num_nodes, a.max_nodes);
-  if (a.best) {
+  // (The first node of a thread is asked for before its target is known.)
+  const bool has = tid < t.nodes;
+  const int parent0 = has ? a.parents[t.first + tid] : -1, draft0 = has ? a.draft[t.first + tid] : 0;
+  if (a.best && a.splits > 1) {
     // 16 lanes to a node.
     const int sub = tid & 15;
-    for (int j0 = 0; j0 < t.nodes; j0 += kAcceptThreads / 16) {
+    for (int j0 = 0; j0 < t.nodes; j0 += threads / 16) {
       const int j = j0 + (tid >> 4);
       uint64_t key = 0;
       if (j < t.nodes) {
@@ -218,20 +237,18 @@ __global__ __launch_bounds__(kAcceptThreads) void accept_tree_kernel(AcceptArgs 
         const uint64_t other = __shfl_xor((unsigned long long)key, o, kWave);
         key = other > key ? other : key;
       }
-      if (sub == 0 && j < t.nodes) {
-        const int32_t v = key ? (int32_t)~(uint32_t)key : 0;  // (nothing above -inf: the first)
-        target[j] = v;
-        a.target[t.first + j] = v;
-      }
+      if (sub == 0 && j < t.nodes) target[j] = a.target[t.first + j] = token_of(key);
     }
+  } else if (a.best) {
+    for (int j = tid; j < t.nodes; j += threads) target[j] = a.target[t.first + j] = token_of(a.best[t.first + j]);
   } else {
-    for (int j = tid; j < t.nodes; j += kAcceptThreads) target[j] = a.target[t.first + j];
+    for (int j = tid; j < t.nodes; j += threads) target[j] = a.target[t.first + j];
   }
-  for (int j = tid; j < t.nodes; j += kAcceptThreads) child[j] = t.nodes;
+  for (int j = tid; j < t.nodes; j += threads) child[j] = t.nodes;
   __syncthreads();
-  for (int j = tid; j < t.nodes; j += kAcceptThreads) {
-    const int p = a.parents[t.first + j];
-    if (p >= 0 && p < j && a.draft[t.first + j] == target[p]) atomicMin(&child[p], j);
+  for (int j = tid; j < t.nodes; j += threads) {
+    const int p = j == tid ? parent0 : a.parents[t.first + j];
+    if (p >= 0 && p < j && (j == tid ? draft0 : a.draft[t.first + j]) == target[p]) atomicMin(&child[p], j);
   }
   __syncthreads();
   if (tid == 0) {
@@ -242,7 +259,7 @@ __global__ __launch_bounds__(kAcceptThreads) void accept_tree_kernel(AcceptArgs 
     a.next[s] = t.nodes > 0 ? target[last] : -1;
   }
   __syncthreads();
-  for (int i = tid; i < a.max_accepted; i += kAcceptThreads) {
+  for (int i = tid; i < a.max_accepted; i += threads) {
     a.accepted[(int64_t)s * a.max_accepted + i] = i < length ? path[i] : -1;
   }
 }
@@ -356,7 +373,8 @@ int check_accept(const char* op, int32_t num_seqs, int32_t num_nodes, int32_t ma
 }
 
 int run_accept(const char* op, const AcceptArgs& a, int32_t num_seqs, hipStream_t s) {
-  hipLaunchKernelGGL(accept_tree_kernel, dim3((unsigned)num_seqs), dim3(kAcceptThreads), 0, s, a);
+  hipLaunchKernelGGL(accept_tree_kernel, dim3((unsigned)num_seqs), dim3(a.splits > 1 ? kAcceptMost : kAcceptThreads), 0, s,
+                     a);
   return check_launch(op);
 }
 

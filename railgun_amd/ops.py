@@ -90,36 +90,58 @@ def _require_scored_lens(scored_lens: Optional[torch.Tensor], batch: int) -> Non
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "scored_lens needs one entry per sequence")
 
 
-def _require_tree_mask(tree_mask: torch.Tensor, nodes: int, max_nodes: int) -> None:
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != nodes or 32 * tree_mask.shape[1] < max_nodes:
+def _require_on(device: int, *tensors: torch.Tensor) -> None:
+    """GPU tensors of that device (-1: of none)."""
+    for t in tensors:
+        if device < 0 or t.get_device() != device:
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "requires GPU tensors, all on one device")
+
+
+def _require_i32_on(device: int, *tensors: torch.Tensor) -> None:
+    """_require_on and _require_i32 in one pass (small calls are bound by the host)."""
+    for t in tensors:
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != device or device < 0:
+            _require_on(device, t)
+            _require_i32(t)
+
+
+def _tree_count(cu_nodes: torch.Tensor) -> int:
+    """Sequences of a call over trees."""
+    if cu_nodes.dim() != 1 or cu_nodes.numel() < 1:
+        raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, f"cu_nodes must be [sequences + 1], got {tuple(cu_nodes.shape)}")
+    return cu_nodes.numel() - 1
+
+
+def _tree_mask_words(tree_mask: torch.Tensor, nodes: int, max_nodes: int) -> int:
+    shape = tree_mask.shape
+    if len(shape) != 2 or shape[0] != nodes or 32 * shape[1] < max_nodes:
         raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                           f"tree_mask must be [{nodes}, words] with 32 words' bits for {max_nodes} nodes, got "
-                           f"{tuple(tree_mask.shape)}")
+                           f"tree_mask must be [{nodes}, words] with a bit for each of {max_nodes} nodes, got {tuple(shape)}")
+    return shape[1]
 
 
-def _require_rows(block_table: torch.Tensor, context_lens: torch.Tensor, seqs: int) -> None:
-    if block_table.dim() != 2 or block_table.shape[0] != seqs or context_lens.numel() != seqs:
+def _tree_table_width(block_table: torch.Tensor, context_lens: torch.Tensor, seqs: int) -> int:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != seqs or context_lens.numel() != seqs:
         raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                           f"block_table must be [{seqs}, max_blocks] and context_lens [{seqs}], got "
-                           f"{tuple(block_table.shape)} and {tuple(context_lens.shape)}")
+                           f"block_table must be [{seqs}, max_blocks] and context_lens [{seqs}], got {tuple(shape)} and "
+                           f"{tuple(context_lens.shape)}")
+    return shape[1]
 
 
-class _on_device:
-    """Makes t's device the current one, if it is not (a launch goes to the current device)."""
-
-    __slots__ = ("wanted", "before")
-
-    def __init__(self, t: torch.Tensor):
-        self.wanted = t.get_device()
-
-    def __enter__(self) -> None:
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.wanted:
-            torch.cuda.set_device(self.wanted)
-
-    def __exit__(self, *exc) -> None:
-        if self.before != self.wanted:
-            torch.cuda.set_device(self.before)
+def _launch_on(device: int, entry, *args) -> None:
+    """entry(*args, stream) on a device and its current torch stream (a launch goes to the current device)."""
+    before = torch._C._cuda_getDevice()
+    if before == device:
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        torch.cuda.set_device(device)
+        try:
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+        finally:
+            torch.cuda.set_device(before)
+    if status != _lib.RG_OK:
+        check(status)
 
 
 def cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
@@ -588,22 +610,24 @@ class PagedAttentionKernels:
         than ``max_nodes`` nodes.  Written: ``tree_mask`` [N, words], ``positions`` [N] (the root's plus the
         node's depth; the root's is ``text_positions`` [S], or the number of tokens before the tree) and
         ``slot_mapping`` [N].  All int32."""
-        n, seqs = self._check_tree(max_nodes, cu_nodes, parents, positions, slot_mapping)
-        self._on_one_device(parents, cu_nodes, context_lens, block_table, text_positions, tree_mask, positions,
-                            slot_mapping)
-        _require_i32(parents, context_lens, block_table, tree_mask, positions, slot_mapping)
-        _require_tree_mask(tree_mask, n, max_nodes)
-        _require_rows(block_table, context_lens, seqs)
+        device = parents.get_device()
+        _require_i32_on(device, parents, cu_nodes, context_lens, block_table, tree_mask, positions, slot_mapping)
         if text_positions is not None:
-            _require_i32(text_positions)
-            if text_positions.numel() != seqs:
-                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "text_positions needs one entry per sequence")
-        _require_int32(block_size=block_size)
-        with _on_device(parents):
-            check(self.lib.rg_tree_layout(
-                parents.data_ptr(), cu_nodes.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
-                _ptr(text_positions), tree_mask.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), block_size,
-                int(block_table.shape[1]), seqs, n, max_nodes, int(tree_mask.shape[1]), _stream(parents)))
+            _require_i32_on(device, text_positions)
+        n, seqs = parents.numel(), _tree_count(cu_nodes)
+        if positions.numel() != n or slot_mapping.numel() != n or \
+                (text_positions is not None and text_positions.numel() != seqs):
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, f"parents, positions and slot_mapping must be of one length and "
+                                                             f"text_positions [{seqs}]")
+        if not (0 <= max_nodes <= 1024 and 0 < block_size < 2**31):
+            _require_int32(block_size=block_size, max_nodes=max_nodes)
+        words = _tree_mask_words(tree_mask, n, max_nodes)
+        max_blocks = _tree_table_width(block_table, context_lens, seqs)
+        _launch_on(
+            device, self.lib.rg_tree_layout, parents.data_ptr(), cu_nodes.data_ptr(), context_lens.data_ptr(),
+            block_table.data_ptr(), None if text_positions is None else text_positions.data_ptr(),
+            tree_mask.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), block_size, max_blocks, seqs, n,
+            max_nodes, words)
 
     def tree_workspace_bytes(self, num_seqs: int, max_nodes: int, num_heads: int, num_kv_heads: int, head_dim: int,
                              block_size: int, max_blocks_per_seq: int) -> int:
@@ -616,31 +640,34 @@ class PagedAttentionKernels:
         that holds their K and V too (rg_paged_attention_tree): a node attends to all positions before its
         tree and to the nodes that its row of ``tree_mask`` [N, words] has set.  ``workspace``:
         tree_workspace_bytes, allocated here when omitted."""
-        n, seqs = self._check_tree(max_nodes, cu_nodes)
-        self._on_one_device(query, key_cache, value_cache, block_table, context_lens, cu_nodes, tree_mask, output,
-                            workspace)
-        _require_i32(block_table, context_lens, tree_mask)
+        device = query.get_device()
+        _require_i32_on(device, block_table, context_lens, cu_nodes, tree_mask)
+        _require_on(device, query, key_cache, value_cache, output)
+        seqs = _tree_count(cu_nodes)
         hkv, bs, d, kv_stride = cache_geometry(key_cache, value_cache)
-        for t in (query, output):
-            if t.dim() != 3 or not t.is_contiguous() or t.shape[2] != d or t.dtype != key_cache.dtype or \
-                    t.shape != query.shape:
-                raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                                   f"query and output must be contiguous [nodes, heads, {d}] of {key_cache.dtype}, got "
-                                   f"{tuple(t.shape)} {t.dtype}")
-        n, heads = int(query.shape[0]), int(query.shape[1])
-        _require_tree_mask(tree_mask, n, max_nodes)
-        _require_rows(block_table, context_lens, seqs)
-        mb = int(block_table.shape[1])
-        with _on_device(query):
-            if workspace is None:
-                nbytes = self._ask("rg_paged_attention_tree_workspace_bytes", seqs, max_nodes, heads, hkv, d, bs, mb)
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
-            check(self.lib.rg_paged_attention_tree(
-                query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
-                context_lens.data_ptr(), cu_nodes.data_ptr(), tree_mask.data_ptr(), output.data_ptr(), float(scale),
-                heads, hkv, d, bs, mb, seqs, n, max_nodes, int(tree_mask.shape[1]), dtype_code(query), kv_stride,
-                _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-                _stream(query)))
+        shape = query.shape
+        if len(shape) != 3 or shape[2] != d or output.shape != shape or query.dtype != key_cache.dtype or \
+                output.dtype != query.dtype or not query.is_contiguous() or not output.is_contiguous():
+            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
+                               f"query and output must be contiguous [nodes, heads, {d}] of {key_cache.dtype}, got "
+                               f"{tuple(shape)} {query.dtype} and {tuple(output.shape)} {output.dtype}")
+        n, heads = shape[0], shape[1]
+        if not 0 <= max_nodes <= 1024:
+            _require_int32(max_nodes=max_nodes)
+        words = _tree_mask_words(tree_mask, n, max_nodes)
+        mb = _tree_table_width(block_table, context_lens, seqs)
+        nbytes = 0
+        if workspace is None:
+            nbytes = self._ask("rg_paged_attention_tree_workspace_bytes", seqs, max_nodes, heads, hkv, d, bs, mb)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+        else:
+            _require_on(device, workspace)
+            nbytes = workspace.numel() * workspace.element_size()
+        _launch_on(
+            device, self.lib.rg_paged_attention_tree, query.data_ptr(), key_cache.data_ptr(),
+            value_cache.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), cu_nodes.data_ptr(),
+            tree_mask.data_ptr(), output.data_ptr(), float(scale), heads, hkv, d, bs, mb, seqs, n, max_nodes, words,
+            dtype_code(query), kv_stride, _ptr(workspace), nbytes)
 
     def verify_tree_workspace_bytes(self, num_nodes: int, vocab_size: int) -> int:
         return int(self.lib.rg_verify_tree_workspace_bytes(num_nodes, vocab_size))
@@ -652,34 +679,35 @@ class PagedAttentionKernels:
         target of the last accepted node is accepted.  Written: ``accepted`` [S, most] (indices in the tree,
         -1 behind them), ``num_accepted`` [S] (node 0 counts) and ``next_tokens`` [S], the last one's target.
         ``workspace``: verify_tree_workspace_bytes, allocated here when omitted."""
-        n, seqs, most = self._check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted,
-                                           num_accepted, next_tokens)
-        self._on_one_device(draft_tokens, logits, workspace)
-        if logits.dim() != 2 or logits.shape[0] != n or logits.shape[1] < 1 or logits.stride(1) != 1 or \
-                (n > 1 and logits.stride(0) < logits.shape[1]):
+        device, n, seqs, most = self._check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted,
+                                                   num_accepted, next_tokens)
+        _require_on(device, logits)
+        shape, strides = logits.shape, logits.stride()
+        if len(shape) != 2 or shape[0] != n or shape[1] < 1 or strides[1] != 1 or (n > 1 and strides[0] < shape[1]):
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                               f"logits must be [{n}, vocab] with unit column stride, got {tuple(logits.shape)}")
-        vocab = int(logits.shape[1])
-        with _on_device(logits):
-            if workspace is None:
-                nbytes = self._ask("rg_verify_tree_workspace_bytes", n, vocab)
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-            check(self.lib.rg_verify_tree(
-                logits.data_ptr(), draft_tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(),
-                target_tokens.data_ptr(), accepted.data_ptr(), num_accepted.data_ptr(), next_tokens.data_ptr(), seqs, n,
-                max_nodes, most, vocab, dtype_code(logits), max(logits.stride(0), vocab), workspace.data_ptr(),
-                workspace.numel() * workspace.element_size(), _stream(logits)))
+                               f"logits must be [{n}, vocab] with unit column stride, got {tuple(shape)}")
+        vocab = shape[1]
+        if workspace is None:
+            nbytes = self._ask("rg_verify_tree_workspace_bytes", n, vocab)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+        else:
+            _require_on(device, workspace)
+            nbytes = workspace.numel() * workspace.element_size()
+        _launch_on(
+            device, self.lib.rg_verify_tree, logits.data_ptr(), draft_tokens.data_ptr(), parents.data_ptr(),
+            cu_nodes.data_ptr(), target_tokens.data_ptr(), accepted.data_ptr(), num_accepted.data_ptr(),
+            next_tokens.data_ptr(), seqs, n, max_nodes, most, vocab, dtype_code(logits), max(strides[0], vocab),
+            workspace.data_ptr(), nbytes)
 
     def launch_accept_tree(self, target_tokens, draft_tokens, parents, cu_nodes, max_nodes: int, accepted, num_accepted,
                            next_tokens) -> None:
         """launch_verify_tree for ``target_tokens`` that a sampler drew (rg_accept_tree)."""
-        n, seqs, most = self._check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted,
-                                           num_accepted, next_tokens)
-        with _on_device(draft_tokens):
-            check(self.lib.rg_accept_tree(
-                target_tokens.data_ptr(), draft_tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(),
-                accepted.data_ptr(), num_accepted.data_ptr(), next_tokens.data_ptr(), seqs, n, max_nodes, most,
-                _stream(draft_tokens)))
+        device, n, seqs, most = self._check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted,
+                                                   num_accepted, next_tokens)
+        _launch_on(
+            device, self.lib.rg_accept_tree, target_tokens.data_ptr(), draft_tokens.data_ptr(), parents.data_ptr(),
+            cu_nodes.data_ptr(), accepted.data_ptr(), num_accepted.data_ptr(), next_tokens.data_ptr(), seqs, n,
+            max_nodes, most)
 
     def launch_compact_tree(self, key_cache, value_cache, scores, block_table, context_lens, cu_nodes, accepted,
                             num_accepted, new_context_lens=None) -> None:
@@ -689,66 +717,59 @@ class PagedAttentionKernels:
 
         Caches ``[NB, H_kv, bs, D]`` or ``[layers, NB, H_kv, bs, D]`` with contiguous blocks, scores fp32 of
         the caches' shape without D."""
-        _, seqs = self._check_tree(0, cu_nodes)
-        self._on_one_device(key_cache, value_cache, scores, block_table, context_lens, cu_nodes, accepted, num_accepted,
-                            new_context_lens)
-        _require_i32(block_table, context_lens, accepted, num_accepted)
-        if key_cache.dim() not in (4, 5) or value_cache.shape != key_cache.shape or \
-                value_cache.dtype != key_cache.dtype or value_cache.stride() != key_cache.stride():
+        device = key_cache.get_device()
+        _require_i32_on(device, block_table, context_lens, cu_nodes, accepted, num_accepted)
+        _require_on(device, key_cache, value_cache)
+        seqs = _tree_count(cu_nodes)
+        shape, strides = key_cache.shape, key_cache.stride()
+        dims = len(shape)
+        if dims not in (4, 5) or value_cache.shape != shape or value_cache.dtype != key_cache.dtype or \
+                value_cache.stride() != strides:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "caches must be [NB, H_kv, bs, D] or [layers, NB, H_kv, "
                                                              "bs, D], alike in shape, strides and dtype")
-        layered = key_cache.dim() == 5
-        layers = int(key_cache.shape[0]) if layered else 1
-        hkv, bs, d = (int(x) for x in key_cache.shape[-3:])
-        if key_cache.stride()[-3:] != (bs * d, d, 1):
+        hkv, bs, d = shape[-3:]
+        if strides[-3:] != (bs * d, d, 1):
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "cache blocks must be contiguous [H_kv, bs, D]")
         _require_blocks_apart(key_cache, -4)
+        layers, layer_stride = (shape[0], strides[0]) if dims == 5 else (1, 0)
+        cells = cell_layer_stride = cell_stride = 0
         if scores is not None:
+            _require_on(device, scores)
             check_scores(scores, key_cache)
-        _require_rows(block_table, context_lens, seqs)
-        if accepted.dim() != 2 or accepted.shape[0] != seqs or num_accepted.numel() != seqs:
+            cells, cell_stride = scores.data_ptr(), scores.stride(-3)
+            cell_layer_stride = scores.stride(0) if dims == 5 else 0
+        mb = _tree_table_width(block_table, context_lens, seqs)
+        most = accepted.shape[1] if accepted.dim() == 2 else 0
+        if accepted.numel() != seqs * most or (most == 0 and seqs > 0) or num_accepted.numel() != seqs:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
                                "accepted must be [sequences, most] and num_accepted [sequences]")
         if new_context_lens is not None:
-            _require_i32(new_context_lens)
+            _require_i32_on(device, new_context_lens)
             if new_context_lens.numel() != seqs:
                 raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "new_context_lens needs one entry per sequence")
-        with _on_device(key_cache):
-            check(self.lib.rg_compact_tree(
-                key_cache.data_ptr(), value_cache.data_ptr(), _ptr(scores), block_table.data_ptr(),
-                context_lens.data_ptr(), cu_nodes.data_ptr(), accepted.data_ptr(), num_accepted.data_ptr(),
-                _ptr(new_context_lens), int(accepted.shape[1]), layers, hkv, d, bs, int(block_table.shape[1]), seqs,
-                2**31 - 1, dtype_code(key_cache), key_cache.stride(0) if layered else 0, key_cache.stride(-4),
-                0 if scores is None or not layered else scores.stride(0), 0 if scores is None else scores.stride(-3),
-                _stream(key_cache)))
+        _launch_on(
+            device, self.lib.rg_compact_tree, key_cache.data_ptr(), value_cache.data_ptr(), cells,
+            block_table.data_ptr(), context_lens.data_ptr(), cu_nodes.data_ptr(), accepted.data_ptr(),
+            num_accepted.data_ptr(), None if new_context_lens is None else new_context_lens.data_ptr(), max(most,
+            1), layers, hkv, d, bs, mb, seqs, 2**31 - 1, dtype_code(key_cache), layer_stride, strides[-4],
+            cell_layer_stride, cell_stride)
 
     @staticmethod
-    def _on_one_device(*tensors: Optional[torch.Tensor]) -> None:
-        _require_cuda(*tensors)
-        if len({t.get_device() for t in tensors if t is not None}) > 1:
-            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT, "tensors must be on one device")
-
-    def _check_tree(self, max_nodes: int, cu_nodes, *per_node) -> tuple:
-        """(nodes, sequences) of one call over trees, as far as its arrays of one entry per node say."""
-        _require_i32(cu_nodes)
-        _require_int32(max_nodes=max_nodes)
-        if cu_nodes.dim() != 1 or cu_nodes.numel() < 1 or len({t.numel() for t in per_node}) > 1:
-            raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                               "cu_nodes must be [sequences + 1], and arrays of the nodes of one length, got "
-                               f"{tuple(cu_nodes.shape)} and {[tuple(t.shape) for t in per_node]}")
-        return (int(per_node[0].numel()) if per_node else 0), int(cu_nodes.numel()) - 1
-
-    def _check_accept(self, draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted, num_accepted,
+    def _check_accept(draft_tokens, parents, cu_nodes, max_nodes, target_tokens, accepted, num_accepted,
                       next_tokens) -> tuple:
-        """(nodes, sequences, most accepted) of a verification."""
-        n, seqs = self._check_tree(max_nodes, cu_nodes, draft_tokens, parents, target_tokens)
-        self._on_one_device(draft_tokens, parents, cu_nodes, target_tokens, accepted, num_accepted, next_tokens)
-        _require_i32(draft_tokens, parents, target_tokens, accepted, num_accepted, next_tokens)
-        if accepted.dim() != 2 or accepted.shape[0] != seqs or num_accepted.numel() != seqs or \
-                next_tokens.numel() != seqs:
+        """(device, nodes, sequences, most accepted) of a verification."""
+        device = cu_nodes.get_device()
+        _require_i32_on(device, cu_nodes, draft_tokens, parents, target_tokens, accepted, num_accepted, next_tokens)
+        n, seqs = draft_tokens.numel(), _tree_count(cu_nodes)
+        shape = accepted.shape
+        if parents.numel() != n or target_tokens.numel() != n or len(shape) != 2 or shape[0] != seqs or \
+                num_accepted.numel() != seqs or next_tokens.numel() != seqs:
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
-                               "accepted must be [sequences, most], num_accepted and next_tokens [sequences]")
-        return n, seqs, int(accepted.shape[1])
+                               "draft_tokens, parents and target_tokens must be of one length, accepted [sequences, most], "
+                               "num_accepted and next_tokens [sequences]")
+        if not 0 <= max_nodes <= 1024:
+            _require_int32(max_nodes=max_nodes)
+        return device, n, seqs, shape[1]
 
     def launch_prefill_packed(self, query, key_cache, value_cache, block_table, context_lens, cu_seqlens,
                               output, scale: float, num_heads: int, num_kv_heads: int, head_dim: int,
