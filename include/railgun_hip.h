@@ -277,7 +277,7 @@ int rg_accept_tree(const int32_t* target_tokens, const int32_t* draft_tokens, co
 
 /* Keeps the accepted nodes: in every layer K and V (and with scores, the scores) of position
  * prior + accepted[s, i] go to prior + i, i < num_accepted[s], and new_context_lens[s] (NULL: not
- * wanted; apart from context_lens and num_accepted) becomes prior + num_accepted[s].  All other cells
+ * wanted; apart from the inputs) becomes prior + num_accepted[s].  All other cells
  * keep what they hold.  accepted rises within a row and lies in [0, L); an entry outside is not
  * moved.  The blocks from position prior on belong to the sequence alone.  Caches and scores as in
  * rg_evict_cache, layer l layer_stride (score_layer_stride) elements behind layer 0. */

@@ -196,6 +196,18 @@ def _tree_depths(tree: DraftTree) -> list:
     return depths
 
 
+def _check_tree_blocks(draft_trees: Sequence[DraftTree], table: np.ndarray, ctx: np.ndarray, block_size: int) -> None:
+    """Blocks that hold a tree's tokens belong to its sequence alone: what is kept of the tree moves in them."""
+    if not draft_trees:
+        return
+    used = np.where(np.arange(table.shape[1]) < -(-ctx // block_size)[:, None], table, -1)
+    first = len(ctx) - len(draft_trees)
+    for s, d in enumerate(draft_trees):
+        written = used[first + s, (d.seq_len - len(d.token_ids)) // block_size:-(-d.seq_len // block_size)]
+        if np.isin(used, written).sum() != len(written):
+            raise ValueError(f"a block of draft tree {s} appears twice in a step")
+
+
 def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[DecodeSlot], block_size: int,
               max_blocks: Optional[int] = None, share_prefix: bool = False, gather_scores: bool = False,
               draft_trees: Sequence[DraftTree] = ()) -> StepBatch:
@@ -272,6 +284,7 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     bt = np.zeros((len(tables), mb), np.int32)
     for r, t in enumerate(tables):
         bt[r, :len(t)] = np.asarray(t, dtype=np.int64).astype(np.int32)
+    _check_tree_blocks(draft_trees, bt, np.asarray(ctx, np.int64), block_size)
     shared = shared_prefix_blocks(decode_slots, block_size) if share_prefix else 0
     lens = np.diff(np.asarray(cu))
     last = np.concatenate([np.asarray(cu[1:], np.int64) - 1,

@@ -537,10 +537,12 @@ extern "C" int rg_compact_tree(void* key_cache, void* value_cache, float* scores
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
   }
   // (Every layer's workgroups read the lengths while the new ones are written.)
-  if (new_context_lens != nullptr &&
-      (overlap(new_context_lens, 4 * (size_t)num_seqs, context_lens, 4 * (size_t)num_seqs) ||
-       overlap(new_context_lens, 4 * (size_t)num_seqs, num_accepted, 4 * (size_t)num_seqs))) {
-    return fail(RG_ERR_INVALID_ARGUMENT, "%s: new_context_lens overlaps context_lens or num_accepted", op);
+  const size_t entries = 4 * (size_t)num_seqs;
+  if (new_context_lens != nullptr && (overlap(new_context_lens, entries, context_lens, entries) ||
+                                      overlap(new_context_lens, entries, num_accepted, entries) ||
+                                      overlap(new_context_lens, entries, accepted, entries * max_accepted) ||
+                                      overlap(new_context_lens, entries, cu_nodes, entries + 4))) {
+    return fail(RG_ERR_INVALID_ARGUMENT, "%s: new_context_lens overlaps an input", op);
   }
   const int64_t layers_apart = num_layers > 1 ? layer_stride : 0;
   auto whole = [&](int64_t elements) { return elements * eb % 16 == 0; };

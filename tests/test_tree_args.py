@@ -107,6 +107,8 @@ COMPACT = dict(k=P, v=P, scores=P, table=P, lens=P, cu=P, accepted=P, count=P, n
     (dict(k=None), INVALID, "null"), (dict(v=None), INVALID, "null"), (dict(table=None), INVALID, "null"),
     (dict(lens=None), INVALID, "null"), (dict(cu=None), INVALID, "null"), (dict(accepted=None), INVALID, "null"),
     (dict(count=None), INVALID, "null"), (dict(new_lens=P), INVALID, "overlaps"), (dict(new_lens=P + 4), INVALID, "overlaps"),
+    (dict(lens=P + 128, count=P + 160, accepted=P + 32, cu=P + 192, new_lens=P + 60), INVALID, "overlaps"),
+    (dict(lens=P + 128, count=P + 160, accepted=P + 192, cu=P + 32, new_lens=P + 40), INVALID, "overlaps"),
 ])
 def test_compact_refusals(change, code, text):
     expect(call("rg_compact_tree", COMPACT, change), code, text)

@@ -41,3 +41,16 @@ def test_steps_without_trees_stay():
 def test_refused_trees(tree, text):
     with pytest.raises(ValueError, match=text):
         pack_step([], [], 4, draft_trees=[tree])
+
+
+def test_blocks_of_a_tree_are_its_own():
+    """Blocks in front of the trees may be shared, those that hold their tokens may not."""
+    def step(a, b, slots=()):
+        return pack_step([], list(slots), 4, draft_trees=[DraftTree([1, 2], [-1, 0], 10, a), DraftTree([1, 2], [-1, 0], 9, b)])
+
+    step([1, 2, 3], [1, 4, 5])                      # the second tree begins in its second block
+    for a, b, slots in (([1, 2, 3], [1, 2, 3], ()), ([1, 2, 3], [4, 5, 3], ()), ([1, 2, 3], [1, 3, 5], ()),
+                        ([1, 2, 2], [4, 5, 6], ()), ([1, 2, 3], [4, 5, 6], [DecodeSlot(1, 9, [7, 8, 3])])):
+        with pytest.raises(ValueError, match="appears twice"):
+            step(a, b, slots)
+    step([1, 2, 3], [4, 5, 6], [DecodeSlot(1, 8, [7, 8, 3])])   # an entry behind the slot's tokens
