@@ -1001,16 +1001,40 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
   }
 }
 
-// The rows of a cut segment: D / 4 lanes have 4 dims each of a row, a wave N times 256 / D rows, the AHEAD next pieces'
-// in flight: a batch of few segments has them in many pieces (N = 1, AHEAD = 8), one of many in two or three (4, 2).
+// The rows of a cut segment: D / 4 lanes have 4 dims each of a row, a wave N times 256 / D rows.  Where a batch is few
+// segments in many pieces (kManyParts), the waves of a workgroup have the same rows (SPLIT), each every fourth piece, and
+// their results are joined in LDS: a wave alone would wait for 64 pieces eight times.  Elsewhere a segment is in two
+// or three.  AHEAD: pieces in flight.  Measured (us, a wave alone / split; bf16, 32 / 8 heads of 128, 16 nodes):
+// one sequence of 32,768 14.5 / 7.4, four of 4,096 6.4 / 6.1, one of 2,048 4.0 / 3.9.
 constexpr int kMergeWaves = 4;
 template <int D> constexpr int merge_rows() { return 256 / D; }
-template <typename T, int D, int N, int AHEAD>
+
+// A row's partials so far, 4 dims of it, and the next.
+struct Partial {
+  float m, l;
+  float4 acc;
+  __device__ __forceinline__ void join(float2 x, float4 v, bool is) {
+    // (A piece without keys for the row has m = -inf and nothing to add; one whose scores are all NaN has m = -inf
+    // too.)
+    const bool counts = is && !(x.x == -INFINITY && x.y == 0.f);
+    const float mn = counts ? fmaxf(m, x.x) : m;
+    const float fo = m == mn ? 1.f : exp2f(m - mn), fq = !counts ? 0.f : x.x == mn ? 1.f : exp2f(x.x - mn);
+    l = l * fo + (counts ? x.y * fq : 0.f);
+    acc.x = acc.x * fo + (counts ? v.x * fq : 0.f);
+    acc.y = acc.y * fo + (counts ? v.y * fq : 0.f);
+    acc.z = acc.z * fo + (counts ? v.z * fq : 0.f);
+    acc.w = acc.w * fo + (counts ? v.w * fq : 0.f);
+    m = mn;
+  }
+};
+
+template <typename T, int D, int N, int AHEAD, bool SPLIT>
 __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a) {
   using S = typename elem<T>::storage;
-  constexpr int LANES = D / 4, ROWS = merge_rows<D>();
+  constexpr int LANES = D / 4, ROWS = merge_rows<D>(), STEP = SPLIT ? kMergeWaves : 1;
   const int s = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63;
-  const int row0 = ((int)blockIdx.x * kMergeWaves + (threadIdx.x >> 6)) * (N * ROWS);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row0 = (SPLIT ? (int)blockIdx.x : (int)blockIdx.x * kMergeWaves + w) * (N * ROWS);
   const int2 cuts = a.cuts[s];  // (not used where the sequence has no tree)
   const Span sp = span_of(arguments(), s);
   const int rows = sp.t.nodes * a.group, n = cuts.y;
@@ -1020,21 +1044,23 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a
   const int64_t first = (int64_t)(cuts.x + kvh * n * sp.row_tiles + rt) * kRows - rt * kRows;
   const int64_t step = (int64_t)sp.row_tiles * kRows;
   int row[N];
-  float m[N], l[N];
-  float4 acc[N];
+  Partial sum[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     row[k] = min(row0 + k * ROWS + lane / LANES, rows - 1);  // (a row tile's rows are written so far)
-    m[k] = -INFINITY;
-    l[k] = 0.f;
-    acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    sum[k] = Partial{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
   }
-  for (int i = 0; i < n; i += AHEAD) {
+  int i = SPLIT ? w : 0;
+  // AHEAD pieces from i on; `left` of them where they are not all there (`all`): then the split form asks for no others,
+  // whose rows four waves would read again.
+  auto take = [&](auto all, int left) __attribute__((always_inline)) {
+    constexpr bool ALL = decltype(all)::value;
     float2 ml[AHEAD][N];
     float4 v[AHEAD][N];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int64_t at = first + min(i + u, n - 1) * step;
+      if (!ALL && SPLIT && u >= left) break;
+      const int64_t at = first + (ALL ? i + u * STEP : min(i + u * STEP, n - 1)) * step;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         ml[u][k] = *reinterpret_cast<const float2*>(a.ml + 2 * (at + row[k]));
@@ -1042,30 +1068,33 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a
       }
     }
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
+    for (int u = 0; u < AHEAD; ++u) {
+      if (!ALL && SPLIT && u >= left) break;
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        // (A piece without keys for the row has m = -inf and nothing to add; one whose scores are all NaN has m = -inf
-        // too.)
-        const float2 x = ml[u][k];
-        const bool counts = i + u < n && !(x.x == -INFINITY && x.y == 0.f);
-        const float mn = counts ? fmaxf(m[k], x.x) : m[k];
-        const float fo = m[k] == mn ? 1.f : exp2f(m[k] - mn), fq = !counts ? 0.f : x.x == mn ? 1.f : exp2f(x.x - mn);
-        l[k] = l[k] * fo + (counts ? x.y * fq : 0.f);
-        acc[k].x = acc[k].x * fo + (counts ? v[u][k].x * fq : 0.f);
-        acc[k].y = acc[k].y * fo + (counts ? v[u][k].y * fq : 0.f);
-        acc[k].z = acc[k].z * fo + (counts ? v[u][k].z * fq : 0.f);
-        acc[k].w = acc[k].w * fo + (counts ? v[u][k].w * fq : 0.f);
-        m[k] = mn;
-      }
+      for (int k = 0; k < N; ++k) sum[k].join(ml[u][k], v[u][k], ALL || u < left);
+    }
+  };
+  for (; i + (AHEAD - 1) * STEP < n; i += AHEAD * STEP) take(std::true_type{}, AHEAD);
+  if (i < n) take(std::false_type{}, (n - i + STEP - 1) / STEP);
+  if constexpr (SPLIT) {
+    static_assert(N == 1, "a row to a lane");
+    __shared__ float2 ml[kMergeWaves][64];
+    __shared__ float4 acc[kMergeWaves][64];
+    ml[w][lane] = make_float2(sum[0].m, sum[0].l);
+    acc[w][lane] = sum[0].acc;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int i = 1; i < kMergeWaves; ++i) sum[0].join(ml[i][lane], acc[i][lane], true);
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     if (row0 + k * ROWS + lane / LANES >= rows) continue;
     const int node = row[k] / a.group, g = row[k] - node * a.group;
     S* out = static_cast<S*>(a.out) + ((int64_t)(sp.t.first + node) * a.num_heads + kvh * a.group + g) * D + d;
-    const float inv = l[k] != 0.f ? 1.f / l[k] : 1.f;
-    const float x0 = acc[k].x * inv, x1 = acc[k].y * inv, x2 = acc[k].z * inv, x3 = acc[k].w * inv;
+    const Partial& x = sum[k];
+    const float inv = x.l != 0.f ? 1.f / x.l : 1.f;
+    const float x0 = x.acc.x * inv, x1 = x.acc.y * inv, x2 = x.acc.z * inv, x3 = x.acc.w * inv;
     if constexpr (std::is_same_v<T, f32_t>) *reinterpret_cast<float4*>(out) = make_float4(x0, x1, x2, x3);
     else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x0, x1), pack2<T>(x2, x3));
   }
@@ -1117,13 +1146,13 @@ template <typename T, int D>
 void launch_product(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
   hipLaunchKernelGGL((tree_kernel<T, D>), dim3((unsigned)p.groups), dim3(kTreeThreads), 0, s, a);
   if (p.tiles <= a.least) return;  // nothing is cut
-  auto merge = [&](auto kernel, int n) {
-    const unsigned rows = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, n * merge_rows<D>() * kMergeWaves);
-    hipLaunchKernelGGL(kernel, dim3(rows, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), dim3(64 * kMergeWaves), 0, s, a);
+  auto merge = [&](auto kernel, int rows) {
+    const unsigned groups = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, rows * merge_rows<D>());
+    hipLaunchKernelGGL(kernel, dim3(groups, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), dim3(64 * kMergeWaves), 0, s, a);
   };
-  if (p.cut_in >= kManyParts) merge(tree_merge_kernel<T, D, 1, 8>, 1);
-  else if (p.cut_in >= 2) merge(tree_merge_kernel<T, D, 2, 4>, 2);
-  else merge(tree_merge_kernel<T, D, 4, 2>, 4);
+  if (p.cut_in >= kManyParts) merge(tree_merge_kernel<T, D, 1, 8, true>, 1);
+  else if (p.cut_in >= 2) merge(tree_merge_kernel<T, D, 2, 4, false>, 2 * kMergeWaves);
+  else merge(tree_merge_kernel<T, D, 4, 2, false>, 4 * kMergeWaves);
 }
 
 }  // namespace
@@ -1132,7 +1161,7 @@ int probe_tree_attention_kernels() {
   hipFuncAttributes at;
   if (hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_generic_kernel<bf16_t>)) != hipSuccess ||
       hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_kernel<bf16_t, 128>)) != hipSuccess ||
-      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_merge_kernel<bf16_t, 128, 1, 8>)) != hipSuccess) {
+      hipFuncGetAttributes(&at, reinterpret_cast<const void*>(tree_merge_kernel<bf16_t, 128, 1, 8, true>)) != hipSuccess) {
     return fail(RG_ERR_HIP, "failed to load the tree attention kernels: %s", hipGetErrorString(hipGetLastError()));
   }
   return RG_OK;

@@ -87,6 +87,14 @@ def test_segments_near_a_round(device, kernels, long, short, d):
     TreeBatch(device, prior, trees(rng, [3] * (long + short)), heads=8, hkv=8, d=d, seed=long).check(kernels)
 
 
+@pytest.mark.parametrize("d,nodes", [(64, 3), (128, 35)])
+def test_parts_of_a_segment(device, kernels, d, nodes):
+    """Segments in one to 66 parts, a key tile each, of one row tile and of two."""
+    rng = np.random.default_rng(d)
+    tiles = rng.permutation([1, 2, 3, 4, 5, 8, 9, 28, 29, 31, 32, 33, 36, 37, 64, 65] if nodes == 3 else [2, 3, 30, 33, 65])
+    TreeBatch(device, 32 * tiles - 5, trees(rng, [nodes] * len(tiles)), "f32", heads=4, hkv=1, d=d, seed=d).check(kernels)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_any_mask(device, kernels, dtype):
     """Masks that are no tree's: dense, empty rows (zeros where nothing lies before), later nodes seen, oneself
