@@ -17,7 +17,8 @@ namespace {
 //   seen[j] |= seen[up[j]],  depth[j] += depth[up[j]],  up[j] = up[up[j]],
 // so a chain of n nodes takes log2 n rounds.  seen is updated in place: what a node reads early are ancestors too.
 // A workgroup has kLayoutWords of a tree's mask words, so that 1,024 nodes' fit in LDS; the positions and slots are
-// written by the first of a tree's.
+// written by the first of a tree's.  Latency: the parents, lengths and table are read in three dependent steps, then a
+// barrier a round.  One tree of 24 nodes 3.5 us (1.3 KB), 256 of up to 128 6.2 us (1.7 MB).
 constexpr int kLayoutThreads = 256;
 constexpr int kLayoutWords = 8;
 
@@ -138,7 +139,8 @@ template <typename T> struct Piece {
 // Workgroup (row, split): the best of one piece of a row of logits.  The row's 16-byte pieces are dealt to the
 // splits; what lies before the first and behind the last goes to the first and the last split.  A thread keeps the
 // largest value and the piece it was in (of equal ones the first, it goes through them in order) and looks for the
-// place in that at the end.  Bound by HBM.
+// place in that at the end.  Bound by HBM: 1,469 rows of 128,256 in bf16 58 us, 6.4 TB/s (a row to a workgroup); 64
+// rows 5.2 us, 16 pieces to a row.
 template <typename T>
 __global__ __launch_bounds__(kArgmaxThreads) void argmax_kernel(const typename elem<T>::storage* __restrict__ logits,
                                                                 int64_t row_stride, int32_t vocab, int32_t splits,
@@ -212,8 +214,9 @@ struct AcceptArgs {
 };
 
 // One workgroup per sequence.  child[p] is the lowest node below p that drafted p's target, found by all nodes at
-// once; the path from the root is then a walk through LDS.  With the rows in many splits (few sequences, then) the
-// workgroups are large, so that all of a tree's are read at once.
+// once; the path from the root is then a walk through LDS, a round trip a token.  With the rows in many splits (few
+// sequences, then) the workgroups are large, so that all of a tree's are read at once.  Latency: 2.6 us for a tree
+// of 64 nodes and 16 splits, 3.2 for 256 trees whose targets are given.
 constexpr int kAcceptThreads = 256, kAcceptMost = 1024;
 __global__ __launch_bounds__(kAcceptMost) void accept_tree_kernel(AcceptArgs a) {
   __shared__ int32_t target[kMaxTreeNodes], child[kMaxTreeNodes], path[kMaxTreeNodes];
@@ -289,7 +292,8 @@ struct CompactArgs {
 // Workgroup (sequence, layer).  The places of up to kMoveTokens moving tokens are looked up by as many threads; then
 // a thread has one piece of a token's rows (K or V, kv-head, place in the row) and takes it from every one of them,
 // kMoveAhead at a time: what a token's move overwrites is read by the same thread, before.  (The accepted list rises,
-// so a later group's sources lie above what an earlier one wrote.)
+// so a later group's sources lie above what an earlier one wrote.)  Latency: list, table, rows; 64 sequences in 16
+// layers, 5.4 MB, 6.7 us, a layer or two of 3 sequences 3.8.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveTokens = 64;
 constexpr int kMoveAhead = 8;

@@ -938,6 +938,17 @@ constexpr int pieces_per_cu(int32_t dtype, int D) { return dtype == RG_DTYPE_F32
 template <typename T, int D>
 constexpr int groups_per_cu() { return pieces_per_cu(std::is_same_v<T, f32_t> ? RG_DTYPE_F32 : RG_DTYPE_BF16, D); }
 
+// A workgroup to a piece.  What bounds it (bf16, 32 / 8 heads of 128; us):
+//  - many sequences, short trees: HBM.  64 of 512 to 4,096 tokens with 8 to 32 nodes, 639 MB: 127, 5.0 TB/s.
+//  - long trees: the waves' LDS reads and the softmax between two products, which other workgroups' waves hide in part.
+//    Four sequences of 30,000 to 32,768 with 101 to 128 nodes, 253 GFLOP: 271, 930 TFLOP/s.  Without the copies to
+//    LDS it takes 15 % less, without the exponentials 7 %, without either product 20 %, without both products and
+//    the exponentials still 53 % of it.  64 rows a wave would read LDS half as often, in 290 registers: one
+//    workgroup a CU.  The next tile's scores under this one's softmax and rings of 4 to 8 tiles gained nothing.
+//  - one sequence: latency.  4,096 tokens with 64 nodes: 20, of them 5 until the first tile is there (the cuts, the
+//    block table, Q and the tile follow each other), 8 tiles at 0.9 and 2 for the partials.
+// fp32: v_mfma_f32_32x32x2 has a sixteenth of the rate, and waves of a row tile that is not full do nothing; 64
+// sequences of 512 to 2,048 with 4 to 8 nodes, 64 dims, 116, 1.6 times the bytes' floor.
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_kernel(TreeArgs) {
   __shared__ __attribute__((aligned(16))) char ring[ring_bytes<T, D>()];
@@ -1102,7 +1113,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a
 
 // ---------------------------------------------------------------- the plan --
 
-// Key tiles of a piece that is worth its partials, 16 bits and fp32 (whose tiles take 16 times the time).
+// Key tiles of a piece that is worth its partials, 16 bits and fp32 (whose tiles take 16 times the time).  In 16 bits 4
+// and 16 measured the same or slower.
 constexpr int kLeast = 8, kLeastF32 = 1;
 
 // Parts of a segment from which on a batch is few segments in many: its pieces are short and end all at once, and what
