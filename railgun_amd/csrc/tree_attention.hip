@@ -1014,9 +1014,11 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
 
 // The rows of a cut segment: D / 4 lanes have 4 dims each of a row, a wave N times 256 / D rows.  Where a batch is few
 // segments in many pieces (kManyParts), the waves of a workgroup have the same rows (SPLIT), each every fourth piece, and
-// their results are joined in LDS: a wave alone would wait for 64 pieces eight times.  Elsewhere a segment is in two
-// or three.  AHEAD: pieces in flight.  Measured (us, a wave alone / split; bf16, 32 / 8 heads of 128, 16 nodes):
-// one sequence of 32,768 14.5 / 7.4, four of 4,096 6.4 / 6.1, one of 2,048 4.0 / 3.9.
+// their results are joined in LDS: a wave alone would wait for 64 pieces eight times.  AHEAD: pieces in flight, 8, or 2
+// where few segments are cut at all.  Measured (us; bf16, 32 / 8 heads of 128, 16 nodes): a wave alone / split, one
+// sequence of 32,768 14.5 / 7.4, four of 4,096 6.4 / 6.1, one of 2,048 4.0 / 3.9.  Two rows a wave and four pieces ahead / one
+// and eight, 17 sequences of up to 3,900 (fp16, 28 / 4 heads) 8.6 / 7.4, four of 32,768 with 128 nodes 12.4 / 11.4; four
+// rows and two pieces / two and two, 64 of up to 4,096 9.1 / 8.0.
 constexpr int kMergeWaves = 4;
 template <int D> constexpr int merge_rows() { return 256 / D; }
 
@@ -1163,8 +1165,8 @@ void launch_product(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3(groups, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), dim3(64 * kMergeWaves), 0, s, a);
   };
   if (p.cut_in >= kManyParts) merge(tree_merge_kernel<T, D, 1, 8, true>, 1);
-  else if (p.cut_in >= 2) merge(tree_merge_kernel<T, D, 2, 4, false>, 2 * kMergeWaves);
-  else merge(tree_merge_kernel<T, D, 4, 2, false>, 4 * kMergeWaves);
+  else if (p.cut_in >= 2) merge(tree_merge_kernel<T, D, 1, 8, false>, kMergeWaves);
+  else merge(tree_merge_kernel<T, D, 2, 2, false>, 2 * kMergeWaves);
 }
 
 }  // namespace
