@@ -87,7 +87,7 @@ struct TreeArgs {
   int32_t group, bs_shift;
   int32_t slots, slots_full;  // pieces that a batch is cut into: as many as are at work together if they are long
   int32_t least;     // key tiles of a piece that is worth its partials
-  int32_t parts_past;  // partials are written past the L2
+  int32_t parts_past;  // partials of short pieces are written past the L2
 };
 
 // Any shape: a wave per (sequence, node, q-head), lane l has dims 4 l .. 4 l + 3, the keys one after the other with
@@ -420,7 +420,7 @@ __device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, cons
     const int64_t at = (int64_t)p.slot * kRows + in;
     float* acc = a.acc + at * D + 4 * hh;
     auto part = [&](int db, int i) { return f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]}; };
-    if (a.parts_past) {
+    if (a.parts_past && p.kt1 - p.kt0 < kLongPiece) {
       asm volatile("" ::: "memory");  // (or the two kinds of stores are made one, before the branch or behind it)
 #pragma unroll
       for (int db = 0; db < D / 32; ++db)
@@ -1119,11 +1119,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a
 // and 16 measured the same or slower.
 constexpr int kLeast = 8, kLeastF32 = 1;
 
-// Parts of a segment from which on a batch is few segments in many: its pieces are short and end all at once, and what
-// the L2s then hold of partials has to leave them before the merge starts.  Written past them the wait is shorter; where
-// the pieces end one after the other it only costs the merge its L2 hits.  Measured (us, through / past; bf16, 32 / 8
-// heads of 128): one sequence of 4,096 with 64 nodes 30.0 / 27.1, four of 4,096 with 16 30.8 / 29.8; 64 of up to 4,096
-// (one or two parts) 133.7 / 139.0; 17 of up to 3,900 (fp16, 28 / 4 heads; three) 38.8 / 42.6.
+// Parts of a segment from which on a batch is few segments in many: if its pieces are short they end all at once, and
+// what the L2s then hold of partials has to leave them before the merge starts.  Written past them the wait is shorter;
+// where pieces end one after the other it only costs the merge its L2 hits.  Measured (us, through / past; bf16, 32 / 8
+// heads of 128): one sequence of 4,096 with 64 nodes 30.3 / 26.6, of 16,384 42.2 / 40.9, in pieces of 32 tiles of 32,768
+// 60.4 / 62.9 and of 65,536 97.9 / 102.5; 64 of up to 4,096 (one or two parts) 133.7 / 139.0; 17 of up to 3,900 (fp16, 28 / 4
+// heads; three) 38.8 / 42.6.
 constexpr int kManyParts = 8;
 
 struct TreePlan {
