@@ -409,39 +409,40 @@ __device__ __forceinline__ float if_bit(uint32_t bits, int b, float x) {
   return __uint_as_float((__float_as_uint(x) & on) | (0xff800000u & ~on));
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, const f32x16_t (&o)[D / 32], float m,
-                                           float l) {
+// The lane's row, NB blocks of 32 dims from d0 on.
+template <typename T, int D, int NB = D / 32>
+__device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, const f32x16_t (&o)[NB], float m, float l,
+                                           int d0 = 0) {
   const Args& a = arguments();
   using S = typename elem<T>::storage;
   const int in = row - p.row0;
   if (row >= p.rows) return;
   if (p.slot >= 0) {
     const int64_t at = (int64_t)p.slot * kRows + in;
-    float* acc = a.acc + at * D + 4 * hh;
+    float* acc = a.acc + at * D + d0 + 4 * hh;
     auto part = [&](int db, int i) { return f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]}; };
     if (a.parts_past && p.kt1 - p.kt0 < kLongPiece) {
       asm volatile("" ::: "memory");  // (or the two kinds of stores are made one, before the branch or behind it)
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           __builtin_nontemporal_store(part(db, i), reinterpret_cast<f32x4_t*>(acc + 32 * db + 8 * i));
       asm volatile("" ::: "memory");
     } else {
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4_t*>(acc + 32 * db + 8 * i) = part(db, i);
     }
-    if (hh == 0) *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(m, l);
+    if (hh == 0 && d0 == 0) *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(m, l);
     return;
   }
   const int node = row / a.group, g = row - node * a.group;
-  S* out = static_cast<S*>(a.out) + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D;
+  S* out = static_cast<S*>(a.out) + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D + d0;
   const float inv = l != 0.f ? 1.f / l : 1.f;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
+  for (int db = 0; db < NB; ++db)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float x0 = o[db][4 * i] * inv, x1 = o[db][4 * i + 1] * inv, x2 = o[db][4 * i + 2] * inv,
@@ -454,9 +455,9 @@ __device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, cons
 
 // Adds to the lane's row what V holds that is not finite, of the keys `sick` that the row attends to (`mine`).  The
 // values come from the cache, 4 dims at a time as the accumulators have them; times any weight they stay what they are.
-template <typename T, int D>
+template <typename T, int D, int NB = D / 32>
 __device__ __forceinline__ void add_not_finite(const Piece& p, int kt, uint32_t sick, uint32_t mine, int hh,
-                                               f32x16_t (&o)[D / 32]) {
+                                               f32x16_t (&o)[NB], int d0 = 0) {
   const Args& a = arguments();
   const int32_t* row_table = a.table + (int64_t)p.seq * a.max_blocks;
   using E = elem<T>;
@@ -466,10 +467,10 @@ __device__ __forceinline__ void add_not_finite(const Piece& p, int kt, uint32_t 
     sick &= sick - 1;
     const int at = kt * kTileKeys + key;
     const S* v = static_cast<const S*>(a.v) + (int64_t)row_table[at / a.block_size] * a.kv_stride +
-                 ((int64_t)p.kvh * a.block_size + at % a.block_size) * D;
+                 ((int64_t)p.kvh * a.block_size + at % a.block_size) * D + d0;
     const bool takes = mine >> key & 1;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -769,21 +770,30 @@ struct KeyTileF32 {
   static constexpr int STAGES = 2;
   static constexpr int CH = D / 4;           // 16-byte chunks of a row
   static constexpr int SUB_COPIES = D / 16;  // 1 KB copies of a sub-block's K, and of its V
+  // The scores that waves exchange, 16 a lane: in K's place where they fit, else behind the ring.
+  static constexpr int SHARED = 64 * kTreeWaves * 16 * 4;
+  static constexpr bool SHARED_IN_RING = KB >= SHARED;
+  static constexpr int LDS = STAGES * BYTES + (SHARED_IN_RING ? 0 : SHARED);
 };
 
-template <int D>
+// WAYS = 2, where a piece has at most 64 rows: waves w and w + 2 have the same rows and half of the dims each.  Each
+// adds up its dims' part of the scores, the two exchange them through LDS (at head_dim 128 over the K that all are
+// done with; a + b is b + a, so both go on with the same scores), and each has its dims of the output.  Otherwise the
+// matrix units of two SIMDs stood idle.  Measured (us, 1 / 2): FIGURES
+template <int D, int WAYS>
 __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t* sick,
-                                        uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
+                                            uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
   const Args& a = arguments();
   using TL = KeyTileF32<D>;
-  constexpr int NDB = D / 32, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF, HD = D / 2;
+  constexpr int NDB = D / 32 / WAYS, HALF = TL::SUB_COPIES / 2, COPIES = 2 * HALF, HD = D / WAYS / 2;
   const float* q = static_cast<const float*>(a.q);
   const float* kc = static_cast<const float*>(a.k);
   const float* vc = static_cast<const float*>(a.v);
   const int32_t* table = a.table + (int64_t)p.seq * a.max_blocks;
   const int j = lane & 31, hh = lane >> 5;
-  const int row = p.row0 + w * 32 + j;
-  const bool busy = p.row0 + w * 32 < p.rows;
+  const int w_row = WAYS == 2 ? w & 1 : w, d0 = WAYS == 2 ? (w >> 1) * (D / 2) : 0;
+  const int row = p.row0 + w_row * 32 + j;
+  const bool busy = p.row0 + w_row * 32 < p.rows;
   const int node = min(row, p.rows - 1) / a.group, g = min(row, p.rows - 1) - node * a.group;
   const int subs = (p.ctx + kBS - 1) / kBS;
   const int cb = w >> 1, cp = w & 1;
@@ -797,7 +807,7 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
   if (masks_from < p.kt1) fill_masks(p, node, masks_from, w * 32 + j, hh, masks);
   float qf[HD];
   {
-    const float4* qr = reinterpret_cast<const float4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D + hh * HD);
+    const float4* qr = reinterpret_cast<const float4*>(q + ((int64_t)(p.first + node) * a.num_heads + p.kvh * a.group + g) * D + d0 + hh * HD);
     const float on = a.q_sign == 0 ? 0.f : a.q_sign & 0x8000u ? -1.f : 1.f;
 #pragma unroll
     for (int i = 0; i < HD / 4; ++i) {
@@ -851,19 +861,22 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
     wave_lds_sync();  // (the copies in flight stay in flight)
     tile_barrier();
   };
-  auto compute = [&](int kt, int st, bool masked) __attribute__((always_inline)) {
+  auto scores = [&](int st) __attribute__((always_inline)) -> f32x16_t {
     const char* krow = lds + st * TL::BYTES + j * (D * 4);
     f32x16_t c;
 #pragma unroll
     for (int v = 0; v < 16; ++v) c[v] = 0.f;
 #pragma unroll
     for (int i = 0; i < HD / 4; ++i) {
-      const float4 k4 = *reinterpret_cast<const float4*>(krow + 16 * ((hh * (HD / 4) + i) ^ (j & 7)));
+      const float4 k4 = *reinterpret_cast<const float4*>(krow + 16 * ((d0 / 4 + hh * (HD / 4) + i) ^ (j & 7)));
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.x, qf[4 * i], c, 0, 0, 0);
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.y, qf[4 * i + 1], c, 0, 0, 0);
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.z, qf[4 * i + 2], c, 0, 0, 0);
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.w, qf[4 * i + 3], c, 0, 0, 0);
     }
+    return c;
+  };
+  auto finish = [&](f32x16_t c, int kt, int st, bool masked) __attribute__((always_inline)) {
     uint32_t mine = ~0u;
     if (masked) {
       if (kt - masks_from >= kMaskTiles) fill_masks(p, node, masks_from = kt, w * 32 + j, hh, masks);
@@ -892,13 +905,38 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
       c[v] = fast_exp2(fmaf(c[v], a.scale_log2, -sub));
       l_run += c[v];
     }
-    const float* vrow = reinterpret_cast<const float*>(lds + st * TL::BYTES + TL::KB) + 4 * hh * D + j;
+    const float* vrow = reinterpret_cast<const float*>(lds + st * TL::BYTES + TL::KB) + 4 * hh * D + d0 + j;
 #pragma unroll
     for (int v = 0; v < 16; ++v)
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
         o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[(8 * (v >> 2) + (v & 3)) * D + 32 * db], c[v], o[db], 0, 0, 0);
-    if (masked && sick[sick_word(p, kt)] != 0) add_not_finite<f32_t, D>(p, kt, sick[sick_word(p, kt)], mine, hh, o);
+    if (masked && sick[sick_word(p, kt)] != 0) add_not_finite<f32_t, D, NDB>(p, kt, sick[sick_word(p, kt)], mine, hh, o, d0);
+  };
+  // Both halves' scores of a row.
+  auto exchange = [&](f32x16_t& c, int st) __attribute__((always_inline)) {
+    float4* const all = reinterpret_cast<float4*>(lds + (TL::SHARED_IN_RING ? st * TL::BYTES : TL::STAGES * TL::BYTES));
+    if constexpr (TL::SHARED_IN_RING) {
+      wave_lds_sync();
+      tile_barrier();  // all are done with K
+    }
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        all[(w * 4 + i) * 64 + lane] = make_float4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+    }
+    wave_lds_sync();
+    tile_barrier();
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 x = all[((w ^ 2) * 4 + i) * 64 + lane];
+        c[4 * i] += x.x;
+        c[4 * i + 1] += x.y;
+        c[4 * i + 2] += x.z;
+        c[4 * i + 3] += x.w;
+      }
+    }
   };
   __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // vmcnt(0): the window and Q
   issue(p.kt0, 0);
@@ -910,27 +948,32 @@ __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t*
     asm volatile("" ::: "memory");
     if (kt + 1 < p.kt1) __builtin_amdgcn_s_waitcnt(COPIES | 0x70 | 0xF00);
     else __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
+    wave_lds_sync();
     tile_barrier();  // tile kt has landed for every wave
     const bool masked = (kt + 1) * kTileKeys > p.prior;
     if (masked) clean(kt, st);
-    if (busy) compute(kt, st, masked);
+    f32x16_t c{};
+    if (busy) c = scores(st);
+    if constexpr (WAYS == 2) exchange(c, st);
+    if (busy) finish(c, kt, st, masked);
     if (kt + 2 < p.kt1) {
       if (kt + 2 - wb >= 64) {
         wb = kt + 2;
         fill();
         __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);
       }
+      wave_lds_sync();
       tile_barrier();  // every wave is done with the stage
       issue(kt + 2, st);
     }
   }
   const float l = l_run + __shfl_xor(l_run, 32, 64);
-  if (busy) store_rows<f32_t, D>(p, row, hh, o, m_run, l);
+  if (busy) store_rows<f32_t, D, NDB>(p, row, hh, o, m_run, l, d0);
 }
 
 template <typename T, int D>
 constexpr int ring_bytes() {
-  if constexpr (std::is_same_v<T, f32_t>) return KeyTileF32<D>::STAGES * KeyTileF32<D>::BYTES;
+  if constexpr (std::is_same_v<T, f32_t>) return KeyTileF32<D>::LDS;
   else return KeyTile<D>::STAGES * KeyTile<D>::BYTES;
 }
 // Workgroups to a CU: what their registers allow (168 a wave for three) and the rings, 64 KB in fp32 at head_dim 128.
@@ -1006,7 +1049,8 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
       for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
     store_rows<T, D>(p, row, lane >> 5, o, -INFINITY, 0.f);
   } else if constexpr (std::is_same_v<T, f32_t>) {
-    product_f32<D>(p, ring, sick, masks, w, lane);
+    if (p.rows - p.row0 <= kRows / 2) product_f32<D, 2>(p, ring, sick, masks, w, lane);
+    else product_f32<D, 1>(p, ring, sick, masks, w, lane);
   } else {
     product<T, D>(p, ring, sick, masks, w, lane);
   }
