@@ -86,7 +86,8 @@ struct TreeArgs {
   uint32_t q_sign;   // bit 0: q is taken (else zeros, a scale of 0), bits 15 and 31: negated (a negative scale)
   int32_t group, bs_shift;
   int32_t slots, slots_full;  // pieces that a batch is cut into: as many as are at work together if they are long
-  int32_t least;     // key tiles of a piece that is worth its partials
+  int32_t least;       // key tiles of a piece that is worth its partials
+  int32_t long_piece;  // and of one that is long
   int32_t parts_past;  // partials of short pieces are written past the L2
 };
 
@@ -222,11 +223,6 @@ __device__ __forceinline__ int ceil_quotient(int x, int d, float by) {
 // total / pieces and total / (pieces - segments), where every segment's last piece may be short, a lane each tries 64
 // lengths; the waves share the sequences.
 // `own`: the thread's sequence of the first kTreeThreads.
-// Key tiles of a piece from which on the chip is filled with them; of shorter ones two go to a CU, whose start and
-// partials cost less than a third hides.  Measured (us, two / three a CU; bf16, 32 / 8 heads of 128): 4 sequences of
-// 32,768 with 128 nodes, 160 to 250 tiles a piece 291 / 279; 17 of up to 3,900 with up to 37 (fp16, 28 / 4 heads), 4 to 15
-// tiles 39 / 45.
-constexpr int kLongPiece = 24;
 struct Cut {
   int tiles, pieces;  // a piece's length; how many there are
   bool alone;         // no sequence has more than one row tile
@@ -263,7 +259,7 @@ __device__ __forceinline__ Cut piece_tiles(const Args& a, CutScratch& sh, const 
   }
   Cut cut{longest, segments, widest == 1};
   if (segments == 0) return cut;
-  const int most = (int)most_pieces(segments, tiles >= kLongPiece * a.slots_full ? a.slots_full : a.slots);
+  const int most = (int)most_pieces(segments, tiles >= a.long_piece * a.slots_full ? a.slots_full : a.slots);
   const int lo = max(a.least, tiles / most), hi = max(lo, min(longest, tiles / (most - segments) + 1));
   if (lo >= longest) return cut;
   const int mine = lo + (hi - lo) * lane / 63;
@@ -421,7 +417,7 @@ __device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, cons
     const int64_t at = (int64_t)p.slot * kRows + in;
     float* acc = a.acc + at * D + d0 + 4 * hh;
     auto part = [&](int db, int i) { return f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]}; };
-    if (a.parts_past && p.kt1 - p.kt0 < kLongPiece) {
+    if (a.parts_past && p.kt1 - p.kt0 < a.long_piece) {
       asm volatile("" ::: "memory");  // (or the two kinds of stores are made one, before the branch or behind it)
 #pragma unroll
       for (int db = 0; db < NB; ++db)
@@ -779,7 +775,8 @@ struct KeyTileF32 {
 // WAYS = 2, where a piece has at most 64 rows: waves w and w + 2 have the same rows and half of the dims each.  Each
 // adds up its dims' part of the scores, the two exchange them through LDS (at head_dim 128 over the K that all are
 // done with; a + b is b + a, so both go on with the same scores), and each has its dims of the output.  Otherwise the
-// matrix units of two SIMDs stood idle.  Measured (us, 1 / 2): FIGURES
+// matrix units of two SIMDs stood idle.  Measured (us, 1 / 2 ways; 32 / 8 heads, 16 sequences of 512 to 2,048 with 8 to 16
+// nodes): head_dim 128 117 / 82, 64 66.7 / 48.6.  Four ways up to 32 rows measured the same as two.
 template <int D, int WAYS>
 __device__ __forceinline__ void product_f32(const Piece& p, char* lds, uint32_t* sick,
                                             uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
@@ -976,8 +973,9 @@ constexpr int ring_bytes() {
   if constexpr (std::is_same_v<T, f32_t>) return KeyTileF32<D>::LDS;
   else return KeyTile<D>::STAGES * KeyTile<D>::BYTES;
 }
-// Workgroups to a CU: what their registers allow (168 a wave for three) and the rings, 64 KB in fp32 at head_dim 128.
-constexpr int pieces_per_cu(int32_t dtype, int D) { return dtype == RG_DTYPE_F32 ? 2 : D == 128 ? 3 : 4; }
+// Workgroups to a CU: what their registers allow (168 a wave for three) and the rings, 64 KB in fp32 at head_dim 128
+// and 48 at 64.
+constexpr int pieces_per_cu(int32_t dtype, int D) { return D == 128 ? (dtype == RG_DTYPE_F32 ? 2 : 3) : dtype == RG_DTYPE_F32 ? 3 : 4; }
 template <typename T, int D>
 constexpr int groups_per_cu() { return pieces_per_cu(std::is_same_v<T, f32_t> ? RG_DTYPE_F32 : RG_DTYPE_BF16, D); }
 
@@ -990,8 +988,8 @@ constexpr int groups_per_cu() { return pieces_per_cu(std::is_same_v<T, f32_t> ? 
 //    workgroup a CU.  The next tile's scores under this one's softmax and rings of 4 to 8 tiles gained nothing.
 //  - one sequence: latency.  4,096 tokens with 64 nodes: 20, of them 5 until the first tile is there (the cuts, the
 //    block table, Q and the tile follow each other), 8 tiles at 0.9 and 2 for the partials.
-// fp32: v_mfma_f32_32x32x2 has a sixteenth of the rate, and waves of a row tile that is not full do nothing; 64
-// sequences of 512 to 2,048 with 4 to 8 nodes, 64 dims, 116, 1.6 times the bytes' floor.
+// fp32: v_mfma_f32_32x32x2 has a sixteenth of the rate, and what a row tile lacks of rows is computed all the same; 64
+// sequences of 512 to 2,048 with 4 to 8 nodes, 64 dims, 108, 1.5 times the bytes' floor.
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_kernel(TreeArgs) {
   __shared__ __attribute__((aligned(16))) char ring[ring_bytes<T, D>()];
@@ -1163,6 +1161,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a
 // and 16 measured the same or slower.
 constexpr int kLeast = 8, kLeastF32 = 1;
 
+// Key tiles of a piece from which on the chip is filled with them; of shorter ones two go to a CU, whose start and
+// partials cost less than a third hides.  Measured (us, two / three a CU; bf16, 32 / 8 heads of 128): 4 sequences of
+// 32,768 with 128 nodes, 160 to 250 tiles a piece 291 / 279; 17 of up to 3,900 with up to 37 (fp16, 28 / 4 heads), 4 to 15
+// tiles 39 / 45.  fp32 of 64 dims, whose tiles take longer: 16 of 512 to 2,048 with 8 to 16 nodes 48.5 / 44.4.
+constexpr int kLongPiece = 24, kLongPieceF32 = 4;
+
 // Parts of a segment from which on a batch is few segments in many: if its pieces are short they end all at once, and
 // what the L2s then hold of partials has to leave them before the merge starts.  Written past them the wait is shorter;
 // where pieces end one after the other it only costs the merge its L2 hits.  Measured (us, through / past; bf16, 32 / 8
@@ -1322,6 +1326,7 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
     a.slots = p.slots;
     a.slots_full = p.slots_full;
     a.least = dtype == RG_DTYPE_F32 ? kLeastF32 : kLeast;
+    a.long_piece = dtype == RG_DTYPE_F32 ? kLongPieceF32 : kLongPiece;
     a.parts_past = p.cut_in >= kManyParts;
     return dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
