@@ -219,6 +219,12 @@ __device__ __forceinline__ int ceil_quotient(int x, int d, float by) {
   return q - ((int)__umul24(q - 1, d) >= x);
 }
 
+// Key tiles of a piece from which on the chip is filled with them; of shorter ones two go to a CU, whose start and
+// partials cost less than a third hides.  Measured (us, two / three a CU; bf16, 32 / 8 heads of 128): 4 sequences of
+// 32,768 with 128 nodes, 160 to 250 tiles a piece 291 / 279; 17 of up to 3,900 with up to 37 (fp16, 28 / 4 heads), 4 to 15
+// tiles 39 / 45.  fp32 of 64 dims, whose tiles take longer: 16 of 512 to 2,048 with 8 to 16 nodes 48.5 / 44.4.
+constexpr int kLongPiece = 24, kLongPieceF32 = 4;
+
 // Key tiles to a piece: the least length (a.least and more) that makes no more pieces than most_pieces.  Between
 // total / pieces and total / (pieces - segments), where every segment's last piece may be short, a lane each tries 64
 // lengths; the waves share the sequences.
@@ -417,7 +423,7 @@ __device__ __forceinline__ void store_rows(const Piece& p, int row, int hh, cons
     const int64_t at = (int64_t)p.slot * kRows + in;
     float* acc = a.acc + at * D + d0 + 4 * hh;
     auto part = [&](int db, int i) { return f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]}; };
-    if (a.parts_past && p.kt1 - p.kt0 < a.long_piece) {
+    if (a.parts_past && p.kt1 - p.kt0 < (std::is_same_v<T, f32_t> ? kLongPieceF32 : kLongPiece)) {
       asm volatile("" ::: "memory");  // (or the two kinds of stores are made one, before the branch or behind it)
 #pragma unroll
       for (int db = 0; db < NB; ++db)
@@ -1160,12 +1166,6 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_merge_kernel(TreeArgs a
 // Key tiles of a piece that is worth its partials, 16 bits and fp32 (whose tiles take 16 times the time).  In 16 bits 4
 // and 16 measured the same or slower.
 constexpr int kLeast = 8, kLeastF32 = 1;
-
-// Key tiles of a piece from which on the chip is filled with them; of shorter ones two go to a CU, whose start and
-// partials cost less than a third hides.  Measured (us, two / three a CU; bf16, 32 / 8 heads of 128): 4 sequences of
-// 32,768 with 128 nodes, 160 to 250 tiles a piece 291 / 279; 17 of up to 3,900 with up to 37 (fp16, 28 / 4 heads), 4 to 15
-// tiles 39 / 45.  fp32 of 64 dims, whose tiles take longer: 16 of 512 to 2,048 with 8 to 16 nodes 48.5 / 44.4.
-constexpr int kLongPiece = 24, kLongPieceF32 = 4;
 
 // Parts of a segment from which on a batch is few segments in many: if its pieces are short they end all at once, and
 // what the L2s then hold of partials has to leave them before the merge starts.  Written past them the wait is shorter;
