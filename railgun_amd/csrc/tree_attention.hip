@@ -87,7 +87,8 @@ struct TreeArgs {
   int32_t group, bs_shift;
   int32_t slots, slots_full;  // pieces that a batch is cut into: as many as are at work together if they are long
   int32_t least;       // key tiles of a piece that is worth its partials
-  int32_t long_piece;  // and of one that is long
+  int32_t long_piece;  // of one that is long
+  int32_t short_piece; // of one that is too short for two a CU
   int32_t parts_past;  // partials of short pieces are written past the L2
 };
 
@@ -224,6 +225,12 @@ __device__ __forceinline__ int ceil_quotient(int x, int d, float by) {
 // 32,768 with 128 nodes, 160 to 250 tiles a piece 291 / 279; 17 of up to 3,900 with up to 37 (fp16, 28 / 4 heads), 4 to 15
 // tiles 39 / 45.  fp32 of 64 dims, whose tiles take longer: 16 of 512 to 2,048 with 8 to 16 nodes 48.5 / 44.4.
 constexpr int kLongPiece = 24, kLongPieceF32 = 4;
+// Shorter than that, two pieces a CU are worse than one of twice the length: half of the partials.  In batches of few
+// segments, whose pieces are all about as long (of many, one a CU is too coarse: 17 of up to 3,900 37 / 42).  Measured
+// (us, two / one a CU; 32 / 8 heads): head_dim 128, one sequence of 16,384 with 16 nodes 30.5 / 26.0, four of 4,096 with 32
+// 40.2 / 33.7, of 6,000 42.9 / 39.2, but one of 16,384 with 64 in pieces of 16 41.3 / 44.5; fp32, one of 2,048 with 16, 64
+// dims, 17.9 / 15.5.  At head_dim 64 in 16 bits no length gained for all (12,288 with 64 nodes 26.7 / 31.9).
+constexpr int kShortPiece = 13, kShortPieceF32 = 2, kFewSegments = 16;
 
 // Key tiles to a piece: the least length (a.least and more) that makes no more pieces than most_pieces.  Between
 // total / pieces and total / (pieces - segments), where every segment's last piece may be short, a lane each tries 64
@@ -265,7 +272,8 @@ __device__ __forceinline__ Cut piece_tiles(const Args& a, CutScratch& sh, const 
   }
   Cut cut{longest, segments, widest == 1};
   if (segments == 0) return cut;
-  const int most = (int)most_pieces(segments, tiles >= a.long_piece * a.slots_full ? a.slots_full : a.slots);
+  const bool few = kFewSegments * segments <= a.slots && tiles < a.short_piece * a.slots;
+  const int most = (int)most_pieces(segments, few ? a.slots / 2 : tiles >= a.long_piece * a.slots_full ? a.slots_full : a.slots);
   const int lo = max(a.least, tiles / most), hi = max(lo, min(longest, tiles / (most - segments) + 1));
   if (lo >= longest) return cut;
   const int mine = lo + (hi - lo) * lane / 63;
@@ -1327,6 +1335,7 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
     a.slots_full = p.slots_full;
     a.least = dtype == RG_DTYPE_F32 ? kLeastF32 : kLeast;
     a.long_piece = dtype == RG_DTYPE_F32 ? kLongPieceF32 : kLongPiece;
+    a.short_piece = dtype == RG_DTYPE_F32 ? kShortPieceF32 : head_dim == 128 ? kShortPiece : 0;
     a.parts_past = p.cut_in >= kManyParts;
     return dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
