@@ -87,6 +87,16 @@ def test_segments_near_a_round(device, kernels, long, short, d):
     TreeBatch(device, prior, trees(rng, [3] * (long + short)), heads=8, hkv=8, d=d, seed=long).check(kernels)
 
 
+@pytest.mark.parametrize("dtype,hkv,d,prior", [("bf16", 4, 128, [6000, 5500, 100, 6100]), ("f16", 8, 128, [27000]),
+                                               ("f32", 2, 64, [5000, 4990]), ("f32", 2, 64, [9000, 8900]),
+                                               ("bf16", 4, 64, [6000, 5500, 100, 6100])])
+def test_few_segments(device, kernels, dtype, hkv, d, prior):
+    """Few segments, cut into as many pieces as the chip has CUs and into more."""
+    rng = np.random.default_rng(len(prior) + d)
+    TreeBatch(device, prior, trees(rng, [3, 9, 1, 5][:len(prior)]), dtype, heads=2 * hkv, hkv=hkv, d=d,
+              seed=len(prior) + d).check(kernels)
+
+
 @pytest.mark.parametrize("d,nodes", [(64, 3), (128, 35)])
 def test_parts_of_a_segment(device, kernels, d, nodes):
     """Segments in one to 66 parts, a key tile each, of one row tile and of two."""
