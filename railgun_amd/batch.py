@@ -204,7 +204,7 @@ def _check_tree_blocks(draft_trees: Sequence[DraftTree], table: np.ndarray, ctx:
     first = len(ctx) - len(draft_trees)
     for s, d in enumerate(draft_trees):
         written = used[first + s, (d.seq_len - len(d.token_ids)) // block_size:-(-d.seq_len // block_size)]
-        if np.isin(used, written).sum() != len(written):
+        if len(np.unique(written)) != len(written) or np.isin(used, written).sum() != len(written):
             raise ValueError(f"a block of draft tree {s} appears twice in a step")
 
 

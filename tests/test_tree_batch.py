@@ -54,3 +54,13 @@ def test_blocks_of_a_tree_are_its_own():
         with pytest.raises(ValueError, match="appears twice"):
             step(a, b, slots)
     step([1, 2, 3], [4, 5, 6], [DecodeSlot(1, 8, [7, 8, 3])])   # an entry behind the slot's tokens
+
+
+@pytest.mark.parametrize("table,nodes", [([5, 5], 20), ([7, 5, 5], 20), ([5, 6, 5], 40), ([4, 4, 6], 33)])
+def test_a_block_twice_in_a_tree(table, nodes):
+    """Two of the tree's own tokens would share a slot."""
+    seq_len = 16 * len(table) - 7
+    tree = DraftTree([1] * nodes, list(range(-1, nodes - 1)), seq_len, table)
+    with pytest.raises(ValueError, match="appears twice"):
+        pack_step([], [], 16, draft_trees=[tree])
+    pack_step([], [], 16, draft_trees=[DraftTree([1] * nodes, tree.parents, seq_len, range(len(table)))])
