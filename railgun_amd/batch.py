@@ -200,12 +200,15 @@ def _check_tree_blocks(draft_trees: Sequence[DraftTree], table: np.ndarray, ctx:
     """Blocks that hold a tree's tokens belong to its sequence alone: what is kept of the tree moves in them."""
     if not draft_trees:
         return
-    used = np.where(np.arange(table.shape[1]) < -(-ctx // block_size)[:, None], table, -1)
-    first = len(ctx) - len(draft_trees)
-    for s, d in enumerate(draft_trees):
-        written = used[first + s, (d.seq_len - len(d.token_ids)) // block_size:-(-d.seq_len // block_size)]
-        if len(np.unique(written)) != len(written) or np.isin(used, written).sum() != len(written):
-            raise ValueError(f"a block of draft tree {s} appears twice in a step")
+    column, first = np.arange(table.shape[1]), len(ctx) - len(draft_trees)
+    ends = -(-ctx // block_size)[:, None]
+    starts = np.asarray([(d.seq_len - len(d.token_ids)) // block_size for d in draft_trees])[:, None]
+    trees, at = np.nonzero((column >= starts) & (column < ends[first:]))
+    # Every entry in use once, sorted; a block is there as often as it is named.
+    used, written = np.sort(table[column < ends]), table[first + trees, at]
+    twice = np.searchsorted(used, written, "right") - np.searchsorted(used, written) != 1
+    if twice.any():
+        raise ValueError(f"a block of draft tree {trees[twice.argmax()]} appears twice in a step")
 
 
 def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[DecodeSlot], block_size: int,
