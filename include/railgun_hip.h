@@ -215,9 +215,9 @@ int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
 /* A step that looks at a tree of drafted tokens per sequence and keeps the path that the model agrees
  * with.  Sequence s owns nodes [cu_nodes[s], cu_nodes[s + 1]) of the packed arrays, L of them (0: a
  * row that pads the batch); nodes from cu_nodes[num_seqs] on belong to nobody and are left as they
- * are.  max_nodes is the largest L, at most 1024.  parents[n] is the index of n's parent in the
- * sequence's own tree, below n's own; any other value (-1) says that n has none.  Node 0 is the token
- * decided last.  In the cache a tree lies behind the tokens before it: context_lens[s] counts its
+ * are.  max_nodes is the largest L, at most 1024; of a longer tree the nodes past it get no results and
+ * are not attended to.  parents[n] is the index of n's parent in the sequence's own tree, below n's
+ * own; any other value (-1) says that n has none.  Node 0 is the token decided last.  In the cache a tree lies behind the tokens before it: context_lens[s] counts its
  * nodes, node j is at position prior + j, prior = max(context_lens[s] - L, 0).  New entries: the
  * reference decodes one token per sequence and step.
  *

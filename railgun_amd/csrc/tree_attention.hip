@@ -158,15 +158,18 @@ __device__ __forceinline__ const Args& arguments() {
 
 // --------------------------------------------------------------- the cuts ---
 
-// A sequence as the cuts see it.
+// A sequence as the cuts see it.  Its context ends with the nodes that are asked for: a tree of more of them than
+// max_nodes says has neither rows for the others nor keys.
 struct Span {
   Tree t;
-  int ctx, tiles, row_tiles;
+  int prior, ctx, tiles, row_tiles;
 };
 __device__ __forceinline__ Span span_of(const Args& a, int s) {
   Span p;
   p.t = tree_of(a.cu, s, a.num_nodes, a.max_nodes);
-  p.ctx = max(0, min(a.context_lens[s], a.max_blocks * a.block_size));
+  const int cached = max(0, min(a.context_lens[s], a.max_blocks * a.block_size));
+  p.prior = max(cached - p.t.len, 0);
+  p.ctx = min(cached, p.prior + p.t.nodes);
   p.row_tiles = (p.t.nodes * a.group + kRows - 1) / kRows;
   // (A tree whose context is empty has one tile, without keys: its rows are cleared there.)
   p.tiles = max(1, (p.ctx + kTileKeys - 1) / kTileKeys);
@@ -396,10 +399,10 @@ __device__ __forceinline__ uint32_t tile_mask(const Piece& p, int node, int kt) 
   return left >= 32 ? m : left > 0 ? m & ((1u << left) - 1u) : 0u;
 }
 
-// Which keys of a tile hold a value that is not finite: a word for every tile that reaches into the tree.  (A tree of
-// more nodes than max_nodes says shares the last one.)
-constexpr int kSickWords = kMaxTreeNodes / kTileKeys + 2;
-__device__ __forceinline__ int sick_word(const Piece& p, int kt) { return min(kt - p.prior / kTileKeys, kSickWords - 1); }
+// Which keys of a tile hold a value that is not finite: a word for every tile that reaches into the tree, one more than
+// its nodes fill where it begins inside a tile.
+constexpr int kSickWords = kMaxTreeNodes / kTileKeys + 1;
+__device__ __forceinline__ int sick_word(const Piece& p, int kt) { return kt - p.prior / kTileKeys; }
 
 // A row's masks of kMaskTiles key tiles from tile `from` on, into LDS; a row's lanes l and l + 32 do half each.  Read
 // by their wave alone.
@@ -1031,8 +1034,8 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
     const int base = __builtin_amdgcn_readfirstlane(sh.base);
     Span sp;
     sp.t.first = __builtin_amdgcn_readfirstlane(sh.span.t.first);
-    sp.t.len = __builtin_amdgcn_readfirstlane(sh.span.t.len);
     sp.t.nodes = __builtin_amdgcn_readfirstlane(sh.span.t.nodes);
+    sp.prior = __builtin_amdgcn_readfirstlane(sh.span.prior);
     sp.ctx = __builtin_amdgcn_readfirstlane(sh.span.ctx);
     sp.tiles = __builtin_amdgcn_readfirstlane(sh.span.tiles);
     sp.row_tiles = __builtin_amdgcn_readfirstlane(sh.span.row_tiles);
@@ -1044,7 +1047,7 @@ __global__ __launch_bounds__(kTreeThreads, (groups_per_cu<T, D>())) void tree_ke
     p.rows = sp.t.nodes * a.group;
     p.first = sp.t.first;
     p.ctx = sp.ctx;
-    p.prior = max(sp.ctx - sp.t.len, 0);
+    p.prior = sp.prior;
     const int each = sp.tiles / n, longer = sp.tiles - each * n;  // the first few are a tile longer
     p.kt0 = each * cut + min(cut, longer);
     p.kt1 = each * (cut + 1) + min(cut + 1, longer);
