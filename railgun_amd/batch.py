@@ -50,8 +50,8 @@ class DecodeSlot:
     larger once tokens have been evicted).  ``scored_len``, for a step that gathers attention weights:
     how many of the leading cached tokens hold a score.  After such a step all seq_len do, whichever
     rows it had, so it is 0 after a prefill of fresh blocks and seq_len - 1 while every step since
-    gathered; a sequence that begins with another's blocks, or with copies of them, says how many of
-    the tokens in those hold one."""
+    gathered or checked a DraftTree (whose accepted tokens hold a score of 0); a sequence that begins with
+    another's blocks, or with copies of them, says how many of the tokens in those hold one."""
 
     last_token_id: int
     seq_len: int
@@ -225,7 +225,7 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     to step.
 
     ``draft_trees``: sequences that check drafted tokens in this step; they neither share a prefix nor
-    gather scores."""
+    gather scores, and their tokens' scores become 0 if the pool has any."""
     tokens, positions, slots, ctx, tables = [], [], [], [], []
     cu = [0]
     for c in prefill_chunks:

@@ -42,10 +42,10 @@ def _pairs(src: Sequence[int], dst: Sequence[int], nsrc: int, ndst: int, device)
     return m.to(device) if device is not None else m.pin_memory()
 
 
-def _new_score_rows(storage: torch.Tensor, **where) -> torch.Tensor:
-    """Zeros, fp32 [layers, NB, H_kv * bs and what rounds a row up to the 16 bytes that block copies go by]."""
+def _new_score_rows(storage: torch.Tensor, spare: int = 0, **where) -> torch.Tensor:
+    """Zeros, fp32 [layers, NB + spare, H_kv * bs and what rounds a row up to the 16 bytes that block copies go by]."""
     layers, blocks, _, hkv, bs, _ = storage.shape
-    return torch.zeros((layers, blocks, -(-hkv * bs // 4) * 4), dtype=torch.float32, **where)
+    return torch.zeros((layers, blocks + spare, -(-hkv * bs // 4) * 4), dtype=torch.float32, **where)
 
 
 class GpuBlockPool:
@@ -68,6 +68,7 @@ class GpuBlockPool:
         self._kernels = kernels
         self._score_rows: Optional[torch.Tensor] = None
         self._scores: Optional[torch.Tensor] = None
+        self._score_cells: Optional[torch.Tensor] = None  # the scores, and a block behind them that is no token's
 
     @staticmethod
     def for_model(cfg, num_blocks: int, block_size: int, device, dtype=torch.bfloat16,
@@ -97,17 +98,25 @@ class GpuBlockPool:
         if self._scores is None:
             if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the pool's scores are first asked for in a graph's capture: ask for them before it")
-            self._score_rows = _new_score_rows(self.storage, device=self.device)
+            rows = _new_score_rows(self.storage, spare=1, device=self.device)
             hkv, bs = self.storage.shape[3:5]
-            self._scores = self._score_rows[..., :hkv * bs].unflatten(-1, (hkv, bs))
+            self._score_cells = rows[..., :hkv * bs].unflatten(-1, (hkv, bs))
+            self._score_rows, self._scores = rows[:, :-1], self._score_cells[:, :-1]
         return self._scores
 
+    @property
+    def has_scores(self) -> bool:
+        """Whether scores have been asked for."""
+        return self._scores is not None
+
     def clear_scores(self, slots: torch.Tensor) -> None:
-        """Sets the scores of the tokens at ``slots`` (block * block_size + offset, on the device) to 0 in
-        every layer: they hold one from then on, of no weight."""
-        at, scores = slots.long(), self.scores
-        # (A zero on the device: a Python one is copied from the host, which a graph's capture refuses.)
-        scores[:, torch.div(at, self.block_size, rounding_mode="floor"), :, at % self.block_size] = scores.new_zeros(())
+        """Sets the scores of the tokens at ``slots`` (block * block_size + offset, on the device; one below 0 is
+        no token's) to 0 in every layer: they hold one from then on, of no weight."""
+        at, zero = slots.long(), self.scores.new_zeros(())
+        # (What has no slot goes to the block behind the pool's.  A zero on the device: a Python one is copied from
+        # the host, which a graph's capture refuses.)
+        block = torch.where(at < 0, self.num_blocks, torch.div(at, self.block_size, rounding_mode="floor"))
+        self._score_cells[:, block, :, at % self.block_size] = zero
 
     def evict(self, block_table: torch.Tensor, context_lens: torch.Tensor, budget: int, recent: int,
               protected_len: int = 0, dst_block_table: Optional[torch.Tensor] = None,
@@ -118,7 +127,8 @@ class GpuBlockPool:
 
         A token whose cell holds no score (cached by a step that did not gather, such as a prefill) ranks
         by whatever the cell holds: keep such within ``protected_len`` and ``recent``, or clear_scores
-        first.  Few long sequences are trimmed faster into other blocks than in place."""
+        first.  The tokens that steps over draft trees kept have a score of 0 and rank behind all that a step
+        gathered for.  Few long sequences are trimmed faster into other blocks than in place."""
         new_lens = torch.empty_like(context_lens)
         self.kernels.launch_evict(self.storage[:, :, 0], self.storage[:, :, 1], self.scores, block_table,
                                   dst_block_table, context_lens, new_lens, kept_positions, budget, recent,
@@ -130,7 +140,11 @@ class GpuBlockPool:
         """Keeps the accepted nodes of trees of drafted tokens, cached at the ends of the sequences of
         ``block_table``: they move down directly behind the tokens before their tree, with their scores if the
         pool has any, every layer in one call (launch_compact_tree); returns the new context lengths, int32 on
-        the device.  The blocks past a sequence's new length hold nothing it needs."""
+        the device.  The blocks past a sequence's new length hold nothing it needs.
+
+        No step gathers attention weights for a tree's tokens, or by them for the tokens before it: the
+        model's step sets their scores to 0 where the pool has some, and a caller who runs the operators one by
+        one calls clear_scores.  From then on they hold a score of no weight."""
         new_lens = torch.empty_like(context_lens)
         self.kernels.launch_compact_tree(self.storage[:, :, 0], self.storage[:, :, 1], self._scores, block_table,
                                          context_lens, cu_nodes, accepted, num_accepted, new_lens)

@@ -587,6 +587,8 @@ class RailgunLlama:
             self.kernels.launch_tree_layout(st.tree_parents, st.tree_cu, st.tree_lens, st.tree_table, st.tree_mask,
                                             st.positions[r:], st.slot_mapping[r:], self.pool.block_size,
                                             st.host.max_tree_nodes, st.tree_places)
+            if self.pool.has_scores:  # (what their cells held is an earlier owner's)
+                self.pool.clear_scores(st.slot_mapping[r:])
         H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
         if st.unscored_slots is not None:
