@@ -1202,9 +1202,9 @@ TreePlan plan_tree(int32_t num_seqs, int32_t max_nodes, int32_t H, int32_t Hkv, 
   // (The kernel goes by either.)
   const int64_t pieces = std::max(most_pieces(segments, p.slots), most_pieces(segments, p.slots_full));
   // (What the product does not take runs on the generic kernel.  The cuts count in 32 bits, a sequence's tiles in 22,
-  // its row tiles in 8.)
+  // its row tiles in 8; a grid has fewer than 2^32 threads.)
   if ((D != 64 && D != 128) || block_shift(bs) < 0 || tiles >= 1 << 22 || row_tiles > 255 ||
-      (double)segments * tiles > INT32_MAX || pieces > INT32_MAX - 8) {
+      (double)segments * tiles > INT32_MAX || pieces > UINT32_MAX / kTreeThreads - 8) {
     return p;
   }
   p.cut_in = (int32_t)std::min<int64_t>(p.slots_full / segments, kManyParts);
@@ -1217,9 +1217,10 @@ TreePlan plan_tree(int32_t num_seqs, int32_t max_nodes, int32_t H, int32_t Hkv, 
 }
 
 template <typename T, int D>
-void launch_product(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
+int launch_product(const char* op, const TreeArgs& a, const TreePlan& p, hipStream_t s) {
   hipLaunchKernelGGL((tree_kernel<T, D>), dim3((unsigned)p.groups), dim3(kTreeThreads), 0, s, a);
-  if (p.tiles <= a.least) return;  // nothing is cut
+  const int st = check_launch(op);                  // (the merge goes by what the product leaves in the workspace)
+  if (st != RG_OK || p.tiles <= a.least) return st;  // nothing is cut
   auto merge = [&](auto kernel, int rows) {
     const unsigned groups = (unsigned)ceil_div((int64_t)a.max_nodes * a.group, rows * merge_rows<D>());
     hipLaunchKernelGGL(kernel, dim3(groups, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), dim3(64 * kMergeWaves), 0, s, a);
@@ -1227,6 +1228,7 @@ void launch_product(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
   if (p.cut_in >= kManyParts) merge(tree_merge_kernel<T, D, 1, 8, true>, 1);
   else if (p.cut_in >= 2) merge(tree_merge_kernel<T, D, 1, 8, false>, kMergeWaves);
   else merge(tree_merge_kernel<T, D, 2, 2, false>, 2 * kMergeWaves);
+  return check_launch(op);
 }
 
 }  // namespace
@@ -1342,9 +1344,8 @@ extern "C" int rg_paged_attention_tree(const void* query, const void* key_cache,
     a.parts_past = p.cut_in >= kManyParts;
     return dispatch_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
-      if (head_dim == 128) launch_product<T, 128>(a, p, as_stream(stream));
-      else launch_product<T, 64>(a, p, as_stream(stream));
-      return check_launch(op);
+      return head_dim == 128 ? launch_product<T, 128>(op, a, p, as_stream(stream))
+                             : launch_product<T, 64>(op, a, p, as_stream(stream));
     });
   }
   const dim3 grid((unsigned)max_nodes, (unsigned)num_heads, (unsigned)num_seqs);

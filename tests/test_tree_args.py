@@ -135,3 +135,11 @@ def test_workspace_queries():
     for bad in ((-1, 6, 8, 2, 64, 16, 4), (2, 0, 8, 2, 64, 16, 4), (2, 6, 7, 2, 64, 16, 4), (2, 6, 8, 0, 64, 16, 4),
                 (2, 2000, 8, 2, 64, 16, 4)):
         assert lib.rg_paged_attention_tree_workspace_bytes(*bad) == 0
+
+
+def test_attention_of_more_pieces_than_a_grid_has():
+    """Segments past the 2^32 threads of a grid go to the form that has a workgroup per node and head (no workspace)."""
+    lib = railgun_amd.load_library()
+    assert lib.rg_paged_attention_tree_workspace_bytes(65535, 1024, 64, 8, 128, 16, 40) == 0
+    assert lib.rg_paged_attention_tree_workspace_bytes(32768, 1024, 64, 8, 128, 16, 40) == 0     # 2^24 segments
+    assert lib.rg_paged_attention_tree_workspace_bytes(32000, 1024, 64, 8, 128, 16, 40) > 0
