@@ -226,7 +226,9 @@ int rg_evict_cache(void* key_cache, void* value_cache, float* scores,
  *     one of its ancestors (mask_words at least max_nodes / 32 rounded up, at most 32; all of a
  *     node's words are written);
  *   positions: text_positions[s] (NULL: prior) plus the node's depth, for the rotation;
- *   slot_mapping: the slot of cache position prior + j, -1 where the context ends before it. */
+ *   slot_mapping: the slot of cache position prior + j, -1 where the context ends before it.  (Rows of
+ *     nobody keep theirs: a caller who replays a captured step with fewer nodes than before sets the
+ *     rest to -1, or the cache write goes to the slots of the earlier ones.) */
 int rg_tree_layout(const int32_t* parents, const int32_t* cu_nodes, const int32_t* context_lens,
                    const int32_t* block_table, const int32_t* text_positions, int32_t* tree_mask,
                    int32_t* positions, int32_t* slot_mapping, int32_t block_size,
