@@ -1,11 +1,16 @@
-"""Attention of draft trees of more nodes than they are declared to have."""
+"""Attention of draft trees past its declared limits, at scores where fp32 runs out of steps, and at long contexts in the
+form that takes any shape; lengths of accepted paths."""
 from __future__ import annotations
+
+import math
 
 import numpy as np
 import pytest
 import torch
 
-from tree64 import TreeBatch, ancestors, random_tree
+from attention64 import HALF_STEP, U
+from test_gpu_tree import check_verify
+from tree64 import TreeBatch, accept, ancestors, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +58,83 @@ def test_values_that_are_not_finite_in_a_tree_past_the_most(device, kernels, dty
     assert torch.isfinite(clean[:1029]).all() and torch.equal(got[:1029][healthy], clean[:1029][healthy])
     assert not torch.isfinite(got[:1029][~healthy]).all(-1).any()
     assert torch.isnan(got[1029:]).all()                               # (left as they were)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("first,step", [(2 ** 20 - 4000, 0), (2 ** 20 - 12, 0), (2 ** 20 - 6, 1), (2 ** 20 - 40, 4),
+                                        (2 ** 20 + 5, 0), (3 * 2 ** 19, 0)])
+def test_scores_around_two_to_the_twenty(device, kernels, dtype, d, first, step):
+    """Scores (in log2 units) of ``first`` and a few more, ``step`` more every 300 tokens, so that the maximum passes
+    2^20, where fp16's probabilities change their factor, in the middle of a piece, between the pieces of one
+    sequence, or nowhere.
+
+    The products are of whole numbers that every type holds: q is 1 in one dim, 2^4 in one and 2^7 in the others, K at
+    most 2^8, so their sums are exact in fp32.  On the matrix cores a score is multiplied and its reference subtracted in
+    one rounding, so its error is relative to the distance from the maximum; the form for other dims rounds the score
+    first, by half a step of fp32 at its size.  In fp16 a probability below 2^-14 is off by 2^-25 at most, where the
+    largest is 1 at least."""
+    n, nodes = 1500, 6
+    b = TreeBatch(device, [n, 40], [random_tree(np.random.default_rng(1), nodes), [-1]], dtype, heads=4, hkv=2, d=d, seed=3,
+                  scale=math.log(2))
+    g = torch.Generator(device=device).manual_seed(first)
+    score = first + torch.randint(0, 7, (b.kc.shape[0], 16), generator=g, device=device)
+    for s in range(2):
+        t = np.arange(int(b.ctx[s]))
+        score[b.table[s, t // 16], t % 16] += torch.as_tensor(t // 300 * step, device=device)
+    # score = 2^7 high + 2^4 k_(d - 2) + k_(d - 1), high spread over the other dims.
+    high = score // 128
+    k = (high // (d - 2))[..., None] + (torch.arange(d, device=device) < (high % (d - 2))[..., None]).long()
+    k[..., d - 2], k[..., d - 1] = score // 16 % 8, score % 16
+    q = torch.full((d,), 128, dtype=torch.int64, device=device)
+    q[d - 2], q[d - 1] = 16, 1
+    assert torch.equal((k * q).sum(-1), score)
+    assert all(torch.equal(x.to(b.kc.dtype).to(torch.int64), x) for x in (k, q))
+    used = ~torch.isnan(b.kc[:, 0, :, 0])
+    b.kc.copy_(torch.where(used[:, None, :, None], k[:, None].to(b.kc.dtype), b.kc))
+    b.q.copy_(q.to(b.q.dtype).expand_as(b.q))
+    got = b.run(kernels).float().cpu().numpy().astype(np.float64)
+    half = HALF_STEP[dtype]
+    at, vc = score.cpu().numpy().astype(np.float64), b.vc.float().cpu().numpy().astype(np.float64)
+    scale = float(np.float32(b.scale))
+    for s, sees in enumerate(b.sees):
+        t = np.arange(int(b.ctx[s]))
+        blocks = b.table[s, t // 16]
+        x = scale * at[blocks, t % 16]
+        for j in range(len(sees)):
+            see = np.concatenate([np.ones(int(b.prior[s]), bool), sees[j]])
+            away = x[see] - x[see].max()
+            p = np.exp(away)
+            # Weights of e^-100 and less count for nothing; the others' relative error: the scale's, the product's and the
+            # difference's rounding (3 U of the distance), the exponential's, and the sum's.
+            dx = 3 * U * min(100.0, float(-away.min())) + 2 * U + (U / 2 * float(np.abs(x).max()) if d == 80 else 0)
+            rel = 2 * (dx + len(t) * U)
+            p /= p.sum()
+            for h in range(b.heads):
+                v = vc[blocks, h // 2, t % 16][see]
+                o, pv = p @ v, p @ np.abs(v)
+                tol = rel * pv * (1 + half) + half * np.abs(o) + 1e-30 + (2 * half * pv if dtype != "f32" else 0)
+                tol = tol + (len(t) * 2.0 ** -25 * np.abs(v).max() if dtype == "f16" else 0)
+                off = np.abs(got[int(b.cu[s]) + j, h] - o)
+                assert (off <= tol).all(), f"sequence {s} node {j} head {h}: {off.max():.3g}, {(off - tol).max():.3g} over"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,hkv,d,bs", [(4, 2, 256, 16), (6, 2, 80, 16), (4, 4, 96, 8)])
+def test_other_shapes_at_long_contexts(device, kernels, dtype, heads, hkv, d, bs):
+    rng = np.random.default_rng(d + heads)
+    TreeBatch(device, [4096, 0, 1777], [random_tree(rng, 24), [-1], random_tree(rng, 7)], dtype, heads, hkv, d, bs,
+              seed=d).check(kernels)
+
+
+@pytest.mark.parametrize("most", [1, 2, 12])
+def test_lengths_of_accepted_paths(device, kernels, most):
+    """Those of the plain walk without a limit, or the limit."""
+    rng = np.random.default_rng(most)
+    sizes = [0, 1, 2, 40, 200, 1024, 33] * 20
+    trees = [random_tree(rng, n, 9, roots=1 + n % 3) for n in sizes]
+    given = dict(agree=0.9, seed=most, sampled=rng.integers(0, 3, sum(sizes)))
+    lengths = check_verify(kernels, device, trees, None, most=most, **given)
+    whole = check_verify(kernels, device, trees, None, most=1024, **given)
+    assert lengths == [min(n, most) for n in whole] and max(whole) >= 9
+    assert accept([-1, 0, 1], [5, 1, 2], [1, 2, 9], 9) == ([0, 1, 2], 9)
