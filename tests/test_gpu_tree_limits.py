@@ -138,3 +138,44 @@ def test_lengths_of_accepted_paths(device, kernels, most):
     whole = check_verify(kernels, device, trees, None, most=1024, **given)
     assert lengths == [min(n, most) for n in whole] and max(whole) >= 9
     assert accept([-1, 0, 1], [5, 1, 2], [1, 2, 9], 9) == ([0, 1, 2], 9)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_as_many_sequences_as_there_may_be(device, kernels, dtype):
+    """65,535, most of them a root alone, which takes its own value; some padded, some long."""
+    rng = np.random.default_rng(4)
+    seqs, some = 65535, [0, 300, 40000, 65534]
+    trees = [[-1] if i % 7 else [] for i in range(seqs)]
+    prior = np.zeros(seqs, np.int64)
+    for s in some:
+        trees[s], prior[s] = random_tree(rng, 9), 500 + s % 100
+    b = TreeBatch(device, prior, trees, dtype, heads=4, hkv=2, d=64, seed=4)
+    got = b.run(kernels)
+    alone = np.asarray([s for s in range(seqs) if len(trees[s]) == 1])
+    rows = torch.as_tensor(b.cu[alone], device=device)
+    values = b.vc[torch.as_tensor(b.table[alone, 0].astype(np.int64), device=device), :, 0]
+    values = values.repeat_interleave(2, 1)
+    # p v / p: in 16 bits p is a power of two.  In fp32 it is 1 but for the rounding of its score, so the product (which
+    # may truncate, U), the quotient 1 / p and the product with that (U / 2 each) are rounded.
+    off = (got[rows].double() - values.double()).abs()
+    assert (off <= (2 * U if dtype == "f32" else 0) * values.double().abs()).all()
+    few = TreeBatch(device, prior[some], [trees[s] for s in some], dtype, heads=4, hkv=2, d=64)
+    few.kc, few.vc, few.table = b.kc, b.vc, b.table[some]
+    few.q = torch.cat([b.q[b.cu[s]:b.cu[s + 1]] for s in some])
+    few.verify(torch.cat([got[b.cu[s]:b.cu[s + 1]] for s in some]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_that_are_not_on_16_bytes(device, kernels, dtype):
+    """Queries, output or caches off the 16 bytes that the matrix cores' form reads: the other form."""
+    rng = np.random.default_rng(6)
+    b = TreeBatch(device, [50, 0, 7], [random_tree(rng, 12), [-1], random_tree(rng, 40)], dtype, seed=6)
+
+    def off(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=device)[1:].view(t.shape)
+        return flat.copy_(t)
+
+    q, kc, vc = b.q, b.kc.contiguous(), b.vc.contiguous()
+    for what in ("q", "out", "k", "v"):
+        b.q, b.kc, b.vc = off(q) if what == "q" else q, off(kc) if what == "k" else kc, off(vc) if what == "v" else vc
+        b.check(kernels, out=off(torch.full_like(q, float("nan"))) if what == "out" else None)
