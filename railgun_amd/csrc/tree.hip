@@ -540,12 +540,13 @@ extern "C" int rg_compact_tree(void* key_cache, void* value_cache, float* scores
   if (!key_cache || !value_cache || !block_table || !context_lens || !cu_nodes || !accepted || !num_accepted) {
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: null pointer argument", op);
   }
-  // (Every layer's workgroups read the lengths while the new ones are written.)
+  // (Every layer's workgroups read the lengths and the table while the new lengths are written.)
   const size_t entries = 4 * (size_t)num_seqs;
   if (new_context_lens != nullptr && (overlap(new_context_lens, entries, context_lens, entries) ||
                                       overlap(new_context_lens, entries, num_accepted, entries) ||
                                       overlap(new_context_lens, entries, accepted, entries * max_accepted) ||
-                                      overlap(new_context_lens, entries, cu_nodes, entries + 4))) {
+                                      overlap(new_context_lens, entries, cu_nodes, entries + 4) ||
+                                      overlap(new_context_lens, entries, block_table, entries * max_blocks_per_seq))) {
     return fail(RG_ERR_INVALID_ARGUMENT, "%s: new_context_lens overlaps an input", op);
   }
   const int64_t layers_apart = num_layers > 1 ? layer_stride : 0;

@@ -143,3 +143,9 @@ def test_attention_of_more_pieces_than_a_grid_has():
     assert lib.rg_paged_attention_tree_workspace_bytes(65535, 1024, 64, 8, 128, 16, 40) == 0
     assert lib.rg_paged_attention_tree_workspace_bytes(32768, 1024, 64, 8, 128, 16, 40) == 0     # 2^24 segments
     assert lib.rg_paged_attention_tree_workspace_bytes(32000, 1024, 64, 8, 128, 16, 40) > 0
+
+
+def test_compaction_refuses_lengths_over_the_block_table():
+    """Every layer's workgroups read the table while the new lengths are written."""
+    for at in (P + 60, P + 64, P + 92):                                # (two rows of four entries from P + 64 on)
+        expect(call("rg_compact_tree", COMPACT, dict(table=P + 64, new_lens=at)), INVALID, "overlaps")
