@@ -242,7 +242,9 @@ int rg_tree_layout(const int32_t* parents, const int32_t* cu_nodes, const int32_
  * it) gets zeros.  What a node does not attend to does not reach it, NaN and infinities included.
  * query / output [num_nodes, num_heads, head_dim].  Any shape of rg_paged_attention_v1; block sizes of
  * 16 * 2^j up to 256 and head_dim 64 or 128 run on the matrix cores, in bf16 / f16 with the
- * probabilities rounded to that type (in f16 times 2^7).  Needs a workspace of
+ * probabilities rounded to that type (in f16 times 2^7).  Other shapes run a wave to a node and head, a
+ * token at a time: as long as rg_paged_attention_v1 takes for a row per node, or up to 90 times that
+ * where sequences and nodes are few.  Needs a workspace of
  * rg_paged_attention_tree_workspace_bytes (16-byte aligned, no clearing) where that is not 0. */
 size_t rg_paged_attention_tree_workspace_bytes(int32_t num_seqs, int32_t max_nodes,
                                                int32_t num_heads, int32_t num_kv_heads,

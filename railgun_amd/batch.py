@@ -225,7 +225,8 @@ def pack_step(prefill_chunks: Sequence[PrefillChunk], decode_slots: Sequence[Dec
     to step.
 
     ``draft_trees``: sequences that check drafted tokens in this step; they neither share a prefix nor
-    gather scores, and their tokens' scores become 0 if the pool has any."""
+    gather scores, and their tokens' scores become 0 if the pool has any.  In bf16 / f16 their probabilities are
+    rounded to that type, where a decode row's stay in fp32."""
     tokens, positions, slots, ctx, tables = [], [], [], [], []
     cu = [0]
     for c in prefill_chunks:

@@ -18,7 +18,7 @@ namespace {
 // so a chain of n nodes takes log2 n rounds.  seen is updated in place: what a node reads early are ancestors too.
 // A workgroup has kLayoutWords of a tree's mask words, so that 1,024 nodes' fit in LDS; the positions and slots are
 // written by the first of a tree's.  Latency: the parents, lengths and table are read in three dependent steps, then a
-// barrier a round.  One tree of 24 nodes 3.5 us (1.3 KB), 256 of up to 128 6.2 us (1.7 MB).
+// barrier a round.  One tree of 64 nodes 3.4 us, 256 of 33 to 256 6.2 us (1.7 MB).
 constexpr int kLayoutThreads = 256;
 constexpr int kLayoutWords = 8;
 

@@ -93,7 +93,11 @@ struct TreeArgs {
 };
 
 // Any shape: a wave per (sequence, node, q-head), lane l has dims 4 l .. 4 l + 3, the keys one after the other with
-// the running maximum m and sum l of their weights.
+// the running maximum m and sum l of their weights.  Bound by a key's chain of load, sum over the wave and exponential,
+// 0.9 us for one of few waves: it is there to be right, and slower than a decode row per node, the more so the fewer of
+// them there are.  Measured (ms; 32 / 8 heads in bf16): 256 dims, one sequence of 4,096 with 64 nodes 3.9 (plain torch
+// operations 0.62, rg_paged_attention_v1 with a row per node 0.18), 64 of 512 to 4,096 with 8 to 32 nodes 21.7 (14.9,
+// 4.0); 96 dims 3.6 (0.57, 0.82) and 22.8 (7.7, 21.8).
 template <typename T>
 __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs a) {
   using E = elem<T>;
@@ -504,8 +508,6 @@ template <typename T> __device__ __forceinline__ uint32_t pair_cleared(uint32_t 
   return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
 }
 
-// Lane l of a wave owns query row l % 32 of it; the other half of that row's keys sits in lane l ^ 32.  sick: a word
-// of LDS per stage.
 // N copies of 1 KB to LDS, `step` bytes apart, non-temporal where they are read once.
 template <int N>
 __device__ __forceinline__ void copy(const char* base, uint32_t step, uint32_t lane_bytes, uint32_t lds_addr, bool once) {
@@ -518,6 +520,8 @@ __device__ __forceinline__ void copy(const char* base, uint32_t step, uint32_t l
   }
 }
 
+// Lane l of a wave owns query row l % 32 of it; the other half of that row's keys sits in lane l ^ 32.  sick: a word of
+// LDS for every tile that reaches into the tree (sick_word).
 template <typename T, int D>
 __device__ __forceinline__ void product(const Piece& p, char* lds, uint32_t* sick,
                                         uint32_t (&masks)[kMaskTiles][kRows], int w, int lane) {
@@ -997,14 +1001,18 @@ template <typename T, int D>
 constexpr int groups_per_cu() { return pieces_per_cu(std::is_same_v<T, f32_t> ? RG_DTYPE_F32 : RG_DTYPE_BF16, D); }
 
 // A workgroup to a piece.  What bounds it (bf16, 32 / 8 heads of 128; us):
-//  - many sequences, short trees: HBM.  64 of 512 to 4,096 tokens with 8 to 32 nodes, 639 MB: 127, 5.0 TB/s.
+//  - many sequences, short trees: HBM, and ends apart.  64 of 512 to 4,096 tokens with 8 to 32 nodes, 639 MB: 121 to
+//    141, 131 with the merge in a row of calls, 4.9 TB/s.  The pieces are of 17 to 40 tiles: their workgroups end 55 to
+//    121 in, at 94 on average.
 //  - long trees: the waves' LDS reads and the softmax between two products, which other workgroups' waves hide in part.
-//    Four sequences of 30,000 to 32,768 with 101 to 128 nodes, 253 GFLOP: 271, 930 TFLOP/s.  Without the copies to
-//    LDS it takes 15 % less, without the exponentials 7 %, without either product 20 %, without both products and
+//    Four sequences of 30,000 to 32,768 with 101 to 128 nodes, 253 GFLOP: 280 with the merge (12) in a row of calls, 900
+//    TFLOP/s; one by one under a profiler the first take 276 to 284, later ones up to 409.  Without the copies to LDS it
+//    takes 15 % less, without the exponentials 7 %, without either product 20 %, without both products and
 //    the exponentials still 53 % of it.  64 rows a wave would read LDS half as often, in 290 registers: one
 //    workgroup a CU.  The next tile's scores under this one's softmax and rings of 4 to 8 tiles gained nothing.
-//  - one sequence: latency.  4,096 tokens with 64 nodes: 20, of them 5 until the first tile is there (the cuts, the
-//    block table, Q and the tile follow each other), 8 tiles at 0.9 and 2 for the partials.
+//  - one sequence: latency.  4,096 tokens with 64 nodes: 20.4.  By stamps in the workgroups, on average: 0.4 until they
+//    start, 2.0 for the lengths and the cut, 0.9 to find the piece, 2.1 until table, masks and Q are there and 0.3 for
+//    the first tile, 6.8 for 8 tiles, 4.5 until the partials are written; the last of them ends at 19.0.
 // fp32: v_mfma_f32_32x32x2 has a sixteenth of the rate, and what a row tile lacks of rows is computed all the same; 64
 // sequences of 512 to 2,048 with 4 to 8 nodes, 64 dims, 108, 1.5 times the bytes' floor.
 template <typename T, int D>

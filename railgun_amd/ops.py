@@ -638,8 +638,13 @@ class PagedAttentionKernels:
                     scale: float, max_nodes: int, workspace: Optional[torch.Tensor] = None) -> None:
         """Attention of the nodes of trees of drafted tokens, query / output [N, H, D], over the paged cache
         that holds their K and V too (rg_paged_attention_tree): a node attends to all positions before its
-        tree and to the nodes that its row of ``tree_mask`` [N, words] has set.  ``workspace``:
-        tree_workspace_bytes, allocated here when omitted."""
+        tree and to the nodes that its row of ``tree_mask`` [N, words] has set.  Of a tree of more than
+        ``max_nodes`` nodes the others are passed over.  ``workspace``: tree_workspace_bytes, allocated here
+        when omitted.
+
+        In bf16 / f16 the probabilities are rounded to that type before the product with V where head_dim is
+        64 or 128 and the block size 16 * 2^j up to 256 (launch_v1 keeps them in fp32); other shapes keep
+        them and are far slower."""
         device = query.get_device()
         _require_i32_on(device, block_table, context_lens, cu_nodes, tree_mask)
         _require_on(device, query, key_cache, value_cache, output)
@@ -901,7 +906,7 @@ class PagedAttentionOp:
                      workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """execute() for trees of drafted tokens: q [N, H, D] of all nodes -> new output [N, H, D], what belongs
         to no sequence left unset (launch_tree); the workspace (tree_workspace_bytes) is allocated here when
-        omitted."""
+        omitted.  In bf16 / f16 the probabilities are rounded to that type (launch_tree)."""
         if q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or k_cache.dim() != 4 or \
                 tuple(k_cache.shape[1:]) != (self.num_kv_heads, self.block_size, self.head_dim):
             raise RailgunError(_lib.RG_ERR_INVALID_ARGUMENT,
